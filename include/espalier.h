@@ -405,6 +405,65 @@ int esp_add_rmsnorm(void* h, const void* d1, const void* d2, const void* w, void
 int esp_argmax(const void* logits, int64_t stride, int64_t T, int64_t N, int dtype, int32_t* ids, int64_t* part,
                int64_t part_numel, int32_t* counters, int64_t counters_numel, void* stream);
 
+/* The norms after and before a block, with its gate and the residual scale: d = d1 + d2 (d2 may be NULL),
+ * u = (d / sqrt(mean(d^2) + eps)) * w_post (u = d when w_post is NULL), z = h + (scale * f(g)) * u, h_out = z in dtype,
+ * out = (h_out / sqrt(mean(h_out^2) + eps)) * w_pre, h_out as stored; everything in fp32, each output rounded once. gate
+ * (may be NULL: f(g) = 1): element i of row t at gate[t * gate_row + i * gate_col], gate_col 1 for a gate an element
+ * (gate_row 0: one row for all), 0 for a gate a row; f is the value itself or, with gate_sigmoid, its sigmoid. h_out may be
+ * h. dtype ESP_BF16 or ESP_F16 for all; [T][D] row-major, D % 8 == 0, D <= 8192, 16-byte aligned (a gate an element with
+ * rows of 16 bytes too). A row's bits depend on that row alone; with d2, gate and w_post NULL and scale 1 they are
+ * esp_add_rmsnorm's. */
+int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d2, const void* w_post, const void* gate,
+                         int64_t gate_row, int64_t gate_col, int gate_sigmoid, double scale, const void* w_pre, void* h_out,
+                         void* out, int64_t T, int64_t D, double eps, int dtype, void* stream);
+
+/* ---- Low-rank adapters of many requests beside a shared projection (csrc/lora.hip). No counterpart in the reference. ---- */
+
+/* For row m of adapter a = rows[m] (int32 on the device) and column n of matrix s of the layer (n_shards, 1 to 4, side by
+ * side in y from column 0, n_cols[s] columns each, multiples of 16):
+ *   out[m][n] = y[m][n] + sum_{j < r} (scales[a][s] * sum_k x[m][k] * A[a][s][j][k]) * B[a][n][j],   r = ranks[a][s],
+ * summed in fp32 and rounded once. A row whose adapter is outside [0, slots) keeps y's bits. x [T][K], y and out [T][N] with
+ * row strides, N = sum(n_cols); A [slots][n_shards][R][K], B [slots][N][R], ranks int32 and scales fp32 [slots][n_shards],
+ * on the device; R (a multiple of 16, at most 256) is the rank rows that the adapters are laid out with, and what lies past
+ * an adapter's rank is not used, whatever it holds. out may be y (in place); columns past N are left as they are. dtype
+ * ESP_BF16 or ESP_F16 for x, y, out, A and B. K a multiple of 16. scratch: at least esp_lora_scratch(T, K, n_shards, R)
+ * floats, any values. Alignment: x, y, out 8 bytes with strides a multiple of 4 elements (16 and 8 are faster), A, B and
+ * scratch 16. A row's bits depend on that row and its adapter alone. */
+int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out, int64_t out_stride,
+             const int32_t* rows, int64_t T, int64_t K, int64_t n_shards, const int64_t* n_cols, const void* A, const void* B,
+             const int32_t* ranks, const float* scales, int64_t slots, int64_t R, int dtype, float* scratch,
+             int64_t scratch_numel, void* stream);
+
+/* Floats of scratch that esp_lora needs. */
+int64_t esp_lora_scratch(int64_t T, int64_t K, int64_t n_shards, int64_t R);
+
+/* ---- Verification of drafted tokens (csrc/verify.hip). No counterpart in the reference. ---- */
+
+/* Request b < B has n = n_drafts[b] drafts drafts[b][0 .. n) (0 <= n <= G) and the rows first[b] .. first[b] + n of the
+ * target's logits [R][V] (row stride `stride`, dtype any of the three): the rows that verify its drafts in order, and the one
+ * behind them. p_j = softmax(row j / temperature[b]); q_j = probs[b][j] (fp32, strides probs_request and probs_row, V
+ * values), what draft j was drawn from, or, with probs NULL, a drafter that was sure of its draft. Draft j is accepted iff
+ * uniform[b][j] * q_j(draft) < p_j(draft) (q_j(draft) = 1 without probs). At the first draft that is not, a token is drawn
+ * from max(p_j - q_j, 0) (p_j without the draft's own probability when probs is NULL; p_j itself where that leaves nothing),
+ * behind n accepted drafts from p_n: the index of the largest w_v / race[b][v] (race fp32, row stride race_stride: exponential
+ * random numbers), the lowest among equal ones. A temperature below 1e-5 (or NaN) means a greedy request: draft j is accepted
+ * iff it is the row's argmax (as esp_argmax: a NaN is the largest; zeros of both signs are equal), which is else the token
+ * drawn.
+ * tokens [B][G + 1] int32: the accepted drafts, then the token drawn, then -1; counts [B]: how many tokens; logprobs
+ * [B][G + 1] fp32: log p_j of each token (of a greedy request at temperature 1), 0 past them. A row without a distribution (a
+ * NaN or +inf in it, or nothing above -inf) accepts nothing and draws nothing if the request is not greedy, and its
+ * log-probabilities are 0. A request with n_drafts outside [0, G] or rows outside the logits has no tokens (-1 and 0: the
+ * padding of a batch). A draft outside [0, V) is never accepted. Arrays contiguous unless a stride is given; rows may start
+ * at any element. B <= 2^20, G <= 1024, B * (G + 1) <= 2^23, V <= 2^24.
+ * scratch: esp_verify_scratch bytes, 16-byte aligned, any values. */
+int esp_verify(const void* logits, int dtype, int64_t stride, int64_t R, int64_t V, const int32_t* first,
+               const int32_t* n_drafts, const int32_t* drafts, int64_t B, int64_t G, const float* uniform, const float* race,
+               int64_t race_stride, const float* temperature, const float* probs, int64_t probs_request, int64_t probs_row,
+               int32_t* tokens, int32_t* counts, float* logprobs, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Bytes of scratch that esp_verify needs. */
+int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

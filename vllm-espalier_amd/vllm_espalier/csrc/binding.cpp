@@ -732,6 +732,132 @@ void argmax(const at::Tensor& logits, at::Tensor ids, std::optional<at::Tensor> 
                     counters.has_value() ? counters->numel() : 0, cur_stream()));
 }
 
+// Every tensor of a call on one device
+static void on_device(const at::Tensor& t, const at::Tensor& first, const char* name) {
+    TORCH_CHECK(t.device() == first.device(), name, ": expected a tensor on ", first.device());
+}
+
+// esp_sandwich_rmsnorm (csrc/sandwich.hip): gate [T, D], [D] (every row's) or [T, 1] (a row's), or none
+void sandwich_rmsnorm(const at::Tensor& h, const at::Tensor& d1, const c10::optional<at::Tensor>& d2,
+                      const c10::optional<at::Tensor>& w_post, const c10::optional<at::Tensor>& gate, bool gate_sigmoid,
+                      double scale, const at::Tensor& w_pre, double eps, at::Tensor h_out, at::Tensor out) {
+    TORCH_CHECK(h.is_cuda() && h.is_contiguous() && h.dim() == 2, "h: [T, D] contiguous");
+    const auto t = h.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, "h: bf16 or fp16");
+    const int64_t T = h.size(0), D = h.size(1);
+    const auto rows = [&](const at::Tensor& v, const char* name) {
+        check(v, t, name);
+        on_device(v, h, name);
+        TORCH_CHECK(v.sizes() == h.sizes(), name, ": h's shape");
+    };
+    const auto weight = [&](const at::Tensor& v, const char* name) {
+        check(v, t, name);
+        on_device(v, h, name);
+        TORCH_CHECK(v.dim() == 1 && v.numel() == D, name, ": [D]");
+    };
+    rows(d1, "d1");
+    if (d2.has_value()) rows(*d2, "d2");
+    rows(h_out, "h_out");
+    rows(out, "out");
+    if (w_post.has_value()) weight(*w_post, "w_post");
+    weight(w_pre, "w_pre");
+    int64_t gate_row = 0, gate_col = 0;
+    if (gate.has_value()) {
+        const at::Tensor& g = *gate;
+        TORCH_CHECK(g.is_cuda() && g.scalar_type() == t, "gate: a CUDA tensor of h's dtype");
+        on_device(g, h, "gate");
+        if (g.dim() == 1) {
+            TORCH_CHECK(g.numel() == D && g.stride(0) == 1, "gate: [T, D], [D] or [T, 1]");
+            gate_col = 1;
+        } else {
+            TORCH_CHECK(g.dim() == 2 && g.size(0) == T && (g.size(1) == D || g.size(1) == 1), "gate: [T, D], [D] or [T, 1]");
+            gate_col = g.size(1) == 1 ? 0 : 1;
+            TORCH_CHECK(gate_col == 0 || g.stride(1) == 1, "gate: unit column stride");
+            gate_row = T > 1 ? g.stride(0) : 0;
+        }
+    }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(h.device());
+    call(esp_sandwich_rmsnorm(h.data_ptr(), d1.data_ptr(), d2.has_value() ? d2->data_ptr() : nullptr,
+                              w_post.has_value() ? w_post->data_ptr() : nullptr,
+                              gate.has_value() ? gate->data_ptr() : nullptr, gate_row, gate_col, gate_sigmoid, scale,
+                              w_pre.data_ptr(), h_out.data_ptr(), out.data_ptr(), T, D, eps, dtype_code(h), cur_stream()));
+}
+
+// esp_lora (csrc/lora.hip): out = y + the rows' own adapters' products; the layer's matrices of n_cols columns side by side
+void lora(const at::Tensor& x, const at::Tensor& y, at::Tensor out, const at::Tensor& rows, const at::Tensor& a,
+          const at::Tensor& b, const at::Tensor& ranks, const at::Tensor& scales, const std::vector<int64_t>& n_cols) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1), "x: [T, K], unit column stride");
+    const auto t = x.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, "x: bf16 or fp16");
+    const int64_t T = x.size(0), K = x.size(1), S = (int64_t)n_cols.size();
+    check(a, t, "a");
+    check(b, t, "b");
+    check(ranks, at::kInt, "ranks");
+    check(scales, at::kFloat, "scales");
+    check(rows, at::kInt, "rows");
+    for (const at::Tensor& v : {y, out, rows, a, b, ranks, scales}) on_device(v, x, "lora");
+    TORCH_CHECK(a.dim() == 4 && a.size(1) == S && a.size(3) == K, "a: [slots, matrices, R, K]");
+    const int64_t slots = a.size(0), R = a.size(2);
+    int64_t N = 0;
+    for (const int64_t n : n_cols) N += n;
+    TORCH_CHECK(b.dim() == 3 && b.size(0) == slots && b.size(1) == N && b.size(2) == R, "b: [slots, N, R]");
+    TORCH_CHECK(ranks.numel() == slots * S && scales.numel() == slots * S, "ranks / scales: [slots, matrices]");
+    TORCH_CHECK(rows.numel() == T, "rows: [T]");
+    for (const at::Tensor& v : {y, out})
+        TORCH_CHECK(v.scalar_type() == t && v.dim() == 2 && v.size(0) == T && v.size(1) >= N && v.stride(1) == 1,
+                    "y / out: [T, at least N columns], x's dtype, unit column stride");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const int64_t numel = esp_lora_scratch(T, K, S, R);
+    const at::Tensor scratch = at::empty({numel}, x.options().dtype(at::kFloat));
+    call(esp_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), cptr<int32_t>(rows), T,
+                  K, S, n_cols.data(), a.data_ptr(), b.data_ptr(), cptr<int32_t>(ranks), cptr<float>(scales), slots, R,
+                  dtype_code(x), mptr<float>(scratch), numel, cur_stream()));
+}
+
+// esp_verify (csrc/verify.hip): drafted tokens [B, G] against the target's logits
+void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor& n_drafts, const at::Tensor& drafts,
+            const at::Tensor& uniform, const at::Tensor& race, const at::Tensor& temperature,
+            const c10::optional<at::Tensor>& probs, at::Tensor tokens, at::Tensor counts, at::Tensor logprobs) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+                "logits: [R, V], unit column stride");
+    const auto t = logits.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, "logits: bf16, fp16 or fp32");
+    check(first, at::kInt, "first");
+    check(n_drafts, at::kInt, "n_drafts");
+    check(drafts, at::kInt, "drafts");
+    check(uniform, at::kFloat, "uniform");
+    check(temperature, at::kFloat, "temperature");
+    check(tokens, at::kInt, "tokens");
+    check(counts, at::kInt, "counts");
+    check(logprobs, at::kFloat, "logprobs");
+    for (const at::Tensor& v : {first, n_drafts, drafts, uniform, race, temperature, tokens, counts, logprobs})
+        on_device(v, logits, "verify");
+    TORCH_CHECK(drafts.dim() == 2, "drafts: [B, G]");
+    const int64_t B = drafts.size(0), G = drafts.size(1), V = logits.size(1);
+    TORCH_CHECK(first.numel() == B && n_drafts.numel() == B && temperature.numel() == B && counts.numel() == B,
+                "first / n_drafts / temperature / counts: [B]");
+    TORCH_CHECK(uniform.sizes() == drafts.sizes(), "uniform: [B, G]");
+    TORCH_CHECK(race.is_cuda() && race.scalar_type() == at::kFloat && race.dim() == 2 && race.size(0) == B &&
+                    race.size(1) == V && (V <= 1 || race.stride(1) == 1), "race: fp32 [B, V], unit column stride");
+    TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == G + 1 && logprobs.sizes() == tokens.sizes(),
+                "tokens / logprobs: [B, G + 1]");
+    if (probs.has_value()) {
+        on_device(*probs, logits, "probs");
+        TORCH_CHECK(probs->is_cuda() && probs->scalar_type() == at::kFloat && probs->dim() == 3 && probs->size(0) == B &&
+                        probs->size(1) == G && probs->size(2) == V && (V <= 1 || probs->stride(2) == 1),
+                    "probs: fp32 [B, G, V], unit column stride");
+    }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+    const int64_t bytes = esp_verify_scratch(B, G, V, dtype_code(logits));
+    const at::Tensor scratch = at::empty({bytes}, logits.options().dtype(at::kByte));
+    call(esp_verify(logits.data_ptr(), dtype_code(logits), logits.stride(0), logits.size(0), V, cptr<int32_t>(first),
+                    cptr<int32_t>(n_drafts), cptr<int32_t>(drafts), B, G, cptr<float>(uniform), cptr<float>(race),
+                    race.stride(0), cptr<float>(temperature), probs.has_value() ? cptr<float>(*probs) : nullptr,
+                    probs.has_value() ? probs->stride(0) : 0, probs.has_value() ? probs->stride(1) : 0,
+                    mptr<int32_t>(tokens), mptr<int32_t>(counts), mptr<float>(logprobs), scratch.data_ptr(), bytes,
+                    cur_stream()));
+}
+
 // several dense launches as one (esp_dense_multi; no reference counterpart): per group its input rows, matrices,
 // output columns and plan; after[g] != 0 when group g's x is a view of group g - 1's y. The optional norm (h, d1, d2,
 // w, h_out, eps) makes group 0's input RMSNorm(h + d1 + d2) * w, as dense_rmsnorm does.
@@ -856,6 +982,9 @@ PYBIND11_MODULE(espalier_ext, m) {
     m.def("dense_own", &dense_own);
     m.def("embed", &embed);
     m.def("add_rmsnorm", &add_rmsnorm);
+    m.def("sandwich_rmsnorm", &sandwich_rmsnorm);
+    m.def("lora", &lora);
+    m.def("verify", &verify);
     m.def("argmax", &argmax, py::arg("logits"), py::arg("ids"), py::arg("part") = py::none(),
           py::arg("counters") = py::none());
 }
