@@ -423,19 +423,24 @@ int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d2, const vo
  * side in y from column 0, n_cols[s] columns each, multiples of 16):
  *   out[m][n] = y[m][n] + sum_{j < r} (scales[a][s] * sum_k x[m][k] * A[a][s][j][k]) * B[a][n][j],   r = ranks[a][s],
  * summed in fp32 and rounded once. A row whose adapter is outside [0, slots) keeps y's bits. x [T][K], y and out [T][N] with
- * row strides, N = sum(n_cols); A [slots][n_shards][R][K], B [slots][N][R], ranks int32 and scales fp32 [slots][n_shards],
- * on the device; R (a multiple of 16, at most 256) is the rank rows that the adapters are laid out with, and what lies past
- * an adapter's rank is not used, whatever it holds. out may be y (in place); columns past N are left as they are. dtype
- * ESP_BF16 or ESP_F16 for x, y, out, A and B. K a multiple of 16. scratch: at least esp_lora_scratch(T, K, n_shards, R)
- * floats, any values. Alignment: x, y, out 8 bytes with strides a multiple of 4 elements (16 and 8 are faster), A, B and
- * scratch 16. A row's bits depend on that row and its adapter alone. */
+ * row strides, N = sum(n_cols); ranks int32 and scales fp32 [slots][n_shards] on the device. out may be y (in place), and must
+ * else overlap neither y nor x; columns past N are left as they are. dtype ESP_BF16 or ESP_F16 for x, y, out, A and B. K a
+ * multiple of 16.
+ * A and B are laid out as the matrix instructions read them, R (a multiple of 16, at most 256) ranks a slot, zeros where an
+ * adapter has nothing (past its rank in its last 16 ranks, past K, past a matrix's columns); 16-rank tiles past the rank are
+ * not used, whatever they hold:
+ *   A [slots][n_shards][R / 16][ceil(K / 32)][4][16][8]: element [..][jt][u][g][j][i] is A[16 jt + j][32 u + 8 g + i];
+ *   B [slots][column tiles][R / 16][8][2][16][8]: each matrix's columns in tiles of 128 of its own; element
+ *     [..][ct][jt][c][h][n][i] is B[128 ct + 8 n + c][16 jt + 8 h + i].
+ * scratch: at least esp_lora_scratch(T, N, n_shards, R) floats, any values. Alignment: x, y, out 8 bytes with strides a
+ * multiple of 4 elements, A, B and scratch 16. A row's bits depend on that row and its adapter alone. */
 int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out, int64_t out_stride,
              const int32_t* rows, int64_t T, int64_t K, int64_t n_shards, const int64_t* n_cols, const void* A, const void* B,
              const int32_t* ranks, const float* scales, int64_t slots, int64_t R, int dtype, float* scratch,
              int64_t scratch_numel, void* stream);
 
 /* Floats of scratch that esp_lora needs. */
-int64_t esp_lora_scratch(int64_t T, int64_t K, int64_t n_shards, int64_t R);
+int64_t esp_lora_scratch(int64_t T, int64_t N, int64_t n_shards, int64_t R);
 
 /* ---- Verification of drafted tokens (csrc/verify.hip). No counterpart in the reference. ---- */
 
@@ -454,7 +459,8 @@ int64_t esp_lora_scratch(int64_t T, int64_t K, int64_t n_shards, int64_t R);
  * NaN or +inf in it, or nothing above -inf) accepts nothing and draws nothing if the request is not greedy, and its
  * log-probabilities are 0. A request with n_drafts outside [0, G] or rows outside the logits has no tokens (-1 and 0: the
  * padding of a batch). A draft outside [0, V) is never accepted. Arrays contiguous unless a stride is given; rows may start
- * at any element. B <= 2^20, G <= 1024, B * (G + 1) <= 2^23, V <= 2^24.
+ * at any element. B <= 2^20, G <= 1024, V <= 2^24,
+ * B * (G + 1) * ceil(V / 4096) < 2^24.
  * scratch: esp_verify_scratch bytes, 16-byte aligned, any values. */
 int esp_verify(const void* logits, int dtype, int64_t stride, int64_t R, int64_t V, const int32_t* first,
                const int32_t* n_drafts, const int32_t* drafts, int64_t B, int64_t G, const float* uniform, const float* race,
@@ -462,7 +468,7 @@ int esp_verify(const void* logits, int dtype, int64_t stride, int64_t R, int64_t
                int32_t* tokens, int32_t* counts, float* logprobs, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* Bytes of scratch that esp_verify needs. */
-int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V, int dtype);
+int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V);
 
 #ifdef __cplusplus
 }

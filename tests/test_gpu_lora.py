@@ -66,7 +66,7 @@ def _rows(T, L, gen, mixed=True):
     return rows.to(torch.int32)
 
 
-@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 33, 256, 257, 530])
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 33, 256, 257, 530, 1601])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_lora_rows(dev, T, dtype):
     print(f"lora rows {T} {dtype}", flush=True)
@@ -87,7 +87,7 @@ def test_lora_rows(dev, T, dtype):
 @pytest.mark.parametrize("K,outs,ranks", [
     (16, [16], [1]), (64, [64], [16, 16]), (80, [16, 16, 16, 16], [2, 5]), (2048, [4096, 512, 512], [16, 64]), (4096, [2048], [8]),
     (512, [2048], [256, 31]), (1040, [80, 1024], [128, 1]), (5120, [32], [33]), (2048, [64] * 4, [64, 48]), (96, [8208], [12])])
-@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("T", [3, 40, 300, 1537])
 def test_lora_shapes(dev, K, outs, ranks, T):
     print(f"lora {K} -> {outs}, ranks {ranks}, {T} rows", flush=True)
     gen = torch.Generator().manual_seed(K + T)
@@ -99,7 +99,7 @@ def test_lora_shapes(dev, K, outs, ranks, T):
     _check(store.apply(x, y, rows.to(dev), out=torch.empty_like(y)), x, y, rows, a, b, scales, outs, dtype)
 
 
-@pytest.mark.parametrize("T", [5, 300])
+@pytest.mark.parametrize("T", [5, 300, 1700])
 def test_lora_rows_alone_equal_batch(dev, T):
     """A row's bits are its own: alone, in windows and in the whole batch, whatever stands beside it."""
     gen = torch.Generator().manual_seed(2)
@@ -109,14 +109,14 @@ def test_lora_rows_alone_equal_batch(dev, T):
     y = torch.randn((T, sum(outs)), generator=gen).to(torch.bfloat16).to(dev)
     rows = _rows(T, 3, gen).to(dev)
     whole = store.apply(x, y, rows, out=torch.empty_like(y))
-    for step in (1, 7, 64, 290):
-        for r0 in range(0, T, step * (1 if step > 1 else 37)):
+    for step in (1, 7, 64, 290, 1543):
+        for r0 in range(0, T, step * (1 if step > 1 else 37) * (1 + T // 600)):
             part = slice(r0, r0 + step)
             got = store.apply(x[part], y[part], rows[part], out=torch.empty_like(y[part]))
             assert torch.equal(got.view(torch.int16), whole[part].view(torch.int16)), (step, r0)
 
 
-@pytest.mark.parametrize("T", [6, 290])
+@pytest.mark.parametrize("T", [6, 290, 1540])
 def test_lora_strides_and_columns(dev, T):
     """Views of wider buffers, whose rows are 8-byte aligned only, a padded output, and rows of no or a far adapter."""
     gen = torch.Generator().manual_seed(4)
@@ -134,16 +134,16 @@ def test_lora_strides_and_columns(dev, T):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("T", [4, 272])
+@pytest.mark.parametrize("T", [4, 272, 1552])
 def test_lora_isolation(dev, T, dtype):
     """What is not a row's own does not reach it: NaN behind a slot's rank, infinities in another adapter, a NaN in another
     row's input; an adapter cleared, loaded again with a smaller rank, or without one of its matrices."""
     gen = torch.Generator().manual_seed(9)
     K, outs = 256, [64, 32]
     store, a, b, scales = _store(K, outs, [5, 24, 16], dtype, gen, dev, max_rank=32)
-    for i, r in enumerate([5, 24, 16]):
-        store.a[i, :, r:] = float("nan")
-        store.b[i, :, r:] = float("nan")
+    for i, r in enumerate([5, 24, 16]):                      # tiles of 16 ranks past the adapter's
+        store.a[i, :, -(-r // 16):] = float("nan")
+        store.b[i, :, -(-r // 16):] = float("nan")
     store.a[2], store.b[2] = float("inf"), float("nan")
     x = torch.randn((T, K), generator=gen).to(dtype).to(dev)
     y = torch.randn((T, sum(outs)), generator=gen).to(dtype).to(dev)
@@ -251,6 +251,6 @@ def test_lora_empty_and_refusals(dev, ext):
         with pytest.raises(RuntimeError):
             store.apply(*args)
     with pytest.raises(RuntimeError):
-        ext.lora(x, y, y, rows, store.a, store.b[:, :16], store.ranks, store.scales, [32])
+        ext.lora(x, y, y, rows, store.a, store.b[:, :0], store.ranks, store.scales, [32])
     with pytest.raises(RuntimeError):
         ext.lora(x, y, y, rows, store.a, store.b, store.ranks, store.scales, [16, 16])

@@ -20,7 +20,7 @@ def lib(ext):
     L.esp_lora.argtypes = [P, I64, P, I64, P, I64, P, I64, I64, I64, ctypes.POINTER(I64), P, P, P, P, I64, I64, INT, P, I64, P]
     L.esp_lora_scratch.argtypes, L.esp_lora_scratch.restype = [I64] * 4, I64
     L.esp_verify.argtypes = [P, INT, I64, I64, I64, P, P, P, I64, I64, P, P, I64, P, P, I64, I64, P, P, P, P, I64, P]
-    L.esp_verify_scratch.argtypes, L.esp_verify_scratch.restype = [I64, I64, I64, INT], I64
+    L.esp_verify_scratch.argtypes, L.esp_verify_scratch.restype = [I64, I64, I64], I64
     return L
 
 
@@ -72,8 +72,8 @@ def test_lora_argument_errors(lib, over, needle):
 def test_scratch_sizes(lib):
     assert lib.esp_lora_scratch(4, 64, 1, 16) >= 64
     assert lib.esp_lora_scratch(0, 64, 1, 16) == 0
-    assert lib.esp_verify_scratch(4, 2, 100, 1) > 0
-    assert lib.esp_verify_scratch(0, 2, 100, 1) == 0
+    assert lib.esp_verify_scratch(4, 2, 100) > 0
+    assert lib.esp_verify_scratch(0, 2, 100) == 0
 
 
 def _verify(lib, **over):
@@ -86,7 +86,7 @@ def _verify(lib, **over):
 
 
 @pytest.mark.parametrize("over,needle", [
-    (dict(dtype=3), "dtype"), (dict(B=-1), "requests"), (dict(B=1 << 21), "requests"), (dict(G=-1), "drafts"),
+    (dict(dtype=3), "dtype"), (dict(B=-1), "requests"), (dict(B=1 << 21), "requests"), (dict(B=1 << 20, V=1 << 24, G=1024), "blocks"), (dict(G=-1), "drafts"),
     (dict(G=1025), "drafts"), (dict(R=1 << 31), "rows"), (dict(V=0), "V"), (dict(V=1 << 28), "V"), (dict(logits=None), "null"),
     (dict(first=None), "null"), (dict(drafts=None), "null"), (dict(race=None), "null"), (dict(scratch=None), "null"),
     (dict(stride=63), "overlap"), (dict(rs=63), "overlap"), (dict(pr=-1), "stride"), (dict(logits=17), "aligned"),
@@ -96,17 +96,35 @@ def test_verify_argument_errors(lib, over, needle):
     assert needle in lib.esp_last_error().decode()
 
 
+def test_adapters_layout():
+    """The places of the elements in a slot, as the C header gives them."""
+    gen = torch.Generator().manual_seed(1)
+    K, outs, r = 48, [144, 16], 19
+    store = Adapters(K, outs, slots=1, max_rank=20, device="cpu")
+    a = [torch.randn((r, K), generator=gen).to(torch.bfloat16) for _ in outs]
+    b = [torch.randn((n, r), generator=gen).to(torch.bfloat16) for n in outs]
+    store.load(0, a, b)
+    for s, first in ((0, 0), (1, 2)):
+        for j, k in ((0, 0), (18, 47), (7, 33), (16, 12)):
+            assert store.a[0, s, j // 16, k // 32, k % 32 // 8, j % 16, k % 8] == a[s][j, k]
+        for n, j in ((0, 0), (outs[s] - 1, 18), (13, 9), (outs[s] // 2, 17)):
+            assert store.b[0, first + n // 128, j // 16, n % 8, j % 16 // 8, n % 128 // 8, j % 8] == b[s][n, j]
+    assert int((store.a != 0).sum()) == sum(int((t != 0).sum()) for t in a)
+    assert int((store.b != 0).sum()) == sum(int((t != 0).sum()) for t in b)
+
+
 def test_adapters_checks():
     for bad in (dict(in_features=24), dict(out_features=[16, 8]), dict(out_features=[]), dict(out_features=[16] * 5), dict(slots=0),
                 dict(max_rank=0), dict(max_rank=257), dict(dtype=torch.float32)):
         with pytest.raises(ValueError):
             Adapters(**{**dict(in_features=32, out_features=[16, 32], slots=2, max_rank=8, device="cpu"), **bad})
     store = Adapters(32, [16, 32], slots=2, max_rank=8, device="cpu")
-    assert store.a.shape == (2, 2, 16, 32) and store.b.shape == (2, 48, 16)
+    assert store.a.shape == (2, 2, 1, 1, 4, 16, 8) and store.b.shape == (2, 2, 1, 8, 2, 16, 8)
     a, b = [torch.ones((4, 32)), None], [torch.ones((16, 4)), None]
     store.load(1, a, b, scale=0.5)
     assert store.ranks.tolist() == [[0, 0], [4, 0]] and store.scales[1, 0] == 0.5
-    assert float(store.a[1, 0, :4].float().sum()) == 128 and float(store.b[1, :16, :4].float().sum()) == 64
+    assert float(store.a[1, 0].float().sum()) == 128 and float(store.b[1, 0].float().sum()) == 64
+    assert not store.a[1, 1].any() and not store.b[1, 1].any()
     bad_b = [torch.ones((16, 5)), None]
     for args in ((2, a, b), (-1, a, b), (0, a[:1], b), (0, a, [b[0], torch.ones((32, 4))]), (0, a, bad_b),
                  (0, [torch.ones((9, 32)), None], [torch.ones((16, 9)), None]), (0, [torch.ones((4, 16)), None], b),

@@ -14,14 +14,34 @@ from .experts import ext
 
 MAX_MATRICES = 4             # matrices of a layer, as one dense launch takes
 MAX_RANK = 256
-RANK_TILE = 16               # slots are laid out in whole tiles of ranks
+RANK_TILE = 16               # slots are laid out in whole tiles of ranks,
+K_UNIT, COLUMN_TILE = 32, 128   # units of k (A) and tiles of a matrix's columns (B): esp_lora's layout
+
+
+def _padded(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """t in the corner of a [rows, cols] of zeros (whole tiles)."""
+    up = lambda n, m: -(-n // m) * m  # noqa: E731
+    return torch.nn.functional.pad(t, (0, up(t.shape[1], cols) - t.shape[1], 0, up(t.shape[0], rows) - t.shape[0]))
+
+
+def pack_a(low: torch.Tensor) -> torch.Tensor:
+    """A [rank, in] as esp_lora reads it: [rank tiles, k units, 4, 16, 8]."""
+    t = _padded(low, RANK_TILE, K_UNIT)
+    return t.view(-1, RANK_TILE, t.shape[1] // K_UNIT, 4, 8).permute(0, 2, 3, 1, 4)
+
+
+def pack_b(high: torch.Tensor) -> torch.Tensor:
+    """B [out, rank] as esp_lora reads it: [column tiles, rank tiles, 8, 2, 16, 8]."""
+    t = _padded(high, COLUMN_TILE, RANK_TILE)
+    return t.view(-1, 16, 8, t.shape[1] // RANK_TILE, 2, 8).permute(0, 3, 2, 4, 1, 5)
 
 
 class Adapters:
     """The adapters of a layer in_features -> sum(out_features), whose matrices' columns stand side by side in its output (the
     Dense layout). in_features and out_features are multiples of 16; dtype is that of the rows (bf16 or fp16).
 
-    Memory: slots * max_rank * (matrices * in_features + sum(out_features)) elements, max_rank rounded up to 16."""
+    Memory: slots * max_rank * (matrices * in_features + sum(out_features)) elements, max_rank rounded up to 16, in_features to
+    32 and every matrix's columns to 128."""
 
     def __init__(self, in_features: int, out_features, slots: int, max_rank: int, dtype=torch.bfloat16, device="cuda"):
         self.in_features, self.out_features = int(in_features), [int(n) for n in out_features]
@@ -34,9 +54,11 @@ class Adapters:
             raise ValueError(f"at least one slot and a max_rank of 1 to {MAX_RANK}")
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("adapters are bf16 or fp16")
-        R, S, self.n = -(-self.max_rank // RANK_TILE) * RANK_TILE, len(self.out_features), sum(self.out_features)
-        self.a = torch.zeros((self.slots, S, R, self.in_features), dtype=dtype, device=device)
-        self.b = torch.zeros((self.slots, self.n, R), dtype=dtype, device=device)
+        tiles, S, self.n = -(-self.max_rank // RANK_TILE), len(self.out_features), sum(self.out_features)
+        self.col_tiles = [-(-n // COLUMN_TILE) for n in self.out_features]
+        units = -(-self.in_features // K_UNIT)
+        self.a = torch.zeros((self.slots, S, tiles, units, 4, 16, 8), dtype=dtype, device=device)
+        self.b = torch.zeros((self.slots, sum(self.col_tiles), tiles, 8, 2, 16, 8), dtype=dtype, device=device)
         self.ranks = torch.zeros((self.slots, S), dtype=torch.int32, device=device)
         self.scales = torch.zeros((self.slots, S), dtype=torch.float32, device=device)
 
@@ -62,11 +84,12 @@ class Adapters:
         for s, (low, high) in enumerate(zip(a, b)):
             if low is not None:
                 rank = low.shape[0]
-                self.a[slot, s, :rank].copy_(low)
-                self.b[slot, col:col + self.out_features[s], :rank].copy_(high)
+                tiles = -(-rank // RANK_TILE)
+                self.a[slot, s, :tiles].copy_(pack_a(low))
+                self.b[slot, col:col + self.col_tiles[s], :tiles].copy_(pack_b(high))
                 self.scales[slot, s] = float(scale)
                 self.ranks[slot, s] = rank
-            col += self.out_features[s]
+            col += self.col_tiles[s]
 
     def clear(self, slot: int) -> None:
         """Empty a slot: its rows are left as the base layer made them."""

@@ -796,18 +796,24 @@ void lora(const at::Tensor& x, const at::Tensor& y, at::Tensor out, const at::Te
     check(scales, at::kFloat, "scales");
     check(rows, at::kInt, "rows");
     for (const at::Tensor& v : {y, out, rows, a, b, ranks, scales}) on_device(v, x, "lora");
-    TORCH_CHECK(a.dim() == 4 && a.size(1) == S && a.size(3) == K, "a: [slots, matrices, R, K]");
-    const int64_t slots = a.size(0), R = a.size(2);
-    int64_t N = 0;
-    for (const int64_t n : n_cols) N += n;
-    TORCH_CHECK(b.dim() == 3 && b.size(0) == slots && b.size(1) == N && b.size(2) == R, "b: [slots, N, R]");
+    // the layouts of include/espalier.h
+    TORCH_CHECK(a.dim() == 7 && a.size(1) == S && a.size(3) == (K + 31) / 32 && a.size(4) == 4 && a.size(5) == 16 &&
+                    a.size(6) == 8, "a: [slots, matrices, R / 16, ceil(K / 32), 4, 16, 8]");
+    const int64_t slots = a.size(0), R = a.size(2) * 16;
+    int64_t N = 0, tiles = 0;
+    for (const int64_t n : n_cols) {
+        N += n;
+        tiles += (n + 127) / 128;
+    }
+    TORCH_CHECK(b.dim() == 7 && b.size(0) == slots && b.size(1) == tiles && b.size(2) * 16 == R && b.size(3) == 8 &&
+                    b.size(4) == 2 && b.size(5) == 16 && b.size(6) == 8, "b: [slots, column tiles, R / 16, 8, 2, 16, 8]");
     TORCH_CHECK(ranks.numel() == slots * S && scales.numel() == slots * S, "ranks / scales: [slots, matrices]");
     TORCH_CHECK(rows.numel() == T, "rows: [T]");
     for (const at::Tensor& v : {y, out})
         TORCH_CHECK(v.scalar_type() == t && v.dim() == 2 && v.size(0) == T && v.size(1) >= N && v.stride(1) == 1,
                     "y / out: [T, at least N columns], x's dtype, unit column stride");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-    const int64_t numel = esp_lora_scratch(T, K, S, R);
+    const int64_t numel = esp_lora_scratch(T, N, S, R);
     const at::Tensor scratch = at::empty({numel}, x.options().dtype(at::kFloat));
     call(esp_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), cptr<int32_t>(rows), T,
                   K, S, n_cols.data(), a.data_ptr(), b.data_ptr(), cptr<int32_t>(ranks), cptr<float>(scales), slots, R,
@@ -848,7 +854,7 @@ void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor&
                     "probs: fp32 [B, G, V], unit column stride");
     }
     c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
-    const int64_t bytes = esp_verify_scratch(B, G, V, dtype_code(logits));
+    const int64_t bytes = esp_verify_scratch(B, G, V);
     const at::Tensor scratch = at::empty({bytes}, logits.options().dtype(at::kByte));
     call(esp_verify(logits.data_ptr(), dtype_code(logits), logits.stride(0), logits.size(0), V, cptr<int32_t>(first),
                     cptr<int32_t>(n_drafts), cptr<int32_t>(drafts), B, G, cptr<float>(uniform), cptr<float>(race),

@@ -2,27 +2,34 @@
 //   out[m, n] = y[m, n] + sum_{j < r} t[m, j] B[a][n][j],   t[m, j] = scale[a][s] * sum_k x[m, k] A[a][s][j][k]
 // for row m of adapter a = rows[m] and column n of the layer's matrix s (r = ranks[a][s]); rows of no adapter keep y.
 //
-// Two launches: the rows' products with A (fp32, in K splits), then those with B and the sum. Both take tiles of 16
-// consecutive rows and, inside a tile, one adapter after the other (the tile's distinct ones, found by a few lane
-// exchanges): a matrix instruction's columns are the rows, so each row keeps the column that its own adapter made and no
-// sorting or grouping launch is needed, whatever the order of the rows. Where a batch is small its distinct adapters are
-// spread over workgroups.
+// Two launches: the rows' products with A, then those with B and the sum. Both take tiles of 16 consecutive rows and, inside a
+// tile, one adapter after the other (the tile's distinct ones, found by ballots): the rows are one side of a matrix instruction,
+// so each row keeps what its own adapter made of it and no sorting or grouping launch is needed, whatever the order of the rows.
+// Where a batch is small its distinct adapters are spread over workgroups.
 //
-// t keeps 32 bits between the launches and enters the second product as a 16-bit high part and the 16-bit rest, side by
-// side in one instruction's k (16 ranks of each), so nothing of it is lost but the rest's own rounding (2^-17 for bf16). fp16's narrow
-// range is kept out of it: a row of t is first scaled by a power of two to below 2.
+// The adapters are laid out as the instructions read them (LoraArgs): a wave's load is one KiB in a row. The quarter of a wave
+// that a CU looks up at once then meets two lines; 16 rows of a plain matrix are 16 lines, and came in at 10 bytes a clock.
+//
+// t is summed in fp32 and enters the second product as a 16-bit high part and the 16-bit rest, side by side in one instruction's
+// k (16 ranks of each), so nothing of it is lost but the rest's own rounding (2^-17 for bf16). fp16's narrow range is kept out of
+// it: 16 ranks of a row are first scaled by a power of two to below 1, and their products scaled back.
+//
+// The order of t's sum is fixed: K in 16 runs of whole 32-k units, a run in its units' order, the runs four by four and the four
+// fours in order; so a row's bits depend on that row and its adapter alone.
 #include "../../../include/espalier.h"
 #include "common.hpp"
 #include "norm.hpp"
+
+#include <algorithm>
 
 namespace esp {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int LORA_ROWS = 16;                  // rows a tile
-constexpr int LORA_CHUNK = 512;               // k a partial sum of t: t is the chunks' sums added in order
+constexpr int LORA_RUNS = 16;                  // runs of k that t is summed in
 constexpr int LORA_MAX_SHARDS = 4;
 constexpr int LORA_MAX_RANK = 256;
+constexpr int LORA_COLS = 128;                 // columns a wave of the second product
 
 struct LoraArgs {
     const uint16_t* x;
@@ -33,14 +40,19 @@ struct LoraArgs {
     int64_t out_stride;
     const int32_t *rows, *ranks;
     const float* scales;
-    const uint16_t *a, *b;
-    float* t;                                  // [SK][T][S * R]
-    int T, K, S, N, R, slots, SK, spread;      // spread: workgroups that share a row tile's adapters
-    int n_cols[LORA_MAX_SHARDS], tiles0[LORA_MAX_SHARDS + 1];   // a matrix's columns, and its first 64-column tile
+    const uint4* a;                            // [slots][S][R / 16][units][64]: lane l of a unit rank l % 16, k 8 (l / 16) .. + 8
+    const uint4* b;                            // [slots][col_tiles][R / 16][8][32]: lane l of instruction c column 8 (l % 16) + c,
+                                               // ranks 8 (l / 16) .. + 8
+    float* part;                               // few rows: [4][row tiles][S * R / 16][16 rows][16 ranks], t's sums of four runs
+    uint4* t;                                  // many: [row tiles][S * R / 16][64], finished: lane l row l % 16, ranks 8 (l / 16
+                                               // % 2) .. + 8, the high parts (l < 32) or the rests
+    int* e;                                    // [row tiles][S * R / 16][16]: fp16's exponents
+    int T, K, S, N, R, slots, spread;          // spread: workgroups that share a row tile's adapters (few rows)
+    int n_cols[LORA_MAX_SHARDS], tiles0[LORA_MAX_SHARDS + 1];   // a matrix's columns, and its first tile of LORA_COLS
 };
 
-// D += P Q^T over 32 k, P's 16 rows and Q's 16 rows 8 k a lane: lane l holds row l & 15, k of its group l >> 4; it gets
-// D[4 * (l >> 4) + i][l & 15]
+// D += P Q^T over 32 k, P's 16 rows and Q's 16 rows 8 k a lane: lane l holds row l % 16, k of its group l / 16; it gets
+// D[4 * (l / 16) + i][l % 16]
 template <int DT>
 __device__ __forceinline__ f32x4 mfma32(uint4 p, uint4 q, f32x4 acc) {
     if constexpr (DT == BF16)
@@ -51,222 +63,504 @@ __device__ __forceinline__ f32x4 mfma32(uint4 p, uint4 q, f32x4 acc) {
                                                       0);
 }
 
-// 8 elements at an 8-byte aligned address (16 with wide)
-__device__ __forceinline__ uint4 load8(const uint16_t* p, bool wide) {
-    if (wide) return *reinterpret_cast<const uint4*>(p);
-    const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 4);
-    return make_uint4(a.x, a.y, b.x, b.y);
+// 8 elements at an 8-byte aligned address: one 16-byte access, which the hardware asks no more of
+typedef uint32_t u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
+__device__ __forceinline__ uint4 load8(const uint16_t* p) {
+    const u32x4_a8 v = *reinterpret_cast<const u32x4_a8*>(p);
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void store8(uint16_t* p, uint4 v) {
+    *reinterpret_cast<u32x4_a8*>(p) = u32x4_a8{v.x, v.y, v.z, v.w};
 }
 
-__device__ __forceinline__ bool wide_rows(const void* p, int64_t stride) {
-    return (uintptr_t)p % 16 == 0 && stride % 8 == 0;
+// a value that every lane of the wave reads, through the scalar cache (nothing writes it while the kernel runs)
+template <typename T>
+__device__ __forceinline__ T load_uniform(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
 }
 
-// The adapter of row row0 + (lane & 15), -1 for none or no such row; leaders: the lanes (0 to 15) that are the first of
-// their adapter in the tile
-__device__ __forceinline__ int tile_adapter(const LoraArgs& a, int row0, uint32_t& leaders) {
-    const int lane = threadIdx.x & 63, m = lane & 15;
-    int id = -1;
-    if (row0 + m < a.T) {
-        id = a.rows[row0 + m];
-        if (id < 0 || id >= a.slots) id = -1;
+// The distinct adapters of a tile of 16 * MG rows (a lane each), one after the other: next() gives an adapter and the mask of
+// its rows, those of `rest` that are left; an id outside [0, slots) is none
+template <int MG>
+struct TileAdapters {
+    int id;
+    uint64_t rest;
+    __device__ __forceinline__ TileAdapters(const LoraArgs& a, int row0) {
+        const int lane = threadIdx.x & 63;
+        id = -1;
+        if (lane < 16 * MG && row0 + lane < a.T) id = a.rows[row0 + lane];
+        if (id >= a.slots) id = -1;
+        rest = __ballot(id >= 0);
     }
-    bool first = id >= 0;
+    __device__ __forceinline__ int next(uint64_t& mask) {
+        const int who = __builtin_amdgcn_readlane(id, __builtin_ctzll(rest));
+        mask = __ballot(id == who) & rest;
+        rest &= ~mask;
+        return who;
+    }
+};
+
+__device__ __forceinline__ int lora_rank(const LoraArgs& a, int who, int s) {
+    return min(load_uniform(a.ranks + (int64_t)who * a.S + s), a.R);
+}
+
+// 4 floats as their 16-bit high parts (hi) and what those leave (lo)
+template <int DT>
+__device__ __forceinline__ void split4(const f32x4& v, uint2& hi, uint2& lo) {
+    uint16_t h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 15; ++k) {
-        const int o = __builtin_amdgcn_readlane(id, k);
-        if (k < m && o == id) first = false;
+    for (int i = 0; i < 4; ++i) {
+        h[i] = to16(v[i], DT == BF16);
+        const float rest = v[i] - from16(h[i], DT == BF16);
+        l[i] = to16(fabsf(rest) < INFINITY ? rest : 0.f, DT == BF16);    // an infinity's or NaN's rest is nothing
     }
-    leaders = (uint32_t)__ballot(first && lane < 16);
-    return id;
+    hi = make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
+    lo = make_uint2((uint32_t)l[0] | ((uint32_t)l[1] << 16), (uint32_t)l[2] | ((uint32_t)l[3] << 16));
 }
 
-// t of a row tile, 16 ranks (blockIdx.y: matrix and rank tile) and one chunk of 512 k (blockIdx.z): a wave 128 k of it, the
-// four waves' sums added in order
+// Row tile of workgroup `block` of n: workgroups go to the eight XCDs in turn, and each XCD takes a run of consecutive tiles, so
+// that the adapters of few requests pass through its L2
+__device__ __forceinline__ int xcd_tile(int block, int n) {
+    const int per = n / 8, more = n % 8, xcd = block % 8;
+    return xcd * per + min(xcd, more) + block / 8;
+}
+
+// The power of two to scale 16 ranks of a row by whose largest magnitude is top
+__device__ __forceinline__ int lora_exponent(float top) {
+    return top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The first product, few rows: the sums of runs 4 z .. 4 z + 3 for 16 rows and LORA_FEW tiles of 16 ranks, a wave a run, in fp32.
+// blockIdx.x the row tile and, spread, its adapters; blockIdx.y the matrix and rank tiles, blockIdx.z the runs: a batch's adapters
+// are read once and come in through many CUs.
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int LORA_FEW = 2;                    // rank tiles whose loads are all in flight at once
+
 template <int DT>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
-    __shared__ f32x4 part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-    const int row0 = (int)(blockIdx.x / a.spread) * LORA_ROWS, d = blockIdx.x % a.spread;
-    const int s = blockIdx.y / (a.R / 16), j0 = (int)(blockIdx.y % (a.R / 16)) * 16;
-    uint32_t leaders;
-    const int id = tile_adapter(a, row0, leaders);
-    const bool wide = wide_rows(a.x, a.x_stride);
-    const uint16_t* xr = a.x + (int64_t)min(row0 + m, a.T - 1) * a.x_stride + 16 * g;
-    const int k0 = (int)blockIdx.z * LORA_CHUNK + wave * (LORA_CHUNK / 4);
-    for (int nth = 0; leaders; ++nth) {
-        const int who = __builtin_amdgcn_readlane(id, __builtin_ctz(leaders));
-        leaders &= leaders - 1;
-        if (nth % a.spread != d || j0 >= a.ranks[who * a.S + s]) continue;
-        const uint16_t* ar = a.a + (((size_t)who * a.S + s) * a.R + j0 + m) * a.K + 16 * g;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = 0; st < LORA_CHUNK / 4 / 64; ++st) {
-            const int k = k0 + 64 * st;
-            uint4 p[2], q[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) p[h] = q[h] = make_uint4(0u, 0u, 0u, 0u);
-            if (k + 16 * g < a.K) {                          // K is a multiple of 16: a lane's 16 k are in or out
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    p[h] = *reinterpret_cast<const uint4*>(ar + k + 8 * h);
-                    q[h] = load8(xr + k + 8 * h, wide);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) acc = mfma32<DT>(p[h], q[h], acc);
-        }
-        part[wave][lane] = acc;
-        __syncthreads();
-        if (wave == 0 && id == who) {
-            const f32x4 sum = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
-            *reinterpret_cast<f32x4*>(a.t + (((size_t)blockIdx.z * a.T + row0 + m) * a.S + s) * a.R + j0 + 4 * g) = sum;
-        }
-        __syncthreads();                                     // part is written again
-    }
-}
-
-__device__ __forceinline__ f32x4 lora_t4(const LoraArgs& a, const float* t, float scale) {
-    f32x4 v = *reinterpret_cast<const f32x4*>(t);
-    for (int z = 1; z < a.SK; ++z) v += *reinterpret_cast<const f32x4*>(t + (size_t)z * a.T * a.S * a.R);
-    return v * scale;
-}
-
-// 8 floats as the 16-bit high parts (low: what they leave)
-template <int DT>
-__device__ __forceinline__ uint4 split8(const float (&v)[8], bool low) {
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        uint16_t h[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float f = v[2 * k + e];
-            h[e] = to16(f, DT == BF16);
-            if (low) {
-                const float hi = from16(h[e], DT == BF16), rest = f - hi;
-                h[e] = to16(rest == rest && fabsf(rest) < INFINITY ? rest : 0.f, DT == BF16);
-            }
-        }
-        w[k] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// 64 columns of one matrix (a wave each) of a row tile: the products of t with B, added to y. Rows of B enter in the order
-// that gives a lane 16 columns in a row of its row of y: instruction q's row 4 c + i is column 16 c + 4 q + i.
-template <int DT>
-__global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs a) {
+    __shared__ f32x4 part[4][LORA_FEW][64];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const int row0 = (int)(blockIdx.x / a.spread) * LORA_ROWS, d = blockIdx.x % a.spread;
-    const int ct = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6);
-    if (ct >= a.tiles0[a.S]) return;
-    int s = 0, c0 = 0;                                       // c0: the matrix's first column in y
-    while (ct >= a.tiles0[s + 1]) c0 += a.n_cols[s++];
-    const int n0 = (ct - a.tiles0[s]) * 64;
-    uint32_t leaders;
-    const int id = tile_adapter(a, row0, leaders);
-    const float* tr = a.t + ((size_t)min(row0 + m, a.T - 1) * a.S + s) * a.R + 8 * (g & 1);
-    bool mine = false;
-    f32x4 sum[4];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int tile_at = blockIdx.x / a.spread, d = blockIdx.x % a.spread;
+    const int rt = a.R / 16, of = (rt + LORA_FEW - 1) / LORA_FEW, s = blockIdx.y / of, j0 = blockIdx.y % of * LORA_FEW;
+    const int units = (a.K + 31) / 32, run = (units + LORA_RUNS - 1) / LORA_RUNS;
+    const int u0 = (4 * (int)blockIdx.z + wave) * run, u1 = min(units, u0 + run);
+    TileAdapters<1> tile(a, 16 * tile_at);
+    for (int nth = 0; tile.rest; nth = nth + 1 == a.spread ? 0 : nth + 1) {
+        uint64_t mask;
+        const int who = tile.next(mask);
+        if (nth != d) continue;
+        const int n = (lora_rank(a, who, s) + 15) / 16 - j0;
+        if (n <= 0) continue;
+        const char* ab = reinterpret_cast<const char*>(a.a + (((int64_t)who * a.S + s) * rt + j0) * units * 64);
+        // rows of other adapters read the first of this one's instead: no line comes in for them
+        const bool mine = (mask >> m) & 1;
+        const int mr = mine ? m : __builtin_ctzll(mask);
+        const uint16_t* xp = a.x + (int64_t)(16 * tile_at + mr) * a.x_stride + 8 * g;
+        f32x4 acc[LORA_FEW];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] = {0.f, 0.f, 0.f, 0.f};
-    const int br = n0 + 16 * (m >> 2) + (m & 3);             // this lane's row of B for q = 0
-    const bool b_in = n0 + 16 * (m >> 2) < a.n_cols[s];      // columns are multiples of 16
-    for (int nth = 0; leaders; ++nth) {
-        const int who = __builtin_amdgcn_readlane(id, __builtin_ctz(leaders));
-        leaders &= leaders - 1;
-        if (nth % a.spread != d) continue;
-        const int r = min(a.ranks[who * a.S + s], a.R);
-        const float scale = a.scales[who * a.S + s];
-        int e = 0;
-        if constexpr (DT == F16) {
-            float top = 0.f;
-            for (int js = 0; js < r; js += 16) {
+        for (int j = 0; j < LORA_FEW; ++j) acc[j] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int u = u0; u < u1; u += 4) {
+            uint4 x[4], p[LORA_FEW][4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x4 v = lora_t4(a, tr + js + 4 * h, scale);
+            for (int j = 0; j < LORA_FEW; ++j)               // units past the run's: its last one again, tiles past the adapter's:
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (js + 8 * (g & 1) + 4 * h + i < r) top = fmaxf(top, fabsf(v[i]));
-                }
+                for (int i = 0; i < 4; ++i)                  // its last one; not used
+                    p[j][i] = *reinterpret_cast<const uint4*>(ab + ((int64_t)min(j, n - 1) * units + min(u + i, u1 - 1)) * 1024 +
+                                                              lane * 16u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = 32 * min(u + i, u1 - 1);
+                x[i] = load8(xp + min(k, a.K - 8 - 8 * g));
+                if (k + 8 * g >= a.K) x[i] = make_uint4(0u, 0u, 0u, 0u);
             }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            if (top > 0.f && top < INFINITY) e = __builtin_amdgcn_frexp_expf(top);
+            __builtin_amdgcn_sched_barrier(0);               // every load before the first use
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (u + i < u1)
+#pragma unroll
+                    for (int j = 0; j < LORA_FEW; ++j) acc[j] = mfma32<DT>(p[j][i], x[i], acc[j]);
         }
-        f32x4 acc[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q] = {0.f, 0.f, 0.f, 0.f};
-        const uint16_t* bp = a.b + ((size_t)who * a.N + c0 + br) * a.R + 8 * (g & 1);
-        for (int js = 0; js < r; js += 16) {
-            const int left = r - js - 8 * (g & 1);           // ranks of this lane's 8 that the adapter has
-            float v[8];
+        for (int j = 0; j < LORA_FEW; ++j) part[wave][j][lane] = acc[j];
+        __syncthreads();
+        if (wave < min(n, LORA_FEW) && mine)
+            *reinterpret_cast<f32x4*>(a.part + (((((int64_t)blockIdx.z * ((a.T + 15) / 16) + tile_at) * a.S + s) * rt + j0 + wave) *
+                                                    16 + m) * 16 + 4 * g) =
+                ((part[0][wave][lane] + part[1][wave][lane]) + part[2][wave][lane]) + part[3][wave][lane];
+        if (tile.rest) __syncthreads();                      // part is written again
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The first product, many rows: 16 rows against all of an adapter's ranks, LORA_BATCH tiles of 16 at a time; sixteen waves, a run
+// of the k each. t leaves finished and split. x comes in once a CU, 256 bytes of a row at a time, and turns into operands through
+// the wave's own 4 KiB of shared memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a
+// quarter-wave meet in a bank either way). The next tiles' A is in flight while a batch is multiplied and summed over the waves.
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int LORA_BATCH = 2;
+constexpr int LORA_ALL_SMEM = LORA_RUNS * (4096 + 2 * LORA_BATCH * 1024);
+
+template <int DT>
+__global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a) {
+    extern __shared__ uint4 xs[];                            // [LORA_RUNS][256], then the sums of two rounds
+    typedef f32x4 Sums[LORA_RUNS][LORA_BATCH][64];
+    Sums* part = reinterpret_cast<Sums*>(xs + LORA_RUNS * 256);
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 16, rt = a.R / 16;   // blockIdx.y: every other adapter
+    const int units = (a.K + 31) / 32, run = (units + LORA_RUNS - 1) / LORA_RUNS, chunks = (run + 3) / 4;
+    const int u0 = wave * run, u1 = min(units, u0 + run);
+    const uint32_t lane16 = lane * 16u;
+    const char* xb = reinterpret_cast<const char*>(a.x + row0 * a.x_stride);
+    uint32_t xrow[4];                                        // bytes to rows g, 4 + g, 8 + g, 12 + g
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const f32x4 t4 = lora_t4(a, tr + js + 4 * h, scale);
+    for (int i = 0; i < 4; ++i) xrow[i] = (uint32_t)(min(4 * i + g, a.T - 1 - row0) * (int)a.x_stride) * 2u;
+    uint4* own = xs + 256 * wave;
+    TileAdapters<1> tile(a, row0);
+    int round = 0;
+    for (int nth = 0; tile.rest; ++nth) {
+        uint64_t mask;
+        const int who = tile.next(mask);
+        if ((nth & 1) != (int)blockIdx.y) continue;
+        int end[LORA_MAX_SHARDS], total = 0;                 // the matrices' rank tiles, one after the other
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * h + i] = 4 * h + i < left ? (DT == F16 ? ldexpf(t4[i], -e) : t4[i]) : 0.f;
+        for (int s = 0; s < LORA_MAX_SHARDS; ++s) {
+            if (s < a.S) total += (max(lora_rank(a, who, s), 0) + 15) / 16;
+            end[s] = total;
+        }
+        if (total == 0) continue;
+        // the place among the layer's S * R / 16 of the adapter's tile i (past the last one: that one)
+        const auto place = [&](int i) __attribute__((always_inline)) {
+            i = min(i, total - 1);
+            int s = 0, first = 0;
+#pragma unroll
+            for (int k = 0; k < LORA_MAX_SHARDS - 1; ++k)
+                if (i >= end[k]) {
+                    s = k + 1;
+                    first = end[k];
+                }
+            return s * rt + i - first;
+        };
+        const char* ab = reinterpret_cast<const char*>(a.a + (int64_t)who * a.S * rt * units * 64);
+        const auto load_a = [&](int i0, int c, uint4(&p)[LORA_BATCH][4]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < LORA_BATCH; ++j) {
+                const char* ap = ab + (int64_t)place(i0 + j) * units * 1024;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    p[j][i] = *reinterpret_cast<const uint4*>(ap + (int64_t)min(u0 + 4 * c + i, u1 - 1) * 1024 + lane16);
             }
-            const uint4 tq = split8<DT>(v, g >= 2);
+        };
+        uint4 x[4], p[LORA_BATCH][4];
+        load_a(0, 0, p);
+#pragma unroll 1
+        for (int i0 = 0; i0 < total; i0 += LORA_BATCH) {
+            f32x4 acc[LORA_BATCH];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint4 bq = make_uint4(0u, 0u, 0u, 0u);
-                if (b_in) bq = *reinterpret_cast<const uint4*>(bp + (size_t)4 * q * a.R + js);
-                if (left < 8) {                              // what lies past the rank is not used, whatever it holds
-                    uint32_t w[4] = {bq.x, bq.y, bq.z, bq.w};
+            for (int j = 0; j < LORA_BATCH; ++j) acc[j] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                const int u = u0 + 4 * c;
+                const bool fresh = chunks > 1 || i0 == 0;    // a single chunk's operands stay in registers
+                if (fresh)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (2 * i >= left) w[i] = 0u;
-                        else if (2 * i + 1 >= left) w[i] &= 0xFFFFu;
+                    for (int i = 0; i < 4; ++i) {            // row 4 i + g, k 32 u + 8 m .. + 8
+                        const int k = 32 * u + 8 * m;        // (of a row that is not the adapter's too: its t is not kept)
+                        x[i] = load8(reinterpret_cast<const uint16_t*>(xb + (xrow[i] + (uint32_t)min(k, a.K - 8) * 2u)));
+                        if (k >= a.K) x[i] = make_uint4(0u, 0u, 0u, 0u);
                     }
-                    bq = make_uint4(w[0], w[1], w[2], w[3]);
+                const bool more = c + 1 < chunks;
+                uint4 next[LORA_BATCH][4];
+                load_a(more ? i0 : i0 + LORA_BATCH, more ? c + 1 : 0, next);
+                __builtin_amdgcn_sched_barrier(0);           // every load before the first use
+                if (fresh) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) own[(4 * i + g) * 16 + (m ^ (4 * i + g))] = x[i];
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = own[m * 16 + ((4 * i + g) ^ m)];
+                    __builtin_amdgcn_wave_barrier();
                 }
-                acc[q] = mfma32<DT>(bq, tq, acc[q]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (u + i < u1)
+#pragma unroll
+                        for (int j = 0; j < LORA_BATCH; ++j) acc[j] = mfma32<DT>(p[j][i], x[i], acc[j]);
+#pragma unroll
+                for (int j = 0; j < LORA_BATCH; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[j][i] = next[j][i];
             }
-        }
-        if (id == who) {
-            mine = true;
+            const int n = min(total - i0, LORA_BATCH), j = (wave - LORA_BATCH * round) & (LORA_RUNS - 1);
+            Sums& sums = part[round++ & 1];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int k = 0; k < LORA_BATCH; ++k) sums[wave][k][lane] = acc[k];
+            lds_barrier();                                   // (the next tiles' loads stay in flight; the sums before the last
+                                                             // ones are read: the waves that do came to this barrier after it)
+            if (j < n) {                                     // a wave a tile, other waves for the next ones
+                const int to = place(i0 + j), s = to / rt, left = lora_rank(a, who, s) - 16 * (to % rt) - 4 * g;
+                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[q][i] = DT == F16 ? ldexpf(acc[q][i], e) : acc[q][i];
+                for (int z = 0; z < LORA_RUNS; z += 4)
+                    sum += ((sums[z][j][lane] + sums[z + 1][j][lane]) + sums[z + 2][j][lane]) + sums[z + 3][j][lane];
+                sum *= load_uniform(a.scales + (int64_t)who * a.S + s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i >= left) sum[i] = 0.f;             // ranks that the adapter does not have
+                const int64_t tile_to = (int64_t)tile_at * a.S * rt + to;
+                if constexpr (DT == F16) {
+                    float top = fmaxf(fmaxf(fabsf(sum[0]), fabsf(sum[1])), fmaxf(fabsf(sum[2]), fabsf(sum[3])));
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const int e = lora_exponent(top);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = ldexpf(sum[i], -e);
+                    if (g == 0 && ((mask >> m) & 1)) a.e[tile_to * 16 + m] = e;
+                }
+                if ((mask >> m) & 1) {                       // ranks 4 g .. + 4 of row m
+                    uint2 hi, lo;
+                    split4<DT>(sum, hi, lo);
+                    uint2* t = reinterpret_cast<uint2*>(a.t + tile_to * 64) + 2 * (16 * (g >> 1) + m) + (g & 1);
+                    t[0] = hi;
+                    t[64] = lo;
+                }
+            }
         }
     }
-    const int row = row0 + m, n = n0 + 16 * g;
-    if (id < 0) mine = d == 0 && a.out != a.y;               // no adapter: y as it is
-    if (!mine || row >= a.T || n >= a.n_cols[s]) return;
-    const uint16_t* yp = a.y + (int64_t)row * a.y_stride + c0 + n;
-    uint16_t* op = a.out + (int64_t)row * a.out_stride + c0 + n;
-    const bool wide_y = wide_rows(a.y, a.y_stride), wide_o = wide_rows(a.out, a.out_stride);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The second product
+// ------------------------------------------------------------------------------------------------------------------
+// 8 columns of a row: y's, with what the adapter adds
+template <int DT>
+__device__ __forceinline__ uint4 lora_add8(uint4 y, const float (&add)[8]) {
+    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = from16((uint16_t)(w[i >> 1] >> (16 * (i & 1))), DT == BF16) + add[i];
+    return pack8_16(v, DT == BF16);
+}
+
+// One rank tile's products: instruction c's are column 8 (lane % 16) + c of rows 4 (lane / 16) .. + 4
+template <int DT>
+__device__ __forceinline__ void lora_rank_tile(const uint4& t, const int (&e)[4], const uint4 (&b)[8], f32x4 (&acc)[8]) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        if constexpr (DT == F16) {
+            const f32x4 v = mfma32<DT>(t, b[c], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][i] += ldexpf(v[i], e[i]);
+        } else {
+            acc[c] = mfma32<DT>(t, b[c], acc[c]);
+        }
+    }
+}
+
+// The matrix that column tile ct lies in: its number, first column of y, and the tile's columns
+struct LoraCols {
+    int s, c0, cols;
+    __device__ __forceinline__ LoraCols(const LoraArgs& a, int ct) : s(0), c0(0) {
+        while (ct >= a.tiles0[s + 1]) c0 += a.n_cols[s++];
+        const int n0 = (ct - a.tiles0[s]) * LORA_COLS;
+        c0 += n0;
+        cols = min(a.n_cols[s] - n0, LORA_COLS);
+    }
+};
+
+// This lane's operand of a rank tile of t from lora_shrink_kernel's four sums (of row `at` of the layer's row tiles): 8 ranks of
+// 16, the high parts (lanes below 32) or the rests; e: fp16's exponents of rows 4 (lane / 16) .. + 4
+template <int DT>
+__device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[4][2], float scale, int left, int (&e)[4]) {
+    const int lane = threadIdx.x & 63;
+    f32x4 v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint4 u = load8(yp + 8 * h, wide_y);
-        if (id >= 0) {
-            float v[8];
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        v[h] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint16_t bits = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-                v[i] = from16(bits, DT == BF16) + sum[2 * h + (i >> 2)][i & 3];
-            }
-            u = pack8_16(v, DT == BF16);
+        for (int z = 0; z < 4; ++z) v[h] += p[z][h];
+        v[h] *= scale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * h + i >= left) v[h][i] = 0.f;
+    }
+    if constexpr (DT == F16) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(v[0][i]), fabsf(v[1][i])));
+        const int mine = lora_exponent(fmaxf(top, __shfl_xor(top, 16)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[h][i] = ldexpf(v[h][i], -mine);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = __shfl(mine, 4 * (lane >> 4) + i);
+    }
+    uint2 hi[2], lo[2];
+    split4<DT>(v[0], hi[0], lo[0]);
+    split4<DT>(v[1], hi[1], lo[1]);
+    return lane >= 32 ? make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y) : make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+}
+
+// Few rows: a wave 128 columns of a row tile (and, spread, its adapters)
+template <int DT>
+__global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
+    const int lane = threadIdx.x, m = lane & 15, g = lane >> 4, rt = a.R / 16, ct = blockIdx.y;
+    const int tile_at = blockIdx.x / a.spread, d = blockIdx.x % a.spread;
+    const LoraCols col(a, ct);
+    const bool in = 8 * m < col.cols;
+    const int64_t row0 = 16 * tile_at + 4 * g, z_at = (int64_t)((a.T + 15) / 16) * a.S * rt * 256;
+    const uint16_t* yp = a.y + row0 * a.y_stride + col.c0 + 8 * m;
+    uint16_t* op = a.out + row0 * a.out_stride + col.c0 + 8 * m;
+    TileAdapters<1> tile(a, 16 * tile_at);
+    if (d == 0 && a.out != a.y) {                            // rows of no adapter: y as it is
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (in && !((tile.rest >> (4 * g + i)) & 1) && row0 + i < a.T) store8(op + i * a.out_stride, load8(yp + i * a.y_stride));
+    }
+    for (int nth = 0; tile.rest; nth = nth + 1 == a.spread ? 0 : nth + 1) {
+        uint64_t mask;
+        const int who = tile.next(mask);
+        if (nth != d) continue;
+        const int r = lora_rank(a, who, col.s);
+        const float scale = load_uniform(a.scales + (int64_t)who * a.S + col.s);
+        const int mr = (mask >> m) & 1 ? m : __builtin_ctzll(mask);
+        const uint32_t own = (uint32_t)mask >> (4 * g);      // this lane's rows 4 g .. + 4
+        const uint4* bp = a.b + ((int64_t)who * a.tiles0[a.S] + ct) * rt * 256 + (lane & 31);
+        const float* pp = a.part + (((int64_t)tile_at * a.S + col.s) * rt * 16 + mr) * 16 + 8 * (g & 1);
+        uint4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (in && ((own >> i) & 1)) y[i] = load8(yp + i * a.y_stride);
+        f32x4 acc[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int j0 = 0; 16 * j0 < r; j0 += LORA_FEW) {
+            f32x4 p[LORA_FEW][4][2];
+            uint4 b[LORA_FEW][8];
+#pragma unroll
+            for (int j = 0; j < LORA_FEW; ++j)
+                if (16 * (j0 + j) < r) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) b[j][c] = bp[(j0 + j) * 256 + 32 * c];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            p[j][z][h] = *reinterpret_cast<const f32x4*>(pp + z * z_at + (j0 + j) * 256 + 4 * h);
+                }
+#pragma unroll
+            for (int j = 0; j < LORA_FEW; ++j)
+                if (16 * (j0 + j) < r) {
+                    int e[4];
+                    const uint4 t = lora_t8<DT>(p[j], scale, r - 16 * (j0 + j) - 8 * (g & 1), e);
+                    lora_rank_tile<DT>(t, e, b[j], acc);
+                }
         }
-        if (wide_o) {
-            *reinterpret_cast<uint4*>(op + 8 * h) = u;
-        } else {
-            *reinterpret_cast<uint2*>(op + 8 * h) = make_uint2(u.x, u.y);
-            *reinterpret_cast<uint2*>(op + 8 * h + 4) = make_uint2(u.z, u.w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (in && ((own >> i) & 1)) {
+                const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
+                store8(op + i * a.out_stride, lora_add8<DT>(y[i], add));
+            }
+    }
+}
+
+constexpr int LORA_HELD = 4;                   // rank tiles of B in shared memory at once
+
+// Many rows: a workgroup of 64 rows (16 a wave) and 128 columns, an adapter's B for them in shared memory
+template <int DT>
+__global__ __launch_bounds__(256) void lora_expand_all_kernel(const LoraArgs a) {
+    __shared__ uint4 bs[LORA_HELD][256];
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 64, rt = a.R / 16;
+    const LoraCols col(a, blockIdx.y);
+    const uint16_t* yp = a.y + (int64_t)(row0 + 16 * wave) * a.y_stride + col.c0 + 8 * m;
+    uint16_t* op = a.out + (int64_t)(row0 + 16 * wave) * a.out_stride + col.c0 + 8 * m;
+    const bool in = 8 * m < col.cols;
+    uint4 y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (in && row0 + 16 * wave + 4 * g + i < a.T) y[i] = load8(yp + (4 * g + i) * a.y_stride);
+    }
+    TileAdapters<4> tile(a, row0);
+    const uint64_t some = tile.rest;
+    while (tile.rest) {
+        uint64_t mask;
+        const int who = tile.next(mask);
+        const int r = lora_rank(a, who, col.s), nt = (r + 15) / 16;
+        const uint4* bp = a.b + ((int64_t)who * a.tiles0[a.S] + blockIdx.y) * rt * 256 + threadIdx.x;
+        const uint32_t rows = (uint32_t)(mask >> (16 * wave)) & 0xFFFFu;
+        const int64_t at = ((int64_t)min(tile_at * 4 + wave, (a.T - 1) / 16) * a.S + col.s) * rt;
+        f32x4 acc[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int j0 = 0; j0 < nt; j0 += LORA_HELD) {
+            uint4 b[LORA_HELD], t[LORA_HELD];
+            int4 e[LORA_HELD];
+#pragma unroll
+            for (int j = 0; j < LORA_HELD; ++j) {            // past the last one: that one again
+                const int jt = min(j0 + j, nt - 1);
+                b[j] = bp[jt * 256];
+                t[j] = a.t[(at + jt) * 64 + lane];
+                if (DT == F16) e[j] = *reinterpret_cast<const int4*>(a.e + (at + jt) * 16 + 4 * g);
+            }
+#pragma unroll
+            for (int j = 0; j < LORA_HELD; ++j) bs[j][threadIdx.x] = b[j];
+            __syncthreads();
+            if (rows) {
+#pragma unroll
+                for (int j = 0; j < LORA_HELD; ++j)
+                    if (j0 + j < nt) {
+                        uint4 bc[8];
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) bc[c] = bs[j][32 * c + (lane & 31)];
+                        int ej[4] = {0, 0, 0, 0};
+                        if constexpr (DT == F16) {
+                            ej[0] = e[j].x; ej[1] = e[j].y; ej[2] = e[j].z; ej[3] = e[j].w;
+                        }
+                        lora_rank_tile<DT>(t[j], ej, bc, acc);
+                    }
+            }
+            __syncthreads();                                 // bs is written again
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (in && ((rows >> (4 * g + i)) & 1)) {
+                const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
+                store8(op + (4 * g + i) * a.out_stride, lora_add8<DT>(y[i], add));
+            }
+    }
+    if (a.out != a.y) {                                      // rows of no adapter: y as it is
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * wave + 4 * g + i;
+            if (in && !((some >> row) & 1) && row0 + row < a.T) store8(op + (4 * g + i) * a.out_stride, y[i]);
         }
     }
 }
 
-constexpr int LORA_SPREAD_ROWS = 256;          // up to this many rows a tile's adapters run in workgroups of their own
-
 template <int DT>
-int lora_launch(const LoraArgs& a, hipStream_t st) {
-    const unsigned tiles = (unsigned)((a.T + LORA_ROWS - 1) / LORA_ROWS) * a.spread;
-    lora_shrink_kernel<DT><<<dim3(tiles, (unsigned)(a.S * (a.R / 16)), (unsigned)a.SK), 256, 0, st>>>(a);
-    lora_expand_kernel<DT><<<dim3(tiles, (unsigned)((a.tiles0[a.S] + 3) / 4)), 256, 0, st>>>(a);
+int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
+    const unsigned tiles = (unsigned)((a.T + 15) / 16), cols = (unsigned)a.tiles0[a.S];
+    if (all) {
+        if (hipFuncSetAttribute((const void*)lora_shrink_all_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                LORA_ALL_SMEM) != hipSuccess)
+            return esp_host::fail(ESP_ERR_HIP, "lora: no %d bytes of shared memory", LORA_ALL_SMEM);
+        lora_shrink_all_kernel<DT><<<dim3(tiles, 2), 1024, LORA_ALL_SMEM, st>>>(a);
+        lora_expand_all_kernel<DT><<<dim3((tiles + 3) / 4, cols), 256, 0, st>>>(a);
+    } else {
+        const unsigned x = tiles * a.spread, ranks = (unsigned)((a.R / 16 + LORA_FEW - 1) / LORA_FEW);
+        lora_shrink_kernel<DT><<<dim3(x, a.S * ranks, LORA_RUNS / 4), 256, 0, st>>>(a);
+        lora_expand_kernel<DT><<<dim3(x, cols), 64, 0, st>>>(a);
+    }
     return esp_host::launch_check("lora");
 }
 
@@ -277,11 +571,26 @@ int lora_launch(const LoraArgs& a, hipStream_t st) {
 // ======================================================================================================================
 using namespace esp;
 
-static int64_t lora_splits(int64_t K) { return (K + LORA_CHUNK - 1) / LORA_CHUNK; }
+// Whether T rows run as the launches for many rows. They take longer to begin with (a CU goes through all ranks of a tile) and
+// less a row. us for T rows, few / many (bf16, graph replays, three requests one after the other):
+//   2048 -> 4096 + 512 + 512, ranks 16: 11.7 / 12.2 at 512, 11.0 / 11.8 at 768, 20 / 13.8 at 1024, 51 / 33 at 4096
+//   4096 -> 2048, rank 16: 8.5 / 10.9 at 768, 13.8 / 11.7 at 1536, 19.4 / 13.8 at 2048
+//   2048 -> 512 + 512, ranks 32: 8.6 / 10.8 at 768, 10.4 / 10.9 at 1536, 15.8 / 12.4 at 2048
+static bool lora_many(int64_t T, int64_t N) { return T * N >= 3 << 20 || T >= 1536; }
 
-extern "C" int64_t esp_lora_scratch(int64_t T, int64_t K, int64_t n_shards, int64_t R) {
-    if (T <= 0 || K <= 0 || n_shards <= 0 || R <= 0) return 0;
-    return lora_splits(K) * T * n_shards * R;
+// The workgroups that a row tile's adapters are dealt to (few rows): up to one a row, and no more than 32 over all tiles, since
+// one that finds nothing costs 2 ns too (a tile of one adapter leaves the others empty). 2048 -> 4096 + 512 + 512, ranks 16 and 64
+// of 32 adapters in random rows, 16 / 32 / 64 workgroups: 16 / 13 / 13 us for 32 rows, 64 / 45 / 51 for 256; in 3 runs of rows
+// 9.8 / 11.3 / 11.3 and 13.0 / 13.2 / 18.5
+static int lora_spread(int64_t T) {
+    const int64_t tiles = (T + 15) / 16;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({16, T, 32 / tiles}));
+}
+
+extern "C" int64_t esp_lora_scratch(int64_t T, int64_t N, int64_t n_shards, int64_t R) {
+    if (T <= 0 || N <= 0 || n_shards <= 0 || R <= 0) return 0;
+    const int64_t rows = (T + 15) / 16 * 16, ranks = n_shards * ((R + 15) / 16);
+    return lora_many(T, N) ? rows * ranks * 17 : rows * ranks * 16 * (LORA_RUNS / 4);
 }
 
 extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out, int64_t out_stride,
@@ -303,19 +612,24 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
         ESP_REQUIRE(n_cols[s] > 0 && n_cols[s] % 16 == 0 && n_cols[s] <= (1 << 21),
                     "lora: columns must be positive multiples of 16, at most 2^21 a matrix");
         a.n_cols[s] = (int)n_cols[s];
-        a.tiles0[s + 1] = a.tiles0[s] + (int)((n_cols[s] + 63) / 64);
+        a.tiles0[s + 1] = a.tiles0[s] + (int)((n_cols[s] + LORA_COLS - 1) / LORA_COLS);
         N += n_cols[s];
     }
+    ESP_REQUIRE(a.tiles0[n_shards] <= 65535, "lora: at most 65535 blocks of %d columns", LORA_COLS);
     if (T == 0) return esp_host::ok();
     ESP_REQUIRE(x && y && out && rows && A && B && ranks && scales && scratch, "lora: null pointer");
     ESP_REQUIRE(T == 1 || (x_stride >= K && y_stride >= N && out_stride >= N), "lora: rows overlap");
+    ESP_REQUIRE(T == 1 || (x_stride <= (1 << 24) && y_stride <= (1 << 24) && out_stride <= (1 << 24)),
+                "lora: row strides of at most 2^24 elements");
     ESP_REQUIRE(out != y || T == 1 || out_stride == y_stride, "lora: in place, out must have y's row stride");
     ESP_REQUIRE(((uintptr_t)x | (uintptr_t)y | (uintptr_t)out) % 8 == 0 &&
                     (T == 1 || (x_stride % 4 == 0 && y_stride % 4 == 0 && out_stride % 4 == 0)),
                 "lora: x, y and out must be 8-byte aligned with row strides a multiple of 4 elements");
     ESP_REQUIRE(((uintptr_t)A | (uintptr_t)B | (uintptr_t)scratch) % 16 == 0,
                 "lora: the adapters and the scratch must be 16-byte aligned");
-    ESP_REQUIRE(scratch_numel >= esp_lora_scratch(T, K, n_shards, R), "lora: the scratch needs esp_lora_scratch floats");
+    ESP_REQUIRE(scratch_numel >= esp_lora_scratch(T, N, n_shards, R), "lora: the scratch needs esp_lora_scratch floats");
+    const bool all = lora_many(T, N);
+    const int64_t tiles = (T + 15) / 16;
     a.x = static_cast<const uint16_t*>(x);
     a.x_stride = x_stride;
     a.y = static_cast<const uint16_t*>(y);
@@ -325,17 +639,18 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
     a.rows = rows;
     a.ranks = ranks;
     a.scales = scales;
-    a.a = static_cast<const uint16_t*>(A);
-    a.b = static_cast<const uint16_t*>(B);
-    a.t = scratch;
+    a.a = static_cast<const uint4*>(A);
+    a.b = static_cast<const uint4*>(B);
+    a.part = scratch;
+    a.t = reinterpret_cast<uint4*>(scratch);
+    a.e = reinterpret_cast<int*>(scratch) + tiles * n_shards * R * 16;
     a.T = (int)T;
     a.K = (int)K;
     a.S = (int)n_shards;
     a.N = (int)N;
     a.R = (int)R;
     a.slots = (int)slots;
-    a.SK = (int)lora_splits(K);
-    a.spread = T > LORA_SPREAD_ROWS ? 1 : (int)(T < LORA_ROWS ? T : LORA_ROWS);
+    a.spread = lora_spread(T);
     const hipStream_t st = (hipStream_t)stream;
-    return dtype == ESP_BF16 ? lora_launch<BF16>(a, st) : lora_launch<F16>(a, st);
+    return dtype == ESP_BF16 ? lora_launch<BF16>(a, all, st) : lora_launch<F16>(a, all, st);
 }

@@ -7,8 +7,11 @@
 // Drawing is a race: argmax of w_v / e_v with e_v exponential random numbers, the lowest index among equal ones. A request
 // whose temperature is below 1e-5 is greedy: a draft is accepted iff it is the row's argmax, which is also the token drawn.
 //
-// Bound by reading the logits: a row is split over many waves, each taking the maximum and the sum of exponentials of its
-// piece from registers, so every logit is read once for the statistics of all rows; the second reading is one row a request.
+// Two launches. The first reads every row once: a wave takes 1024 logits into registers and leaves their maximum and their sum of
+// exponentials (a greedy request's: the place of the maximum too), so no workgroup waits for another and nothing is rescaled. The
+// second runs over the one row of a request that is drawn from: each of its workgroups puts the request's rows together from the
+// waves' pieces and decides the drafts for itself (a few hundred bytes out of the L2 and 64-bit sums, a wave a row, while its
+// random numbers are on the way), then races its 4096 entries; the last of a request's to arrive writes the outcome.
 #include "../../../include/espalier.h"
 #include "common.hpp"
 #include "norm.hpp"
@@ -16,81 +19,87 @@
 namespace esp {
 
 constexpr float GREEDY_BELOW = 1e-5f;
-constexpr int VERIFY_VECS = 2;                 // 16-byte loads of logits a lane, all in flight
+constexpr int PIECE_GROUPS = 2;                // groups of 8 logits a lane of a wave's piece, all in flight
+constexpr int PIECE = 64 * 8 * PIECE_GROUPS;
+constexpr int RACE_GROUPS = 2;                 // groups of 8 entries a thread of a race
+constexpr int RACE = 256 * 8 * RACE_GROUPS;
 
-// one wave's piece of one row: the largest logit (NaN if there is one), the sum of exp((l - m) / temperature), the index of m
+// one wave's piece of one row: the largest logit and the sum of exp((l - m) / temperature), NaN where a logit is NaN or +inf
 struct Piece {
     float m, s;
-    int idx, pad;
-};
-
-// what the race of a request needs, written by the decision
-struct Drawn {
-    int row;              // the logits row, -1: nothing to draw
-    int j;                // the token's place
-    int draft;            // the rejected draft, -1: none was (the row behind the last draft)
-    float m, c_hi, c_lo, rz;
-    double log_z;
 };
 
 struct VerifyArgs {
     const void* logits;
     int64_t stride, R;
-    int V, B, G, pieces;
+    int V, B, G, pieces, races;
     const int32_t *first, *n_drafts, *drafts;
     const float *uniform, *race, *temperature, *probs;
     int64_t race_stride, probs_request, probs_row;
     int32_t *tokens, *counts;
     float* logprobs;
+    unsigned long long* keys;                   // [B][races]
     Piece* part;                                // [B][G + 1][pieces]
-    unsigned long long* keys;                   // [B][pieces][2]
-    Drawn* drawn;                               // [B]
+    int* best;                                  // [B][G + 1][pieces]: the place of m (the first NaN, if any), greedy requests
+    int* arrived;                               // [B][CNT_STRIDE], made zero by the first launch
 };
 
 // unaligned 16-byte loads: rows start at any element (an odd vocabulary)
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// elements i .. i + 8 of a row of V, `past` past its end
 template <int DT>
-struct Elems {
-    static constexpr int VEC = DT == F32 ? 4 : 8;
-    static __device__ __forceinline__ float at(const void* row, int i) { return load_elem(row, DT, (size_t)i); }
-    // elements i .. i + VEC of a row of V, -inf past its end
-    static __device__ __forceinline__ void load(const void* row, int i, int V, float (&v)[VEC]) {
-        if (i + VEC <= V) {
-            if constexpr (DT == F32) {
-                const f32x4_a4 u = *reinterpret_cast<const f32x4_a4*>(static_cast<const float*>(row) + i);
-                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-            } else {
-                const u32x4_a2 u = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(row) + i);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void load_group(const void* row, int i, int V, float past, float (&v)[8]) {
+    if (i + 8 <= V) {
+        if constexpr (DT == F32) {
+            const f32x4_a4* p = reinterpret_cast<const f32x4_a4*>(static_cast<const float*>(row) + i);
+            const f32x4_a4 a = p[0], b = p[1];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[2 * k] = from16((uint16_t)(w[k] & 0xFFFFu), DT == BF16);
-                    v[2 * k + 1] = from16((uint16_t)(w[k] >> 16), DT == BF16);
-                }
+            for (int k = 0; k < 4; ++k) {
+                v[k] = a[k];
+                v[4 + k] = b[k];
             }
         } else {
+            const u32x4_a2 u = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(row) + i);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[k] = i + k < V ? at(row, i + k) : -INFINITY;
+            for (int k = 0; k < 4; ++k) {
+                v[2 * k] = from16((uint16_t)(u[k] & 0xFFFFu), DT == BF16);
+                v[2 * k + 1] = from16((uint16_t)(u[k] >> 16), DT == BF16);
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k) {
+            const float f = i + k < V ? load_elem(row, DT, (size_t)(i + k)) : past;
+#pragma unroll
+            for (int l = 0; l < 8; ++l)
+                if (l == k) v[l] = f;
         }
     }
-};
-
-// f's order among all floats as an unsigned integer, zeros of both signs alike, NaN above everything
-__device__ __forceinline__ uint32_t order32(float f) {
-    if (f != f) return 0xFFFFFFFFu;
-    const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+
+// f's order among all floats as an unsigned integer, zeros of both signs alike, NaN above everything; above the complemented
+// index, so that the largest key is the largest value at its lowest index
 __device__ __forceinline__ unsigned long long key32(float f, int idx) {
-    return ((unsigned long long)order32(f) << 32) | (uint32_t)~(uint32_t)idx;
+    const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.0f);
+    const uint32_t o = f != f ? 0xFFFFFFFFu : u & 0x80000000u ? ~u : u | 0x80000000u;
+    return ((unsigned long long)o << 32) | (uint32_t)~(uint32_t)idx;
 }
 
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ float dpp_of(float v) {           // -inf where the row mask excludes the lane
+    return __builtin_bit_cast(float, dpp_u32<CTRL, ROW_MASK>(__builtin_bit_cast(uint32_t, v), 0xFF800000u));
+}
+// the wave's maximum, in every lane; a NaN is passed over
 __device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
+    v = fmaxf(v, dpp_of<0xB1>(v));
+    v = fmaxf(v, dpp_of<0x4E>(v));
+    v = fmaxf(v, dpp_of<0x141>(v));
+    v = fmaxf(v, dpp_of<0x140>(v));
+    v = fmaxf(v, dpp_of<0x142, 0xA>(v));
+    v = fmaxf(v, dpp_of<0x143, 0xC>(v));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, v), 63));
 }
 __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k) {
 #pragma unroll
@@ -128,230 +137,243 @@ __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) {
     const int64_t f = a.first[b];
     return n >= 0 && n <= a.G && f >= 0 && f + n < a.R ? n : -1;
 }
-__device__ __forceinline__ const void* logits_row(const VerifyArgs& a, int64_t row, int dt) {
-    return static_cast<const char*>(a.logits) + row * a.stride * (dt == F32 ? 4 : 2);
+template <int DT>
+__device__ __forceinline__ const void* logits_row(const VerifyArgs& a, int64_t row) {
+    return static_cast<const char*>(a.logits) + row * a.stride * (DT == F32 ? 4 : 2);
 }
 
-// The statistics of one piece (64 * VERIFY_VECS vectors) of one row: a wave each, blockIdx.x a row of a request
+// The statistics of the rows: a wave a piece, four to a workgroup
 template <int DT>
 __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
-    constexpr int VEC = Elems<DT>::VEC;
-    const int b = blockIdx.x / (a.G + 1), j = blockIdx.x % (a.G + 1);
-    const int piece = blockIdx.y * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n = drafts_of(a, b);
-    if (j > n || piece >= a.pieces) return;
-    const void* row = logits_row(a, (int64_t)a.first[b] + j, DT);
-    float hi, lo;
-    exponent_factor(inv_temperature(a.temperature[b]), hi, lo);
-    const int i0 = (piece * VERIFY_VECS * 64 + lane) * VEC;
-    float v[VERIFY_VECS][VEC];
+    const int quads = (a.pieces + 3) / 4, at = blockIdx.x / quads, b = at / (a.G + 1), j = at % (a.G + 1);
+    const int lane = threadIdx.x & 63;
+    const int piece = (int)(blockIdx.x % quads) * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (j == 0 && piece == 0 && lane == 0) a.arrived[(size_t)b * CNT_STRIDE] = 0;
+    if (j > drafts_of(a, b) || piece >= a.pieces) return;
+    const void* row = logits_row<DT>(a, (int64_t)a.first[b] + j);
+    const float temperature = a.temperature[b];
+    const int i0 = piece * PIECE + lane * 8;
+    float v[PIECE_GROUPS][8];
 #pragma unroll
-    for (int u = 0; u < VERIFY_VECS; ++u) Elems<DT>::load(row, i0 + u * 64 * VEC, a.V, v[u]);
+    for (int u = 0; u < PIECE_GROUPS; ++u) load_group<DT>(row, i0 + u * 512, a.V, -INFINITY, v[u]);
+    float hi, lo;
+    exponent_factor(inv_temperature(temperature), hi, lo);
     float m = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < VERIFY_VECS; ++u)
+    for (int u = 0; u < PIECE_GROUPS; ++u)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m = fmaxf(m, v[u][k]);
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, v[u][k]);
     m = wave_max_f32(m);                                    // NaN is passed over here and found in the sum
     const float base = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
-    for (int u = 0; u < VERIFY_VECS; ++u)
+    for (int u = 0; u < PIECE_GROUPS; ++u)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) s += exp_scaled(v[u][k] - base, hi, lo);
+        for (int k = 0; k < 8; ++k) s += exp_scaled(v[u][k] - base, hi, lo);
     s = wave_sum_f32(s);
-    const bool odd = s != s;                                // a NaN or +inf among the logits
-    int idx = 0x7FFFFFFF;
-    bool nan = false;
+    const size_t to = (size_t)at * a.pieces + piece;
+    if (lane == 0) a.part[to] = {m, s};
+    if (!is_greedy(temperature)) return;
+    const bool nan = s != s;                                // a NaN or +inf; the first NaN, if there is one, is the largest
+    int idx = 0x7FFFFFFF, nan_at = 0x7FFFFFFF;
 #pragma unroll
-    for (int u = VERIFY_VECS - 1; u >= 0; --u)
+    for (int u = PIECE_GROUPS - 1; u >= 0; --u)
 #pragma unroll
-        for (int k = VEC - 1; k >= 0; --k)
-            if (v[u][k] == m) idx = i0 + u * 64 * VEC + k;  // (a -inf past the row's end has the highest indices)
-    if (odd) {
-        int at = 0x7FFFFFFF;
-#pragma unroll
-        for (int u = VERIFY_VECS - 1; u >= 0; --u)
-#pragma unroll
-            for (int k = VEC - 1; k >= 0; --k)
-                if (v[u][k] != v[u][k]) at = i0 + u * 64 * VEC + k;
-        nan = __ballot(at != 0x7FFFFFFF) != 0;
-        if (nan) idx = at;
-    }
+        for (int k = 7; k >= 0; --k) {
+            if (v[u][k] == m) idx = i0 + u * 512 + k;       // (a -inf past the row's end has the highest indices)
+            if (nan && v[u][k] != v[u][k]) nan_at = i0 + u * 512 + k;
+        }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_xor(idx, d);
-        idx = o < idx ? o : idx;
+        idx = min(idx, __shfl_xor(idx, d));
+        nan_at = min(nan_at, __shfl_xor(nan_at, d));
     }
-    if (lane == 0) a.part[(size_t)blockIdx.x * a.pieces + piece] = {nan ? __builtin_nanf("") : m, s, idx, 0};
+    if (lane == 0) {
+        const bool has = nan_at != 0x7FFFFFFF;
+        a.best[to] = has ? nan_at : idx;
+        if (has) a.part[to].m = __builtin_nanf("");
+    }
 }
 
-// One workgroup a request: every row's statistics from its pieces (a wave a row), then the drafts in order
+// What a workgroup knows of each of its request's rows
+struct Row {
+    double z;                                   // the sum of exponentials over m, no finite positive number: no distribution
+    double arg;                                 // (the logit of the draft, or of a greedy row's argmax, - m) / temperature
+    float m;
+    int token;                                  // the draft, if it is accepted, else -1; the argmax of a greedy row
+};
+
+__device__ __forceinline__ bool distribution(double z) { return z > 0.0 && z < INFINITY; }
+
+// Row j of request b from its pieces, by one wave; the decision about its draft (j < n)
 template <int DT>
-__global__ __launch_bounds__(256) void verify_decide_kernel(const VerifyArgs a) {
-    extern __shared__ double row_z[];                        // [G + 1] sums, then maxima and argmaxima
-    float* row_m = reinterpret_cast<float*>(row_z + a.G + 1);
-    int* row_best = reinterpret_cast<int*>(row_m + a.G + 1);
-    const int b = blockIdx.x, lane = threadIdx.x & 63;
-    const int n = drafts_of(a, b);
-    const double inv_t = inv_temperature(a.temperature[b]);
-    for (int j = threadIdx.x >> 6; j <= n; j += 4) {
-        const Piece* p = a.part + ((size_t)b * (a.G + 1) + j) * a.pieces;
-        unsigned long long key = 0;
-        float m = -INFINITY;
-        for (int i = lane; i < a.pieces; i += 64) {
-            const Piece q = p[i];
-            const unsigned long long k = key32(q.m, q.idx);
-            key = k > key ? k : key;
-            m = fmaxf(m, q.m);
-        }
-        key = wave_max_key(key);
-        m = wave_max_f32(m);
-        double z = 0.0;
-        for (int i = lane; i < a.pieces; i += 64) {
-            const Piece q = p[i];
-            if (q.s != 0.f) z += (double)q.s * exp(((double)q.m - (double)m) * inv_t);
-        }
-        z = wave_sum_f64_dpp(z);
-        if (lane == 0) {
-            row_z[j] = z;
-            row_m[j] = m;
-            row_best[j] = (int)~(uint32_t)key;
-        }
+__device__ __forceinline__ Row verify_row(const VerifyArgs& a, int b, int j, int n, bool greedy, double inv_t) {
+    const int lane = threadIdx.x & 63;
+    const size_t at = (size_t)b * (a.G + 1) + j;
+    const Piece* p = a.part + at * a.pieces;
+    const int x = j < n ? a.drafts[(size_t)b * a.G + j] : -1;
+    const bool in = x >= 0 && x < a.V;
+    const void* row = logits_row<DT>(a, (int64_t)a.first[b] + j);
+    float lx = 0.f, u = 0.f, q = 1.f;
+    if (in && !greedy) {
+        lx = load_elem(row, DT, (size_t)x);
+        u = a.uniform[(size_t)b * a.G + j];
+        if (a.probs) q = a.probs[b * a.probs_request + j * a.probs_row + x];
     }
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    const size_t o = (size_t)b * (a.G + 1);
-    Drawn d = {-1, 0, -1, 0.f, 0.f, 0.f, 0.f, 0.0};
-    int emitted = 0;
-    if (n >= 0) {
-        const bool greedy = is_greedy(a.temperature[b]);
-        for (int j = 0; j <= n; ++j) {
-            const void* row = logits_row(a, (int64_t)a.first[b] + j, DT);
-            const double z = row_z[j], m = row_m[j];
-            const bool some = z > 0.0 && z < INFINITY;       // false too for a NaN: no distribution
-            const double log_z = some ? log(z) : 0.0;
-            const int x = j < n ? a.drafts[(size_t)b * a.G + j] : -1;
-            const bool in = x >= 0 && x < a.V;
-            int token = -1;
-            if (greedy) {
-                token = row_best[j];
-                if (j < n && x == token) {
-                    a.tokens[o + j] = token;
-                    a.logprobs[o + j] = some ? (float)((Elems<DT>::at(row, token) - m) * inv_t - log_z) : 0.f;
-                    ++emitted;
-                    continue;
-                }
-                a.tokens[o + j] = token;
-                a.logprobs[o + j] = some ? (float)((Elems<DT>::at(row, token) - m) * inv_t - log_z) : 0.f;
-                ++emitted;
-                break;
-            }
-            if (in && some && j < n) {
-                const double arg = (Elems<DT>::at(row, x) - m) * inv_t;
-                const double q = a.probs ? (double)a.probs[b * a.probs_request + j * a.probs_row + x] : 1.0;
-                if ((double)a.uniform[(size_t)b * a.G + j] * q < exp(arg) / z) {
-                    a.tokens[o + j] = x;
-                    a.logprobs[o + j] = (float)(arg - log_z);
-                    ++emitted;
-                    continue;
-                }
-            }
-            if (some) {
-                d.row = a.first[b] + j;
-                d.j = j;
-                d.draft = j < n ? x : -1;
-                d.m = row_m[j];
-                exponent_factor(inv_t, d.c_hi, d.c_lo);
-                d.rz = (float)(1.0 / z);
-                d.log_z = log_z;
-                ++emitted;
-            }
-            break;
-        }
+    constexpr int HELD = 4;                                  // pieces a lane keeps (a vocabulary of 262144); more are read twice
+    Piece held[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) held[k] = lane + 64 * k < a.pieces ? p[lane + 64 * k] : Piece{-INFINITY, 0.f};
+    Row r;
+    unsigned long long key = 0;
+    if (greedy)
+        for (int i = lane; i < a.pieces; i += 64) key = max(key, key32(p[i].m, a.best[at * a.pieces + i]));
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) m = fmaxf(m, held[k].m);
+    for (int i = lane + 64 * HELD; i < a.pieces; i += 64) m = fmaxf(m, p[i].m);
+    r.m = m = wave_max_f32(m);
+    double z = 0.0;
+    const auto add = [&](const Piece& v) __attribute__((always_inline)) {
+        if (v.s != 0.f) z += (double)v.s * exp(((double)v.m - (double)m) * inv_t);
+    };
+#pragma unroll 1
+    for (int k = 0; k < HELD; ++k) {
+        add(held[0]);
+        held[0] = held[1], held[1] = held[2], held[2] = held[3];
     }
-    a.drawn[b] = d;
-    a.counts[b] = emitted;
-    for (int j = emitted - (d.row >= 0); j <= a.G; ++j) {    // the race's token overwrites its place
-        a.tokens[o + j] = -1;
-        a.logprobs[o + j] = 0.f;
+    for (int i = lane + 64 * HELD; i < a.pieces; i += 64) add(p[i]);
+    r.z = z = wave_sum_f64_dpp(z);
+    if (greedy) {
+        r.token = (int)~(uint32_t)wave_max_key(key);
+        r.arg = ((double)load_elem(row, DT, (size_t)r.token) - (double)m) * inv_t;
+    } else {
+        r.arg = ((double)lx - (double)m) * inv_t;
+        r.token = in && distribution(z) && (double)u * (double)q < exp(r.arg) / z ? x : -1;
     }
+    return r;
 }
 
-// The race over one piece of request blockIdx.x's row: the largest key of w / e, and that of p / e
+// This thread's entries of the race from entry i0 on (RACE_GROUPS groups of 8, 2048 apart): the largest w / e with w above 0, w = p
+// without draft probabilities q (0 at the draft itself), else p - q
+template <int DT>
+__device__ __forceinline__ unsigned long long race_best(const VerifyArgs& a, const void* row, const float* e, const float* q,
+                                                        int draft, float m, float hi, float lo, float rz, int i0,
+                                                        const float (&ev)[RACE_GROUPS][8]) {
+    float v[RACE_GROUPS][8], qv[RACE_GROUPS][8];
+#pragma unroll
+    for (int u = 0; u < RACE_GROUPS; ++u) {
+        load_group<DT>(row, i0 + u * 2048, a.V, -INFINITY, v[u]);
+        if (q) load_group<F32>(q, i0 + u * 2048, a.V, 0.f, qv[u]);
+    }
+    float best = -INFINITY;
+    int idx = -1;
+#pragma unroll
+    for (int u = 0; u < RACE_GROUPS; ++u)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + u * 2048 + k;
+            float w = exp_scaled(v[u][k] - m, hi, lo) * rz;
+            if (q) w -= qv[u][k];
+            else if (i == draft) w = 0.f;
+            const float key = w * __builtin_amdgcn_rcpf(ev[u][k]);
+            if (w > 0.f && key > best) {                     // in the order of the indices: the lowest of equal ones stays
+                best = key;
+                idx = i;
+            }
+        }
+    return idx < 0 ? 0ull : key32(best, idx);
+}
+
+// A request's outcome: tokens, counts and log-probabilities from its rows (rows below `taken` accepted, the token of row `taken`
+// drawn, -1: none)
+__device__ __forceinline__ void verify_write(const VerifyArgs& a, int b, const Row* rows, int taken, int drawn, double drawn_arg) {
+    const size_t o = (size_t)b * (a.G + 1);
+    for (int j = threadIdx.x; j <= a.G; j += 256) {
+        const int token = j < taken ? rows[j].token : j == taken ? drawn : -1;
+        const bool some = token >= 0 && distribution(rows[j].z);
+        a.tokens[o + j] = token;
+        a.logprobs[o + j] = some ? (float)((j < taken ? rows[j].arg : drawn_arg) - log(rows[j].z)) : 0.f;
+    }
+    if (threadIdx.x == 0) a.counts[b] = taken + (drawn >= 0);
+}
+
+__device__ __forceinline__ unsigned long long block_max_key(unsigned long long k, unsigned long long* sh) {
+    k = wave_max_key(k);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = k;
+    __syncthreads();
+    k = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
+    __syncthreads();
+    return k;
+}
+
+// The drafts' decisions and a request's race: a workgroup RACE entries of one request
 template <int DT>
 __global__ __launch_bounds__(256) void verify_race_kernel(const VerifyArgs a) {
-    constexpr int VEC = Elems<DT>::VEC;
-    const int b = blockIdx.x, piece = blockIdx.y * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (piece >= a.pieces) return;
-    const Drawn d = a.drawn[b];
-    if (d.row < 0) return;
+    extern __shared__ Row rows[];                            // [G + 1]
+    __shared__ unsigned long long sh[4];
+    __shared__ int last;
+    const int b = blockIdx.x / a.races, at = blockIdx.x % a.races;
     const int n = drafts_of(a, b);
-    const void* row = logits_row(a, d.row, DT);
-    const float* e = a.race + b * a.race_stride;
-    const float* q = a.probs && d.j < n ? a.probs + b * a.probs_request + d.j * a.probs_row : nullptr;
-    const int i0 = (piece * VERIFY_VECS * 64 + lane) * VEC;
-    unsigned long long best_w = 0, best_p = 0;
-#pragma unroll
-    for (int u = 0; u < VERIFY_VECS; ++u) {
-        const int i = i0 + u * 64 * VEC;
-        float v[VEC];
-        Elems<DT>::load(row, i, a.V, v);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            if (i + k >= a.V) break;
-            const float p = exp_scaled(v[k] - d.m, d.c_hi, d.c_lo) * d.rz;
-            float w = p;
-            if (q) w = p - q[i + k];
-            else if (d.draft == i + k) w = 0.f;
-            const float kp = p / e[i + k], kw = w / e[i + k];
-            if (p > 0.f && kp == kp) best_p = max(best_p, key32(kp, i + k));
-            if (w > 0.f && kw == kw) best_w = max(best_w, key32(kw, i + k));
-        }
-    }
-    best_w = wave_max_key(best_w);
-    best_p = wave_max_key(best_p);
-    if (lane == 0) {
-        unsigned long long* k = a.keys + ((size_t)b * a.pieces + piece) * 2;
-        k[0] = best_w;
-        k[1] = best_p;
-    }
-}
-
-// The winner of every request's race: a wave a request
-template <int DT>
-__global__ __launch_bounds__(64) void verify_finish_kernel(const VerifyArgs a) {
-    const int b = blockIdx.x, lane = threadIdx.x;
-    const Drawn d = a.drawn[b];
-    if (d.row < 0) return;
-    unsigned long long w = 0, p = 0;
-    for (int i = lane; i < a.pieces; i += 64) {
-        const unsigned long long* k = a.keys + ((size_t)b * a.pieces + i) * 2;
-        w = max(w, k[0]);
-        p = max(p, k[1]);
-    }
-    w = wave_max_key(w);
-    p = wave_max_key(p);
-    if (lane != 0) return;
-    const unsigned long long key = w ? w : p;
-    const size_t o = (size_t)b * (a.G + 1) + d.j;
-    if (!key) {                                              // every random number of the row is unusable
-        a.counts[b] = d.j;
+    const float temperature = a.temperature[b];
+    const bool greedy = is_greedy(temperature);
+    if ((n < 0 || greedy) && at != 0) return;
+    if (n < 0) {
+        verify_write(a, b, rows, 0, -1, 0.0);
         return;
     }
-    const int token = (int)~(uint32_t)key;
-    const double inv_t = inv_temperature(a.temperature[b]);
-    a.tokens[o] = token;
-    a.logprobs[o] = (float)(((double)Elems<DT>::at(logits_row(a, d.row, DT), token) - (double)d.m) * inv_t - d.log_z);
+    const float* e = a.race + b * a.race_stride;
+    const int i0 = at * RACE + (int)threadIdx.x * 8;
+    float ev[RACE_GROUPS][8];
+    if (!greedy)
+#pragma unroll
+        for (int u = 0; u < RACE_GROUPS; ++u) load_group<F32>(e, i0 + u * 2048, a.V, 1.f, ev[u]);
+    const double inv_t = inv_temperature(temperature);
+    for (int j = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); j <= n; j += 4) {
+        const Row r = verify_row<DT>(a, b, j, n, greedy, inv_t);
+        if ((threadIdx.x & 63) == 0) rows[j] = r;
+    }
+    __syncthreads();
+    int taken = 0;
+    while (taken < n && (greedy ? rows[taken].token == a.drafts[(size_t)b * a.G + taken] : rows[taken].token >= 0)) ++taken;
+    const Row r = rows[taken];
+    if (greedy || !distribution(r.z)) {                      // nothing to race for
+        if (at == 0) verify_write(a, b, rows, taken, greedy ? r.token : -1, r.arg);
+        return;
+    }
+    const void* row = logits_row<DT>(a, (int64_t)a.first[b] + taken);
+    const float* q = a.probs && taken < n ? a.probs + b * a.probs_request + taken * a.probs_row : nullptr;
+    const int draft = taken < n ? a.drafts[(size_t)b * a.G + taken] : -1;
+    float hi, lo;
+    exponent_factor(inv_t, hi, lo);
+    const float rz = (float)(1.0 / r.z);
+    unsigned long long key = block_max_key(race_best<DT>(a, row, e, q, draft, r.m, hi, lo, rz, i0, ev), sh);
+    unsigned long long* keys = a.keys + (size_t)b * a.races;
+    if (a.races > 1) {
+        if (threadIdx.x == 0) store_dev(keys + at, key);
+        if (!arrive_last(a.arrived + (size_t)b * CNT_STRIDE, a.races, &last)) return;
+        key = 0;
+        for (int i = threadIdx.x; i < a.races; i += 256) key = max(key, load_dev(keys + i));
+        key = block_max_key(key, sh);
+    }
+    if (!key && taken < n) {                                 // q covers p (or the draft was all of it): p itself, rarely
+        for (int k = 0; k < a.races; ++k) {
+            const int i1 = k * RACE + (int)threadIdx.x * 8;
+#pragma unroll
+            for (int u = 0; u < RACE_GROUPS; ++u) load_group<F32>(e, i1 + u * 2048, a.V, 1.f, ev[u]);
+            key = max(key, race_best<DT>(a, row, e, nullptr, -1, r.m, hi, lo, rz, i1, ev));
+        }
+        key = block_max_key(key, sh);
+    }
+    const int token = key ? (int)~(uint32_t)key : -1;        // -1: every random number of the row is unusable
+    verify_write(a, b, rows, taken, token,
+                 token < 0 ? 0.0 : ((double)load_elem(row, DT, (size_t)token) - (double)r.m) * inv_t);
 }
 
 template <int DT>
 int verify_launch(const VerifyArgs& a, hipStream_t st) {
-    const unsigned blocks = (unsigned)((a.pieces + 3) / 4);
-    verify_stats_kernel<DT><<<dim3((unsigned)(a.B * (a.G + 1)), blocks), 256, 0, st>>>(a);
-    verify_decide_kernel<DT><<<(unsigned)a.B, 256, (size_t)(a.G + 1) * 16, st>>>(a);
-    verify_race_kernel<DT><<<dim3((unsigned)a.B, blocks), 256, 0, st>>>(a);
-    verify_finish_kernel<DT><<<(unsigned)a.B, 64, 0, st>>>(a);
+    verify_stats_kernel<DT><<<(unsigned)(a.B * (a.G + 1) * ((a.pieces + 3) / 4)), 256, 0, st>>>(a);
+    verify_race_kernel<DT><<<(unsigned)(a.B * a.races), 256, (size_t)(a.G + 1) * sizeof(Row), st>>>(a);
     return esp_host::launch_check("verify");
 }
 
@@ -362,15 +384,17 @@ int verify_launch(const VerifyArgs& a, hipStream_t st) {
 // ======================================================================================================================
 using namespace esp;
 
-static int64_t verify_pieces(int64_t V, int dtype) {
-    const int64_t one = 64 * VERIFY_VECS * (dtype == ESP_F32 ? 4 : 8);
-    return (V + one - 1) / one;
-}
+struct VerifySizes {
+    int64_t pieces, races, part, best, arrived, bytes;       // byte offsets behind the keys
+    VerifySizes(int64_t B, int64_t G, int64_t V)
+        : pieces((V + PIECE - 1) / PIECE), races((V + RACE - 1) / RACE), part(B * races * 8),
+          best(part + B * (G + 1) * pieces * (int64_t)sizeof(Piece)), arrived(best + B * (G + 1) * pieces * 4),
+          bytes(arrived + B * CNT_STRIDE * 4) {}
+};
 
-extern "C" int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V, int dtype) {
+extern "C" int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V) {
     if (B <= 0 || G < 0 || V <= 0 || B > (1 << 20) || G > 1024 || V > (1 << 24)) return 0;
-    const int64_t np = verify_pieces(V, dtype);
-    return B * (G + 1) * np * (int64_t)sizeof(Piece) + B * np * 16 + B * (int64_t)sizeof(Drawn);
+    return VerifySizes(B, G, V).bytes;
 }
 
 extern "C" int esp_verify(const void* logits, int dtype, int64_t stride, int64_t R, int64_t V, const int32_t* first,
@@ -382,14 +406,15 @@ extern "C" int esp_verify(const void* logits, int dtype, int64_t stride, int64_t
     ESP_REQUIRE(B >= 0 && B <= (1 << 20) && G >= 0 && G <= 1024, "verify: at most 2^20 requests of at most 1024 drafts");
     ESP_REQUIRE(R >= 0 && R < (1ll << 31) && V > 0 && V <= (1 << 24), "verify: need R < 2^31 rows and 0 < V <= 2^24");
     if (B == 0) return esp_host::ok();
-    ESP_REQUIRE(B * (G + 1) <= (1 << 23), "verify: at most 2^23 rows over all requests");
+    const VerifySizes z(B, G, V);
+    ESP_REQUIRE(B * (G + 1) * ((z.pieces + 3) / 4) < (1 << 24), "verify: at most 2^24 - 1 blocks of 4096 logits over all rows");
     ESP_REQUIRE((logits || R == 0) && first && n_drafts && race && temperature && tokens && counts && logprobs && scratch &&
                     (G == 0 || (drafts && uniform)), "verify: null pointer");
     ESP_REQUIRE((R <= 1 || stride >= V) && (B <= 1 || race_stride >= V), "verify: rows overlap");
     ESP_REQUIRE(probs_request >= 0 && probs_row >= 0, "verify: negative stride");
     ESP_REQUIRE((uintptr_t)logits % (dtype == ESP_F32 ? 4 : 2) == 0 && (uintptr_t)scratch % 16 == 0,
                 "verify: logits must be aligned to an element, the scratch to 16 bytes");
-    ESP_REQUIRE(scratch_bytes >= esp_verify_scratch(B, G, V, dtype), "verify: the scratch needs esp_verify_scratch bytes");
+    ESP_REQUIRE(scratch_bytes >= z.bytes, "verify: the scratch needs esp_verify_scratch bytes");
     VerifyArgs a;
     a.logits = logits;
     a.stride = stride;
@@ -397,7 +422,8 @@ extern "C" int esp_verify(const void* logits, int dtype, int64_t stride, int64_t
     a.V = (int)V;
     a.B = (int)B;
     a.G = (int)G;
-    a.pieces = (int)verify_pieces(V, dtype);
+    a.pieces = (int)z.pieces;
+    a.races = (int)z.races;
     a.first = first;
     a.n_drafts = n_drafts;
     a.drafts = drafts;
@@ -411,9 +437,11 @@ extern "C" int esp_verify(const void* logits, int dtype, int64_t stride, int64_t
     a.tokens = tokens;
     a.counts = counts;
     a.logprobs = logprobs;
-    a.part = static_cast<Piece*>(scratch);
-    a.keys = reinterpret_cast<unsigned long long*>(a.part + B * (G + 1) * a.pieces);
-    a.drawn = reinterpret_cast<Drawn*>(a.keys + B * a.pieces * 2);
+    char* base = static_cast<char*>(scratch);
+    a.keys = reinterpret_cast<unsigned long long*>(base);
+    a.part = reinterpret_cast<Piece*>(base + z.part);
+    a.best = reinterpret_cast<int*>(base + z.best);
+    a.arrived = reinterpret_cast<int*>(base + z.arrived);
     const hipStream_t st = (hipStream_t)stream;
     return dtype == ESP_F32 ? verify_launch<F32>(a, st) : dtype == ESP_BF16 ? verify_launch<BF16>(a, st)
                                                                             : verify_launch<F16>(a, st);
