@@ -86,7 +86,7 @@ def _verify(lib, **over):
 
 
 @pytest.mark.parametrize("over,needle", [
-    (dict(dtype=3), "dtype"), (dict(B=-1), "requests"), (dict(B=1 << 21), "requests"), (dict(B=1 << 20, V=1 << 24, G=1024), "blocks"), (dict(G=-1), "drafts"),
+    (dict(dtype=3), "dtype"), (dict(B=-1), "requests"), (dict(B=1 << 21), "requests"), (dict(B=1 << 20, V=1 << 24, stride=1 << 24, rs=1 << 24, G=1024), "blocks"), (dict(G=-1), "drafts"),
     (dict(G=1025), "drafts"), (dict(R=1 << 31), "rows"), (dict(V=0), "V"), (dict(V=1 << 28), "V"), (dict(logits=None), "null"),
     (dict(first=None), "null"), (dict(drafts=None), "null"), (dict(race=None), "null"), (dict(scratch=None), "null"),
     (dict(stride=63), "overlap"), (dict(rs=63), "overlap"), (dict(pr=-1), "stride"), (dict(logits=17), "aligned"),

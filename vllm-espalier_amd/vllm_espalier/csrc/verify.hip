@@ -10,17 +10,19 @@
 // Two launches. The first reads every row once: a wave takes 1024 logits into registers and leaves their maximum and their sum of
 // exponentials (a greedy request's: the place of the maximum too), so no workgroup waits for another and nothing is rescaled. The
 // second runs over the one row of a request that is drawn from: each of its workgroups puts the request's rows together from the
-// waves' pieces and decides the drafts for itself (a few hundred bytes out of the L2 and 64-bit sums, a wave a row, while its
-// random numbers are on the way), then races its 4096 entries; the last of a request's to arrive writes the outcome.
+// waves' pieces and decides the drafts for itself (a few hundred bytes out of the L2, a wave a row, while its random numbers are
+// on the way), then races its share of the entries, 4096 at a time; the last of a request's to arrive writes the outcome.
 #include "../../../include/espalier.h"
 #include "common.hpp"
 #include "norm.hpp"
+
+#include <algorithm>
 
 namespace esp {
 
 constexpr float GREEDY_BELOW = 1e-5f;
 constexpr int PIECE_GROUPS = 2;                // groups of 8 logits a lane of a wave's piece, all in flight
-constexpr int PIECE = 64 * 8 * PIECE_GROUPS;
+constexpr int PIECE = 64 * 8 * PIECE_GROUPS;    // (2048 a wave: 7.0 us instead of 5.0 for the four rows of one request, 79 / 76 for 768)
 constexpr int RACE_GROUPS = 2;                 // groups of 8 entries a thread of a race
 constexpr int RACE = 256 * 8 * RACE_GROUPS;
 
@@ -32,13 +34,14 @@ struct Piece {
 struct VerifyArgs {
     const void* logits;
     int64_t stride, R;
-    int V, B, G, pieces, races;
+    int V, B, G, pieces, races, chunks;         // races: workgroups a request, that share its chunks of RACE entries
     const int32_t *first, *n_drafts, *drafts;
     const float *uniform, *race, *temperature, *probs;
     int64_t race_stride, probs_request, probs_row;
     int32_t *tokens, *counts;
     float* logprobs;
     unsigned long long* keys;                   // [B][races]
+    float* winners;                             // [B][races]: the keys' logits
     Piece* part;                                // [B][G + 1][pieces]
     int* best;                                  // [B][G + 1][pieces]: the place of m (the first NaN, if any), greedy requests
     int* arrived;                               // [B][CNT_STRIDE], made zero by the first launch
@@ -131,10 +134,16 @@ __device__ __forceinline__ float exp_scaled(float d, float hi, float lo) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, hi, d * lo));
 }
 
+// a value that every lane of the wave reads, through the scalar cache (nothing writes it while the kernel runs)
+template <typename T>
+__device__ __forceinline__ T load_uniform(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 // the drafts of request b, -1 where there is no such request (or its rows lie outside the logits)
 __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) {
-    const int n = a.n_drafts[b];
-    const int64_t f = a.first[b];
+    const int n = load_uniform(a.n_drafts + b);
+    const int64_t f = load_uniform(a.first + b);
     return n >= 0 && n <= a.G && f >= 0 && f + n < a.R ? n : -1;
 }
 template <int DT>
@@ -150,8 +159,8 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
     const int piece = (int)(blockIdx.x % quads) * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (j == 0 && piece == 0 && lane == 0) a.arrived[(size_t)b * CNT_STRIDE] = 0;
     if (j > drafts_of(a, b) || piece >= a.pieces) return;
-    const void* row = logits_row<DT>(a, (int64_t)a.first[b] + j);
-    const float temperature = a.temperature[b];
+    const void* row = logits_row<DT>(a, (int64_t)load_uniform(a.first + b) + j);
+    const float temperature = load_uniform(a.temperature + b);
     const int i0 = piece * PIECE + lane * 8;
     float v[PIECE_GROUPS][8];
 #pragma unroll
@@ -207,27 +216,24 @@ __device__ __forceinline__ bool distribution(double z) { return z > 0.0 && z < I
 
 // Row j of request b from its pieces, by one wave; the decision about its draft (j < n)
 template <int DT>
-__device__ __forceinline__ Row verify_row(const VerifyArgs& a, int b, int j, int n, bool greedy, double inv_t) {
+__device__ __forceinline__ Row verify_row(const VerifyArgs& a, int b, int j, int n, bool greedy, double inv_t, float hi, float lo) {
     const int lane = threadIdx.x & 63;
     const size_t at = (size_t)b * (a.G + 1) + j;
     const Piece* p = a.part + at * a.pieces;
-    const int x = j < n ? a.drafts[(size_t)b * a.G + j] : -1;
-    const bool in = x >= 0 && x < a.V;
-    const void* row = logits_row<DT>(a, (int64_t)a.first[b] + j);
-    float lx = 0.f, u = 0.f, q = 1.f;
-    if (in && !greedy) {
-        lx = load_elem(row, DT, (size_t)x);
-        u = a.uniform[(size_t)b * a.G + j];
-        if (a.probs) q = a.probs[b * a.probs_request + j * a.probs_row + x];
-    }
     constexpr int HELD = 4;                                  // pieces a lane keeps (a vocabulary of 262144); more are read twice
     Piece held[HELD];
 #pragma unroll
     for (int k = 0; k < HELD; ++k) held[k] = lane + 64 * k < a.pieces ? p[lane + 64 * k] : Piece{-INFINITY, 0.f};
+    const int x = j < n ? load_uniform(a.drafts + (size_t)b * a.G + j) : -1;
+    const bool in = x >= 0 && x < a.V;
+    const void* row = logits_row<DT>(a, (int64_t)load_uniform(a.first + b) + j);
+    float lx = 0.f, u = 0.f, q = 1.f;
+    if (in && !greedy) {
+        lx = load_elem(row, DT, (size_t)x);
+        u = load_uniform(a.uniform + (size_t)b * a.G + j);
+        if (a.probs) q = load_uniform(a.probs + b * a.probs_request + j * a.probs_row + x);
+    }
     Row r;
-    unsigned long long key = 0;
-    if (greedy)
-        for (int i = lane; i < a.pieces; i += 64) key = max(key, key32(p[i].m, a.best[at * a.pieces + i]));
     float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < HELD; ++k) m = fmaxf(m, held[k].m);
@@ -235,39 +241,40 @@ __device__ __forceinline__ Row verify_row(const VerifyArgs& a, int b, int j, int
     r.m = m = wave_max_f32(m);
     double z = 0.0;
     const auto add = [&](const Piece& v) __attribute__((always_inline)) {
-        if (v.s != 0.f) z += (double)v.s * exp(((double)v.m - (double)m) * inv_t);
+        if (v.s != 0.f) z += (double)(v.s * exp_scaled(v.m - m, hi, lo));
     };
-#pragma unroll 1
-    for (int k = 0; k < HELD; ++k) {
-        add(held[0]);
-        held[0] = held[1], held[1] = held[2], held[2] = held[3];
-    }
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) add(held[k]);
     for (int i = lane + 64 * HELD; i < a.pieces; i += 64) add(p[i]);
     r.z = z = wave_sum_f64_dpp(z);
     if (greedy) {
+        unsigned long long key = 0;
+        for (int i = lane; i < a.pieces; i += 64) key = max(key, key32(p[i].m, a.best[at * a.pieces + i]));
         r.token = (int)~(uint32_t)wave_max_key(key);
-        r.arg = ((double)load_elem(row, DT, (size_t)r.token) - (double)m) * inv_t;
+        lx = load_elem(row, DT, (size_t)r.token);
     } else {
-        r.arg = ((double)lx - (double)m) * inv_t;
-        r.token = in && distribution(z) && (double)u * (double)q < exp(r.arg) / z ? x : -1;
+        r.token = -1;
     }
+    r.arg = ((double)lx - (double)m) * inv_t;
+    if (in && !greedy && distribution(z) && (double)u * (double)q < exp(r.arg) / z) r.token = x;
     return r;
 }
 
-// This thread's entries of the race from entry i0 on (RACE_GROUPS groups of 8, 2048 apart): the largest w / e with w above 0, w = p
-// without draft probabilities q (0 at the draft itself), else p - q
+// This thread's entries of the race from entry i0 on (RACE_GROUPS groups of 8, 2048 apart) into its best: the largest w / e with w
+// above 0, w = p without draft probabilities q (0 at the draft itself), else p - q
+struct Best {
+    float key, logit;
+    int idx;
+};
 template <int DT>
-__device__ __forceinline__ unsigned long long race_best(const VerifyArgs& a, const void* row, const float* e, const float* q,
-                                                        int draft, float m, float hi, float lo, float rz, int i0,
-                                                        const float (&ev)[RACE_GROUPS][8]) {
+__device__ __forceinline__ void race_best(const VerifyArgs& a, const void* row, const float* q, int draft, float m, float hi,
+                                          float lo, float rz, int i0, const float (&ev)[RACE_GROUPS][8], Best& best) {
     float v[RACE_GROUPS][8], qv[RACE_GROUPS][8];
 #pragma unroll
     for (int u = 0; u < RACE_GROUPS; ++u) {
         load_group<DT>(row, i0 + u * 2048, a.V, -INFINITY, v[u]);
         if (q) load_group<F32>(q, i0 + u * 2048, a.V, 0.f, qv[u]);
     }
-    float best = -INFINITY;
-    int idx = -1;
 #pragma unroll
     for (int u = 0; u < RACE_GROUPS; ++u)
 #pragma unroll
@@ -277,12 +284,8 @@ __device__ __forceinline__ unsigned long long race_best(const VerifyArgs& a, con
             if (q) w -= qv[u][k];
             else if (i == draft) w = 0.f;
             const float key = w * __builtin_amdgcn_rcpf(ev[u][k]);
-            if (w > 0.f && key > best) {                     // in the order of the indices: the lowest of equal ones stays
-                best = key;
-                idx = i;
-            }
-        }
-    return idx < 0 ? 0ull : key32(best, idx);
+            if (w > 0.f && key > best.key) best = {key, v[u][k], i};     // in the order of the indices: the lowest of equal
+        }                                                                // ones stays
 }
 
 // A request's outcome: tokens, counts and log-probabilities from its rows (rows below `taken` accepted, the token of row `taken`
@@ -298,24 +301,30 @@ __device__ __forceinline__ void verify_write(const VerifyArgs& a, int b, const R
     if (threadIdx.x == 0) a.counts[b] = taken + (drawn >= 0);
 }
 
-__device__ __forceinline__ unsigned long long block_max_key(unsigned long long k, unsigned long long* sh) {
-    k = wave_max_key(k);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = k;
+// The largest key of the workgroup, and its logit
+struct Winner {
+    unsigned long long key[4];
+    float logit;
+};
+__device__ __forceinline__ unsigned long long block_max_key(unsigned long long mine, float logit, Winner& sh) {
+    const unsigned long long k = wave_max_key(mine);
+    if ((threadIdx.x & 63) == 0) sh.key[threadIdx.x >> 6] = k;
     __syncthreads();
-    k = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
+    const unsigned long long all = max(max(sh.key[0], sh.key[1]), max(sh.key[2], sh.key[3]));
+    if (all && mine == all) sh.logit = logit;                // one thread: a key holds its index
     __syncthreads();
-    return k;
+    return all;
 }
 
-// The drafts' decisions and a request's race: a workgroup RACE entries of one request
+// The drafts' decisions and a request's race: a.races workgroups a request, each of which takes every a.races-th chunk
 template <int DT>
 __global__ __launch_bounds__(256) void verify_race_kernel(const VerifyArgs a) {
     extern __shared__ Row rows[];                            // [G + 1]
-    __shared__ unsigned long long sh[4];
+    __shared__ Winner sh;
     __shared__ int last;
     const int b = blockIdx.x / a.races, at = blockIdx.x % a.races;
     const int n = drafts_of(a, b);
-    const float temperature = a.temperature[b];
+    const float temperature = load_uniform(a.temperature + b);
     const bool greedy = is_greedy(temperature);
     if ((n < 0 || greedy) && at != 0) return;
     if (n < 0) {
@@ -323,51 +332,68 @@ __global__ __launch_bounds__(256) void verify_race_kernel(const VerifyArgs a) {
         return;
     }
     const float* e = a.race + b * a.race_stride;
-    const int i0 = at * RACE + (int)threadIdx.x * 8;
+    const int i0 = (int)threadIdx.x * 8;
     float ev[RACE_GROUPS][8];
-    if (!greedy)
+    const auto load_e = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < RACE_GROUPS; ++u) load_group<F32>(e, i0 + u * 2048, a.V, 1.f, ev[u]);
+        for (int u = 0; u < RACE_GROUPS; ++u) load_group<F32>(e, c * RACE + i0 + u * 2048, a.V, 1.f, ev[u]);
+    };
+    if (!greedy) load_e(at);
     const double inv_t = inv_temperature(temperature);
+    float hi, lo;
+    exponent_factor(inv_t, hi, lo);
     for (int j = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); j <= n; j += 4) {
-        const Row r = verify_row<DT>(a, b, j, n, greedy, inv_t);
+        const Row r = verify_row<DT>(a, b, j, n, greedy, inv_t, hi, lo);
         if ((threadIdx.x & 63) == 0) rows[j] = r;
     }
     __syncthreads();
+    const int32_t* drafts = a.drafts + (size_t)b * a.G;
     int taken = 0;
-    while (taken < n && (greedy ? rows[taken].token == a.drafts[(size_t)b * a.G + taken] : rows[taken].token >= 0)) ++taken;
+    while (taken < n && (greedy ? rows[taken].token == load_uniform(drafts + taken) : rows[taken].token >= 0)) ++taken;
+    taken = __builtin_amdgcn_readfirstlane(taken);
     const Row r = rows[taken];
     if (greedy || !distribution(r.z)) {                      // nothing to race for
         if (at == 0) verify_write(a, b, rows, taken, greedy ? r.token : -1, r.arg);
         return;
     }
-    const void* row = logits_row<DT>(a, (int64_t)a.first[b] + taken);
+    const void* row = logits_row<DT>(a, (int64_t)load_uniform(a.first + b) + taken);
     const float* q = a.probs && taken < n ? a.probs + b * a.probs_request + taken * a.probs_row : nullptr;
-    const int draft = taken < n ? a.drafts[(size_t)b * a.G + taken] : -1;
-    float hi, lo;
-    exponent_factor(inv_t, hi, lo);
+    const int draft = taken < n ? load_uniform(drafts + taken) : -1;
     const float rz = (float)(1.0 / r.z);
-    unsigned long long key = block_max_key(race_best<DT>(a, row, e, q, draft, r.m, hi, lo, rz, i0, ev), sh);
-    unsigned long long* keys = a.keys + (size_t)b * a.races;
+    Best best = {-INFINITY, 0.f, -1};
+    for (int c = at; c < a.chunks; c += a.races) {
+        if (c != at) load_e(c);
+        race_best<DT>(a, row, q, draft, r.m, hi, lo, rz, c * RACE + i0, ev, best);
+    }
+    unsigned long long key = block_max_key(best.idx < 0 ? 0ull : key32(best.key, best.idx), best.logit, sh);
     if (a.races > 1) {
-        if (threadIdx.x == 0) store_dev(keys + at, key);
+        const size_t to = (size_t)b * a.races;
+        if (threadIdx.x == 0) {
+            store_dev(a.winners + to + at, sh.logit);
+            store_dev(a.keys + to + at, key);
+        }
         if (!arrive_last(a.arrived + (size_t)b * CNT_STRIDE, a.races, &last)) return;
         key = 0;
-        for (int i = threadIdx.x; i < a.races; i += 256) key = max(key, load_dev(keys + i));
-        key = block_max_key(key, sh);
+        float logit = 0.f;
+        for (int i = threadIdx.x; i < a.races; i += 256) {
+            const unsigned long long k = load_dev(a.keys + to + i);
+            const float l = load_dev(a.winners + to + i);
+            if (k > key) {
+                key = k;
+                logit = l;
+            }
+        }
+        key = block_max_key(key, logit, sh);
     }
     if (!key && taken < n) {                                 // q covers p (or the draft was all of it): p itself, rarely
-        for (int k = 0; k < a.races; ++k) {
-            const int i1 = k * RACE + (int)threadIdx.x * 8;
-#pragma unroll
-            for (int u = 0; u < RACE_GROUPS; ++u) load_group<F32>(e, i1 + u * 2048, a.V, 1.f, ev[u]);
-            key = max(key, race_best<DT>(a, row, e, nullptr, -1, r.m, hi, lo, rz, i1, ev));
+        for (int c = 0; c < a.chunks; ++c) {
+            load_e(c);
+            race_best<DT>(a, row, nullptr, -1, r.m, hi, lo, rz, c * RACE + i0, ev, best);
         }
-        key = block_max_key(key, sh);
+        key = block_max_key(best.idx < 0 ? 0ull : key32(best.key, best.idx), best.logit, sh);
     }
-    const int token = key ? (int)~(uint32_t)key : -1;        // -1: every random number of the row is unusable
-    verify_write(a, b, rows, taken, token,
-                 token < 0 ? 0.0 : ((double)load_elem(row, DT, (size_t)token) - (double)r.m) * inv_t);
+    // no key: every random number of the row is unusable
+    verify_write(a, b, rows, taken, key ? (int)~(uint32_t)key : -1, ((double)sh.logit - (double)r.m) * inv_t);
 }
 
 template <int DT>
@@ -384,12 +410,24 @@ int verify_launch(const VerifyArgs& a, hipStream_t st) {
 // ======================================================================================================================
 using namespace esp;
 
+// A request's race is shared by as many workgroups as it has chunks of entries, but 1280 over all requests (five a CU, what
+// fits at once): each of them decides the drafts first, which takes longer than a chunk. The launch of 128 requests
+// of 151936 fp32 logits, 5 drafts and draft probabilities: 51.5 us with 38 workgroups a request, 49.5 with 19, 48.5 with 10
+constexpr int64_t VERIFY_RACES = 1280;
+
 struct VerifySizes {
-    int64_t pieces, races, part, best, arrived, bytes;       // byte offsets behind the keys
-    VerifySizes(int64_t B, int64_t G, int64_t V)
-        : pieces((V + PIECE - 1) / PIECE), races((V + RACE - 1) / RACE), part(B * races * 8),
-          best(part + B * (G + 1) * pieces * (int64_t)sizeof(Piece)), arrived(best + B * (G + 1) * pieces * 4),
-          bytes(arrived + B * CNT_STRIDE * 4) {}
+    int64_t pieces, chunks, races, winners, part, best, arrived, bytes;       // byte offsets behind the keys
+    VerifySizes(int64_t B, int64_t G, int64_t V) {
+        pieces = (V + PIECE - 1) / PIECE;
+        chunks = (V + RACE - 1) / RACE;
+        const int64_t loops = std::max<int64_t>(1, (B * chunks + VERIFY_RACES - 1) / VERIFY_RACES);
+        races = (chunks + loops - 1) / loops;
+        winners = B * races * 8;
+        part = winners + (B * races * 4 + 7) / 8 * 8;
+        best = part + B * (G + 1) * pieces * (int64_t)sizeof(Piece);
+        arrived = best + B * (G + 1) * pieces * 4;
+        bytes = arrived + B * CNT_STRIDE * 4;
+    }
 };
 
 extern "C" int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V) {
@@ -424,6 +462,7 @@ extern "C" int esp_verify(const void* logits, int dtype, int64_t stride, int64_t
     a.G = (int)G;
     a.pieces = (int)z.pieces;
     a.races = (int)z.races;
+    a.chunks = (int)z.chunks;
     a.first = first;
     a.n_drafts = n_drafts;
     a.drafts = drafts;
@@ -439,6 +478,7 @@ extern "C" int esp_verify(const void* logits, int dtype, int64_t stride, int64_t
     a.logprobs = logprobs;
     char* base = static_cast<char*>(scratch);
     a.keys = reinterpret_cast<unsigned long long*>(base);
+    a.winners = reinterpret_cast<float*>(base + z.winners);
     a.part = reinterpret_cast<Piece*>(base + z.part);
     a.best = reinterpret_cast<int*>(base + z.best);
     a.arrived = reinterpret_cast<int*>(base + z.arrived);
