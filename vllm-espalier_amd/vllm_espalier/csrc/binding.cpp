@@ -736,6 +736,10 @@ void argmax(const at::Tensor& logits, at::Tensor ids, std::optional<at::Tensor> 
 static void on_device(const at::Tensor& t, const at::Tensor& first, const char* name) {
     TORCH_CHECK(t.device() == first.device(), name, ": expected a tensor on ", first.device());
 }
+template <typename... Ts>
+static void all_on_device(const char* name, const at::Tensor& first, const Ts&... ts) {
+    (on_device(ts, first, name), ...);
+}
 
 // esp_sandwich_rmsnorm (csrc/sandwich.hip): gate [T, D], [D] (every row's) or [T, 1] (a row's), or none
 void sandwich_rmsnorm(const at::Tensor& h, const at::Tensor& d1, const c10::optional<at::Tensor>& d2,
@@ -795,7 +799,7 @@ void lora(const at::Tensor& x, const at::Tensor& y, at::Tensor out, const at::Te
     check(ranks, at::kInt, "ranks");
     check(scales, at::kFloat, "scales");
     check(rows, at::kInt, "rows");
-    for (const at::Tensor& v : {y, out, rows, a, b, ranks, scales}) on_device(v, x, "lora");
+    all_on_device("lora", x, y, out, rows, a, b, ranks, scales);
     // the layouts of include/espalier.h
     TORCH_CHECK(a.dim() == 7 && a.size(1) == S && a.size(3) == (K + 31) / 32 && a.size(4) == 4 && a.size(5) == 16 &&
                     a.size(6) == 8, "a: [slots, matrices, R / 16, ceil(K / 32), 4, 16, 8]");
@@ -809,8 +813,8 @@ void lora(const at::Tensor& x, const at::Tensor& y, at::Tensor out, const at::Te
                     b.size(4) == 2 && b.size(5) == 16 && b.size(6) == 8, "b: [slots, column tiles, R / 16, 8, 2, 16, 8]");
     TORCH_CHECK(ranks.numel() == slots * S && scales.numel() == slots * S, "ranks / scales: [slots, matrices]");
     TORCH_CHECK(rows.numel() == T, "rows: [T]");
-    for (const at::Tensor& v : {y, out})
-        TORCH_CHECK(v.scalar_type() == t && v.dim() == 2 && v.size(0) == T && v.size(1) >= N && v.stride(1) == 1,
+    for (const at::Tensor* v : {&y, static_cast<const at::Tensor*>(&out)})
+        TORCH_CHECK(v->scalar_type() == t && v->dim() == 2 && v->size(0) == T && v->size(1) >= N && v->stride(1) == 1,
                     "y / out: [T, at least N columns], x's dtype, unit column stride");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     const int64_t numel = esp_lora_scratch(T, N, S, R);
@@ -836,8 +840,7 @@ void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor&
     check(tokens, at::kInt, "tokens");
     check(counts, at::kInt, "counts");
     check(logprobs, at::kFloat, "logprobs");
-    for (const at::Tensor& v : {first, n_drafts, drafts, uniform, race, temperature, tokens, counts, logprobs})
-        on_device(v, logits, "verify");
+    all_on_device("verify", logits, first, n_drafts, drafts, uniform, race, temperature, tokens, counts, logprobs);
     TORCH_CHECK(drafts.dim() == 2, "drafts: [B, G]");
     const int64_t B = drafts.size(0), G = drafts.size(1), V = logits.size(1);
     TORCH_CHECK(first.numel() == B && n_drafts.numel() == B && temperature.numel() == B && counts.numel() == B,

@@ -73,6 +73,12 @@ __device__ __forceinline__ void store8(uint16_t* p, uint4 v) {
     *reinterpret_cast<u32x4_a8*>(p) = u32x4_a8{v.x, v.y, v.z, v.w};
 }
 
+// past the L2's present contents: 42 MB of a prompt's outputs pushed out what its other workgroups read again (the expanding
+// launch of 4096 rows through 2048 -> 5120 25.9 -> 21.8 us, the one before it 22.4 -> 20.6)
+__device__ __forceinline__ void store8_nt(uint16_t* p, uint4 v) {
+    __builtin_nontemporal_store(u32x4_a8{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_a8*>(p));
+}
+
 // a value that every lane of the wave reads, through the scalar cache (nothing writes it while the kernel runs)
 template <typename T>
 __device__ __forceinline__ T load_uniform(const T* p) {
@@ -195,132 +201,147 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// The first product, many rows: 16 rows against all of an adapter's ranks, LORA_BATCH tiles of 16 at a time; sixteen waves, a run
-// of the k each. t leaves finished and split. x comes in once a CU, 256 bytes of a row at a time, and turns into operands through
-// the wave's own 4 KiB of shared memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a
-// quarter-wave meet in a bank either way). The next tiles' A is in flight while a batch is multiplied and summed over the waves.
+// The first product, many rows: 16 G rows against an adapter's rank tiles (G = 1: all of them, two a round; G = 2: every other
+// one, blockIdx.y), sixteen waves, a run of the k each; blockIdx.z: a row tile's first, third, ... adapter or the others. t leaves
+// finished and split. x comes in once, 256 bytes of a row at a time, and turns into operands through the wave's own 4 KiB of shared
+// memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a quarter-wave meet in a bank either
+// way). The next round's A is in flight while a round is multiplied and summed over the waves. 4096 rows of 2048 against 48 and
+// 192 ranks: 22 us, of which 1.4 until a workgroup knows its adapter and ranks, 5.6 for the first 320 KiB, then 1.4 a round; the
+// second adapter of a tile adds its 6 at the end.
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int LORA_BATCH = 2;
-constexpr int LORA_ALL_SMEM = LORA_RUNS * (4096 + 2 * LORA_BATCH * 1024);
+constexpr int LORA_ALL_SMEM = LORA_RUNS * (4096 + 2 * 2 * 1024);
 
-template <int DT>
+template <int DT, int G>
 __global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a) {
+    constexpr int B = 2 / G;                                 // rank tiles a round
     extern __shared__ uint4 xs[];                            // [LORA_RUNS][256], then the sums of two rounds
-    typedef f32x4 Sums[LORA_RUNS][LORA_BATCH][64];
+    typedef f32x4 Sums[LORA_RUNS][2][64];                    // of a round's B tiles and G row groups
     Sums* part = reinterpret_cast<Sums*>(xs + LORA_RUNS * 256);
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 16, rt = a.R / 16;   // blockIdx.y: every other adapter
+    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 16 * G, rt = a.R / 16, half = blockIdx.y;
     const int units = (a.K + 31) / 32, run = (units + LORA_RUNS - 1) / LORA_RUNS, chunks = (run + 3) / 4;
     const int u0 = wave * run, u1 = min(units, u0 + run);
     const uint32_t lane16 = lane * 16u;
     const char* xb = reinterpret_cast<const char*>(a.x + row0 * a.x_stride);
-    uint32_t xrow[4];                                        // bytes to rows g, 4 + g, 8 + g, 12 + g
+    uint32_t xrow[G][4];                                     // bytes to rows g, 4 + g, 8 + g, 12 + g of a group
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xrow[i] = (uint32_t)(min(4 * i + g, a.T - 1 - row0) * (int)a.x_stride) * 2u;
+    for (int q = 0; q < G; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xrow[q][i] = (uint32_t)(min(16 * q + 4 * i + g, a.T - 1 - row0) * (int)a.x_stride) * 2u;
     uint4* own = xs + 256 * wave;
-    TileAdapters<1> tile(a, row0);
+    TileAdapters<G> tile(a, row0);
     int round = 0;
     for (int nth = 0; tile.rest; ++nth) {
         uint64_t mask;
         const int who = tile.next(mask);
-        if ((nth & 1) != (int)blockIdx.y) continue;
-        int end[LORA_MAX_SHARDS], total = 0;                 // the matrices' rank tiles, one after the other
+        if ((nth & 1) != (int)blockIdx.z) continue;
+        // the adapter's rank tiles, matrix after matrix, a lane each: the tile's place among the layer's S * R / 16, its ranks
+        // that the adapter has and its scale
+        const int sl = min(lane, a.S - 1);
+        const int rank_of = min(max(a.ranks[(int64_t)who * a.S + sl], 0), a.R);
+        const float scale_of = a.scales[(int64_t)who * a.S + sl];
+        int total = 0, place = 0, ranks = 0;
+        float scale = 0.f;
 #pragma unroll
-        for (int s = 0; s < LORA_MAX_SHARDS; ++s) {
-            if (s < a.S) total += (max(lora_rank(a, who, s), 0) + 15) / 16;
-            end[s] = total;
-        }
-        if (total == 0) continue;
-        // the place among the layer's S * R / 16 of the adapter's tile i (past the last one: that one)
-        const auto place = [&](int i) __attribute__((always_inline)) {
-            i = min(i, total - 1);
-            int s = 0, first = 0;
-#pragma unroll
-            for (int k = 0; k < LORA_MAX_SHARDS - 1; ++k)
-                if (i >= end[k]) {
-                    s = k + 1;
-                    first = end[k];
+        for (int s = 0; s < LORA_MAX_SHARDS; ++s)
+            if (s < a.S) {
+                const int r = __builtin_amdgcn_readlane(rank_of, s);
+                if (lane >= total) {
+                    place = s * rt + lane - total;
+                    ranks = r - 16 * (lane - total);
+                    scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale_of), s));
                 }
-            return s * rt + i - first;
-        };
+                total += (r + 15) / 16;
+            }
+        if (half >= total) continue;
         const char* ab = reinterpret_cast<const char*>(a.a + (int64_t)who * a.S * rt * units * 64);
-        const auto load_a = [&](int i0, int c, uint4(&p)[LORA_BATCH][4]) __attribute__((always_inline)) {
+        const auto load_a = [&](int i0, int c, uint4(&p)[B][4]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < LORA_BATCH; ++j) {
-                const char* ap = ab + (int64_t)place(i0 + j) * units * 1024;
+            for (int j = 0; j < B; ++j) {                    // past the last one: that one again, and not used
+                const char* ap = ab + (int64_t)__builtin_amdgcn_readlane(place, min(i0 + j * G, total - 1)) * (units * 1024);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     p[j][i] = *reinterpret_cast<const uint4*>(ap + (int64_t)min(u0 + 4 * c + i, u1 - 1) * 1024 + lane16);
             }
         };
-        uint4 x[4], p[LORA_BATCH][4];
-        load_a(0, 0, p);
+        uint4 x[G][4], p[B][4];
+        load_a(half, 0, p);
 #pragma unroll 1
-        for (int i0 = 0; i0 < total; i0 += LORA_BATCH) {
-            f32x4 acc[LORA_BATCH];
+        for (int i0 = half; i0 < total; i0 += 2) {
+            f32x4 acc[B][G];
 #pragma unroll
-            for (int j = 0; j < LORA_BATCH; ++j) acc[j] = {0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < B; ++j)
+#pragma unroll
+                for (int q = 0; q < G; ++q) acc[j][q] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
             for (int c = 0; c < chunks; ++c) {
                 const int u = u0 + 4 * c;
-                const bool fresh = chunks > 1 || i0 == 0;    // a single chunk's operands stay in registers
+                const bool fresh = chunks > 1 || i0 == half; // a single chunk's operands stay in registers
                 if (fresh)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {            // row 4 i + g, k 32 u + 8 m .. + 8
-                        const int k = 32 * u + 8 * m;        // (of a row that is not the adapter's too: its t is not kept)
-                        x[i] = load8(reinterpret_cast<const uint16_t*>(xb + (xrow[i] + (uint32_t)min(k, a.K - 8) * 2u)));
-                        if (k >= a.K) x[i] = make_uint4(0u, 0u, 0u, 0u);
-                    }
+                    for (int q = 0; q < G; ++q)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {        // row 4 i + g of group q, k 32 u + 8 m .. + 8
+                            const int k = 32 * u + 8 * m;    // (of a row that is not the adapter's too: its t is not kept)
+                            x[q][i] = load8(reinterpret_cast<const uint16_t*>(xb + (xrow[q][i] + (uint32_t)min(k, a.K - 8) * 2u)));
+                            if (k >= a.K) x[q][i] = make_uint4(0u, 0u, 0u, 0u);
+                        }
                 const bool more = c + 1 < chunks;
-                uint4 next[LORA_BATCH][4];
-                load_a(more ? i0 : i0 + LORA_BATCH, more ? c + 1 : 0, next);
+                uint4 next[B][4];
+                load_a(more ? i0 : i0 + 2, more ? c + 1 : 0, next);
                 __builtin_amdgcn_sched_barrier(0);           // every load before the first use
-                if (fresh) {
+                if (fresh)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) own[(4 * i + g) * 16 + (m ^ (4 * i + g))] = x[i];
-                    __builtin_amdgcn_wave_barrier();
+                    for (int q = 0; q < G; ++q) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = own[m * 16 + ((4 * i + g) ^ m)];
-                    __builtin_amdgcn_wave_barrier();
-                }
+                        for (int i = 0; i < 4; ++i) own[(4 * i + g) * 16 + (m ^ (4 * i + g))] = x[q][i];
+                        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[q][i] = own[m * 16 + ((4 * i + g) ^ m)];
+                        __builtin_amdgcn_wave_barrier();
+                    }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (u + i < u1)
 #pragma unroll
-                        for (int j = 0; j < LORA_BATCH; ++j) acc[j] = mfma32<DT>(p[j][i], x[i], acc[j]);
+                        for (int j = 0; j < B; ++j)
 #pragma unroll
-                for (int j = 0; j < LORA_BATCH; ++j)
+                            for (int q = 0; q < G; ++q) acc[j][q] = mfma32<DT>(p[j][i], x[q][i], acc[j][q]);
+#pragma unroll
+                for (int j = 0; j < B; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) p[j][i] = next[j][i];
             }
-            const int n = min(total - i0, LORA_BATCH), j = (wave - LORA_BATCH * round) & (LORA_RUNS - 1);
+            // two waves finish a round's two sums, other waves the next one's
+            const int w = (wave - 2 * round) & (LORA_RUNS - 1), i = i0 + (G == 1 ? w : 0), q = G == 1 ? 0 : w;
             Sums& sums = part[round++ & 1];
 #pragma unroll
-            for (int k = 0; k < LORA_BATCH; ++k) sums[wave][k][lane] = acc[k];
+            for (int j = 0; j < 2; ++j) sums[wave][j][lane] = G == 1 ? acc[j % B][0] : acc[0][j % G];
             lds_barrier();                                   // (the next tiles' loads stay in flight; the sums before the last
                                                              // ones are read: the waves that do came to this barrier after it)
-            if (j < n) {                                     // a wave a tile, other waves for the next ones
-                const int to = place(i0 + j), s = to / rt, left = lora_rank(a, who, s) - 16 * (to % rt) - 4 * g;
+            if (w < 2 && i < total) {
+                const bool mine = (mask >> (16 * q + m)) & 1;
+                const int left = __builtin_amdgcn_readlane(ranks, i) - 4 * g;
                 f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int z = 0; z < LORA_RUNS; z += 4)
-                    sum += ((sums[z][j][lane] + sums[z + 1][j][lane]) + sums[z + 2][j][lane]) + sums[z + 3][j][lane];
-                sum *= load_uniform(a.scales + (int64_t)who * a.S + s);
+                    sum += ((sums[z][w][lane] + sums[z + 1][w][lane]) + sums[z + 2][w][lane]) + sums[z + 3][w][lane];
+                sum *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), i));
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i >= left) sum[i] = 0.f;             // ranks that the adapter does not have
-                const int64_t tile_to = (int64_t)tile_at * a.S * rt + to;
+                for (int k = 0; k < 4; ++k)
+                    if (k >= left) sum[k] = 0.f;             // ranks that the adapter does not have
+                const int64_t tile_to = ((int64_t)tile_at * G + q) * a.S * rt + __builtin_amdgcn_readlane(place, i);
                 if constexpr (DT == F16) {
                     float top = fmaxf(fmaxf(fabsf(sum[0]), fabsf(sum[1])), fmaxf(fabsf(sum[2]), fabsf(sum[3])));
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
                     const int e = lora_exponent(top);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[i] = ldexpf(sum[i], -e);
-                    if (g == 0 && ((mask >> m) & 1)) a.e[tile_to * 16 + m] = e;
+                    for (int k = 0; k < 4; ++k) sum[k] = ldexpf(sum[k], -e);
+                    if (g == 0 && mine) a.e[tile_to * 16 + m] = e;
                 }
-                if ((mask >> m) & 1) {                       // ranks 4 g .. + 4 of row m
+                if (mine) {                                  // ranks 4 g .. + 4 of row m
                     uint2 hi, lo;
                     split4<DT>(sum, hi, lo);
                     uint2* t = reinterpret_cast<uint2*>(a.t + tile_to * 64) + 2 * (16 * (g >> 1) + m) + (g & 1);
@@ -474,7 +495,7 @@ constexpr int LORA_HELD = 4;                   // rank tiles of B in shared memo
 
 // Many rows: a workgroup of 64 rows (16 a wave) and 128 columns, an adapter's B for them in shared memory
 template <int DT>
-__global__ __launch_bounds__(256) void lora_expand_all_kernel(const LoraArgs a) {
+__global__ __launch_bounds__(256, DT == BF16 ? 4 : 3) void lora_expand_all_kernel(const LoraArgs a) {
     __shared__ uint4 bs[LORA_HELD][256];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -535,14 +556,14 @@ __global__ __launch_bounds__(256) void lora_expand_all_kernel(const LoraArgs a) 
         for (int i = 0; i < 4; ++i)
             if (in && ((rows >> (4 * g + i)) & 1)) {
                 const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
-                store8(op + (4 * g + i) * a.out_stride, lora_add8<DT>(y[i], add));
+                store8_nt(op + (4 * g + i) * a.out_stride, lora_add8<DT>(y[i], add));
             }
     }
     if (a.out != a.y) {                                      // rows of no adapter: y as it is
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 16 * wave + 4 * g + i;
-            if (in && !((some >> row) & 1) && row0 + row < a.T) store8(op + (4 * g + i) * a.out_stride, y[i]);
+            if (in && !((some >> row) & 1) && row0 + row < a.T) store8_nt(op + (4 * g + i) * a.out_stride, y[i]);
         }
     }
 }
@@ -551,10 +572,14 @@ template <int DT>
 int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
     const unsigned tiles = (unsigned)((a.T + 15) / 16), cols = (unsigned)a.tiles0[a.S];
     if (all) {
-        if (hipFuncSetAttribute((const void*)lora_shrink_all_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                LORA_ALL_SMEM) != hipSuccess)
+        // 32 rows and half of the rank tiles a workgroup take in less than 16 rows and all, where x is taken in once (K up to
+        // 2048) or few tiles follow: 2048 -> 4096 + 512 + 512, ranks 16 and 64, 4096 rows 38.6 -> 35.9 us in all, 4096 -> 2048,
+        // ranks up to 64, 28.9 -> 24.5; 4096 -> 4096, rank 128, 8192 rows 101 -> 133
+        const unsigned group = a.K <= 2048 || a.S * (a.R / 16) <= 4 ? 2 : 1;
+        const auto shrink = group == 1 ? lora_shrink_all_kernel<DT, 1> : lora_shrink_all_kernel<DT, 2>;
+        if (hipFuncSetAttribute((const void*)shrink, hipFuncAttributeMaxDynamicSharedMemorySize, LORA_ALL_SMEM) != hipSuccess)
             return esp_host::fail(ESP_ERR_HIP, "lora: no %d bytes of shared memory", LORA_ALL_SMEM);
-        lora_shrink_all_kernel<DT><<<dim3(tiles, 2), 1024, LORA_ALL_SMEM, st>>>(a);
+        shrink<<<dim3((tiles + group - 1) / group, group, 2), 1024, LORA_ALL_SMEM, st>>>(a);
         lora_expand_all_kernel<DT><<<dim3((tiles + 3) / 4, cols), 256, 0, st>>>(a);
     } else {
         const unsigned x = tiles * a.spread, ranks = (unsigned)((a.R / 16 + LORA_FEW - 1) / LORA_FEW);
