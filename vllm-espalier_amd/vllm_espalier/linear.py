@@ -12,6 +12,8 @@ How a layer is held here:
     shards' EspMatrix objects in vLLM's output order, their tensors as non-persistent buffers (a compiled graph then
     takes them as inputs rather than constants), and the output padding (a vocabulary padded past the matrix).
     Each shard keeps its own suh / svh, so the matrices are never concatenated into one trellis.
+  * attach_adapters gives layer.espalier a store of low-rank adapters (adapters.Adapters); apply then adds each row's own
+    when it is told the rows' slots.
   * apply runs layer.espalier: with DENSE the whole layer is one espalier::dense call (one esp_dense launch for all
     its matrices up to 32 rows, more rows as ESPALIER_PREFILL_MODE says); without it each matrix goes through
     espalier::matmul and the outputs are joined.
@@ -92,6 +94,7 @@ class TrellisLinear(torch.nn.Module):
             self.register_buffer(f"trellis_{i}", m.trellis, persistent=False)
             self.register_buffer(f"suh_{i}", m.suh, persistent=False)
             self.register_buffer(f"svh_{i}", m.svh, persistent=False)
+        self.adapters = None
         self.dense_key = None
         if fused and mats and all(m.in_features % 128 == 0 and m.out_features % 128 == 0 for m in mats):
             from . import dense, ops
@@ -102,7 +105,28 @@ class TrellisLinear(torch.nn.Module):
     def tensors(self, name: str) -> list[torch.Tensor]:
         return [getattr(self, f"{name}_{i}") for i in range(len(self.mats))]
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def attach_adapters(self, slots: int, max_rank: int, dtype=torch.bfloat16):
+        """A store of low-rank adapters for this layer (adapters.Adapters, to load into), which forward adds to the rows that
+        name its slots. dtype: that of the rows."""
+        from .adapters import Adapters
+        if not self.mats:
+            raise RuntimeError("this layer has no matrices to put adapters beside")
+        self.adapters = Adapters(self.mats[0].in_features, [m.out_features for m in self.mats], slots, max_rank, dtype,
+                                 self.mats[0].trellis.device)
+        return self.adapters
+
+    def forward(self, x: torch.Tensor, adapter_rows: torch.Tensor | None = None) -> torch.Tensor:
+        """adapter_rows: int32, the slot of every row of x (attach_adapters), outside [0, slots) for a row without one."""
+        y = self._base(x)
+        if adapter_rows is not None:
+            if self.adapters is None:
+                raise RuntimeError("rows name adapters, but none were attached to this layer")
+            s = self.adapters
+            torch.ops.espalier.add_adapters(y.view(-1, self.out_features), x.reshape(-1, x.shape[-1]), adapter_rows.reshape(-1),
+                                            s.a, s.b, s.ranks, s.scales, s.out_features)
+        return y
+
+    def _base(self, x: torch.Tensor) -> torch.Tensor:
         from . import ops  # noqa: F401  (registers the espalier::* ops)
         if not self.mats:
             raise RuntimeError("this layer's matrices were never loaded (a drafter's head, replaced by the target's)")
@@ -151,6 +175,7 @@ class EspLinearMethod(_Base):
                                f"the layer ({k_in} in, {n_out} out)")
         layer.espalier = TrellisLinear(mats, n_out, fused=DENSE)
 
-    def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
-        y = layer.espalier(x)
+    def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None = None,
+              adapter_rows: torch.Tensor | None = None) -> torch.Tensor:
+        y = layer.espalier(x) if adapter_rows is None else layer.espalier(x, adapter_rows)
         return y if bias is None else y + bias

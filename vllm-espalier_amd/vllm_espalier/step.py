@@ -23,6 +23,14 @@ MoE after the routing is one chained launch too (experts.routed2: esp_moe_chain)
 
 Rows never interact (the dense and grouped kernels keep rows apart, norms are per row), so a window of T rows
 gives each row the bits it gets alone.
+
+Three things of a served model can stand in the step, off by default:
+  * use_adapters(slots, max_rank): low-rank adapters beside qkv and o, each row's own (Buffers.rows names their slots);
+  * post_norms=True: every block's output has a norm of its own before it joins the residual (sandwich_rmsnorm instead of
+    add_rmsnorm);
+  * verify(b, ...): the rows of a pass are requests' last tokens and their drafts, verified against the logits
+    (speculative.verify).
+With the first two the launches run apart (qkv's adapters stand between qkv and o); rows stay independent.
 """
 from __future__ import annotations
 
@@ -32,7 +40,9 @@ import torch
 
 from . import dense as Dn
 from . import experts as G
+from . import speculative
 from . import workloads as WL
+from .adapters import Adapters
 from .experts import ext
 
 D_MODEL = 2048
@@ -57,6 +67,15 @@ class DecoderLayer:
     moe: G.Layer
     experts: list                # [(gate, up, down) EspMatrix] routed, in id order
     shared: tuple                # the shared expert's (gate, up, down)
+    post_in: torch.Tensor | None = None      # the norms behind the previous layer's MoE and behind this layer's o
+    post_o: torch.Tensor | None = None
+    qkv_adapters: Adapters | None = None
+    o_adapters: Adapters | None = None
+
+    @property
+    def plain(self) -> bool:
+        """Whether the layer runs in the launches that hold several of its steps."""
+        return self.post_o is None and self.qkv_adapters is None
 
 
 def _norm_weight(gen, dev, D):
@@ -92,6 +111,7 @@ class Buffers:
         self.T = T
         self.ids_in = torch.zeros((T,), dtype=torch.int32, device=dev)
         self.ids_out = torch.zeros((T,), dtype=torch.int32, device=dev)
+        self.rows = torch.full((T,), -1, dtype=torch.int32, device=dev)       # every row's adapter slot (use_adapters)
         self.h = torch.zeros((T, D), dtype=bf, device=dev)
         self.h2 = torch.zeros((T, D), dtype=bf, device=dev)      # the residual between the qkv and routing launches
         self.a = torch.zeros((T, D), dtype=bf, device=dev)
@@ -106,7 +126,7 @@ class Buffers:
 
 class SyntheticDecoder:
     def __init__(self, n_layers: int = 40, seed: int = 5, device="cuda", E: int = 256, vocab: int = VOCAB,
-                 head_bits: int = 6):
+                 head_bits: int = 6, post_norms: bool = False):
         dev = torch.device(device)
         gen = torch.Generator(device=dev).manual_seed(seed)
         self.dev, self.vocab, self.E = dev, vocab, E
@@ -116,6 +136,31 @@ class SyntheticDecoder:
         self.head = Dn.Dense([WL.matrix(D_MODEL, vocab, head_bits, "mcg", gen, dev)])
         self.scratch = G.scratch(self.layers[0].moe, Dn.MAX_ROWS, TOPK + 1, dev)
         self._bufs: dict[int, Buffers] = {}
+        self.final_post = None
+        if post_norms:                            # drawn apart, so that the other weights stay what they are
+            post = torch.Generator(device=dev).manual_seed(seed + 1)
+            weights = [_norm_weight(post, dev, D_MODEL) for _ in range(2 * n_layers)]
+            for i, L in enumerate(self.layers):
+                L.post_in, L.post_o = weights[2 * i - 1] if i else None, weights[2 * i]
+            self.final_post = weights[-1]
+
+    def use_adapters(self, slots: int, max_rank: int) -> None:
+        """Low-rank adapters beside every layer's qkv and o (DecoderLayer.qkv_adapters, o_adapters, to load into)."""
+        for L in self.layers:
+            L.qkv_adapters = Adapters(D_MODEL, [Q_OUT, KV_OUT, KV_OUT], slots, max_rank, device=self.dev)
+            L.o_adapters = Adapters(Q_OUT, [D_MODEL], slots, max_rank, device=self.dev)
+
+    def verify(self, b: Buffers, first, n_drafts, drafts, uniform, race, temperature, draft_probs=None, out=None):
+        """The drafts of the requests whose rows a pass over b ran, against its logits (speculative.verify)."""
+        return speculative.verify(b.logits, first, n_drafts, drafts, uniform, race, temperature, draft_probs, out)
+
+    def _join(self, b: Buffers, d1, d2, post, w) -> None:
+        """A block's outputs d1 (+ d2) into the residual b.h, through the block's own norm if it has one; b.a = the next
+        block's input."""
+        if post is None:
+            ext().add_rmsnorm(b.h, d1, d2, w, b.a, EPS)
+        else:
+            ext().sandwich_rmsnorm(b.h, d1, d2, post, None, False, 1.0, w, EPS, b.h, b.a)
 
     def buffers(self, T: int) -> Buffers:
         if T not in self._bufs:
@@ -126,10 +171,10 @@ class SyntheticDecoder:
 
     def fused_norms(self, T: int) -> bool:
         """Whether the layers' norms run inside the qkv and routing launches for T rows."""
-        return FUSE_NORMS and T <= 4 and self.layers[0].qkv.norm_fusable(T)
+        return FUSE_NORMS and T <= 4 and self.layers[0].plain and self.layers[0].qkv.norm_fusable(T)
 
     def fused_head_norm(self, T: int) -> bool:
-        return FUSE_NORMS and self.head.norm_fusable(T)
+        return FUSE_NORMS and self.final_post is None and self.head.norm_fusable(T)
 
     def layer_forward(self, L: DecoderLayer, b: Buffers, first: bool, picks: list | None = None):
         e = ext()
@@ -143,13 +188,16 @@ class SyntheticDecoder:
                 L.o.forward(q, out=b.o)
             G.route_rmsnorm(b.h2, b.o, L.norm2, EPS, b.h, b.a, L.router, TOPK, L.moe, self.scratch)
         else:
-            e.add_rmsnorm(b.h, d1, d2, L.norm1, b.a, EPS)
-            if MULTI_ATTN:
+            self._join(b, d1, d2, L.post_in, L.norm1)
+            if L.qkv_adapters is not None:
+                L.qkv_adapters.apply(b.a, L.qkv.forward(b.a, out=b.qkv), b.rows)
+                L.o_adapters.apply(q, L.o.forward(q, out=b.o), b.rows)
+            elif MULTI_ATTN:
                 L.attn.forward([b.a, q], [b.qkv, b.o])
             else:
                 L.qkv.forward(b.a, out=b.qkv)
                 L.o.forward(q, out=b.o)
-            e.add_rmsnorm(b.h, b.o, None, L.norm2, b.a, EPS)
+            self._join(b, b.o, None, L.post_o, L.norm2)
             G.route(b.a, L.router, TOPK, L.moe, self.scratch)
         if picks is not None:                     # eager runs only: the distinct experts this layer reads
             n = int(self.scratch.count.item())
@@ -167,7 +215,7 @@ class SyntheticDecoder:
             if self.fused_head_norm(T):
                 self.head.forward_rmsnorm(b.h, b.moe, b.moe_shared, self.final_norm, EPS, b.h2, out=b.logits)
             else:
-                e.add_rmsnorm(b.h, b.moe, b.moe_shared, self.final_norm, b.a, EPS)
+                self._join(b, b.moe, b.moe_shared, self.final_post, self.final_norm)
                 self.head.forward(b.a, out=b.logits)
             e.argmax(b.logits, b.ids_out, b.argmax_part, b.argmax_cnt)
         return b
@@ -188,12 +236,16 @@ class SyntheticDecoder:
     def prefill_layer(self, L: DecoderLayer, b: Buffers, first: bool, ps: G.PrefillScratch):
         """One layer of prefill over the rows of b: the dense layers as prompt launches, the MoE over the whole prompt
         (its picks left in ps.pick, slots a row)."""
-        e = ext()
         d1, d2 = (None, None) if first else (b.moe, b.moe_shared)
-        e.add_rmsnorm(b.h, d1, d2, L.norm1, b.a, EPS)
+        q = b.qkv[:, :Q_OUT]
+        self._join(b, d1, d2, L.post_in, L.norm1)
         L.qkv.forward_tile(b.a, out=b.qkv)
-        L.o.forward_tile(b.qkv[:, :Q_OUT], out=b.o)
-        e.add_rmsnorm(b.h, b.o, None, L.norm2, b.a, EPS)
+        if L.qkv_adapters is not None:
+            L.qkv_adapters.apply(b.a, b.qkv, b.rows)
+        L.o.forward_tile(q, out=b.o)
+        if L.o_adapters is not None:
+            L.o_adapters.apply(q, b.o, b.rows)
+        self._join(b, b.o, None, L.post_o, L.norm2)
         G.prefill(b.a, None, None, L.moe, ps, TOPK, gate=L.router, out=b.moe, out_shared=b.moe_shared)
 
     def prefill(self, T: int, head_rows: int = 1) -> Buffers:
@@ -209,7 +261,7 @@ class SyntheticDecoder:
         self.head.reserve_prompt(head_rows)
         for i, L in enumerate(self.layers):
             self.prefill_layer(L, b, i == 0, ps)
-        e.add_rmsnorm(b.h, b.moe, b.moe_shared, self.final_norm, b.a, EPS)
+        self._join(b, b.moe, b.moe_shared, self.final_post, self.final_norm)
         tail = slice(T - head_rows, T)
         self.head.forward_tile(b.a[tail], out=b.logits[tail])
         e.argmax(b.logits[tail], b.ids_out[tail])
