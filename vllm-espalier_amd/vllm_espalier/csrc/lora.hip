@@ -14,8 +14,8 @@
 // k (16 ranks of each), so nothing of it is lost but the rest's own rounding (2^-17 for bf16). fp16's narrow range is kept out of
 // it: 16 ranks of a row are first scaled by a power of two to below 1, and their products scaled back.
 //
-// The order of t's sum is fixed: K in 16 runs of whole 32-k units, a run in its units' order, the runs four by four and the four
-// fours in order; so a row's bits depend on that row and its adapter alone.
+// The order of t's sum is fixed: K in 16 runs of whole 32-k units, a run in its units' order, the runs four by four in order, and
+// of the four fours the first two and the last two; so a row's bits depend on that row and its adapter alone.
 #include "../../../include/espalier.h"
 #include "common.hpp"
 #include "norm.hpp"
@@ -323,10 +323,12 @@ __global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a)
             if (w < 2 && i < total) {
                 const bool mine = (mask >> (16 * q + m)) & 1;
                 const int left = __builtin_amdgcn_readlane(ranks, i) - 4 * g;
-                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+                f32x4 four[4];
 #pragma unroll
-                for (int z = 0; z < LORA_RUNS; z += 4)
-                    sum += ((sums[z][w][lane] + sums[z + 1][w][lane]) + sums[z + 2][w][lane]) + sums[z + 3][w][lane];
+                for (int z = 0; z < 4; ++z)
+                    four[z] = ((sums[4 * z][w][lane] + sums[4 * z + 1][w][lane]) + sums[4 * z + 2][w][lane]) +
+                              sums[4 * z + 3][w][lane];
+                f32x4 sum = (four[0] + four[1]) + (four[2] + four[3]);
                 sum *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), i));
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
@@ -392,21 +394,24 @@ struct LoraCols {
     }
 };
 
-// This lane's operand of a rank tile of t from lora_shrink_kernel's four sums (of row `at` of the layer's row tiles): 8 ranks of
-// 16, the high parts (lanes below 32) or the rests; e: fp16's exponents of rows 4 (lane / 16) .. + 4
+// v of the lanes below 32 plus v of those 32 above, in all of them
+__device__ __forceinline__ float add_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// This lane's operand of a rank tile of t from lora_shrink_kernel's four sums, of which the lanes below 32 hold the first two and
+// those above the last two: 8 ranks of 16, the high parts (lanes below 32) or the rests; e: fp16's exponents of rows
+// 4 (lane / 16) .. + 4
 template <int DT>
-__device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[4][2], float scale, int left, int (&e)[4]) {
+__device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[2][2], float scale, int left, int (&e)[4]) {
     const int lane = threadIdx.x & 63;
     f32x4 v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        v[h] = {0.f, 0.f, 0.f, 0.f};
+        v[h] = p[0][h] + p[1][h];
 #pragma unroll
-        for (int z = 0; z < 4; ++z) v[h] += p[z][h];
-        v[h] *= scale;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (4 * h + i >= left) v[h][i] = 0.f;
+        for (int i = 0; i < 4; ++i) v[h][i] = 4 * h + i < left ? add_halves(v[h][i]) * scale : 0.f;
     }
     if constexpr (DT == F16) {
         float top = 0.f;
@@ -451,7 +456,7 @@ __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
         const int mr = (mask >> m) & 1 ? m : __builtin_ctzll(mask);
         const uint32_t own = (uint32_t)mask >> (4 * g);      // this lane's rows 4 g .. + 4
         const uint4* bp = a.b + ((int64_t)who * a.tiles0[a.S] + ct) * rt * 256 + (lane & 31);
-        const float* pp = a.part + (((int64_t)tile_at * a.S + col.s) * rt * 16 + mr) * 16 + 8 * (g & 1);
+        const float* pp = a.part + 2 * (g >> 1) * z_at + (((int64_t)tile_at * a.S + col.s) * rt * 16 + mr) * 16 + 8 * (g & 1);
         uint4 y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -461,7 +466,7 @@ __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
         for (int c = 0; c < 8; ++c) acc[c] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int j0 = 0; 16 * j0 < r; j0 += LORA_FEW) {
-            f32x4 p[LORA_FEW][4][2];
+            f32x4 p[LORA_FEW][2][2];
             uint4 b[LORA_FEW][8];
 #pragma unroll
             for (int j = 0; j < LORA_FEW; ++j)
@@ -469,7 +474,7 @@ __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c) b[j][c] = bp[(j0 + j) * 256 + 32 * c];
 #pragma unroll
-                    for (int z = 0; z < 4; ++z)
+                    for (int z = 0; z < 2; ++z)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
                             p[j][z][h] = *reinterpret_cast<const f32x4*>(pp + z * z_at + (j0 + j) * 256 + 4 * h);
@@ -606,10 +611,13 @@ static bool lora_many(int64_t T, int64_t N) { return T * N >= 3 << 20 || T >= 15
 // The workgroups that a row tile's adapters are dealt to (few rows): up to one a row, and no more than 32 over all tiles, since
 // one that finds nothing costs 2 ns too (a tile of one adapter leaves the others empty). 2048 -> 4096 + 512 + 512, ranks 16 and 64
 // of 32 adapters in random rows, 16 / 32 / 64 workgroups: 16 / 13 / 13 us for 32 rows, 64 / 45 / 51 for 256; in 3 runs of rows
-// 9.8 / 11.3 / 11.3 and 13.0 / 13.2 / 18.5
-static int lora_spread(int64_t T) {
+// 9.8 / 11.3 / 11.3 and 13.0 / 13.2 / 18.5. Two even so where the second product has few columns (1280 of its waves), so that a
+// prompt's tiles of two requests do not take twice as long: 512 rows in 3 runs, one and two: 4096 -> 2048 11.0 and 8.8 us,
+// 2048 -> 512 + 512 10.3 and 8.7; 2048 -> 4096 + 512 + 512 11.7 and 13.8
+static int lora_spread(int64_t T, int64_t cols) {
     const int64_t tiles = (T + 15) / 16;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({16, T, 32 / tiles}));
+    const int64_t spread = std::max<int64_t>(32 / tiles, 2 * tiles * cols <= 1280 ? 2 : 1);
+    return (int)std::min<int64_t>({16, T, spread});
 }
 
 extern "C" int64_t esp_lora_scratch(int64_t T, int64_t N, int64_t n_shards, int64_t R) {
@@ -675,7 +683,7 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
     a.N = (int)N;
     a.R = (int)R;
     a.slots = (int)slots;
-    a.spread = lora_spread(T);
+    a.spread = lora_spread(T, a.tiles0[n_shards]);
     const hipStream_t st = (hipStream_t)stream;
     return dtype == ESP_BF16 ? lora_launch<BF16>(a, all, st) : lora_launch<F16>(a, all, st);
 }
