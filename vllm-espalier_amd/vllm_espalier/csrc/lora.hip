@@ -2,7 +2,7 @@
 //   out[m, n] = y[m, n] + sum_{j < r} t[m, j] B[a][n][j],   t[m, j] = scale[a][s] * sum_k x[m, k] A[a][s][j][k]
 // for row m of adapter a = rows[m] and column n of the layer's matrix s (r = ranks[a][s]); rows of no adapter keep y.
 //
-// Two launches: the rows' products with A, then those with B and the sum. Both take tiles of 16 consecutive rows and, inside a
+// Two launches: the rows' products with A, then those with B and the sum; one for a few rows and ranks. All take tiles of 16 consecutive rows and, inside a
 // tile, one adapter after the other (the tile's distinct ones, found by ballots): the rows are one side of a matrix instruction,
 // so each row keeps what its own adapter made of it and no sorting or grouping launch is needed, whatever the order of the rows.
 // Where a batch is small its distinct adapters are spread over workgroups.
@@ -400,19 +400,15 @@ __device__ __forceinline__ float add_halves(float v) {
     return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
-// This lane's operand of a rank tile of t from lora_shrink_kernel's four sums, of which the lanes below 32 hold the first two and
-// those above the last two: 8 ranks of 16, the high parts (lanes below 32) or the rests; e: fp16's exponents of rows
-// 4 (lane / 16) .. + 4
+// This lane's operand of a rank tile of t: 8 ranks v of 16 of row lane % 16, the high parts (lanes below 32) or the rests; e: fp16's
+// exponents of rows 4 (lane / 16) .. + 4
 template <int DT>
-__device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[2][2], float scale, int left, int (&e)[4]) {
+__device__ __forceinline__ uint4 lora_operand(f32x4 (&v)[2], float scale, int left, int (&e)[4]) {
     const int lane = threadIdx.x & 63;
-    f32x4 v[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        v[h] = p[0][h] + p[1][h];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[h][i] = 4 * h + i < left ? add_halves(v[h][i]) * scale : 0.f;
-    }
+        for (int i = 0; i < 4; ++i) v[h][i] = 4 * h + i < left ? v[h][i] * scale : 0.f;
     if constexpr (DT == F16) {
         float top = 0.f;
 #pragma unroll
@@ -429,6 +425,19 @@ __device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[2][2], float scale, in
     split4<DT>(v[0], hi[0], lo[0]);
     split4<DT>(v[1], hi[1], lo[1]);
     return lane >= 32 ? make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y) : make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+}
+
+// lora_operand from lora_shrink_kernel's four sums, of which the lanes below 32 hold the first two and those above the last two
+template <int DT>
+__device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[2][2], float scale, int left, int (&e)[4]) {
+    f32x4 v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        v[h] = p[0][h] + p[1][h];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[h][i] = add_halves(v[h][i]);
+    }
+    return lora_operand<DT>(v, scale, left, e);
 }
 
 // Few rows: a wave 128 columns of a row tile (and, spread, its adapters)
@@ -493,6 +502,112 @@ __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
                 const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
                 store8(op + i * a.out_stride, lora_add8<DT>(y[i], add));
             }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Both products in one launch, for a few rows and ranks: sixteen waves make t of a row tile and adapter (blockIdx.x), a run of the
+// k each, and four of them go on to 128 columns of one matrix each (blockIdx.y). Every workgroup makes its t itself: at 16 ranks of
+// 2048 it takes in 64 KiB of A, which costs less than a launch more and the way through memory.
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int LORA_ONE_TILES = 2;              // rank tiles
+
+template <int DT>
+__global__ __launch_bounds__(1024) void lora_one_kernel(const LoraArgs a) {
+    __shared__ f32x4 part[LORA_ONE_TILES][LORA_RUNS][64];
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, rt = a.R / 16;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    int s = 0, c0 = 0, block = blockIdx.y, tiles;            // the matrix, its first column, and four of its column tiles
+    while (block >= ((tiles = a.tiles0[s + 1] - a.tiles0[s]) + 3) / 4) {
+        block -= (tiles + 3) / 4;
+        c0 += a.n_cols[s++];
+    }
+    const int ct = 4 * block + wave, n0 = ct * LORA_COLS;
+    const bool expands = wave < 4 && ct < tiles, in = expands && n0 + 8 * m < a.n_cols[s];
+    const uint16_t* yp = a.y + 4 * g * a.y_stride + c0 + n0 + 8 * m;
+    uint16_t* op = a.out + 4 * g * a.out_stride + c0 + n0 + 8 * m;
+    uint4 y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (in && 4 * g + i < a.T) y[i] = load8(yp + i * a.y_stride);
+    TileAdapters<1> tile(a, 0);
+    if (blockIdx.x == 0 && a.out != a.y) {                   // rows of no adapter: y as it is
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (in && !((tile.rest >> (4 * g + i)) & 1) && 4 * g + i < a.T) store8(op + i * a.out_stride, y[i]);
+    }
+    const int units = (a.K + 31) / 32, run = (units + LORA_RUNS - 1) / LORA_RUNS;
+    const int u0 = wave * run, u1 = min(units, u0 + run);
+    for (int nth = 0; tile.rest; ++nth) {
+        uint64_t mask;
+        const int who = tile.next(mask);
+        if (nth != (int)blockIdx.x) continue;
+        const int r = lora_rank(a, who, s), nt = (r + 15) / 16;
+        const float scale = load_uniform(a.scales + (int64_t)who * a.S + s);
+        const uint4* bp = a.b + ((int64_t)who * a.tiles0[a.S] + a.tiles0[s] + ct) * rt * 256 + (lane & 31);
+        uint4 b[LORA_ONE_TILES][8];
+        if (expands)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) b[0][c] = bp[32 * c];
+        const int mr = (mask >> m) & 1 ? m : __builtin_ctzll(mask);     // rows of others: the first of this one's
+        const uint16_t* xp = a.x + (int64_t)mr * a.x_stride + 8 * g;
+        const char* ab = reinterpret_cast<const char*>(a.a + ((int64_t)who * a.S + s) * rt * units * 64);
+        f32x4 sum[LORA_ONE_TILES];
+#pragma unroll
+        for (int j = 0; j < LORA_ONE_TILES; ++j) sum[j] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int u = u0; u < u1; u += 4) {
+            uint4 x[4], p[LORA_ONE_TILES][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                    // units past the run's: its last one again, and not used
+                const int v = min(u + i, u1 - 1);
+#pragma unroll
+                for (int j = 0; j < LORA_ONE_TILES; ++j)
+                    if (j == 0 || j < nt) p[j][i] = *reinterpret_cast<const uint4*>(ab + ((int64_t)j * units + v) * 1024 + lane * 16u);
+                x[i] = load8(xp + min(32 * v, a.K - 8 - 8 * g));
+                if (32 * v + 8 * g >= a.K) x[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int j = 0; j < LORA_ONE_TILES; ++j)
+                if (j < nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (u + i < u1) sum[j] = mfma32<DT>(p[j][i], x[i], sum[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < LORA_ONE_TILES; ++j) part[j][wave][lane] = sum[j];
+        if (expands && nt > 1)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) b[1][c] = bp[256 + 32 * c];
+        lds_barrier();
+        if (!expands) return;                                // (a workgroup has one adapter)
+        f32x4 acc[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < LORA_ONE_TILES; ++j)
+            if (j < nt) {
+                f32x4 v[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {                // ranks 8 (g % 2) + 4 h .. + 4 of row m
+                    const f32x4* from = &part[j][0][(2 * (g & 1) + h) * 16 + m];
+                    f32x4 four[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                        four[z] = ((from[256 * z] + from[256 * z + 64]) + from[256 * z + 128]) + from[256 * z + 192];
+                    v[h] = (four[0] + four[1]) + (four[2] + four[3]);
+                }
+                int e[4];
+                const uint4 t = lora_operand<DT>(v, scale, r - 16 * j - 8 * (g & 1), e);
+                lora_rank_tile<DT>(t, e, b[j], acc);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (in && ((mask >> (4 * g + i)) & 1)) {
+                const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
+                store8(op + i * a.out_stride, lora_add8<DT>(y[i], add));
+            }
+        return;
     }
 }
 
@@ -573,6 +688,21 @@ __global__ __launch_bounds__(256, DT == BF16 ? 4 : 3) void lora_expand_all_kerne
     }
 }
 
+// The one launch's workgroups a row tile and adapter
+static int lora_one_blocks(const LoraArgs& a) {
+    int blocks = 0;
+    for (int s = 0; s < a.S; ++s) blocks += (a.tiles0[s + 1] - a.tiles0[s] + 3) / 4;
+    return blocks;
+}
+
+// Whether both products run in one launch: one row tile, at most 64 Ki elements of A a matrix, which every workgroup takes in, and
+// no more workgroups than CUs. us in two launches / in one, one row: 2048 -> 4096 + 512 + 512, rank 16 6.2 / 4.6, rank 32 6.6 / 5.9;
+// 4096 -> 2048 6.5 / 5.3 and 6.9 / 7.1; 8192 -> 8192, rank 16 7.5 / 7.3; 2048 -> 50048, rank 16, two and four rows 6.4 / 4.8 and
+// 7.0 / 8.5
+static bool lora_one(const LoraArgs& a) {
+    return a.T <= 16 && a.R <= 16 * LORA_ONE_TILES && (int64_t)a.R * a.K <= 1 << 16 && a.T * lora_one_blocks(a) <= 256;
+}
+
 template <int DT>
 int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
     const unsigned tiles = (unsigned)((a.T + 15) / 16), cols = (unsigned)a.tiles0[a.S];
@@ -586,6 +716,8 @@ int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
             return esp_host::fail(ESP_ERR_HIP, "lora: no %d bytes of shared memory", LORA_ALL_SMEM);
         shrink<<<dim3((tiles + group - 1) / group, group, 2), 1024, LORA_ALL_SMEM, st>>>(a);
         lora_expand_all_kernel<DT><<<dim3((tiles + 3) / 4, cols), 256, 0, st>>>(a);
+    } else if (lora_one(a)) {
+        lora_one_kernel<DT><<<dim3(a.T, lora_one_blocks(a)), 1024, 0, st>>>(a);
     } else {
         const unsigned x = tiles * a.spread, ranks = (unsigned)((a.R / 16 + LORA_FEW - 1) / LORA_FEW);
         lora_shrink_kernel<DT><<<dim3(x, a.S * ranks, LORA_RUNS / 4), 256, 0, st>>>(a);
