@@ -71,13 +71,15 @@ __device__ __forceinline__ void load_group(const void* row, int i, int V, float 
                 v[2 * k + 1] = from16((uint16_t)(u[k] >> 16), DT == BF16);
             }
         }
-    } else {
-#pragma unroll 1
-        for (int k = 0; k < 8; ++k) {
-            const float f = i + k < V ? load_elem(row, DT, (size_t)(i + k)) : past;
+    } else {                                                 // eight loads at once here too, and none wholly past the end
 #pragma unroll
-            for (int l = 0; l < 8; ++l)
-                if (l == k) v[l] = f;
+        for (int k = 0; k < 8; ++k) v[k] = past;
+        if (i < V) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = load_elem(row, DT, (size_t)min(i + k, V - 1));
+                if (i + k < V) v[k] = f;
+            }
         }
     }
 }
