@@ -824,10 +824,11 @@ void lora(const at::Tensor& x, const at::Tensor& y, at::Tensor out, const at::Te
                   dtype_code(x), mptr<float>(scratch), numel, cur_stream()));
 }
 
-// esp_verify (csrc/verify.hip): drafted tokens [B, G] against the target's logits
-void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor& n_drafts, const at::Tensor& drafts,
-            const at::Tensor& uniform, const at::Tensor& race, const at::Tensor& temperature,
-            const c10::optional<at::Tensor>& probs, at::Tensor tokens, at::Tensor counts, at::Tensor logprobs) {
+// esp_verify (csrc/verify.hip): drafted tokens [B, G] against the target's logits; (tokens, counts, logprobs), `out`'s own if given
+std::tuple<at::Tensor, at::Tensor, at::Tensor> verify(
+    const at::Tensor& logits, const at::Tensor& first, const at::Tensor& n_drafts, const at::Tensor& drafts,
+    const at::Tensor& uniform, const at::Tensor& race, const at::Tensor& temperature, const c10::optional<at::Tensor>& probs,
+    const c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>>& out) {
     TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
                 "logits: [R, V], unit column stride");
     const auto t = logits.scalar_type();
@@ -837,19 +838,13 @@ void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor&
     check(drafts, at::kInt, "drafts");
     check(uniform, at::kFloat, "uniform");
     check(temperature, at::kFloat, "temperature");
-    check(tokens, at::kInt, "tokens");
-    check(counts, at::kInt, "counts");
-    check(logprobs, at::kFloat, "logprobs");
-    all_on_device("verify", logits, first, n_drafts, drafts, uniform, race, temperature, tokens, counts, logprobs);
+    all_on_device("verify", logits, first, n_drafts, drafts, uniform, race, temperature);
     TORCH_CHECK(drafts.dim() == 2, "drafts: [B, G]");
     const int64_t B = drafts.size(0), G = drafts.size(1), V = logits.size(1);
-    TORCH_CHECK(first.numel() == B && n_drafts.numel() == B && temperature.numel() == B && counts.numel() == B,
-                "first / n_drafts / temperature / counts: [B]");
+    TORCH_CHECK(first.numel() == B && n_drafts.numel() == B && temperature.numel() == B, "first / n_drafts / temperature: [B]");
     TORCH_CHECK(uniform.sizes() == drafts.sizes(), "uniform: [B, G]");
     TORCH_CHECK(race.is_cuda() && race.scalar_type() == at::kFloat && race.dim() == 2 && race.size(0) == B &&
                     race.size(1) == V && (V <= 1 || race.stride(1) == 1), "race: fp32 [B, V], unit column stride");
-    TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == G + 1 && logprobs.sizes() == tokens.sizes(),
-                "tokens / logprobs: [B, G + 1]");
     if (probs.has_value()) {
         on_device(*probs, logits, "probs");
         TORCH_CHECK(probs->is_cuda() && probs->scalar_type() == at::kFloat && probs->dim() == 3 && probs->size(0) == B &&
@@ -857,6 +852,20 @@ void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor&
                     "probs: fp32 [B, G, V], unit column stride");
     }
     c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+    at::Tensor tokens, counts, logprobs;
+    if (out.has_value()) {
+        std::tie(tokens, counts, logprobs) = *out;
+        check(tokens, at::kInt, "tokens");
+        check(counts, at::kInt, "counts");
+        check(logprobs, at::kFloat, "logprobs");
+        all_on_device("verify", logits, tokens, counts, logprobs);
+        TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == G + 1 && logprobs.sizes() == tokens.sizes() &&
+                        counts.numel() == B, "tokens / logprobs: [B, G + 1]; counts: [B]");
+    } else {
+        tokens = at::empty({B, G + 1}, drafts.options());
+        counts = at::empty({B}, drafts.options());
+        logprobs = at::empty({B, G + 1}, uniform.options());
+    }
     const int64_t bytes = esp_verify_scratch(B, G, V);
     const at::Tensor scratch = at::empty({bytes}, logits.options().dtype(at::kByte));
     call(esp_verify(logits.data_ptr(), dtype_code(logits), logits.stride(0), logits.size(0), V, cptr<int32_t>(first),
@@ -865,6 +874,7 @@ void verify(const at::Tensor& logits, const at::Tensor& first, const at::Tensor&
                     probs.has_value() ? probs->stride(0) : 0, probs.has_value() ? probs->stride(1) : 0,
                     mptr<int32_t>(tokens), mptr<int32_t>(counts), mptr<float>(logprobs), scratch.data_ptr(), bytes,
                     cur_stream()));
+    return {tokens, counts, logprobs};
 }
 
 // several dense launches as one (esp_dense_multi; no reference counterpart): per group its input rows, matrices,

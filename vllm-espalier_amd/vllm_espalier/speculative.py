@@ -3,8 +3,6 @@ rows of a batch are a request's last token and its drafts (an MTP drafter's or a
 """
 from __future__ import annotations
 
-import torch
-
 from .experts import ext
 
 
@@ -24,10 +22,4 @@ def verify(logits, first, n_drafts, drafts, uniform, race, temperature, draft_pr
     out          (tokens, counts, logprobs) to write into; otherwise new ones
 
     With fixed arrays a captured graph replays it; nothing is kept between calls, so calls on several streams do not meet."""
-    if out is None:
-        B, G = drafts.shape
-        out = (torch.empty((B, G + 1), dtype=torch.int32, device=logits.device),
-               torch.empty((B,), dtype=torch.int32, device=logits.device),
-               torch.empty((B, G + 1), dtype=torch.float32, device=logits.device))
-    ext().verify(logits, first, n_drafts, drafts, uniform, race, temperature, draft_probs, *out)
-    return out
+    return ext().verify(logits, first, n_drafts, drafts, uniform, race, temperature, draft_probs, out)
