@@ -181,6 +181,69 @@ def test_lora_fp16_range(dev, size):
     _check(store.apply(x, y, rows.to(dev), out=torch.empty_like(y)), x, y, rows, a, b, scales, outs, dtype)
 
 
+@pytest.mark.parametrize("T,ranks", [(3, [8, 8]), (20, [8, 40]), (1600, [16, 64])])
+def test_lora_untouched_bits(dev, T, ranks):
+    """Matrices without ranks, cleared slots and rows without adapters: y's bits, zeros of both signs and NaN among them, in place
+    and not; the other matrix of the same adapter as ever."""
+    gen = torch.Generator().manual_seed(19)
+    K, outs, dtype = 128, [48, 80], torch.bfloat16
+    store, a, b, scales = _store(K, outs, ranks, dtype, gen, dev, skip={(0, 1)})
+    store.clear(1)
+    x = torch.randn((T, K), generator=gen).to(dtype).to(dev)
+    y = torch.randn((T, 128), generator=gen).to(dtype)
+    y[:, ::3] = -0.0
+    y[:, 60] = float("nan")
+    y = y.to(dev)
+    rows = torch.tensor([0, 1, -1] * -(-T // 3), dtype=torch.int32)[:T]
+    for out in (torch.zeros_like(y), y.clone()):
+        got = store.apply(x, y if out.any() == 0 else out, rows.to(dev), out=out)
+        assert torch.equal(got[:, 48:].view(torch.int16), y[:, 48:].view(torch.int16))
+        bare = rows != 0
+        assert torch.equal(got[bare.to(dev)].view(torch.int16), y[bare.to(dev)].view(torch.int16))
+        _check(got[:, :48], x, y[:, :48], torch.where(rows == 0, 0, -1), [a[0][:1]], [b[0][:1]], scales, outs[:1], dtype)
+
+
+def test_lora_prompt_in_a_graph(dev):
+    """The launches for many rows captured, and replayed with other rows and inputs."""
+    gen = torch.Generator().manual_seed(23)
+    K, outs, T = 256, [256, 128], 1700
+    store, a, b, scales = _store(K, outs, [16, 70], torch.bfloat16, gen, dev)
+    x = torch.randn((T, K), generator=gen).to(torch.bfloat16).to(dev)
+    y = torch.randn((T, 384), generator=gen).to(torch.bfloat16).to(dev)
+    rows, out = torch.zeros((T,), dtype=torch.int32, device=dev), torch.empty_like(y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        store.apply(x, y, rows, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        store.apply(x, y, rows, out=out)
+    for k in range(3):
+        rows.copy_(_rows(T, 2, gen, mixed=k == 1))
+        x.copy_(torch.randn((T, K), generator=gen).to(torch.bfloat16))
+        out.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        eager = store.apply(x, y, rows, out=torch.empty_like(y))
+        assert torch.equal(eager.view(torch.int16), out.view(torch.int16)), k
+    _check(out, x, y, rows.cpu(), a, b, scales, outs, torch.bfloat16)
+
+
+def test_lora_long_rows_and_many_columns(dev):
+    """Long K with few and many rows (x in several parts a run), and more columns than the one launch takes."""
+    gen = torch.Generator().manual_seed(27)
+    for K, outs, ranks, T in ((10256, [64], [16, 33], 9), (10256, [64], [16, 33], 1590), (64, [40000], [16], 16), (6160, [128], [4], 16)):
+        print(f"lora {K} -> {outs}, {T} rows", flush=True)
+        store, a, b, scales = _store(K, outs, ranks, torch.bfloat16, gen, dev)
+        x = torch.randn((T, K), generator=gen).to(torch.bfloat16).to(dev)
+        y = torch.randn((T, sum(outs)), generator=gen).to(torch.bfloat16).to(dev)
+        rows = _rows(T, len(ranks), gen)
+        out = store.apply(x, y, rows.to(dev), out=torch.empty_like(y))
+        some = torch.arange(0, T, max(1, T // 40))
+        _check(out[some], x[some], y[some], rows[some], a, b, scales, outs, torch.bfloat16)
+
+
 def test_lora_beside_dense_in_a_graph(dev):
     """As it is used: a trellis layer, then its adapters in place, captured once and replayed while the rows' adapters change
     and a slot is loaded anew; every replay equals the eager calls."""
@@ -236,6 +299,16 @@ def test_lora_two_streams(dev):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(w.view(torch.int16), o.view(torch.int16)) for o in g)
+
+
+def test_lora_loaded_from_views(dev):
+    """Adapters given as transposed views, in another dtype and on the CPU or the device, in tiles that need no padding."""
+    gen = torch.Generator().manual_seed(33)
+    store = Adapters(64, [128], slots=2, max_rank=16, device=dev)
+    a, b = torch.randn((64, 16), generator=gen), torch.randn((16, 128), generator=gen)
+    store.load(0, [a.t()], [b.t()])
+    store.load(1, [a.to(dev).t().contiguous().to(torch.bfloat16)], [b.to(dev).t()])
+    assert torch.equal(store.a[0], store.a[1]) and torch.equal(store.b[0], store.b[1]) and store.b.any()
 
 
 def test_lora_empty_and_refusals(dev, ext):

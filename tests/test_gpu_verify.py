@@ -146,6 +146,13 @@ def test_verify_batches(dev, B, G, probs):
     _check(i, _call(i, dev), few=0.2)
 
 
+def test_verify_many_requests(dev):
+    """More chunks of entries than workgroups race: a workgroup several of them."""
+    gen = torch.Generator().manual_seed(2)
+    i = _inputs(700, 1, 9001, torch.bfloat16, True, gen, greedy_every=5)
+    _check(i, _call(i, dev), few=0.02)
+
+
 def test_verify_large_vocabulary(dev):
     gen = torch.Generator().manual_seed(1)
     i = _inputs(3, 3, 151936, torch.bfloat16, True, gen, ragged=False)

@@ -27,13 +27,13 @@ def _padded(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
 def pack_a(low: torch.Tensor) -> torch.Tensor:
     """A [rank, in] as esp_lora reads it: [rank tiles, k units, 4, 16, 8]."""
     t = _padded(low, RANK_TILE, K_UNIT)
-    return t.view(-1, RANK_TILE, t.shape[1] // K_UNIT, 4, 8).permute(0, 2, 3, 1, 4)
+    return t.reshape(-1, RANK_TILE, t.shape[1] // K_UNIT, 4, 8).permute(0, 2, 3, 1, 4)
 
 
 def pack_b(high: torch.Tensor) -> torch.Tensor:
     """B [out, rank] as esp_lora reads it: [column tiles, rank tiles, 8, 2, 16, 8]."""
     t = _padded(high, COLUMN_TILE, RANK_TILE)
-    return t.view(-1, 16, 8, t.shape[1] // RANK_TILE, 2, 8).permute(0, 3, 2, 4, 1, 5)
+    return t.reshape(-1, 16, 8, t.shape[1] // RANK_TILE, 2, 8).permute(0, 3, 2, 4, 1, 5)
 
 
 class Adapters:

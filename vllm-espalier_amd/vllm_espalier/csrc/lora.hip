@@ -358,7 +358,7 @@ __global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a)
 // ------------------------------------------------------------------------------------------------------------------
 // The second product
 // ------------------------------------------------------------------------------------------------------------------
-// 8 columns of a row: y's, with what the adapter adds
+// 8 columns of a row: y's, with what the adapter adds (only where it has ranks: y + 0 is not y's bits for -0 and NaN)
 template <int DT>
 __device__ __forceinline__ uint4 lora_add8(uint4 y, const float (&add)[8]) {
     const uint32_t w[4] = {y.x, y.y, y.z, y.w};
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
         for (int i = 0; i < 4; ++i)
             if (in && ((own >> i) & 1)) {
                 const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
-                store8(op + i * a.out_stride, lora_add8<DT>(y[i], add));
+                store8(op + i * a.out_stride, r > 0 ? lora_add8<DT>(y[i], add) : y[i]);
             }
     }
 }
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(1024) void lora_one_kernel(const LoraArgs a) {
         for (int i = 0; i < 4; ++i)
             if (in && ((mask >> (4 * g + i)) & 1)) {
                 const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
-                store8(op + i * a.out_stride, lora_add8<DT>(y[i], add));
+                store8(op + i * a.out_stride, r > 0 ? lora_add8<DT>(y[i], add) : y[i]);
             }
         return;
     }
@@ -676,7 +676,7 @@ __global__ __launch_bounds__(256, DT == BF16 ? 4 : 3) void lora_expand_all_kerne
         for (int i = 0; i < 4; ++i)
             if (in && ((rows >> (4 * g + i)) & 1)) {
                 const float add[8] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
-                store8_nt(op + (4 * g + i) * a.out_stride, lora_add8<DT>(y[i], add));
+                store8_nt(op + (4 * g + i) * a.out_stride, r > 0 ? lora_add8<DT>(y[i], add) : y[i]);
             }
     }
     if (a.out != a.y) {                                      // rows of no adapter: y as it is
