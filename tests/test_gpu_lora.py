@@ -244,6 +244,26 @@ def test_lora_long_rows_and_many_columns(dev):
         _check(out[some], x[some], y[some], rows[some], a, b, scales, outs, torch.bfloat16)
 
 
+@pytest.mark.parametrize("K", [16, 96, 1040, 2048, 2064, 4096, 4112, 8192, 8208])
+@pytest.mark.parametrize("ranks,dtype", [([5, 16], torch.bfloat16), ([96, 16, 40, 33, 81], torch.bfloat16),
+                                         ([96, 16, 40, 33, 81], torch.float16)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_lora_prompt_tiles(dev, K, ranks, dtype, mixed):
+    """A prompt's rows, in tiles of every height, have the bits that they have in short batches; some of them in 64 bits too."""
+    print(f"lora prompt tiles K={K} ranks={ranks} {dtype} mixed={mixed}", flush=True)
+    gen = torch.Generator().manual_seed(K)
+    T, outs = 1301, [32, 144, 16]
+    store, a, b, scales = _store(K, outs, ranks, dtype, gen, dev, skip={(1, 1)})
+    x = torch.randn((T, K), generator=gen).to(dtype).to(dev)
+    y = torch.randn((T, sum(outs)), generator=gen).to(dtype).to(dev)
+    rows = _rows(T, len(ranks), gen, mixed).to(dev)
+    got = store.apply(x, y, rows, out=torch.empty_like(y))
+    short = torch.cat([store.apply(x[t:t + 100], y[t:t + 100].clone(), rows[t:t + 100]) for t in range(0, T, 100)])
+    assert torch.equal(got.view(torch.int16), short.view(torch.int16))
+    some = torch.randperm(T, generator=gen)[:24].to(dev)
+    _check(got[some], x[some], y[some], rows[some], a, b, scales, outs, dtype)
+
+
 def test_lora_beside_dense_in_a_graph(dev):
     """As it is used: a trellis layer, then its adapters in place, captured once and replayed while the rows' adapters change
     and a slot is loaded anew; every replay equals the eager calls."""

@@ -2,10 +2,10 @@
 //   out[m, n] = y[m, n] + sum_{j < r} t[m, j] B[a][n][j],   t[m, j] = scale[a][s] * sum_k x[m, k] A[a][s][j][k]
 // for row m of adapter a = rows[m] and column n of the layer's matrix s (r = ranks[a][s]); rows of no adapter keep y.
 //
-// Two launches: the rows' products with A, then those with B and the sum; one for a few rows and ranks. All take tiles of 16 consecutive rows and, inside a
-// tile, one adapter after the other (the tile's distinct ones, found by ballots): the rows are one side of a matrix instruction,
-// so each row keeps what its own adapter made of it and no sorting or grouping launch is needed, whatever the order of the rows.
-// Where a batch is small its distinct adapters are spread over workgroups.
+// Two launches: the rows' products with A, then those with B and the sum; one for a few rows and ranks. All take tiles of 16 to 64
+// consecutive rows and, inside a tile, one adapter after the other (the tile's distinct ones, found by ballots): the rows are one
+// side of a matrix instruction, so each row keeps what its own adapter made of it and no sorting or grouping launch is needed,
+// whatever the order of the rows. Where a batch is small its distinct adapters are spread over workgroups.
 //
 // The adapters are laid out as the instructions read them (LoraArgs): a wave's load is one KiB in a row. The quarter of a wave
 // that a CU looks up at once then meets two lines; 16 rows of a plain matrix are 16 lines, and came in at 10 bytes a clock.
@@ -124,6 +124,17 @@ __device__ __forceinline__ void split4(const f32x4& v, uint2& hi, uint2& lo) {
     lo = make_uint2((uint32_t)l[0] | ((uint32_t)l[1] << 16), (uint32_t)l[2] | ((uint32_t)l[3] << 16));
 }
 
+// 16 bytes a lane of a KiB that starts where all lanes have it alike, its address in scalar registers
+__device__ __forceinline__ uint4 load_kib(const char* p, int lane) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32));
+    typedef const __attribute__((address_space(1))) char* global;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 r = *(const __attribute__((address_space(1))) u32x4*)((global)(uintptr_t)((hi << 32) | lo) + (uint32_t)(lane * 16));
+    return make_uint4(r.x, r.y, r.z, r.w);
+}
+
 // Row tile of workgroup `block` of n: workgroups go to the eight XCDs in turn, and each XCD takes a run of consecutive tiles, so
 // that the adapters of few requests pass through its L2
 __device__ __forceinline__ int xcd_tile(int block, int n) {
@@ -139,7 +150,8 @@ __device__ __forceinline__ int lora_exponent(float top) {
 // ------------------------------------------------------------------------------------------------------------------
 // The first product, few rows: the sums of runs 4 z .. 4 z + 3 for 16 rows and LORA_FEW tiles of 16 ranks, a wave a run, in fp32.
 // blockIdx.x the row tile and, spread, its adapters; blockIdx.y the matrix and rank tiles, blockIdx.z the runs: a batch's adapters
-// are read once and come in through many CUs.
+// are read once and come in through many CUs. Bound by its three dependent round trips (rows, ranks, operands): 32 rows of 24
+// adapters, ranks up to 64 of 4096, 5.2 us for 5.3 MB; 509 rows of 3 adapters of rank 32 of 2048 5.2 us.
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int LORA_FEW = 2;                    // rank tiles whose loads are all in flight at once
 
@@ -200,157 +212,274 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------------
-// The first product, many rows: 16 G rows against an adapter's rank tiles (G = 1: all of them, two a round; G = 2: every other
-// one, blockIdx.y), sixteen waves, a run of the k each; blockIdx.z: a row tile's first, third, ... adapter or the others. t leaves
-// finished and split. x comes in once, 256 bytes of a row at a time, and turns into operands through the wave's own 4 KiB of shared
-// memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a quarter-wave meet in a bank either
-// way). The next round's A is in flight while a round is multiplied and summed over the waves. 4096 rows of 2048 against 48 and
-// 192 ranks: 22 us, of which 1.4 until a workgroup knows its adapter and ranks, 5.6 for the first 320 KiB, then 1.4 a round; the
-// second adapter of a tile adds its 6 at the end.
-// ------------------------------------------------------------------------------------------------------------------
-constexpr int LORA_ALL_SMEM = LORA_RUNS * (4096 + 2 * 2 * 1024);
+// Many rows. An adapter's rank tiles, matrix after matrix, a lane each: the tile's place among the layer's S * R / 16, how many of its
+// ranks the adapter has, and their scale
+struct RankTiles {
+    int total, place, ranks;
+    float scale;
+    __device__ __forceinline__ RankTiles(const LoraArgs& a, int who) : total(0), place(0), ranks(0), scale(0.f) {
+        const int lane = threadIdx.x & 63, rt = a.R / 16;
+        int r[LORA_MAX_SHARDS];
+        float f[LORA_MAX_SHARDS];
+#pragma unroll
+        for (int s = 0; s < LORA_MAX_SHARDS; ++s) {
+            r[s] = load_uniform(a.ranks + (int64_t)who * a.S + min(s, a.S - 1));
+            f[s] = load_uniform(a.scales + (int64_t)who * a.S + min(s, a.S - 1));
+        }
+        asm volatile("" : "+s"(r[0]), "+s"(r[1]), "+s"(r[2]), "+s"(r[3]), "+s"(f[0]), "+s"(f[1]), "+s"(f[2]), "+s"(f[3]));
+#pragma unroll                                               // (all eight on their way before the first is waited for)
+        for (int s = 0; s < LORA_MAX_SHARDS; ++s)
+            if (s < a.S) {
+                const int n = min(max(r[s], 0), a.R);
+                if (lane >= total) {
+                    place = s * rt + lane - total;
+                    ranks = n - 16 * (lane - total);
+                    scale = f[s];
+                }
+                total += (n + 15) / 16;
+            }
+    }
+    __device__ __forceinline__ int place_of(int i) const { return __builtin_amdgcn_readlane(place, i); }
+    __device__ __forceinline__ int ranks_of(int i) const { return __builtin_amdgcn_readlane(ranks, i); }
+    __device__ __forceinline__ float scale_of(int i) const {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), i));
+    }
+};
 
-template <int DT, int G>
-__global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a) {
-    constexpr int B = 2 / G;                                 // rank tiles a round
+// The runs' sums of NS tiles of 16 ranks x 16 rows, as the matrix instruction leaves them but for the lanes' order, which keeps apart
+// in the banks what lora_sum reads at once: rank l % 16 of row m = 4 (wave % 4) + l / 16 of tile q = wave / 4, in every lane l
+template <int NS>
+using LoraSums = f32x4[LORA_RUNS][NS][64];
+__device__ __forceinline__ int sums_lane(int l) { return l ^ (l >> 4 << 2); }
+template <int NS>
+__device__ __forceinline__ float lora_sum(const LoraSums<NS>& sums, int q, int m, int l) {
+    const int g = (l >> 2) & 3;
+    const float* from = reinterpret_cast<const float*>(&sums[0][q][16 * g + (m ^ (4 * g))]) + (l & 3);
+    float v[LORA_RUNS], four[4];
+#pragma unroll
+    for (int z = 0; z < LORA_RUNS; ++z) v[z] = from[z * 256 * NS];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) four[z] = ((v[4 * z] + v[4 * z + 1]) + v[4 * z + 2]) + v[4 * z + 3];
+    return (four[0] + four[1]) + (four[2] + four[3]);
+}
+
+// That sum into t: scaled, none of the ranks past `left`, split
+template <int DT>
+__device__ __forceinline__ void lora_put(const LoraArgs& a, float sum, float scale, int left, int64_t tile_to, int m, int l, bool mine) {
+    sum *= scale;
+    if ((l & 15) >= left) sum = 0.f;
+    if constexpr (DT == F16) {
+        float top = fabsf(sum);                              // of the row's 16 lanes; a NaN is passed over
+        top = fmaxf(top, dpp_f32<0xB1>(top));
+        top = fmaxf(top, dpp_f32<0x4E>(top));
+        top = fmaxf(top, dpp_f32<0x141>(top));
+        top = fmaxf(top, dpp_f32<0x140>(top));
+        const int e = lora_exponent(top);
+        sum = ldexpf(sum, -e);
+        if ((l & 15) == 0 && mine) a.e[tile_to * 16 + m] = e;
+    }
+    const uint32_t hi = to16(sum, DT == BF16);
+    const float rest = sum - from16((uint16_t)hi, DT == BF16);
+    const uint32_t lo = to16(fabsf(rest) < INFINITY ? rest : 0.f, DT == BF16);
+    // even lanes store two ranks' high parts, odd ones the two rests
+    const uint32_t other = dpp_u32<0xB1>(l & 1 ? hi : lo, 0u);
+    const uint32_t two = l & 1 ? other | (lo << 16) : hi | (other << 16);
+    const int g = (l >> 2) & 3;
+    if (mine)
+        reinterpret_cast<uint32_t*>(a.t + tile_to * 64)[4 * (16 * (g >> 1) + m) + 2 * (g & 1) + ((l >> 1) & 1) + (l & 1) * 128] = two;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The first product, many rows, K up to 8192: 16 G rows against `per` of an adapter's rank tiles (blockIdx.x: the row tile and its
+// share of the rank tiles), sixteen waves, a run of the k each. t leaves finished and split. A workgroup has a CU to itself, whose
+// intake bounds it (~25 bytes a ns from memory, ~50 from the L2), so it takes x in once and keeps it in registers, G C = 4 KiB of it
+// a wave, whatever the ranks and adapters that follow, and the shares are as many as there are CUs for: 64 rows against 48 ranks of
+// 2048 are 452 KiB, where 32 rows against 96 were 520. x comes in 256 bytes of a row at a time and turns into operands through the
+// wave's own 4 KiB of shared memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a quarter-wave
+// meet in a bank either way). The next rank tile is in flight while one is multiplied and summed over the waves; the sums of a tile are
+// finished by all waves, a rank a lane (the same xor keeps its reads apart). 4096 rows of 2048 against 48 and 192 ranks: 16.4 us.
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int LORA_ALL_SMEM = 2 * LORA_RUNS * 4096;
+
+template <int DT, int G, int C>
+__global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a, int shares, int per) {
+    extern __shared__ uint4 xs[];                            // [LORA_RUNS][256] for x, then every other round's sums
+    typedef LoraSums<G> Sums;                                // of a round's row groups
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int item = xcd_tile(blockIdx.x, gridDim.x), tile_at = item / shares, first = item % shares * per;
+    const int row0 = tile_at * 16 * G, rt = a.R / 16;
+    const int units = (a.K + 31) / 32, run = (units + LORA_RUNS - 1) / LORA_RUNS;      // (at most 4 C)
+    const int u0 = wave * run, u1 = min(units, u0 + run);
+    TileAdapters<G> tile(a, row0);
+    uint4 x[G][C][4];
+    {
+        const int m = lane & 15, g = lane >> 4;
+        const char* xb = reinterpret_cast<const char*>(a.x + row0 * a.x_stride);
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)                  // row 4 i + g of group q, k 32 (u0 + 4 c) + 8 m .. + 8
+                    x[q][c][i] = load8(reinterpret_cast<const uint16_t*>(
+                        xb + ((uint32_t)(min(16 * q + 4 * i + g, a.T - 1 - row0) * (int)a.x_stride) * 2u +
+                              (uint32_t)min(32 * (u0 + 4 * c) + 8 * m, min(32 * u1, a.K) - 8) * 2u)));
+    }
+    bool fresh = true;
+    int round = 1;
+    while (tile.rest) {
+        uint64_t mask;
+        const int who = tile.next(mask);
+        const RankTiles tiles(a, who);
+        if (first >= tiles.total) continue;
+        const int last = min(tiles.total, first + per) - 1;
+        const char* ab = reinterpret_cast<const char*>(a.a + (int64_t)who * a.S * rt * units * 64);
+        const auto load_a = [&](int i0, int c, uint4(&p)[4]) __attribute__((always_inline)) {
+            const char* ap = ab + (int64_t)tiles.place_of(min(i0, last)) * (units * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = load_kib(ap + min(u0 + 4 * c + i, u1 - 1) * 1024, lane);
+        };
+        uint4 p[4];
+        load_a(first, 0, p);
+        __builtin_amdgcn_sched_barrier(0);
+        if (fresh) {
+            int l = lane;
+            asm volatile("" : "+v"(l));                      // (addresses made here, not kept in registers)
+            const int m = l & 15, g = l >> 4;
+            uint4* own = xs + 256 * wave;
+#pragma unroll
+            for (int q = 0; q < G; ++q)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const bool past = 32 * (u0 + 4 * c) + 8 * m >= a.K;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        own[(4 * i + g) * 16 + (m ^ (4 * i + g))] = past ? make_uint4(0u, 0u, 0u, 0u) : x[q][c][i];
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[q][c][i] = own[m * 16 + ((4 * i + g) ^ m)];
+                    __builtin_amdgcn_wave_barrier();
+                }
+            fresh = false;
+        }
+#pragma unroll 1
+        for (int i0 = first; i0 <= last; ++i0) {
+            f32x4 acc[G];
+            uint4 next[4];
+#pragma unroll
+            for (int q = 0; q < G; ++q) acc[q] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                load_a(c + 1 < C ? i0 : i0 + 1, (c + 1) % C, next);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (u0 + 4 * c + i < u1)
+#pragma unroll
+                        for (int q = 0; q < G; ++q) acc[q] = mfma32<DT>(p[i], x[q][c][i], acc[q]);
+                if (c + 1 < C)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] = next[i];
+            }
+            Sums& sums = *reinterpret_cast<Sums*>(xs + (round++ & 1) * (LORA_RUNS * 256));
+            int l = lane;
+            asm volatile("" : "+v"(l));
+#pragma unroll
+            for (int j = 0; j < G; ++j) sums[wave][j][sums_lane(l)] = acc[j];
+            lds_barrier();                                   // (the sums before the last ones are read: who does came here after it)
+            const int q = (wave >> 2) % G, m = 4 * (wave & 3) + (l >> 4);
+            const float sum = lora_sum<G>(sums, q, m, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                    // (before the store, which would be waited for with them)
+                p[i] = next[i];
+                asm volatile("" : "+v"(p[i].x), "+v"(p[i].y), "+v"(p[i].z), "+v"(p[i].w));
+            }
+            lora_put<DT>(a, sum, tiles.scale_of(i0), tiles.ranks_of(i0),
+                         ((int64_t)tile_at * G + q) * a.S * rt + tiles.place_of(i0), m, l,
+                         wave < 4 * G && (mask >> (16 * q + m)) & 1);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The first product, many rows, K past 8192: 16 rows against all of an adapter's rank tiles, two a round, sixteen waves, a run of the
+// k each; x, which no wave can hold, comes in again every round. blockIdx.y: a row tile's first, third, ... adapter or the others.
+// ------------------------------------------------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(1024) void lora_shrink_long_kernel(const LoraArgs a, int, int) {
     extern __shared__ uint4 xs[];                            // [LORA_RUNS][256], then the sums of two rounds
-    typedef f32x4 Sums[LORA_RUNS][2][64];                    // of a round's B tiles and G row groups
+    typedef LoraSums<2> Sums;                                // of a round's two tiles
     Sums* part = reinterpret_cast<Sums*>(xs + LORA_RUNS * 256);
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 16 * G, rt = a.R / 16, half = blockIdx.y;
+    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 16, rt = a.R / 16;
     const int units = (a.K + 31) / 32, run = (units + LORA_RUNS - 1) / LORA_RUNS, chunks = (run + 3) / 4;
     const int u0 = wave * run, u1 = min(units, u0 + run);
-    const uint32_t lane16 = lane * 16u;
     const char* xb = reinterpret_cast<const char*>(a.x + row0 * a.x_stride);
-    uint32_t xrow[G][4];                                     // bytes to rows g, 4 + g, 8 + g, 12 + g of a group
+    uint32_t xrow[4];                                        // bytes to rows g, 4 + g, 8 + g, 12 + g
 #pragma unroll
-    for (int q = 0; q < G; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xrow[q][i] = (uint32_t)(min(16 * q + 4 * i + g, a.T - 1 - row0) * (int)a.x_stride) * 2u;
+    for (int i = 0; i < 4; ++i) xrow[i] = (uint32_t)(min(4 * i + g, a.T - 1 - row0) * (int)a.x_stride) * 2u;
     uint4* own = xs + 256 * wave;
-    TileAdapters<G> tile(a, row0);
+    TileAdapters<1> tile(a, row0);
     int round = 0;
     for (int nth = 0; tile.rest; ++nth) {
         uint64_t mask;
         const int who = tile.next(mask);
-        if ((nth & 1) != (int)blockIdx.z) continue;
-        // the adapter's rank tiles, matrix after matrix, a lane each: the tile's place among the layer's S * R / 16, its ranks
-        // that the adapter has and its scale
-        const int sl = min(lane, a.S - 1);
-        const int rank_of = min(max(a.ranks[(int64_t)who * a.S + sl], 0), a.R);
-        const float scale_of = a.scales[(int64_t)who * a.S + sl];
-        int total = 0, place = 0, ranks = 0;
-        float scale = 0.f;
-#pragma unroll
-        for (int s = 0; s < LORA_MAX_SHARDS; ++s)
-            if (s < a.S) {
-                const int r = __builtin_amdgcn_readlane(rank_of, s);
-                if (lane >= total) {
-                    place = s * rt + lane - total;
-                    ranks = r - 16 * (lane - total);
-                    scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale_of), s));
-                }
-                total += (r + 15) / 16;
-            }
-        if (half >= total) continue;
+        if ((nth & 1) != (int)blockIdx.y) continue;
+        const RankTiles tiles(a, who);
+        if (tiles.total == 0) continue;
         const char* ab = reinterpret_cast<const char*>(a.a + (int64_t)who * a.S * rt * units * 64);
-        const auto load_a = [&](int i0, int c, uint4(&p)[B][4]) __attribute__((always_inline)) {
+        const auto load_a = [&](int i0, int c, uint4(&p)[2][4]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < B; ++j) {                    // past the last one: that one again, and not used
-                const char* ap = ab + (int64_t)__builtin_amdgcn_readlane(place, min(i0 + j * G, total - 1)) * (units * 1024);
+            for (int j = 0; j < 2; ++j) {                    // past the last one: that one again, and not used
+                const char* ap = ab + (int64_t)tiles.place_of(min(i0 + j, tiles.total - 1)) * (units * 1024);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    p[j][i] = *reinterpret_cast<const uint4*>(ap + (int64_t)min(u0 + 4 * c + i, u1 - 1) * 1024 + lane16);
+                for (int i = 0; i < 4; ++i) p[j][i] = load_kib(ap + (int64_t)min(u0 + 4 * c + i, u1 - 1) * 1024, lane);
             }
         };
-        uint4 x[G][4], p[B][4];
-        load_a(half, 0, p);
+        uint4 x[4], p[2][4];
+        load_a(0, 0, p);
 #pragma unroll 1
-        for (int i0 = half; i0 < total; i0 += 2) {
-            f32x4 acc[B][G];
-#pragma unroll
-            for (int j = 0; j < B; ++j)
-#pragma unroll
-                for (int q = 0; q < G; ++q) acc[j][q] = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < tiles.total; i0 += 2) {
+            f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 1
             for (int c = 0; c < chunks; ++c) {
                 const int u = u0 + 4 * c;
-                const bool fresh = chunks > 1 || i0 == half; // a single chunk's operands stay in registers
-                if (fresh)
 #pragma unroll
-                    for (int q = 0; q < G; ++q)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {        // row 4 i + g of group q, k 32 u + 8 m .. + 8
-                            const int k = 32 * u + 8 * m;    // (of a row that is not the adapter's too: its t is not kept)
-                            x[q][i] = load8(reinterpret_cast<const uint16_t*>(xb + (xrow[q][i] + (uint32_t)min(k, a.K - 8) * 2u)));
-                            if (k >= a.K) x[q][i] = make_uint4(0u, 0u, 0u, 0u);
-                        }
+                for (int i = 0; i < 4; ++i) {                // row 4 i + g, k 32 u + 8 m .. + 8
+                    const int k = 32 * u + 8 * m;            // (of a row that is not the adapter's too: its t is not kept)
+                    x[i] = load8(reinterpret_cast<const uint16_t*>(xb + (xrow[i] + (uint32_t)min(k, a.K - 8) * 2u)));
+                    if (k >= a.K) x[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
                 const bool more = c + 1 < chunks;
-                uint4 next[B][4];
+                uint4 next[2][4];
                 load_a(more ? i0 : i0 + 2, more ? c + 1 : 0, next);
                 __builtin_amdgcn_sched_barrier(0);           // every load before the first use
-                if (fresh)
 #pragma unroll
-                    for (int q = 0; q < G; ++q) {
+                for (int i = 0; i < 4; ++i) own[(4 * i + g) * 16 + (m ^ (4 * i + g))] = x[i];
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) own[(4 * i + g) * 16 + (m ^ (4 * i + g))] = x[q][i];
-                        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[q][i] = own[m * 16 + ((4 * i + g) ^ m)];
-                        __builtin_amdgcn_wave_barrier();
-                    }
+                for (int i = 0; i < 4; ++i) x[i] = own[m * 16 + ((4 * i + g) ^ m)];
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (u + i < u1)
 #pragma unroll
-                        for (int j = 0; j < B; ++j)
+                        for (int j = 0; j < 2; ++j) acc[j] = mfma32<DT>(p[j][i], x[i], acc[j]);
 #pragma unroll
-                            for (int q = 0; q < G; ++q) acc[j][q] = mfma32<DT>(p[j][i], x[q][i], acc[j][q]);
-#pragma unroll
-                for (int j = 0; j < B; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) p[j][i] = next[j][i];
             }
-            // two waves finish a round's two sums, other waves the next one's
-            const int w = (wave - 2 * round) & (LORA_RUNS - 1), i = i0 + (G == 1 ? w : 0), q = G == 1 ? 0 : w;
             Sums& sums = part[round++ & 1];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) sums[wave][j][lane] = G == 1 ? acc[j % B][0] : acc[0][j % G];
-            lds_barrier();                                   // (the next tiles' loads stay in flight; the sums before the last
-                                                             // ones are read: the waves that do came to this barrier after it)
-            if (w < 2 && i < total) {
-                const bool mine = (mask >> (16 * q + m)) & 1;
-                const int left = __builtin_amdgcn_readlane(ranks, i) - 4 * g;
-                f32x4 four[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-                    four[z] = ((sums[4 * z][w][lane] + sums[4 * z + 1][w][lane]) + sums[4 * z + 2][w][lane]) +
-                              sums[4 * z + 3][w][lane];
-                f32x4 sum = (four[0] + four[1]) + (four[2] + four[3]);
-                sum *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), i));
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k >= left) sum[k] = 0.f;             // ranks that the adapter does not have
-                const int64_t tile_to = ((int64_t)tile_at * G + q) * a.S * rt + __builtin_amdgcn_readlane(place, i);
-                if constexpr (DT == F16) {
-                    float top = fmaxf(fmaxf(fabsf(sum[0]), fabsf(sum[1])), fmaxf(fabsf(sum[2]), fabsf(sum[3])));
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const int e = lora_exponent(top);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sum[k] = ldexpf(sum[k], -e);
-                    if (g == 0 && mine) a.e[tile_to * 16 + m] = e;
-                }
-                if (mine) {                                  // ranks 4 g .. + 4 of row m
-                    uint2 hi, lo;
-                    split4<DT>(sum, hi, lo);
-                    uint2* t = reinterpret_cast<uint2*>(a.t + tile_to * 64) + 2 * (16 * (g >> 1) + m) + (g & 1);
-                    t[0] = hi;
-                    t[64] = lo;
-                }
-            }
+            for (int j = 0; j < 2; ++j) sums[wave][j][sums_lane(lane)] = acc[j];
+            lds_barrier();
+            const int q = (wave >> 2) & 1, at = min(i0 + q, tiles.total - 1), row = 4 * (wave & 3) + g;
+            lora_put<DT>(a, lora_sum<2>(sums, q, row, lane), tiles.scale_of(at), tiles.ranks_of(at),
+                         (int64_t)tile_at * a.S * rt + tiles.place_of(at), row, lane,
+                         wave < 8 && i0 + q < tiles.total && (mask >> row) & 1);
         }
     }
 }
@@ -440,7 +569,8 @@ __device__ __forceinline__ uint4 lora_t8(const f32x4 (&p)[2][2], float scale, in
     return lora_operand<DT>(v, scale, left, e);
 }
 
-// Few rows: a wave 128 columns of a row tile (and, spread, its adapters)
+// Few rows: a wave 128 columns of a row tile (and, spread, its adapters). The same 32 rows, 2048 columns: 5.9 us for 2.5 MB, the same
+// round trips; loading before the ranks are known gained nothing, four rank tiles at once (308 registers) lost.
 template <int DT>
 __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4, rt = a.R / 16, ct = blockIdx.y;
@@ -508,7 +638,8 @@ __global__ __launch_bounds__(64) void lora_expand_kernel(const LoraArgs a) {
 // ------------------------------------------------------------------------------------------------------------------
 // Both products in one launch, for a few rows and ranks: sixteen waves make t of a row tile and adapter (blockIdx.x), a run of the
 // k each, and four of them go on to 128 columns of one matrix each (blockIdx.y). Every workgroup makes its t itself: at 16 ranks of
-// 2048 it takes in 64 KiB of A, which costs less than a launch more and the way through memory.
+// 2048 it takes in 64 KiB of A, which costs less than a launch more and the way through memory. One row, 2048 -> 4096 + 512 + 512,
+// rank 16: 4.7 us, a launch and four dependent round trips.
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int LORA_ONE_TILES = 2;              // rank tiles
 
@@ -613,7 +744,9 @@ __global__ __launch_bounds__(1024) void lora_one_kernel(const LoraArgs a) {
 
 constexpr int LORA_HELD = 4;                   // rank tiles of B in shared memory at once
 
-// Many rows: a workgroup of 64 rows (16 a wave) and 128 columns, an adapter's B for them in shared memory
+// Many rows: a workgroup of 64 rows (16 a wave) and 128 columns, an adapter's B for them in shared memory. Bound by memory: y comes in
+// and out goes out, 84 MB for 4096 rows of 5120 columns in 22 us (3.8 TB/s) under the profiler. All waves of a SIMD busy matters more than
+// loads in flight: 5 or 6 waves a SIMD by spilling 23 and 36 us, several column tiles a workgroup 31 to 55.
 template <int DT>
 __global__ __launch_bounds__(256, DT == BF16 ? 4 : 3) void lora_expand_all_kernel(const LoraArgs a) {
     __shared__ uint4 bs[LORA_HELD][256];
@@ -707,14 +840,23 @@ template <int DT>
 int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
     const unsigned tiles = (unsigned)((a.T + 15) / 16), cols = (unsigned)a.tiles0[a.S];
     if (all) {
-        // 32 rows and half of the rank tiles a workgroup take in less than 16 rows and all, where x is taken in once (K up to
-        // 2048) or few tiles follow: 2048 -> 4096 + 512 + 512, ranks 16 and 64, 4096 rows 38.6 -> 35.9 us in all, 4096 -> 2048,
-        // ranks up to 64, 28.9 -> 24.5; 4096 -> 4096, rank 128, 8192 rows 101 -> 133
-        const unsigned group = a.K <= 2048 || a.S * (a.R / 16) <= 4 ? 2 : 1;
-        const auto shrink = group == 1 ? lora_shrink_all_kernel<DT, 1> : lora_shrink_all_kernel<DT, 2>;
+        const int rank_tiles = a.S * (a.R / 16), chunks = a.K <= 2048 ? 1 : a.K <= 4096 ? 2 : 4;
+        int groups = a.K <= 8192 ? 4 / chunks : 1;
+        // half the rows where there are few tiles, so that more CUs have one. us of both launches, 4 / 2 groups: 2048 -> 4096 + 512 +
+        // 512, rank 16, 2048 rows 20.6 / 18.9, 8192 rows 46.8 / 47.9; 2048 -> 2048, rank 128, 1536 rows 13.0 / 12.3, 8192 rows 43 / 48
+        if (groups > 1 && (a.T + 16 * groups - 1) / (16 * groups) * rank_tiles < 256) groups /= 2;
+        const int row_tiles = (a.T + 16 * groups - 1) / (16 * groups);
+        const int want = std::min(rank_tiles, std::max(1, 256 / row_tiles));         // a workgroup a CU
+        const int per = (rank_tiles + want - 1) / want, shares = (rank_tiles + per - 1) / per;
+        const auto shrink = a.K > 8192                    ? lora_shrink_long_kernel<DT>
+                            : chunks == 4                 ? lora_shrink_all_kernel<DT, 1, 4>
+                            : chunks == 2 && groups == 2  ? lora_shrink_all_kernel<DT, 2, 2>
+                            : chunks == 2                 ? lora_shrink_all_kernel<DT, 1, 2>
+                            : groups == 4                 ? lora_shrink_all_kernel<DT, 4, 1>
+                                                          : lora_shrink_all_kernel<DT, 2, 1>;
         if (hipFuncSetAttribute((const void*)shrink, hipFuncAttributeMaxDynamicSharedMemorySize, LORA_ALL_SMEM) != hipSuccess)
             return esp_host::fail(ESP_ERR_HIP, "lora: no %d bytes of shared memory", LORA_ALL_SMEM);
-        shrink<<<dim3((tiles + group - 1) / group, group, 2), 1024, LORA_ALL_SMEM, st>>>(a);
+        shrink<<<a.K > 8192 ? dim3(tiles, 2) : dim3(row_tiles * shares), 1024, LORA_ALL_SMEM, st>>>(a, shares, per);
         lora_expand_all_kernel<DT><<<dim3((tiles + 3) / 4, cols), 256, 0, st>>>(a);
     } else if (lora_one(a)) {
         lora_one_kernel<DT><<<dim3(a.T, lora_one_blocks(a)), 1024, 0, st>>>(a);
@@ -733,12 +875,16 @@ int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
 // ======================================================================================================================
 using namespace esp;
 
-// Whether T rows run as the launches for many rows. They take longer to begin with (a CU goes through all ranks of a tile) and
-// less a row. us for T rows, few / many (bf16, graph replays, three requests one after the other):
-//   2048 -> 4096 + 512 + 512, ranks 16: 11.7 / 12.2 at 512, 11.0 / 11.8 at 768, 20 / 13.8 at 1024, 51 / 33 at 4096
-//   4096 -> 2048, rank 16: 8.5 / 10.9 at 768, 13.8 / 11.7 at 1536, 19.4 / 13.8 at 2048
-//   2048 -> 512 + 512, ranks 32: 8.6 / 10.8 at 768, 10.4 / 10.9 at 1536, 15.8 / 12.4 at 2048
-static bool lora_many(int64_t T, int64_t N) { return T * N >= 3 << 20 || T >= 1536; }
+// Whether T rows run as the launches for many rows. They take longer to begin with (a CU goes through a tile's adapters one after
+// the other) and less a row, column and rank. us for T rows, few / many (bf16, graph replays, three requests one after the other):
+//   2048 -> 4096 + 512 + 512, ranks 16: 8.3 / 9.1 at 384, 11.6 / 11.6 at 512; ranks up to 64: 14.0 / 9.8, 17.9 / 12.5
+//   2048 -> 2048, rank 128: 11.9 / 14.6 at 256, 14.7 / 10.8 at 384, 24.1 / 14.9 at 1024
+//   512 -> 2048, ranks 64: 10.4 / 12.0 at 512, 10.0 / 9.5 at 768; ranks 16: 7.4 / 8.8 at 768, 10.0 / 11.0 at 1024
+//   2048 -> 512 + 512, ranks 32: 9.6 / 9.1 at 768, 11.1 / 11.5 at 1024, 13.0 / 11.9 at 1280
+// and 32 requests one after the other, 2048 -> 4096 + 512 + 512, ranks up to 64: 13.8 / 27.2 at 256, 17.6 / 24.8 at 384, 15.0 / 18.5
+static bool lora_many(int64_t T, int64_t N, int64_t rank_tiles) {
+    return T >= 1152 || (T >= 384 && T * N * rank_tiles >= 6 << 20);
+}
 
 // The workgroups that a row tile's adapters are dealt to (few rows): up to one a row, and no more than 32 over all tiles, since
 // one that finds nothing costs 2 ns too (a tile of one adapter leaves the others empty). 2048 -> 4096 + 512 + 512, ranks 16 and 64
@@ -755,7 +901,7 @@ static int lora_spread(int64_t T, int64_t cols) {
 extern "C" int64_t esp_lora_scratch(int64_t T, int64_t N, int64_t n_shards, int64_t R) {
     if (T <= 0 || N <= 0 || n_shards <= 0 || R <= 0) return 0;
     const int64_t rows = (T + 15) / 16 * 16, ranks = n_shards * ((R + 15) / 16);
-    return lora_many(T, N) ? rows * ranks * 17 : rows * ranks * 16 * (LORA_RUNS / 4);
+    return lora_many(T, N, ranks) ? rows * ranks * 17 : rows * ranks * 16 * (LORA_RUNS / 4);
 }
 
 extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out, int64_t out_stride,
@@ -793,7 +939,7 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
     ESP_REQUIRE(((uintptr_t)A | (uintptr_t)B | (uintptr_t)scratch) % 16 == 0,
                 "lora: the adapters and the scratch must be 16-byte aligned");
     ESP_REQUIRE(scratch_numel >= esp_lora_scratch(T, N, n_shards, R), "lora: the scratch needs esp_lora_scratch floats");
-    const bool all = lora_many(T, N);
+    const bool all = lora_many(T, N, n_shards * (R / 16));
     const int64_t tiles = (T + 15) / 16;
     a.x = static_cast<const uint16_t*>(x);
     a.x_stride = x_stride;
