@@ -59,6 +59,7 @@ def _lora(lib, **over):
 @pytest.mark.parametrize("over,needle", [
     (dict(dtype=2), "bf16"), (dict(T=-1), "rows"), (dict(T=1 << 24), "rows"), (dict(S=0), "matrices"),
     (dict(S=5, cols=[16] * 5), "matrices"), (dict(K=72), "multiple of 16"), (dict(K=0), "multiple of 16"),
+    (dict(T=(1 << 24) - 1, cols=[8192]), "blocks of 64 rows"),
     (dict(R=8), "multiple of 16"), (dict(R=272), "at most"), (dict(slots=0), "adapters"), (dict(cols=[24]), "columns"),
     (dict(cols=[0]), "columns"), (dict(x=None), "null"), (dict(scratch=None), "null"), (dict(ranks=None), "null"),
     (dict(xs=32), "overlap"), (dict(ys=16), "overlap"), (dict(os=36), "in place"), (dict(x=20), "aligned"),

@@ -745,15 +745,17 @@ __global__ __launch_bounds__(1024) void lora_one_kernel(const LoraArgs a) {
 constexpr int LORA_HELD = 4;                   // rank tiles of B in shared memory at once
 
 // Many rows: a workgroup of 64 rows (16 a wave) and 128 columns, an adapter's B for them in shared memory. Bound by memory: y comes in
-// and out goes out, 84 MB for 4096 rows of 5120 columns in 22 us (3.8 TB/s) under the profiler. All waves of a SIMD busy matters more than
-// loads in flight: 5 or 6 waves a SIMD by spilling 23 and 36 us, several column tiles a workgroup 31 to 55.
+// and out goes out, 84 MB for 4096 rows of 5120 columns in 20.6 us (4.1 TB/s) under the profiler. All waves of a SIMD busy matters more than
+// loads in flight: 5 or 6 waves a SIMD by spilling 23 and 36 us, several column tiles a workgroup 31 to 55. An XCD's workgroups go
+// through the columns of a row tile first, so that whole rows of y pass at a time (the rows first: 22.1 us).
 template <int DT>
 __global__ __launch_bounds__(256, DT == BF16 ? 4 : 3) void lora_expand_all_kernel(const LoraArgs a) {
     __shared__ uint4 bs[LORA_HELD][256];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int tile_at = xcd_tile(blockIdx.x, gridDim.x), row0 = tile_at * 64, rt = a.R / 16;
-    const LoraCols col(a, blockIdx.y);
+    const int cts = a.tiles0[a.S], item = xcd_tile(blockIdx.x, gridDim.x), tile_at = item / cts, ct = item % cts;
+    const int row0 = tile_at * 64, rt = a.R / 16;
+    const LoraCols col(a, ct);
     const uint16_t* yp = a.y + (int64_t)(row0 + 16 * wave) * a.y_stride + col.c0 + 8 * m;
     uint16_t* op = a.out + (int64_t)(row0 + 16 * wave) * a.out_stride + col.c0 + 8 * m;
     const bool in = 8 * m < col.cols;
@@ -769,7 +771,7 @@ __global__ __launch_bounds__(256, DT == BF16 ? 4 : 3) void lora_expand_all_kerne
         uint64_t mask;
         const int who = tile.next(mask);
         const int r = lora_rank(a, who, col.s), nt = (r + 15) / 16;
-        const uint4* bp = a.b + ((int64_t)who * a.tiles0[a.S] + blockIdx.y) * rt * 256 + threadIdx.x;
+        const uint4* bp = a.b + ((int64_t)who * cts + ct) * rt * 256 + threadIdx.x;
         const uint32_t rows = (uint32_t)(mask >> (16 * wave)) & 0xFFFFu;
         const int64_t at = ((int64_t)min(tile_at * 4 + wave, (a.T - 1) / 16) * a.S + col.s) * rt;
         f32x4 acc[8];
@@ -857,7 +859,7 @@ int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
         if (hipFuncSetAttribute((const void*)shrink, hipFuncAttributeMaxDynamicSharedMemorySize, LORA_ALL_SMEM) != hipSuccess)
             return esp_host::fail(ESP_ERR_HIP, "lora: no %d bytes of shared memory", LORA_ALL_SMEM);
         shrink<<<a.K > 8192 ? dim3(tiles, 2) : dim3(row_tiles * shares), 1024, LORA_ALL_SMEM, st>>>(a, shares, per);
-        lora_expand_all_kernel<DT><<<dim3((tiles + 3) / 4, cols), 256, 0, st>>>(a);
+        lora_expand_all_kernel<DT><<<(tiles + 3) / 4 * cols, 256, 0, st>>>(a);
     } else if (lora_one(a)) {
         lora_one_kernel<DT><<<dim3(a.T, lora_one_blocks(a)), 1024, 0, st>>>(a);
     } else {
@@ -927,6 +929,7 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
         N += n_cols[s];
     }
     ESP_REQUIRE(a.tiles0[n_shards] <= 65535, "lora: at most 65535 blocks of %d columns", LORA_COLS);
+    ESP_REQUIRE((T + 63) / 64 * a.tiles0[n_shards] < (1 << 24), "lora: at most 2^24 - 1 blocks of 64 rows and %d columns", LORA_COLS);
     if (T == 0) return esp_host::ok();
     ESP_REQUIRE(x && y && out && rows && A && B && ranks && scales && scratch, "lora: null pointer");
     ESP_REQUIRE(T == 1 || (x_stride >= K && y_stride >= N && out_stride >= N), "lora: rows overlap");
