@@ -30,7 +30,7 @@ Three things of a served model can stand in the step, off by default:
     add_rmsnorm);
   * verify(b, ...): the rows of a pass are requests' last tokens and their drafts, verified against the logits
     (speculative.verify).
-With the first two the launches run apart (qkv's adapters stand between qkv and o); rows stay independent.
+A layer that has one of the first two runs its launches apart (qkv's adapters stand between qkv and o); rows stay independent.
 """
 from __future__ import annotations
 
@@ -73,9 +73,13 @@ class DecoderLayer:
     o_adapters: Adapters | None = None
 
     @property
+    def adapted(self) -> bool:
+        return self.qkv_adapters is not None or self.o_adapters is not None
+
+    @property
     def plain(self) -> bool:
-        """Whether the layer runs in the launches that hold several of its steps."""
-        return self.post_o is None and self.qkv_adapters is None
+        """Whether the layer runs in the launches that hold several of its steps: none of what may stand between them."""
+        return self.post_in is None and self.post_o is None and not self.adapted
 
 
 def _norm_weight(gen, dev, D):
@@ -169,9 +173,14 @@ class SyntheticDecoder:
             self._bufs[T] = Buffers(T, self.vocab, self.dev)
         return self._bufs[T]
 
+    def _fused(self, L: DecoderLayer, T: int) -> bool:
+        """Whether L's norms run inside its qkv and routing launches for T rows. (Either way the residual comes in and goes out in
+        Buffers.h, so neighbours may differ.)"""
+        return FUSE_NORMS and T <= 4 and L.plain and L.qkv.norm_fusable(T)
+
     def fused_norms(self, T: int) -> bool:
-        """Whether the layers' norms run inside the qkv and routing launches for T rows."""
-        return FUSE_NORMS and T <= 4 and self.layers[0].plain and self.layers[0].qkv.norm_fusable(T)
+        """Whether all layers' norms run inside the qkv and routing launches for T rows."""
+        return all(self._fused(L, T) for L in self.layers)
 
     def fused_head_norm(self, T: int) -> bool:
         return FUSE_NORMS and self.final_post is None and self.head.norm_fusable(T)
@@ -180,7 +189,7 @@ class SyntheticDecoder:
         e = ext()
         q = b.qkv[:, :Q_OUT]
         d1, d2 = (None, None) if first else (b.moe, b.moe_shared)
-        if self.fused_norms(b.T):
+        if self._fused(L, b.T):
             if MULTI_ATTN:
                 L.attn.forward([None, q], [b.qkv, b.o], norm=(b.h, d1, d2, L.norm1, EPS, b.h2))
             else:
@@ -189,14 +198,15 @@ class SyntheticDecoder:
             G.route_rmsnorm(b.h2, b.o, L.norm2, EPS, b.h, b.a, L.router, TOPK, L.moe, self.scratch)
         else:
             self._join(b, d1, d2, L.post_in, L.norm1)
-            if L.qkv_adapters is not None:
-                L.qkv_adapters.apply(b.a, L.qkv.forward(b.a, out=b.qkv), b.rows)
-                L.o_adapters.apply(q, L.o.forward(q, out=b.o), b.rows)
-            elif MULTI_ATTN:
+            if MULTI_ATTN and not L.adapted:
                 L.attn.forward([b.a, q], [b.qkv, b.o])
             else:
                 L.qkv.forward(b.a, out=b.qkv)
+                if L.qkv_adapters is not None:
+                    L.qkv_adapters.apply(b.a, b.qkv, b.rows)
                 L.o.forward(q, out=b.o)
+                if L.o_adapters is not None:
+                    L.o_adapters.apply(q, b.o, b.rows)
             self._join(b, b.o, None, L.post_o, L.norm2)
             G.route(b.a, L.router, TOPK, L.moe, self.scratch)
         if picks is not None:                     # eager runs only: the distinct experts this layer reads
