@@ -424,9 +424,9 @@ int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d2, const vo
  *   out[m][n] = y[m][n] + sum_{j < r} (scales[a][s] * sum_k x[m][k] * A[a][s][j][k]) * B[a][n][j],   r = ranks[a][s],
  * summed in fp32 and rounded once. A row whose adapter is outside [0, slots), and the columns of a matrix for which its adapter
  * has no ranks, keep y's bits. x [T][K], y and out [T][N] with row strides, N = sum(n_cols); ranks int32 and scales fp32
- * [slots][n_shards] on the device. out may be y (in place), and must else overlap neither y nor x; columns past N are left as
- * they are. dtype ESP_BF16 or ESP_F16 for x, y, out, A and B. K a multiple of 16, T < 2^24, at most 2^24 - 1 blocks of 64 rows and
- * 128 columns of a matrix.
+ * [slots][n_shards] on the device. out may be y (in place), and must else overlap neither y nor x (refused), nor any other input;
+ * columns past N are left as they are. dtype ESP_BF16 or ESP_F16 for x, y, out, A and B. K a multiple of 16, T < 2^24, at most
+ * 2^24 - 1 blocks of 64 rows and 128 columns of a matrix.
  * A and B are laid out as the matrix instructions read them, R (a multiple of 16, at most 256) ranks a slot, zeros where an
  * adapter has nothing (past its rank in its last 16 ranks, past K, past a matrix's columns); 16-rank tiles past the rank are
  * not used, whatever they hold:

@@ -1,0 +1,40 @@
+"""GPU checks of calls of the adapters, the verification and the norms around a block that other tests do not make: views of one
+buffer side by side, calls that would overwrite what they read."""
+import pytest
+import torch
+
+from vllm_espalier.adapters import Adapters
+
+pytestmark = pytest.mark.gpu
+
+
+def _store(K, outs, ranks, dtype, gen, dev, slots=None):
+    store = Adapters(K, outs, slots=slots or len(ranks), max_rank=max(ranks), dtype=dtype, device=dev)
+    for i, r in enumerate(ranks):
+        store.load(i, [(torch.randn((r, K), generator=gen) * K ** -0.5).to(dtype) for _ in outs],
+                   [(torch.randn((n, r), generator=gen) * r ** -0.5).to(dtype) for n in outs], 0.5)
+    return store
+
+
+@pytest.mark.parametrize("T", [1, 5, 300, 1200])
+def test_lora_views_of_one_buffer(dev, T):
+    """x, y and out side by side in the rows of one buffer are no overlap; x as y is one."""
+    gen = torch.Generator().manual_seed(T)
+    K = N = 64
+    store = _store(K, [N], [8, 20], torch.bfloat16, gen, dev)
+    wide = torch.randn((T, 3 * 64 + 4), generator=gen).to(torch.bfloat16).to(dev)
+    before = wide.clone()
+    rows = (torch.arange(T, dtype=torch.int32) % 3 - 1).to(dev)
+    want = store.apply(before[:, :64].contiguous(), before[:, 64:128].contiguous(), rows, out=torch.empty((T, N), dtype=torch.bfloat16, device=dev))
+    store.apply(wide[:, :64], wide[:, 64:128], rows, out=wide[:, 128:192])
+    assert torch.equal(wide[:, 128:192].view(torch.int16), want.view(torch.int16))
+    store.apply(wide[:, :64], wide[:, 64:128], rows)
+    assert torch.equal(wide[:, 64:128].view(torch.int16), want.view(torch.int16))
+    assert torch.equal(wide[:, :64], before[:, :64]) and torch.equal(wide[:, 192:], before[:, 192:])
+    x = before[:, :64].contiguous()
+    keep = x.clone()
+    for y, out in ((x, None), (before[:, 64:128], x), (before[:, 60:124], before[:, 64:128])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            store.apply(x if y is x or out is x else wide[:, :64], y, rows, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(x, keep)

@@ -1,10 +1,24 @@
 """Calls of the adapters, the verification and the norms around a block that have to be refused, or must leave nothing behind, on
 the CPU: the package's own checks in front of the extension, and the C ABI's before any HIP call."""
+import ctypes
+from pathlib import Path
+
 import pytest
 import torch
 
 from vllm_espalier import linear as LN
 from vllm_espalier.adapters import Adapters
+
+LIB = Path(__file__).resolve().parent.parent / "vllm-espalier_amd" / "vllm_espalier" / "libespalier_hip.so"
+P, I64, INT, F64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double
+
+
+@pytest.fixture(scope="module")
+def lib(ext):
+    L = ctypes.CDLL(str(LIB))
+    L.esp_last_error.restype = ctypes.c_char_p
+    L.esp_lora.argtypes = [P, I64, P, I64, P, I64, P, I64, I64, I64, ctypes.POINTER(I64), P, P, P, P, I64, I64, INT, P, I64, P]
+    return L
 
 
 def _layer(monkeypatch, in_features, outs):
@@ -27,3 +41,21 @@ def test_rows_of_another_width_refused(monkeypatch, have, given):
         store.apply(x[0], y, rows)
     with pytest.raises(RuntimeError, match="in_features"):
         _layer(monkeypatch, have, [32])(x.view(1, 3, given), rows)
+
+
+@pytest.mark.parametrize("x,xs,y,ys,out,os,needle", [
+    (4096, 64, 4096, 64, 4096, 64, "overlaps x"),            # y = x, in place: rows that other workgroups still read
+    (4096, 64, 65536, 64, 4096, 64, "overlaps x"),           # out = x
+    (4096, 64, 65536, 64, 4096 + 3 * 128 + 64, 64, "overlaps x"),        # the last row alone
+    (4096, 128, 65536, 128, 4096 + 96, 128, "overlaps x"),   # side by side in one buffer, but for 16 columns
+    (4096, 128, 65536, 128, 4096 - 96, 128, "overlaps x"),
+    (4096, 100, 65536, 64, 4096 + 2 * 136, 68, "overlaps x"),      # different strides
+    (65536, 64, 4096, 64, 4096 + 128, 64, "overlaps y"),     # a row further
+    (65536, 64, 4096, 128, 4096 + 32, 128, "overlaps y"),
+    (65536, 64, 4096, 128, 4096 + 64, 68, "overlaps y")])
+def test_lora_overlap_refused(lib, x, xs, y, ys, out, os, needle):
+    """4 rows of 64 -> 64 in 16-bit elements at made-up addresses: refused before anything reads them."""
+    rc = lib.esp_lora(x, xs, y, ys, out, os, 16, 4, 64, 1, (I64 * 1)(64), 16, 16, 16, 16, 1, 16, 1, 16, 1 << 20, None)
+    assert rc == 1 and needle in lib.esp_last_error().decode()
+    one = lib.esp_lora(x, xs, y, ys, x, os, 16, 1, 64, 1, (I64 * 1)(64), 16, 16, 16, 16, 1, 16, 1, 16, 1 << 20, None)
+    assert one == 1 and "overlaps x" in lib.esp_last_error().decode()

@@ -108,7 +108,8 @@ class Adapters:
     def apply(self, x: torch.Tensor, y: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """y [T, at least sum(out_features)] plus, for every row, the product of x [T, in_features] with the adapter in slot
         rows[t] (int32 [T], on the device; outside [0, slots): none, and the row keeps y's bits). In place unless `out` is
-        given; columns past the matrices' are not touched. A row's bits do not depend on the other rows."""
+        given; what is written may not overlap x, nor y without being y. Columns past the matrices' are not touched. A row's bits
+        do not depend on the other rows."""
         self.check_rows(x)
         out = y if out is None else out
         if x.stride(-1) != 1:

@@ -7,6 +7,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
+
 namespace esp {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -369,6 +371,23 @@ int moe_prompt_status(int clear, hipStream_t st, int* out); // moe_prompt.hip: t
 // Whether row strides (elements) fit the kernels' 32-bit ones; one row's stride is not used
 inline bool strides_fit(int64_t rows, int64_t a, int64_t b = 0) {
     return rows <= 1 || (a < (int64_t(1) << 31) && b < (int64_t(1) << 31));
+}
+// Whether any of `rows` rows of a bytes at p, p_stride bytes apart, shares a byte with one of b bytes at q, q_stride apart. Exact:
+// columns of one buffer side by side do not meet.
+inline bool rows_meet(const void* p, int64_t p_stride, int64_t a, const void* q, int64_t q_stride, int64_t b, int64_t rows) {
+    const int64_t d = (int64_t)((uintptr_t)q - (uintptr_t)p), last = rows - 1;
+    if (rows <= 0 || last * p_stride + a <= d || d + last * q_stride + b <= 0) return false;
+    if (last == 0) return true;
+    const auto floor_div = [](int64_t n, int64_t m) { return n >= 0 ? n / m : -((-n + m - 1) / m); };
+    if (p_stride == q_stride && p_stride > 0) {              // row j of q against row i of p: the last start below p's end
+        const int64_t k = std::min(floor_div(a - 1 - d, p_stride), last);
+        return k >= -last && d + k * p_stride + b > 0;
+    }
+    for (int64_t i = 0; i < rows; ++i) {
+        const int64_t top = i * p_stride + a - 1 - d, j = q_stride > 0 ? std::min(floor_div(top, q_stride), last) : top >= 0 ? last : -1;
+        if (j >= 0 && d + j * q_stride + b > i * p_stride) return true;
+    }
+    return false;
 }
 }  // namespace esp_host
 

@@ -942,6 +942,10 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
     ESP_REQUIRE(((uintptr_t)A | (uintptr_t)B | (uintptr_t)scratch) % 16 == 0,
                 "lora: the adapters and the scratch must be 16-byte aligned");
     ESP_REQUIRE(scratch_numel >= esp_lora_scratch(T, N, n_shards, R), "lora: the scratch needs esp_lora_scratch floats");
+    ESP_REQUIRE(!esp_host::rows_meet(out, out_stride * 2, N * 2, x, x_stride * 2, K * 2, T),
+                "lora: out overlaps x, which other workgroups still read");
+    ESP_REQUIRE(out == y || !esp_host::rows_meet(out, out_stride * 2, N * 2, y, y_stride * 2, N * 2, T),
+                "lora: out overlaps y without being y");
     const bool all = lora_many(T, N, n_shards * (R / 16));
     const int64_t tiles = (T + 15) / 16;
     a.x = static_cast<const uint16_t*>(x);
