@@ -38,3 +38,13 @@ def test_lora_views_of_one_buffer(dev, T):
             store.apply(x if y is x or out is x else wide[:, :64], y, rows, out=out)
     torch.cuda.synchronize()
     assert torch.equal(x, keep)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+def test_sandwich_of_no_rows(dev, ext, gate):
+    rows = torch.empty((0, 64), dtype=torch.bfloat16, device=dev)
+    w = torch.ones((64,), dtype=torch.bfloat16, device=dev)
+    g = {"none": None, "channel": w, "token": rows[:, :1], "element": rows}[gate]
+    out = torch.empty_like(rows)
+    ext.sandwich_rmsnorm(rows, rows, rows, w, g, True, 0.5, w, 1e-6, rows, out)
+    assert out.shape == (0, 64)

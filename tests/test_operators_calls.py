@@ -18,6 +18,7 @@ def lib(ext):
     L = ctypes.CDLL(str(LIB))
     L.esp_last_error.restype = ctypes.c_char_p
     L.esp_lora.argtypes = [P, I64, P, I64, P, I64, P, I64, I64, I64, ctypes.POINTER(I64), P, P, P, P, I64, I64, INT, P, I64, P]
+    L.esp_sandwich_rmsnorm.argtypes = [P, P, P, P, P, I64, I64, INT, F64, P, P, P, I64, I64, F64, INT, P]
     return L
 
 
@@ -59,3 +60,10 @@ def test_lora_overlap_refused(lib, x, xs, y, ys, out, os, needle):
     assert rc == 1 and needle in lib.esp_last_error().decode()
     one = lib.esp_lora(x, xs, y, ys, x, os, 16, 1, 64, 1, (I64 * 1)(64), 16, 16, 16, 16, 1, 16, 1, 16, 1 << 20, None)
     assert one == 1 and "overlaps x" in lib.esp_last_error().decode()
+
+
+def test_sandwich_of_no_rows(lib):
+    """A batch of no rows, whose tensors have no address, is no error; what does not fit is one even so."""
+    none = lambda D, dtype=1: lib.esp_sandwich_rmsnorm(None, None, None, 16, None, 0, 0, 0, 1.0, 16, None, None, 0, D, 1e-6, dtype, None)  # noqa: E731
+    assert none(64) == 0
+    assert none(12) == 1 and none(64, 2) == 1

@@ -134,18 +134,18 @@ using namespace esp;
 extern "C" int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d2, const void* w_post, const void* gate,
                                     int64_t gate_row, int64_t gate_col, int gate_sigmoid, double scale, const void* w_pre,
                                     void* h_out, void* out, int64_t T, int64_t D, double eps, int dtype, void* stream) {
-    ESP_REQUIRE(h && d1 && w_pre && h_out && out, "sandwich_rmsnorm: null pointer");
     ESP_REQUIRE(dtype == ESP_BF16 || dtype == ESP_F16, "sandwich_rmsnorm: dtype must be bf16 or fp16");
     ESP_REQUIRE(D > 0 && D % 8 == 0 && D <= NORM_MAX_D, "sandwich_rmsnorm: D must be a positive multiple of 8, at most %d",
                 NORM_MAX_D);
     ESP_REQUIRE(T < (1 << 24), "sandwich_rmsnorm: at most 2^24 - 1 rows");
+    if (T <= 0) return esp_host::ok();                       // (no rows have no address)
+    ESP_REQUIRE(h && d1 && w_pre && h_out && out, "sandwich_rmsnorm: null pointer");
     ESP_REQUIRE(((uintptr_t)h | (uintptr_t)d1 | (uintptr_t)d2 | (uintptr_t)w_post | (uintptr_t)w_pre | (uintptr_t)h_out |
                  (uintptr_t)out) % 16 == 0, "sandwich_rmsnorm: every tensor must be 16-byte aligned");
     ESP_REQUIRE(gate_row >= 0 && (gate_col == 0 || gate_col == 1),
                 "sandwich_rmsnorm: a gate has a row stride of at least 0 and a column stride of 0 (one a row) or 1");
     ESP_REQUIRE(!gate || (gate_col == 0 ? (uintptr_t)gate % 2 == 0 : ((uintptr_t)gate % 16 == 0 && gate_row % 8 == 0)),
                 "sandwich_rmsnorm: a gate an element must have 16-byte aligned rows");
-    if (T <= 0) return esp_host::ok();
     SandwichArgs a;
     a.h = static_cast<const uint16_t*>(h);
     a.d1 = static_cast<const uint16_t*>(d1);
