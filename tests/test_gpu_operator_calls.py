@@ -48,3 +48,30 @@ def test_sandwich_of_no_rows(dev, ext, gate):
     out = torch.empty_like(rows)
     ext.sandwich_rmsnorm(rows, rows, rows, w, g, True, 0.5, w, 1e-6, rows, out)
     assert out.shape == (0, 64)
+
+
+@pytest.mark.parametrize("T", [1, 9, 700])
+def test_sandwich_in_place(dev, ext, T):
+    """Either output in the place of h, a delta or a whole gate: the bits of outputs of their own."""
+    gen = torch.Generator().manual_seed(T)
+    rnd = lambda *s: torch.randn(s, generator=gen).to(torch.bfloat16).to(dev)  # noqa: E731
+    tensors = {n: rnd(T, 520) for n in ("h", "d1", "d2", "gate")}
+    post, pre = rnd(520), rnd(520)
+
+    def run(ho, out):
+        t = {n: v.clone() for n, v in tensors.items()}
+        ho, out = (t[n] if n else torch.empty_like(t["h"]) for n in (ho, out))
+        ext.sandwich_rmsnorm(t["h"], t["d1"], t["d2"], post, t["gate"], True, 0.5, pre, 1e-6, ho, out)
+        return ho.view(torch.int16), out.view(torch.int16)
+
+    want = run(None, None)
+    for ho, out in (("h", None), ("h", "d1"), ("h", "d2"), ("h", "gate"), ("d1", "h"), ("gate", "d1"), ("d2", "gate")):
+        assert all(torch.equal(w, g) for w, g in zip(want, run(ho, out))), (ho, out)
+    for ho, out in (("h", "h"), ("d1", "d1")):
+        with pytest.raises(RuntimeError, match="overlap"):
+            run(ho, out)
+    if T == 1:
+        return
+    both = rnd(T + 1, 520)                                   # a row further
+    with pytest.raises(RuntimeError, match="overlap"):
+        ext.sandwich_rmsnorm(tensors["h"], both[1:], None, post, None, False, 1.0, pre, 1e-6, torch.empty_like(tensors["h"]), both[:T])

@@ -67,3 +67,21 @@ def test_sandwich_of_no_rows(lib):
     none = lambda D, dtype=1: lib.esp_sandwich_rmsnorm(None, None, None, 16, None, 0, 0, 0, 1.0, 16, None, None, 0, D, 1e-6, dtype, None)  # noqa: E731
     assert none(64) == 0
     assert none(12) == 1 and none(64, 2) == 1
+
+
+FAR = 1 << 20                                                # 4 rows of 64 elements of 16 bits: 512 bytes a tensor
+
+
+@pytest.mark.parametrize("over,needle", [
+    (dict(out=0), "two outputs"), (dict(out=2 * FAR, ho=2 * FAR + 256), "two outputs"),
+    (dict(ho=128), "other rows"), (dict(out=FAR + 128), "other rows"), (dict(out=3 * FAR - 128), "other rows"),
+    (dict(out=4 * FAR - 384), "weight"), (dict(ho=5 * FAR), "weight"), (dict(out=6 * FAR), "gate"),
+    (dict(out=6 * FAR, row=64, col=0), "gate"), (dict(out=6 * FAR + 128, row=64), "gate"), (dict(ho=6 * FAR, row=72), "gate")])
+def test_sandwich_overlap_refused(lib, over, needle):
+    """An output over another one, another row of an input, a weight, or a gate that other workgroups read: refused."""
+    a = dict(ho=0, out=7 * FAR, row=0, col=1)                # h_out = h; h, d1, d2, the weights and the gate far apart
+    a.update(over)
+    at = lambda n: FAR + n  # noqa: E731
+    rc = lib.esp_sandwich_rmsnorm(at(0), at(FAR), at(3 * FAR), at(4 * FAR), at(6 * FAR), a["row"], a["col"], 0, 1.0, at(5 * FAR),
+                                  at(a["ho"]), at(a["out"]), 4, 64, 1e-6, 1, None)
+    assert rc == 1 and needle in lib.esp_last_error().decode()
