@@ -3,6 +3,8 @@ buffer side by side, calls that would overwrite what they read."""
 import pytest
 import torch
 
+from vllm_espalier import linear as LN
+from vllm_espalier import workloads as WL
 from vllm_espalier.adapters import Adapters
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +77,38 @@ def test_sandwich_in_place(dev, ext, T):
     both = rnd(T + 1, 520)                                   # a row further
     with pytest.raises(RuntimeError, match="overlap"):
         ext.sandwich_rmsnorm(tensors["h"], both[1:], None, post, None, False, 1.0, pre, 1e-6, torch.empty_like(tensors["h"]), both[:T])
+
+
+VIEWS = {"transposed": lambda rnd, T: rnd(256, T).t(), "every other column": lambda rnd, T: rnd(T, 512)[:, ::2],
+         "odd stride": lambda rnd, T: rnd(T, 259)[:, :256], "odd start": lambda rnd, T: rnd(T * 256 + 1)[1:].view(T, 256),
+         "expanded": lambda rnd, T: rnd(1, 256).expand(T, 256)}
+
+
+@pytest.mark.parametrize("T", [1, 5, 1300])
+@pytest.mark.parametrize("view", VIEWS)
+def test_lora_rows_of_any_strides(dev, view, T):
+    gen = torch.Generator().manual_seed(T)
+    rnd = lambda *s: torch.randn(s, generator=gen).to(torch.bfloat16).to(dev)  # noqa: E731
+    store = _store(256, [128, 16], [8, 20], torch.bfloat16, gen, dev)
+    x, y = VIEWS[view](rnd, T), rnd(T, 144)
+    rows = torch.stack([torch.randint(-1, 2, (T,), generator=gen), torch.full((T,), 7)], 1).to(torch.int32).to(dev)[:, 0]
+    plain = x.clone(memory_format=torch.contiguous_format)
+    want = store.apply(plain, y, rows.clone(memory_format=torch.contiguous_format), out=torch.empty_like(y))
+    got = store.apply(x, y, rows, out=torch.empty_like(y))
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and (T < 5 or not torch.equal(got, y))
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("view", ["transposed", "every other column", "odd stride"])
+def test_layer_rows_of_any_strides(dev, fused, view):
+    """A layer takes the rows with adapters that it takes without."""
+    gen = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(s, generator=gen).to(torch.bfloat16).to(dev)  # noqa: E731
+    layer = LN.TrellisLinear([WL.matrix(256, 128, 4, "int6", torch.Generator(device=dev).manual_seed(1), dev)], 128, fused)
+    store = layer.attach_adapters(2, 8)
+    for i in range(2):
+        store.load(i, [rnd(8, 256) / 16], [rnd(128, 8)], 0.5)
+    x = VIEWS[view](rnd, 5)
+    rows = torch.tensor([0, 9, 1, 9, -1, 9, 1, 9, 0, 9], dtype=torch.int32, device=dev)[::2]
+    want = layer(x.contiguous(), rows.contiguous())
+    assert torch.equal(layer(x, rows).view(torch.int16), want.view(torch.int16)) and not torch.equal(want, layer(x))

@@ -112,7 +112,5 @@ class Adapters:
         do not depend on the other rows."""
         self.check_rows(x)
         out = y if out is None else out
-        if x.stride(-1) != 1:
-            x = x.contiguous()
         ext().lora(x, y, out, rows, self.a, self.b, self.ranks, self.scales, self.out_features)
         return out

@@ -787,13 +787,19 @@ void sandwich_rmsnorm(const at::Tensor& h, const at::Tensor& d1, const c10::opti
                               w_pre.data_ptr(), h_out.data_ptr(), out.data_ptr(), T, D, eps, dtype_code(h), cur_stream()));
 }
 
-// esp_lora (csrc/lora.hip): out = y + the rows' own adapters' products; the layer's matrices of n_cols columns side by side
-void lora(const at::Tensor& x, const at::Tensor& y, at::Tensor out, const at::Tensor& rows, const at::Tensor& a,
+// esp_lora (csrc/lora.hip): out = y + the rows' own adapters' products; the layer's matrices of n_cols columns side by side. x and
+// rows of any strides: copied where the launches cannot read them in place (columns apart, rows that overlap or do not start at
+// multiples of 8 bytes)
+void lora(const at::Tensor& x_any, const at::Tensor& y, at::Tensor out, const at::Tensor& rows_any, const at::Tensor& a,
           const at::Tensor& b, const at::Tensor& ranks, const at::Tensor& scales, const std::vector<int64_t>& n_cols) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1), "x: [T, K], unit column stride");
-    const auto t = x.scalar_type();
+    TORCH_CHECK(x_any.is_cuda() && x_any.dim() == 2, "x: [T, K]");
+    const auto t = x_any.scalar_type();
     TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, "x: bf16 or fp16");
-    const int64_t T = x.size(0), K = x.size(1), S = (int64_t)n_cols.size();
+    const int64_t T = x_any.size(0), K = x_any.size(1), S = (int64_t)n_cols.size();
+    const bool in_place = x_any.stride(1) == 1 && (uintptr_t)x_any.data_ptr() % 8 == 0 &&
+                          (T <= 1 || (x_any.stride(0) >= K && x_any.stride(0) % 4 == 0));
+    const at::Tensor x = in_place ? x_any : x_any.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor rows = rows_any.contiguous();
     check(a, t, "a");
     check(b, t, "b");
     check(ranks, at::kInt, "ranks");
