@@ -1,6 +1,8 @@
 """Calls of the adapters, the verification and the norms around a block that have to be refused, or must leave nothing behind, on
 the CPU: the package's own checks in front of the extension, and the C ABI's before any HIP call."""
 import ctypes
+import gc
+import weakref
 from pathlib import Path
 
 import pytest
@@ -85,3 +87,21 @@ def test_sandwich_overlap_refused(lib, over, needle):
     rc = lib.esp_sandwich_rmsnorm(at(0), at(FAR), at(3 * FAR), at(4 * FAR), at(6 * FAR), a["row"], a["col"], 0, 1.0, at(5 * FAR),
                                   at(a["ho"]), at(a["out"]), 4, 64, 1e-6, 1, None)
     assert rc == 1 and needle in lib.esp_last_error().decode()
+
+
+def test_loaded_parameters_leave_no_graph():
+    """Parameters that require grad, loaded with grad mode on: the store's tensors stay plain, and hold none of what was loaded."""
+    store = Adapters(32, [16, 32], slots=2, max_rank=8, device="cpu")
+    kept = []
+    for k in range(2):
+        a = [torch.nn.Parameter(torch.randn((4, 32))) for _ in range(2)]
+        b = [torch.nn.Parameter(torch.randn((n, 4))) for n in (16, 32)]
+        store.load(k, a, [p * 2 for p in b])
+        kept += [weakref.ref(p) for p in a + b]
+        assert torch.equal(store.a[k, 1, 0, 0, :, :4].transpose(0, 1).reshape(4, 32), a[1].detach().to(torch.bfloat16))
+    store.clear(0)
+    for t in (store.a, store.b, store.ranks, store.scales):
+        assert not t.requires_grad and t.grad_fn is None
+    del a, b
+    gc.collect()
+    assert not any(r() is not None for r in kept)

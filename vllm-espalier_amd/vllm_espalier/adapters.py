@@ -62,10 +62,12 @@ class Adapters:
         self.ranks = torch.zeros((self.slots, S), dtype=torch.int32, device=device)
         self.scales = torch.zeros((self.slots, S), dtype=torch.float32, device=device)
 
+    @torch.no_grad()
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """Put an adapter into a slot: a[s] [rank_s, in_features] and b[s] [out_features[s], rank_s] for matrix s, None for
-        both where it leaves the matrix alone; its product with a row is scaled by `scale` (alpha / rank). Runs on the
-        current stream; rows that name the slot must not be in flight on another one."""
+        both where it leaves the matrix alone; its product with a row is scaled by `scale` (alpha / rank). Values are copied:
+        tensors that require grad may be given, and the store keeps nothing of them. Runs on the current stream; rows that name
+        the slot must not be in flight on another one."""
         self._slot(slot)
         if len(a) != len(self.out_features) or len(b) != len(self.out_features):
             raise ValueError(f"an adapter has one A and one B for each of the {len(self.out_features)} matrices")
@@ -91,6 +93,7 @@ class Adapters:
                 self.ranks[slot, s] = rank
             col += self.col_tiles[s]
 
+    @torch.no_grad()
     def clear(self, slot: int) -> None:
         """Empty a slot: its rows are left as the base layer made them."""
         self._slot(slot)
