@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from vllm_espalier import linear as LN
+from vllm_espalier import workloads as WL
 from vllm_espalier.adapters import Adapters
 
 LIB = Path(__file__).resolve().parent.parent / "vllm-espalier_amd" / "vllm_espalier" / "libespalier_hip.so"
@@ -105,3 +106,21 @@ def test_loaded_parameters_leave_no_graph():
     del a, b
     gc.collect()
     assert not any(r() is not None for r in kept)
+
+
+def test_adapters_move_with_their_layer():
+    """To another device (that of no data here) with the layer's buffers, before the adapters are attached or after; a change of
+    dtype, which is no move, leaves them as they are."""
+    gen = torch.Generator().manual_seed(1)
+    mats = [WL.matrix(128, n, 4, "int6", gen, torch.device("cpu")) for n in (128, 256)]
+    layer = LN.TrellisLinear(mats, 384, False)
+    store = layer.attach_adapters(2, 8, torch.float16)
+    a, scales = store.a, store.scales
+    layer.float()
+    layer.to("cpu")
+    assert store.a is a and store.scales is scales and store.a.dtype == torch.float16 and store.scales.dtype == torch.float32
+    outer = torch.nn.Sequential(layer).to("meta")
+    assert outer[0].adapters is store and layer.trellis_0.device.type == "meta"
+    for t in (store.a, store.b, store.ranks, store.scales):
+        assert t.device.type == "meta"
+    assert layer.attach_adapters(2, 8).a.device.type == "meta"

@@ -62,6 +62,12 @@ class Adapters:
         self.ranks = torch.zeros((self.slots, S), dtype=torch.int32, device=device)
         self.scales = torch.zeros((self.slots, S), dtype=torch.float32, device=device)
 
+    def to(self, device):
+        """The store on another device (its dtypes stay); where it is there already, its addresses stay too."""
+        for name in ("a", "b", "ranks", "scales"):
+            setattr(self, name, getattr(self, name).to(device))
+        return self
+
     @torch.no_grad()
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """Put an adapter into a slot: a[s] [rank_s, in_features] and b[s] [out_features[s], rank_s] for matrix s, None for

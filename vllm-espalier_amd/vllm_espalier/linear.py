@@ -105,6 +105,13 @@ class TrellisLinear(torch.nn.Module):
     def tensors(self, name: str) -> list[torch.Tensor]:
         return [getattr(self, f"{name}_{i}") for i in range(len(self.mats))]
 
+    def _apply(self, fn, *args, **kwargs):
+        """A move of the layer's buffers takes its adapters along."""
+        super()._apply(fn, *args, **kwargs)
+        if self.adapters is not None:
+            self.adapters.to(self.trellis_0.device)
+        return self
+
     def attach_adapters(self, slots: int, max_rank: int, dtype=torch.bfloat16):
         """A store of low-rank adapters for this layer (adapters.Adapters, to load into), which forward adds to the rows that
         name its slots. dtype: that of the rows."""
@@ -112,7 +119,7 @@ class TrellisLinear(torch.nn.Module):
         if not self.mats:
             raise RuntimeError("this layer has no matrices to put adapters beside")
         self.adapters = Adapters(self.mats[0].in_features, [m.out_features for m in self.mats], slots, max_rank, dtype,
-                                 self.mats[0].trellis.device)
+                                 self.trellis_0.device)
         return self.adapters
 
     def forward(self, x: torch.Tensor, adapter_rows: torch.Tensor | None = None) -> torch.Tensor:
