@@ -112,3 +112,26 @@ def test_layer_rows_of_any_strides(dev, fused, view):
     rows = torch.tensor([0, 9, 1, 9, -1, 9, 1, 9, 0, 9], dtype=torch.int32, device=dev)[::2]
     want = layer(x.contiguous(), rows.contiguous())
     assert torch.equal(layer(x, rows).view(torch.int16), want.view(torch.int16)) and not torch.equal(want, layer(x))
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_layer_with_adapters_compiled(dev, fused):
+    """espalier::add_adapters through torch.library's own checks, and a layer with adapters traced whole: the eager bits, with
+    other rows and after a slot is loaded anew too."""
+    gen = torch.Generator().manual_seed(7)
+    rnd = lambda *s: torch.randn(s, generator=gen).to(torch.bfloat16).to(dev)  # noqa: E731
+    mats = [WL.matrix(256, n, 4, "int6", torch.Generator(device=dev).manual_seed(n), dev) for n in (256, 128)]
+    layer = LN.TrellisLinear(mats, 384, fused)
+    store = layer.attach_adapters(2, 8)
+    load = lambda i: store.load(i, [rnd(8, 256) / 16, None], [rnd(256, 8), None], 0.5)  # noqa: E731
+    load(0), load(1)
+    x, rows = rnd(5, 256), torch.tensor([0, -1, 1, 1, 0], dtype=torch.int32, device=dev)
+    torch.library.opcheck(torch.ops.espalier.add_adapters.default,
+                          (rnd(5, 384), x, rows, store.a, store.b, store.ranks, store.scales, store.out_features),
+                          test_utils=("test_schema", "test_faketensor"))
+    traced = torch.compile(layer, backend="aot_eager", fullgraph=True)
+    for k in range(3):
+        x, rows = rnd(5, 256), (rows + k) % 3 - 1
+        with torch.no_grad():
+            assert torch.equal(traced(x, rows).view(torch.int16), layer(x, rows).view(torch.int16)), k
+        load(k % 2)

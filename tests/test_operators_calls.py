@@ -7,8 +7,10 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from vllm_espalier import linear as LN
+from vllm_espalier import ops  # noqa: F401  (registers the espalier::* ops)
 from vllm_espalier import workloads as WL
 from vllm_espalier.adapters import Adapters
 
@@ -124,3 +126,15 @@ def test_adapters_move_with_their_layer():
     for t in (store.a, store.b, store.ranks, store.scales):
         assert t.device.type == "meta"
     assert layer.attach_adapters(2, 8).a.device.type == "meta"
+
+
+def test_add_adapters_fake_form():
+    """Under fake tensors the op gives nothing, reaches no extension, and is known to change y alone."""
+    with FakeTensorMode():
+        store = Adapters(64, [32], slots=1, max_rank=4, device="cpu")
+        y = torch.empty((3, 32), dtype=torch.bfloat16)
+        got = torch.ops.espalier.add_adapters(y, torch.empty((3, 64), dtype=torch.bfloat16), torch.empty((3,), dtype=torch.int32),
+                                              store.a, store.b, store.ranks, store.scales, store.out_features)
+    assert got is None
+    args = torch.ops.espalier.add_adapters.default._schema.arguments
+    assert [a.name for a in args if a.alias_info is not None and a.alias_info.is_write] == ["y"]
