@@ -135,3 +135,19 @@ def test_layer_with_adapters_compiled(dev, fused):
         with torch.no_grad():
             assert torch.equal(traced(x, rows).view(torch.int16), layer(x, rows).view(torch.int16)), k
         load(k % 2)
+
+
+@pytest.mark.parametrize("T", [384, 700, 1151, 1152])
+@pytest.mark.parametrize("slots", [16, 17, 40])
+def test_lora_bits_whatever_the_slots(dev, T, slots):
+    """As many slots as let the launches for many rows run, and more: the bits of short batches."""
+    print(f"lora {T} rows, {slots} slots", flush=True)
+    gen = torch.Generator().manual_seed(T)
+    store = _store(512, [1024, 640], [16, 64, 40, 9] * 4, torch.bfloat16, gen, dev, slots=slots)
+    x = torch.randn((T, 512), generator=gen).to(torch.bfloat16).to(dev)
+    y = torch.randn((T, 1664), generator=gen).to(torch.bfloat16).to(dev)
+    for rows in (torch.randint(-1, slots + 1, (T,), generator=gen), torch.arange(T) * 17 // T):
+        rows = rows.to(torch.int32).to(dev)
+        got = store.apply(x, y, rows, out=torch.full_like(y, float("nan")))
+        short = torch.cat([store.apply(x[t:t + 90], y[t:t + 90].clone(), rows[t:t + 90]) for t in range(0, T, 90)])
+        assert torch.equal(got.view(torch.int16), short.view(torch.int16))

@@ -23,6 +23,7 @@ def lib(ext):
     L = ctypes.CDLL(str(LIB))
     L.esp_last_error.restype = ctypes.c_char_p
     L.esp_lora.argtypes = [P, I64, P, I64, P, I64, P, I64, I64, I64, ctypes.POINTER(I64), P, P, P, P, I64, I64, INT, P, I64, P]
+    L.esp_lora_scratch.argtypes, L.esp_lora_scratch.restype = [I64] * 4, I64
     L.esp_sandwich_rmsnorm.argtypes = [P, P, P, P, P, I64, I64, INT, F64, P, P, P, I64, I64, F64, INT, P]
     return L
 
@@ -138,3 +139,12 @@ def test_add_adapters_fake_form():
     assert got is None
     args = torch.ops.espalier.add_adapters.default._schema.arguments
     assert [a.name for a in args if a.alias_info is not None and a.alias_info.is_write] == ["y"]
+
+
+@pytest.mark.parametrize("T", [1, 16, 383, 384, 512, 1000, 1151, 1152, 4096])
+@pytest.mark.parametrize("N,S,R", [(5120, 3, 64), (2048, 1, 128), (64, 1, 16)])
+def test_lora_scratch_of_either_launches(lib, T, N, S, R):
+    """The size does not know the slots, which choose between the launches for few and for many rows below 1152: it covers the four
+    sums of 16 x 16 that the few keep a rank tile and 16 rows, and from there on the many's operands and exponents."""
+    tiles = -(-T // 16) * S * (R // 16)
+    assert lib.esp_lora_scratch(T, N, S, R) >= tiles * (4 * 256 if T < 1152 else 256 + 16)

@@ -877,15 +877,28 @@ int lora_launch(const LoraArgs& a, bool all, hipStream_t st) {
 // ======================================================================================================================
 using namespace esp;
 
-// Whether T rows run as the launches for many rows. They take longer to begin with (a CU goes through a tile's adapters one after
-// the other) and less a row, column and rank. us for T rows, few / many (bf16, graph replays, three requests one after the other):
-//   2048 -> 4096 + 512 + 512, ranks 16: 8.3 / 9.1 at 384, 11.6 / 11.6 at 512; ranks up to 64: 14.0 / 9.8, 17.9 / 12.5
-//   2048 -> 2048, rank 128: 11.9 / 14.6 at 256, 14.7 / 10.8 at 384, 24.1 / 14.9 at 1024
-//   512 -> 2048, ranks 64: 10.4 / 12.0 at 512, 10.0 / 9.5 at 768; ranks 16: 7.4 / 8.8 at 768, 10.0 / 11.0 at 1024
-//   2048 -> 512 + 512, ranks 32: 9.6 / 9.1 at 768, 11.1 / 11.5 at 1024, 13.0 / 11.9 at 1280
-// and 32 requests one after the other, 2048 -> 4096 + 512 + 512, ranks up to 64: 13.8 / 27.2 at 256, 17.6 / 24.8 at 384, 15.0 / 18.5
-static bool lora_many(int64_t T, int64_t N, int64_t rank_tiles) {
-    return T >= 1152 || (T >= 384 && T * N * rank_tiles >= 6 << 20);
+// Whether T rows run as the launches for many rows. They take longer to begin with and less a row, column and rank; but a workgroup of
+// theirs goes through all adapters of its 64 rows one after the other, where the few's are dealt out. How many a batch mixes the host
+// does not know, only how many there are: up to 16, the rows and the work decide (they cross between 4 and 8 Mi); past 16, a mixed
+// batch would lose up to 90 us where a batch of few adapters gains up to 11, so the few's run until 1152 rows, where their own cost
+// a row has caught up. us for T rows, few / many (bf16, graph replays): the adapters in runs of rows; 32 rows of any behind a prompt of
+// two; all in random order:
+//   2048 -> 4096 + 512 + 512, ranks 16, 3 adapters: 8/9  13/14  14/14 at 384, 10/10  15/14  17/15 at 768, 15/10  19/15  25/16 at 1151
+//     8 adapters: 8/12  23/26  24/28 at 384, 11/10  26/31  30/31 at 768, 16/13  28/28  44/34 at 1151
+//     16 adapters: 9/10  34/52  38/54 at 512, 12/12  34/44  42/53 at 768, 20/13  36/49  59/56 at 1151
+//     32 adapters: 11/19  37/76  42/84 at 384, 15/14  40/70  48/85 at 768, 20/15  42/70  70/92 at 1151
+//   ranks 16 and 64, 3 adapters: 11/10  15/14  16/15 at 384, 15/11  20/19  23/20 at 768, 20/13  24/20  32/22 at 1151
+//     8 adapters: 12/12  32/34  36/36 at 384, 18/12  36/43  46/44 at 768, 23/16  36/39  67/46 at 1151
+//     16 adapters: 15/11  50/61  60/64 at 512, 18/16  46/61  68/79 at 768, 26/18  50/69  97/84 at 1151
+//     32 adapters: 18/25  47/84  65/98 at 384, 21/21  57/101  86/125 at 768, 28/21  55/98  128/137 at 1151
+//   2048 -> 2048, rank 128, 8 adapters: 16/15  31/50  37/52 at 384, 18/14  55/51  62/52 at 768, 22/17  53/59  76/59 at 1151
+//     32 adapters: 17/37  43/116  67/157 at 384, 25/26  76/105  122/165 at 768, 31/25  92/153  153/187 at 1151
+//   512 -> 2048, ranks 64, 3 adapters: 10/9  13/15  14/15 at 384, 10/10  17/15  18/16 at 768; 8 adapters: 10/12  20/29  21/30 at 384,
+//     10/11  26/26  36/30 at 768, 13/13  35/30  43/32 at 1151
+//   2048 -> 512 + 512, ranks 32, 8 adapters: 8/12  16/27  16/28 at 384, 10/10  16/24  19/29 at 768, 13/12  21/28  24/28 at 1151
+constexpr int64_t LORA_MANY_ROWS = 1152;       // from here on whatever the adapters
+static bool lora_many(int64_t T, int64_t N, int64_t rank_tiles, int64_t slots) {
+    return T >= LORA_MANY_ROWS || (slots <= 16 && T >= 384 && T * N * rank_tiles >= 6 << 20);
 }
 
 // The workgroups that a row tile's adapters are dealt to (few rows): up to one a row, and no more than 32 over all tiles, since
@@ -903,7 +916,8 @@ static int lora_spread(int64_t T, int64_t cols) {
 extern "C" int64_t esp_lora_scratch(int64_t T, int64_t N, int64_t n_shards, int64_t R) {
     if (T <= 0 || N <= 0 || n_shards <= 0 || R <= 0) return 0;
     const int64_t rows = (T + 15) / 16 * 16, ranks = n_shards * ((R + 15) / 16);
-    return lora_many(T, N, ranks) ? rows * ranks * 17 : rows * ranks * 16 * (LORA_RUNS / 4);
+    // (below LORA_MANY_ROWS either launches may run, as the slots are, and the few's need more)
+    return T >= LORA_MANY_ROWS ? rows * ranks * 17 : rows * ranks * 16 * (LORA_RUNS / 4);
 }
 
 extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out, int64_t out_stride,
@@ -946,7 +960,7 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
                 "lora: out overlaps x, which other workgroups still read");
     ESP_REQUIRE(out == y || !esp_host::rows_meet(out, out_stride * 2, N * 2, y, y_stride * 2, N * 2, T),
                 "lora: out overlaps y without being y");
-    const bool all = lora_many(T, N, n_shards * (R / 16));
+    const bool all = lora_many(T, N, n_shards * (R / 16), slots);
     const int64_t tiles = (T + 15) / 16;
     a.x = static_cast<const uint16_t*>(x);
     a.x_stride = x_stride;
