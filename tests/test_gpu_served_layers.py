@@ -84,3 +84,11 @@ def test_plain_layers_stay_fused(dev, monkeypatch):
     monkeypatch.setattr(S, "FUSE_NORMS", False)
     monkeypatch.setattr(S, "MULTI_ATTN", False)
     assert torch.equal(_run(dec, slice(0, 1)), got)
+
+
+def test_algorithmic_bytes_count_every_norm(dev):
+    """The weights of the norms behind the blocks: two a layer, of which the last MoE's runs before the head."""
+    picks = [torch.empty((0,), dtype=torch.int32)] * 2
+    plain, posts = _decoder(dev), S.SyntheticDecoder(n_layers=2, seed=9, device=dev, E=16, vocab=VOCAB, post_norms=True)
+    assert posts.algorithmic_bytes(picks, 3) - plain.algorithmic_bytes(picks, 3) == 4 * S.D_MODEL * 2
+    assert posts.algorithmic_bytes(picks, 3, head=False) - plain.algorithmic_bytes(picks, 3, head=False) == 3 * S.D_MODEL * 2

@@ -279,15 +279,15 @@ class SyntheticDecoder:
 
     def algorithmic_bytes(self, picks: list[torch.Tensor], tokens: int, head: bool = True) -> int:
         """Weight bytes a pass over `tokens` rows reads: trellis + suh + svh of q/k/v/o, of the shared expert and of
-        every distinct routed expert picked (picks from an eager forward), the bf16 router, the RMSNorm weights, one
-        embedding row a token, and the head."""
+        every distinct routed expert picked (picks from an eager forward), the bf16 router, the RMSNorm weights (behind
+        the blocks too), one embedding row a token, and the head. Adapters, of which rows name the slots, are not in it."""
         total = tokens * D_MODEL * 2
         for L, ids in zip(self.layers, picks):
             total += WL.nbytes(L.qkv.mats) + WL.nbytes(L.o.mats) + WL.nbytes(L.shared)
-            total += L.router.numel() * 2 + (L.norm1.numel() + L.norm2.numel()) * 2
+            total += L.router.numel() * 2 + WL.norm_bytes(L.norm1, L.norm2, L.post_in, L.post_o)
             for u in ids.tolist():
                 if u < len(L.experts):
                     total += WL.nbytes(L.experts[u])
         if head:
-            total += WL.nbytes(self.head.mats) + self.final_norm.numel() * 2
+            total += WL.nbytes(self.head.mats) + WL.norm_bytes(self.final_norm, self.final_post)
         return total

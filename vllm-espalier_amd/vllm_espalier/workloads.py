@@ -42,3 +42,8 @@ def matrix(K: int, N: int, bits: int, grid: str, gen: torch.Generator, device) -
 def nbytes(mats) -> int:
     """Algorithmic bytes of matrices: trellis + suh + svh."""
     return sum(m.trellis.numel() * 2 + (m.suh.numel() + m.svh.numel()) * 2 for m in mats)
+
+
+def norm_bytes(*weights) -> int:
+    """Bytes of bf16 norm weights, None for one that is not there."""
+    return sum(w.numel() * 2 for w in weights if w is not None)
