@@ -422,11 +422,13 @@ int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d2, const vo
 /* For row m of adapter a = rows[m] (int32 on the device) and column n of matrix s of the layer (n_shards, 1 to 4, side by
  * side in y from column 0, n_cols[s] columns each, multiples of 16):
  *   out[m][n] = y[m][n] + sum_{j < r} (scales[a][s] * sum_k x[m][k] * A[a][s][j][k]) * B[a][n][j],   r = ranks[a][s],
- * summed in fp32 and rounded once. A row whose adapter is outside [0, slots), and the columns of a matrix for which its adapter
- * has no ranks, keep y's bits. x [T][K], y and out [T][N] with row strides, N = sum(n_cols); ranks int32 and scales fp32
- * [slots][n_shards] on the device. out may be y (in place), and must else overlap neither y nor x (refused), nor any other input;
- * columns past N are left as they are. dtype ESP_BF16 or ESP_F16 for x, y, out, A and B. K a multiple of 16, T < 2^24, at most
- * 2^24 - 1 blocks of 64 rows and 128 columns of a matrix.
+ * summed in fp32 and rounded to dtype once. Between the products, the scaled sums over k are held as a value of dtype and the rest
+ * of it in dtype too: off by at most 2^-17 of themselves in bf16, by 2^-23 of the largest of a row's 16 ranks in fp16. A row whose
+ * adapter is outside [0, slots), and the columns of a matrix for which its adapter has no ranks, keep y's bits. x [T][K], y and
+ * out [T][N] with row strides, N = sum(n_cols); ranks int32 and scales fp32 [slots][n_shards] on the device. out may be y (in
+ * place), and must else overlap neither y nor x (refused), nor any other input; columns past N are left as they are. dtype
+ * ESP_BF16 or ESP_F16 for x, y, out, A and B. K a multiple of 16, T < 2^24, at most 2^24 - 1 blocks of 64 rows and 128 columns of
+ * a matrix.
  * A and B are laid out as the matrix instructions read them, R (a multiple of 16, at most 256) ranks a slot, zeros where an
  * adapter has nothing (past its rank in its last 16 ranks, past K, past a matrix's columns); 16-rank tiles past the rank are
  * not used, whatever they hold:
@@ -455,12 +457,14 @@ int64_t esp_lora_scratch(int64_t T, int64_t N, int64_t n_shards, int64_t R);
  * random numbers), the lowest among equal ones. A temperature below 1e-5 (or NaN) means a greedy request: draft j is accepted
  * iff it is the row's argmax (as esp_argmax: a NaN is the largest; zeros of both signs are equal), which is else the token
  * drawn.
+ * A row's exponentials are summed in fp32 within 1024 logits and in fp64 above; the race runs in fp32, with the hardware's
+ * exponential and reciprocal. A draft or a race that is decided by less than about 2^-19 of p may fall on either side.
  * tokens [B][G + 1] int32: the accepted drafts, then the token drawn, then -1; counts [B]: how many tokens; logprobs
  * [B][G + 1] fp32: log p_j of each token (of a greedy request at temperature 1), 0 past them. A row without a distribution (a
  * NaN or +inf in it, or nothing above -inf) accepts nothing and draws nothing if the request is not greedy, and its
  * log-probabilities are 0. A request with n_drafts outside [0, G] or rows outside the logits has no tokens (-1 and 0: the
- * padding of a batch). A draft outside [0, V) is never accepted. Arrays contiguous unless a stride is given; rows may start
- * at any element. B <= 2^20, G <= 1024, V <= 2^24,
+ * padding of a batch). A draft outside [0, V) is never accepted. The outputs must overlap no input, nor one another. Arrays
+ * contiguous unless a stride is given; rows may start at any element. B <= 2^20, G <= 1024, V <= 2^24,
  * B * (G + 1) * ceil(V / 4096) < 2^24.
  * scratch: esp_verify_scratch bytes, 16-byte aligned, any values. */
 int esp_verify(const void* logits, int dtype, int64_t stride, int64_t R, int64_t V, const int32_t* first,

@@ -47,7 +47,7 @@ struct LoraArgs {
     uint4* t;                                  // many: [row tiles][S * R / 16][64], finished: lane l row l % 16, ranks 8 (l / 16
                                                // % 2) .. + 8, the high parts (l < 32) or the rests
     int* e;                                    // [row tiles][S * R / 16][16]: fp16's exponents
-    int T, K, S, N, R, slots, spread;          // spread: workgroups that share a row tile's adapters (few rows)
+    int T, K, S, R, slots, spread;             // spread: workgroups that share a row tile's adapters (few rows)
     int n_cols[LORA_MAX_SHARDS], tiles0[LORA_MAX_SHARDS + 1];   // a matrix's columns, and its first tile of LORA_COLS
 };
 
@@ -294,7 +294,7 @@ __device__ __forceinline__ void lora_put(const LoraArgs& a, float sum, float sca
 // share of the rank tiles), sixteen waves, a run of the k each. t leaves finished and split. A workgroup has a CU to itself, whose
 // intake bounds it (~25 bytes a ns from memory, ~50 from the L2), so it takes x in once and keeps it in registers, G C = 4 KiB of it
 // a wave, whatever the ranks and adapters that follow, and the shares are as many as there are CUs for: 64 rows against 48 ranks of
-// 2048 are 452 KiB, where 32 rows against 96 were 520. x comes in 256 bytes of a row at a time and turns into operands through the
+// 2048 are 448 KiB (256 of x, 192 of A), where 32 rows against 96 are 512. x comes in 256 bytes of a row at a time and turns into operands through the
 // wave's own 4 KiB of shared memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a quarter-wave
 // meet in a bank either way). The next rank tile is in flight while one is multiplied and summed over the waves; the sums of a tile are
 // finished by all waves, a rank a lane (the same xor keeps its reads apart). 4096 rows of 2048 against 48 and 192 ranks: 16.4 us.
@@ -405,6 +405,8 @@ __global__ __launch_bounds__(1024) void lora_shrink_all_kernel(const LoraArgs a,
 // ------------------------------------------------------------------------------------------------------------------
 // The first product, many rows, K past 8192: 16 rows against all of an adapter's rank tiles, two a round, sixteen waves, a run of the
 // k each; x, which no wave can hold, comes in again every round. blockIdx.y: a row tile's first, third, ... adapter or the others.
+// Bound by that intake of x: 14336 -> 4096, three adapters in runs, 2048 rows against 16 ranks 17.6 us (59 MB of x, 3.3 TB/s), 4096 rows
+// 42.2 (2.8 TB/s), against 16 and 64 ranks, two rounds for a third of the rows, 56.2.
 // ------------------------------------------------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(1024) void lora_shrink_long_kernel(const LoraArgs a, int, int) {
@@ -979,7 +981,6 @@ extern "C" int esp_lora(const void* x, int64_t x_stride, const void* y, int64_t 
     a.T = (int)T;
     a.K = (int)K;
     a.S = (int)n_shards;
-    a.N = (int)N;
     a.R = (int)R;
     a.slots = (int)slots;
     a.spread = lora_spread(T, a.tiles0[n_shards]);

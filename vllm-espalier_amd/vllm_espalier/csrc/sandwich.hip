@@ -43,8 +43,11 @@ __device__ __forceinline__ void store16(uint16_t* p, uint4 v) {
 }
 
 // One workgroup of 256 a row; thread t holds elements (c * 256 + t) * 8 .. + 8. Bound by memory from a few hundred rows on (8192 x
-// 4096 with a gate an element, 336 MB: 64 us, 5.2 TB/s; a copy of such a size reaches 4.7 to 5.5), by the launch and two dependent
-// round trips below (3.3 us for one row). NT: outputs stored past the L2, see the launch.
+// 4096 with a gate an element, 336 MB: 64 us, 5.2 TB/s; a copy of such a size reaches 4.7 to 5.5), below by the launch and its chain
+// of round trips: each operand's load is waited for before the next one's begins, d1, d2, w_post, gate, h and w_pre, three to six for a
+// chunk of 2048 and, chunk after chunk, up to four times as many for 8192. One row, graph replays: 2048 with one delta and a channel
+// gate 3.7 us, with two deltas and a gate an element 4.1; 8192 8.3 and 9.7 (add_rmsnorm, which issues a row's loads together, 3.3 and
+// 6.7). NT: outputs stored past the L2, see the launch.
 template <bool NT>
 __global__ __launch_bounds__(256) void sandwich_rmsnorm_kernel(const SandwichArgs a) {
     __shared__ float part[2][4];

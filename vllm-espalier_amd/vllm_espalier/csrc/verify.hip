@@ -265,7 +265,8 @@ __device__ __forceinline__ Row verify_row(const VerifyArgs& a, int b, int j, int
 }
 
 // This thread's entries of the race from entry i0 on (RACE_GROUPS groups of 8, 2048 apart) into its best: the largest w / e with w
-// above 0, w = p without draft probabilities q (0 at the draft itself), else p - q
+// above 0, w = p without draft probabilities q (0 at the draft itself), else p - q. In fp32 with the hardware's exponential and
+// reciprocal, since only the keys' order is wanted: two that are nearer than about 2^-19 of p may change places
 struct Best {
     float key, logit;
     int idx;

@@ -19,7 +19,10 @@ def verify(logits, first, n_drafts, drafts, uniform, race, temperature, draft_pr
                  first rejected draft, p behind the last accepted one
     temperature  fp32 [B]; below 1e-5: greedy (a draft is accepted iff it is the row's argmax)
     draft_probs  fp32 [B, G, V], what the drafts were drawn from (q); None: the drafter was sure (q = 1 at its draft)
-    out          (tokens, counts, logprobs) to write into; otherwise new ones
+    out          (tokens, counts, logprobs) to write into, apart from one another and from the inputs; otherwise new ones
+
+    Acceptance is decided in 64 bits from sums of 32, the race in 32 bits: what is decided by less than about 2^-19 of p may fall on
+    either side, the same one in every call with these inputs.
 
     With fixed arrays a captured graph replays it; nothing is kept between calls, so calls on several streams do not meet."""
     return ext().verify(logits, first, n_drafts, drafts, uniform, race, temperature, draft_probs, out)
