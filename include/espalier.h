@@ -410,7 +410,7 @@ int esp_argmax(const void* logits, int64_t stride, int64_t T, int64_t N, int dty
  * out = (h_out / sqrt(mean(h_out^2) + eps)) * w_pre, h_out as stored; everything in fp32, each output rounded once. gate
  * (may be NULL: f(g) = 1): element i of row t at gate[t * gate_row + i * gate_col], gate_col 1 for a gate an element
  * (gate_row 0: one row for all), 0 for a gate a row; f is the value itself or, with gate_sigmoid, its sigmoid. h_out and
- * out may each be one of h, d1, d2 and a gate of [T][D], and must overlap nothing else, nor one another (refused). dtype
+ * out may each be one of h, d1 and d2 and hold their own row's gate, and must overlap nothing else, nor one another (refused). dtype
  * ESP_BF16 or ESP_F16 for all; [T][D] row-major, D % 8 == 0, D <= 8192, 16-byte aligned (a gate an element with rows of 16
  * bytes too). A row's bits depend on that row alone; with d2, gate and w_post NULL and scale 1 they are esp_add_rmsnorm's. */
 int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d2, const void* w_post, const void* gate,

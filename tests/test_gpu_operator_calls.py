@@ -69,6 +69,14 @@ def test_sandwich_in_place(dev, ext, T):
     want = run(None, None)
     for ho, out in (("h", None), ("h", "d1"), ("h", "d2"), ("h", "gate"), ("d1", "h"), ("gate", "d1"), ("d2", "gate")):
         assert all(torch.equal(w, g) for w, g in zip(want, run(ho, out))), (ho, out)
+    h, d1 = tensors["h"].clone(), tensors["d1"]                # a row's gate that stands in the row itself
+    for gate in (h[:, :1], h[:, 519:], h[:, 7:8]):
+        alone = [torch.empty_like(h) for _ in range(2)]
+        ext.sandwich_rmsnorm(tensors["h"], d1, None, post, gate.clone(), False, 0.5, pre, 1e-6, *alone)
+        out = torch.empty_like(h)
+        ext.sandwich_rmsnorm(h, d1, None, post, gate, False, 0.5, pre, 1e-6, h, out)
+        assert torch.equal(h.view(torch.int16), alone[0].view(torch.int16)) and torch.equal(out.view(torch.int16), alone[1].view(torch.int16))
+        h.copy_(tensors["h"])
     for ho, out in (("h", "h"), ("d1", "d1")):
         with pytest.raises(RuntimeError, match="overlap"):
             run(ho, out)

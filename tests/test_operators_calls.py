@@ -82,7 +82,7 @@ FAR = 1 << 20                                                # 4 rows of 64 elem
     (dict(out=0), "two outputs"), (dict(out=2 * FAR, ho=2 * FAR + 256), "two outputs"),
     (dict(ho=128), "other rows"), (dict(out=FAR + 128), "other rows"), (dict(out=3 * FAR - 128), "other rows"),
     (dict(out=4 * FAR - 384), "weight"), (dict(ho=5 * FAR), "weight"), (dict(out=6 * FAR), "gate"),
-    (dict(out=6 * FAR, row=64, col=0), "gate"), (dict(out=6 * FAR + 128, row=64), "gate"), (dict(ho=6 * FAR, row=72), "gate")])
+    (dict(out=6 * FAR, row=128, col=0), "gate"), (dict(ho=6 * FAR + 256, row=64, col=0), "gate"), (dict(out=6 * FAR + 128, row=64), "gate"), (dict(ho=6 * FAR, row=72), "gate")])
 def test_sandwich_overlap_refused(lib, over, needle):
     """An output over another one, another row of an input, a weight, or a gate that other workgroups read: refused."""
     a = dict(ho=0, out=7 * FAR, row=0, col=1)                # h_out = h; h, d1, d2, the weights and the gate far apart

@@ -149,15 +149,16 @@ extern "C" int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d
                 "sandwich_rmsnorm: a gate has a row stride of at least 0 and a column stride of 0 (one a row) or 1");
     ESP_REQUIRE(!gate || (gate_col == 0 ? (uintptr_t)gate % 2 == 0 : ((uintptr_t)gate % 16 == 0 && gate_row % 8 == 0)),
                 "sandwich_rmsnorm: a gate an element must have 16-byte aligned rows");
-    // A workgroup has read all of its row when it stores it: an output may be an input of whole rows, and nothing else
+    // A workgroup has read all of its row but w_pre when it stores it: an output may lie where its own row's inputs do
     const auto meet = [](const void* p, int64_t n, const void* q, int64_t m) { return q && esp_host::rows_meet(p, 0, n, q, 0, m, 1); };
     for (const void* o : {h_out, out}) {
         for (const void* i : {h, d1, d2})
-            ESP_REQUIRE(i == o || !meet(o, T * D * 2, i, T * D * 2), "sandwich_rmsnorm: an output overlaps other rows of an input");
+            ESP_REQUIRE(i == o || T == 1 || !meet(o, T * D * 2, i, T * D * 2), "sandwich_rmsnorm: an output overlaps other rows of an input");
         ESP_REQUIRE(!meet(o, T * D * 2, w_post, D * 2) && !meet(o, T * D * 2, w_pre, D * 2),
                     "sandwich_rmsnorm: an output overlaps a weight");
         const int64_t g = gate_col ? D * 2 : 2;
-        ESP_REQUIRE(!gate || (gate == o && gate_col && (gate_row == D || T == 1)) ||
+        const bool own_row = gate_row == D && (uintptr_t)gate - (uintptr_t)o <= (uintptr_t)(D * 2 - g);
+        ESP_REQUIRE(!gate || T == 1 || own_row ||
                         !(gate_row ? esp_host::rows_meet(o, D * 2, D * 2, gate, gate_row * 2, g, T) : meet(o, T * D * 2, gate, g)),
                     "sandwich_rmsnorm: an output overlaps the gate");
     }
