@@ -27,7 +27,7 @@ def test_lora_views_of_one_buffer(dev, T):
     wide = torch.randn((T, 3 * 64 + 4), generator=gen).to(torch.bfloat16).to(dev)
     before = wide.clone()
     rows = (torch.arange(T, dtype=torch.int32) % 3 - 1).to(dev)
-    want = store.apply(before[:, :64].contiguous(), before[:, 64:128].contiguous(), rows, out=torch.empty((T, N), dtype=torch.bfloat16, device=dev))
+    want = store.apply(before[:, :64].contiguous(), before[:, 64:128].contiguous(), rows)
     store.apply(wide[:, :64], wide[:, 64:128], rows, out=wide[:, 128:192])
     assert torch.equal(wide[:, 128:192].view(torch.int16), want.view(torch.int16))
     store.apply(wide[:, :64], wide[:, 64:128], rows)
@@ -75,7 +75,7 @@ def test_sandwich_in_place(dev, ext, T):
         ext.sandwich_rmsnorm(tensors["h"], d1, None, post, gate.clone(), False, 0.5, pre, 1e-6, *alone)
         out = torch.empty_like(h)
         ext.sandwich_rmsnorm(h, d1, None, post, gate, False, 0.5, pre, 1e-6, h, out)
-        assert torch.equal(h.view(torch.int16), alone[0].view(torch.int16)) and torch.equal(out.view(torch.int16), alone[1].view(torch.int16))
+        assert all(torch.equal(g.view(torch.int16), w.view(torch.int16)) for g, w in zip((h, out), alone))
         h.copy_(tensors["h"])
     for ho, out in (("h", "h"), ("d1", "d1")):
         with pytest.raises(RuntimeError, match="overlap"):

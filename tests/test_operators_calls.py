@@ -48,6 +48,8 @@ def test_rows_of_another_width_refused(monkeypatch, have, given):
         store.apply(x[0], y, rows)
     with pytest.raises(RuntimeError, match="in_features"):
         _layer(monkeypatch, have, [32])(x.view(1, 3, given), rows)
+    with pytest.raises(RuntimeError, match="in_features"):
+        torch.ops.espalier.add_adapters(y, x, rows, store.a, store.b, store.ranks, store.scales, store.out_features, have)
 
 
 @pytest.mark.parametrize("x,xs,y,ys,out,os,needle", [
@@ -70,7 +72,8 @@ def test_lora_overlap_refused(lib, x, xs, y, ys, out, os, needle):
 
 def test_sandwich_of_no_rows(lib):
     """A batch of no rows, whose tensors have no address, is no error; what does not fit is one even so."""
-    none = lambda D, dtype=1: lib.esp_sandwich_rmsnorm(None, None, None, 16, None, 0, 0, 0, 1.0, 16, None, None, 0, D, 1e-6, dtype, None)  # noqa: E731
+    none = lambda D, dtype=1: lib.esp_sandwich_rmsnorm(None, None, None, 16, None, 0, 0, 0, 1.0, 16, None, None, 0, D, 1e-6,  # noqa: E731
+                                                       dtype, None)
     assert none(64) == 0
     assert none(12) == 1 and none(64, 2) == 1
 
@@ -82,7 +85,8 @@ FAR = 1 << 20                                                # 4 rows of 64 elem
     (dict(out=0), "two outputs"), (dict(out=2 * FAR, ho=2 * FAR + 256), "two outputs"),
     (dict(ho=128), "other rows"), (dict(out=FAR + 128), "other rows"), (dict(out=3 * FAR - 128), "other rows"),
     (dict(out=4 * FAR - 384), "weight"), (dict(ho=5 * FAR), "weight"), (dict(out=6 * FAR), "gate"),
-    (dict(out=6 * FAR, row=128, col=0), "gate"), (dict(ho=6 * FAR + 256, row=64, col=0), "gate"), (dict(out=6 * FAR + 128, row=64), "gate"), (dict(ho=6 * FAR, row=72), "gate")])
+    (dict(out=6 * FAR, row=128, col=0), "gate"), (dict(ho=6 * FAR + 256, row=64, col=0), "gate"),
+    (dict(out=6 * FAR + 128, row=64), "gate"), (dict(ho=6 * FAR, row=72), "gate")])
 def test_sandwich_overlap_refused(lib, over, needle):
     """An output over another one, another row of an input, a weight, or a gate that other workgroups read: refused."""
     a = dict(ho=0, out=7 * FAR, row=0, col=1)                # h_out = h; h, d1, d2, the weights and the gate far apart

@@ -109,17 +109,11 @@ class Adapters:
         if not 0 <= slot < self.slots:
             raise ValueError(f"slot {slot} is outside [0, {self.slots})")
 
-    def check_rows(self, x: torch.Tensor) -> None:
-        """Refuse rows of another width. The padded A does not show it: 48 and 64 columns are two units of k both."""
-        if x.dim() != 2 or x.shape[1] != self.in_features:
-            raise RuntimeError(f"x: expected [T, in_features = {self.in_features}], got {tuple(x.shape)}")
-
     def apply(self, x: torch.Tensor, y: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """y [T, at least sum(out_features)] plus, for every row, the product of x [T, in_features] with the adapter in slot
         rows[t] (int32 [T], on the device; outside [0, slots): none, and the row keeps y's bits). In place unless `out` is
         given; what is written may not overlap x, nor y without being y. Columns past the matrices' are not touched. A row's bits
         do not depend on the other rows."""
-        self.check_rows(x)
         out = y if out is None else out
-        ext().lora(x, y, out, rows, self.a, self.b, self.ranks, self.scales, self.out_features)
+        ext().lora(x, y, out, rows, self.a, self.b, self.ranks, self.scales, self.out_features, self.in_features)
         return out

@@ -789,9 +789,13 @@ void sandwich_rmsnorm(const at::Tensor& h, const at::Tensor& d1, const c10::opti
 
 // esp_lora (csrc/lora.hip): out = y + the rows' own adapters' products; the layer's matrices of n_cols columns side by side. x and
 // rows of any strides: copied where the launches cannot read them in place (columns apart, rows that overlap or do not start at
-// multiples of 8 bytes)
+// multiples of 8 bytes). in_features: the width that x must have, which the padded a does not show (48 and 64 columns are two units
+// of k both); 0: any
 void lora(const at::Tensor& x_any, const at::Tensor& y, at::Tensor out, const at::Tensor& rows_any, const at::Tensor& a,
-          const at::Tensor& b, const at::Tensor& ranks, const at::Tensor& scales, const std::vector<int64_t>& n_cols) {
+          const at::Tensor& b, const at::Tensor& ranks, const at::Tensor& scales, const std::vector<int64_t>& n_cols,
+          int64_t in_features) {
+    TORCH_CHECK(in_features == 0 || (x_any.dim() == 2 && x_any.size(1) == in_features), "x: expected [T, in_features = ",
+                in_features, "], got ", x_any.sizes());
     TORCH_CHECK(x_any.is_cuda() && x_any.dim() == 2, "x: [T, K]");
     const auto t = x_any.scalar_type();
     TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, "x: bf16 or fp16");
@@ -1008,7 +1012,8 @@ PYBIND11_MODULE(espalier_ext, m) {
     m.def("embed", &embed);
     m.def("add_rmsnorm", &add_rmsnorm);
     m.def("sandwich_rmsnorm", &sandwich_rmsnorm);
-    m.def("lora", &lora);
+    m.def("lora", &lora, py::arg("x"), py::arg("y"), py::arg("out"), py::arg("rows"), py::arg("a"), py::arg("b"),
+          py::arg("ranks"), py::arg("scales"), py::arg("n_cols"), py::arg("in_features") = 0);
     m.def("verify", &verify);
     m.def("argmax", &argmax, py::arg("logits"), py::arg("ids"), py::arg("part") = py::none(),
           py::arg("counters") = py::none());

@@ -294,9 +294,9 @@ __device__ __forceinline__ void lora_put(const LoraArgs& a, float sum, float sca
 // share of the rank tiles), sixteen waves, a run of the k each. t leaves finished and split. A workgroup has a CU to itself, whose
 // intake bounds it (~25 bytes a ns from memory, ~50 from the L2), so it takes x in once and keeps it in registers, G C = 4 KiB of it
 // a wave, whatever the ranks and adapters that follow, and the shares are as many as there are CUs for: 64 rows against 48 ranks of
-// 2048 are 448 KiB (256 of x, 192 of A), where 32 rows against 96 are 512. x comes in 256 bytes of a row at a time and turns into operands through the
-// wave's own 4 KiB of shared memory (16-byte units of a row in the place of their number xor the row's: no two lanes of a quarter-wave
-// meet in a bank either way). The next rank tile is in flight while one is multiplied and summed over the waves; the sums of a tile are
+// 2048 are 448 KiB (256 of x, 192 of A), where 32 rows against 96 are 512. x comes in 256 bytes of a row at a time and turns into
+// operands through the wave's own 4 KiB of shared memory (16-byte units of a row in the place of their number xor the row's: no two
+// lanes of a quarter-wave meet in a bank either way). The next rank tile is in flight while one is multiplied and summed over the waves; the sums of a tile are
 // finished by all waves, a rank a lane (the same xor keeps its reads apart). 4096 rows of 2048 against 48 and 192 ranks: 16.4 us.
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int LORA_ALL_SMEM = 2 * LORA_RUNS * 4096;

@@ -153,7 +153,8 @@ extern "C" int esp_sandwich_rmsnorm(const void* h, const void* d1, const void* d
     const auto meet = [](const void* p, int64_t n, const void* q, int64_t m) { return q && esp_host::rows_meet(p, 0, n, q, 0, m, 1); };
     for (const void* o : {h_out, out}) {
         for (const void* i : {h, d1, d2})
-            ESP_REQUIRE(i == o || T == 1 || !meet(o, T * D * 2, i, T * D * 2), "sandwich_rmsnorm: an output overlaps other rows of an input");
+            ESP_REQUIRE(i == o || T == 1 || !meet(o, T * D * 2, i, T * D * 2),
+                        "sandwich_rmsnorm: an output overlaps other rows of an input");
         ESP_REQUIRE(!meet(o, T * D * 2, w_post, D * 2) && !meet(o, T * D * 2, w_pre, D * 2),
                     "sandwich_rmsnorm: an output overlaps a weight");
         const int64_t g = gate_col ? D * 2 : 2;

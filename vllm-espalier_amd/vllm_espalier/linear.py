@@ -128,10 +128,9 @@ class TrellisLinear(torch.nn.Module):
         if adapter_rows is not None:
             if self.adapters is None:
                 raise RuntimeError("rows name adapters, but none were attached to this layer")
-            s, rows = self.adapters, x.reshape(-1, x.shape[-1])
-            s.check_rows(rows)
-            torch.ops.espalier.add_adapters(y.view(-1, self.out_features), rows, adapter_rows.reshape(-1), s.a, s.b, s.ranks,
-                                            s.scales, s.out_features)
+            s = self.adapters
+            torch.ops.espalier.add_adapters(y.view(-1, self.out_features), x.reshape(-1, x.shape[-1]), adapter_rows.reshape(-1),
+                                            s.a, s.b, s.ranks, s.scales, s.out_features, s.in_features)
         return y
 
     def _base(self, x: torch.Tensor) -> torch.Tensor:

@@ -6,8 +6,9 @@ espalier::matmul(x, trellis, suh, svh, K, cb) -> fp16 [m, out]
 espalier::dense(x, trellis[], suh[], svh[], key) -> [m, n_out] in x's dtype
     every matrix of one vLLM layer, the Dense registered under `key` in DENSE_LAYERS.
 
-espalier::add_adapters(y!, x, rows, a, b, ranks, scales, n_cols)
-    every row's own low-rank adapter added to y [m, at least sum(n_cols)], the slots of an adapters.Adapters store.
+espalier::add_adapters(y!, x, rows, a, b, ranks, scales, n_cols, in_features=0)
+    every row's own low-rank adapter added to y [m, at least sum(n_cols)], the slots of an adapters.Adapters store; rows of
+    another width than in_features are refused (the padded a does not show it; 0: taken as they are).
 
 Rows beyond one launch (prefill) follow ESPALIER_PREFILL_MODE:
     chunk  (default) a row gets exactly its decode bits: the decode kernels over windows of MAX_ROWS rows, or from
@@ -119,13 +120,13 @@ def dense(x: torch.Tensor, trellis: list[torch.Tensor], suh: list[torch.Tensor],
 
 @torch.library.custom_op("espalier::add_adapters", mutates_args=("y",))
 def add_adapters(y: torch.Tensor, x: torch.Tensor, rows: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ranks: torch.Tensor,
-                 scales: torch.Tensor, n_cols: list[int]) -> None:
+                 scales: torch.Tensor, n_cols: list[int], in_features: int = 0) -> None:
     from .experts import ext
-    ext().lora(x, y, y, rows, a, b, ranks, scales, n_cols)
+    ext().lora(x, y, y, rows, a, b, ranks, scales, n_cols, in_features)
 
 
 @add_adapters.register_fake
-def _add_adapters_shape(y, x, rows, a, b, ranks, scales, n_cols):
+def _add_adapters_shape(y, x, rows, a, b, ranks, scales, n_cols, in_features=0):
     return None
 
 
