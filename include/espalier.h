@@ -8,7 +8,7 @@
  *     capture. The caller owns every buffer.
  * Errors: a call returns ESP_OK (0) or an ESP_ERR_* code, and esp_last_error() holds a message. The reference
  * raises these as TORCH_CHECK failures (RuntimeError in Python); the torch binding raises the same.
- * dtype codes: ESP_F16 0, ESP_BF16 1, ESP_F32 2.
+ * dtype codes: ESP_F16 0, ESP_BF16 1, ESP_F32 2, ESP_E4M3 3 (8 bits: a paged cache only).
  * Codebook ids are the kernels' (1 mcg, 3 E2M1, 6 int5, 7 int6), K2 = 2 * bits; the supported (cb, K2) pairs are
  * mcg at K2 2..16 (even), E2M1 at 2, 4, 6, int5 at 4, 6, 8, int6 at 6, 8, 10 (experts_grouped.cuh:227-229).
  */
@@ -29,6 +29,7 @@ extern "C" {
 #define ESP_F16 0
 #define ESP_BF16 1
 #define ESP_F32 2
+#define ESP_E4M3 3
 
 /* Bits of the device status word (esp_status). */
 #define ESP_STATUS_NO_KERNEL 1    /* a grouped launch met an expert whose (codebook, K2) has no kernel */
@@ -474,6 +475,83 @@ int esp_verify(const void* logits, int dtype, int64_t stride, int64_t R, int64_t
 
 /* Bytes of scratch that esp_verify needs. */
 int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V);
+
+/* ---- A paged cache of keys and values, and attention over it (csrc/cache.hip, csrc/attention.hip). No counterpart in the
+ * reference. ---- */
+
+/* `pages` pages of `page` tokens (a multiple of 16, at most 65536), `heads` heads of dim (64, 128 or 256) elements each: element d
+ * of head h of token t of page p at k[p * k_page + t * k_token + h * k_head + d] and v likewise, strides in elements. dtype
+ * ESP_F16, ESP_BF16, or ESP_E4M3 with k_scale and v_scale (fp32 [heads] on the device, positive): a value stands for itself times
+ * its head's scale; without scales NULL. k, v and every stride 16-byte aligned; k_token, v_token at least dim. */
+typedef struct esp_kv_cache {
+    void* k;
+    void* v;
+    int dtype;
+    int64_t pages, page, heads, dim;
+    int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+    const float* k_scale;
+    const float* v_scale;
+} esp_kv_cache;
+
+/* The rows of T new tokens, between a layer's projections and its attention: queries q [T][Hq][dim], keys and values k, v
+ * [T][cache->heads][dim] (dtype ESP_BF16 or ESP_F16, row and head strides in elements). Queries and keys go through an RMSNorm of
+ * their own a head (q_weight, k_weight [dim], either may be NULL: none), (x / sqrt(mean(x^2) + eps)) * w, and the rotation of their first 2 * half
+ * elements: pair f < half, elements f and half + f (or, adjacent, 2 f and 2 f + 1), becomes rot_scale * (a cos t - b sin t,
+ * b cos t + a sin t) with t = positions[axis * pos_axis + token] * inv_freq[f] (inv_freq fp64 on the device), axis = axes[f] (int32
+ * on the device, taken into [0, n_axes); NULL: 0). In fp32 (the angles in fp64), rounded once where it is stored: queries to out
+ * [T][Hq][dim], keys and values to slot slots[token] = page * cache->page + token in the page. A token whose slot lies outside the
+ * cache (-1: the padding of a batch) stores no key and value, its queries are turned all the same. Slots of a call are distinct;
+ * of tokens that share one, each 16 bytes are either's. e4m3: to nearest even of the value over the head's scale, beyond +-448
+ * (infinities too) +-448. half a multiple of 8 (0: no rotation). out may be q (in place) and must else overlap none of q, k and v
+ * (refused), nor the cache any of them. Alignment: rows and weights 16 bytes, strides a multiple of 8 elements. T < 2^24. A row's
+ * bits depend on that row alone. */
+int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                     int64_t v_row, int64_t v_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
+                     const int64_t* slots, const int64_t* positions, int64_t pos_axis, int64_t n_axes, const double* inv_freq,
+                     const int32_t* axes, int64_t half, int adjacent, double rot_scale, const void* q_weight,
+                     const void* k_weight, double eps, void* out, int64_t out_row, int64_t out_head, void* stream);
+
+/* Attention of new tokens over the cache. Request b has n = n_new[b] new tokens (at most max_new; NULL: 1), whose queries are rows
+ * first[b] .. first[b] + n of q (NULL: row b), and lengths[b] tokens in the cache, the new ones the last of them; token j is in
+ * page tables[b * table_row + j / page] at j % page. New token i, at position p = lengths[b] - n + i, sees the tokens j <= p, of
+ * a window (0: none) those with j > p - window, that lie in the table (j < max_pages * page) and in a page that exists (a table
+ * entry outside [0, pages) hides its tokens): out = sum_j softmax_j(scale * q k_j) v_j, query head h over the cache's head
+ * h / (Hq / heads), zeros where it sees nothing. What a row does not see does not change it, whatever it holds. Rows of no request,
+ * and those of a request with n outside [0, max_new] or rows outside [0, T), are left as they are. Scores and sums in fp32, the
+ * weights rounded to dtype for the product with the values.
+ * split: tokens a piece of a request's keys (a multiple of 128); pieces run apart and are joined in order. 0: chosen from all the
+ * batch's lengths, so that a row's bits depend on them; with a split of its own a row's bits depend on that row alone.
+ * q, out [T][Hq][dim] of dtype ESP_BF16 or ESP_F16 with row and head strides, 16-byte aligned (strides multiples of 8); out must
+ * not overlap q (refused), nor anything else. Hq a multiple of heads; scale > 0; max_pages * page <= 2^28. scratch: at least
+ * esp_paged_attention_scratch bytes, 16-byte aligned, any values. */
+int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
+                        const int32_t* tables, int64_t table_row, int64_t max_pages, const int32_t* lengths,
+                        const int32_t* first, const int32_t* n_new, int64_t B, int64_t max_new, double scale, int64_t window,
+                        int64_t split, void* out, int64_t out_row, int64_t out_head, void* scratch, int64_t scratch_bytes,
+                        void* stream);
+
+/* Bytes of scratch that esp_paged_attention needs (the cache's heads, dim and page are read). */
+int64_t esp_paged_attention_scratch(int64_t B, int64_t max_new, int64_t Hq, const esp_kv_cache* cache, int64_t max_pages,
+                                    int64_t split);
+
+/* ---- Log-probabilities of given tokens (csrc/logprobs.hip). No counterpart in the reference. ---- */
+
+/* For row r of the logits [R][V] (row stride `stride`, dtype any of the three), with p = softmax(row / temperature[r])
+ * (temperature NULL, or below 1e-5 or NaN: 1) and token t = tokens[r] (int32):
+ *   logprobs[r] = log p_t, ranks[r] = 1 + how many tokens come before t (a larger logit, or an equal one at a lower index; a NaN is
+ *   the largest, zeros of both signs are equal), entropies[r] = -sum p log p, and the `top` (at most 64) first tokens in that
+ *   order, top_ids[r][..], with their top_logprobs[r][..].
+ * A token outside [0, V) has rank 0 and log-probability 0. A row without a distribution (a NaN or +inf in it, or nothing above
+ * -inf) has NaN for its entropy and all its log-probabilities; ids and ranks as ever. Exponentials are summed in fp32 within 1024
+ * logits, in fp64 above. ranks, entropies may be NULL; top <= V. Outputs contiguous, apart from one another and from the inputs.
+ * Rows may start at any element. R < 2^31, V <= 2^24, R * ceil(V / 4096) < 2^24. scratch: esp_token_logprobs_scratch bytes,
+ * 16-byte aligned, any values. A row's bits depend on that row alone. */
+int esp_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t R, int64_t V, const int32_t* tokens,
+                       const float* temperature, int64_t top, float* logprobs, int32_t* ranks, float* entropies,
+                       int32_t* top_ids, float* top_logprobs, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Bytes of scratch that esp_token_logprobs needs. */
+int64_t esp_token_logprobs_scratch(int64_t R, int64_t V, int64_t top);
 
 #ifdef __cplusplus
 }

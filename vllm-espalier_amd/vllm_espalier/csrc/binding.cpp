@@ -887,6 +887,196 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify(
     return {tokens, counts, logprobs};
 }
 
+// A paged cache of its tensors [pages, page, heads, dim] (any strides, elements of a head side by side), scales [heads] where it
+// is of 8 bits
+static esp_kv_cache kv_cache(const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& k_scale,
+                             const c10::optional<at::Tensor>& v_scale) {
+    TORCH_CHECK(k.is_cuda() && k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && k.stride(3) == 1 &&
+                    v.stride(3) == 1, "cache: k and v [pages, page, heads, dim] of one dtype, unit stride in dim");
+    const auto t = k.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat8_e4m3fn, "cache: bf16, fp16 or e4m3");
+    on_device(v, k, "v cache");
+    esp_kv_cache c = {};
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.dtype = t == at::kFloat8_e4m3fn ? ESP_E4M3 : dtype_code(k);
+    c.pages = k.size(0);
+    c.page = k.size(1);
+    c.heads = k.size(2);
+    c.dim = k.size(3);
+    // (of a dimension of one element the stride says nothing)
+    const auto stride = [](const at::Tensor& x, int d, int64_t one) { return x.size(d) > 1 ? x.stride(d) : one; };
+    c.k_page = stride(k, 0, 0);
+    c.k_token = k.stride(1);
+    c.k_head = stride(k, 2, 0);
+    c.v_page = stride(v, 0, 0);
+    c.v_token = v.stride(1);
+    c.v_head = stride(v, 2, 0);
+    for (const auto* s : {&k_scale, &v_scale})
+        if (s->has_value()) {
+            check(**s, at::kFloat, "cache scales");
+            on_device(**s, k, "cache scales");
+            TORCH_CHECK((*s)->numel() == c.heads, "cache scales: one a head");
+        }
+    c.k_scale = k_scale.has_value() ? cptr<float>(*k_scale) : nullptr;
+    c.v_scale = v_scale.has_value() ? cptr<float>(*v_scale) : nullptr;
+    return c;
+}
+// Rows [T, heads, dim] as the launches read them (16-byte pieces): x itself, or a copy where it does not fit
+static at::Tensor head_rows(const at::Tensor& x, at::ScalarType t, const at::Tensor& first, int64_t T, int64_t dim, const char* name) {
+    TORCH_CHECK(x.is_cuda() && x.scalar_type() == t && x.dim() == 3 && x.size(0) == T && x.size(2) == dim, name,
+                ": [T, heads, dim], q's dtype");
+    on_device(x, first, name);
+    const auto fits = [&](int d) { return x.size(d) <= 1 || x.stride(d) % 8 == 0; };
+    return x.stride(2) == 1 && (uintptr_t)x.data_ptr() % 16 == 0 && fits(0) && fits(1) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+static int64_t row_stride(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1) * x.size(2); }
+static int64_t head_stride(const at::Tensor& x) { return x.size(1) > 1 ? x.stride(1) : x.size(2); }
+static at::Tensor head_out(const c10::optional<at::Tensor>& out, const at::Tensor& q) {
+    if (!out.has_value()) return at::empty(q.sizes(), q.options());
+    TORCH_CHECK(out->is_cuda() && out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && out->stride(2) == 1,
+                "out: q's shape and dtype, unit stride in dim");
+    on_device(*out, q, "out");
+    return *out;
+}
+
+// esp_cache_append (csrc/cache.hip): q [T, Hq, dim], k and v [T, heads, dim]; the queries that attend (out's own if given)
+at::Tensor cache_append(const at::Tensor& q_any, const at::Tensor& k_any, const at::Tensor& v_any, const at::Tensor& k_cache,
+                        const at::Tensor& v_cache, const c10::optional<at::Tensor>& k_scale,
+                        const c10::optional<at::Tensor>& v_scale, const at::Tensor& slots,
+                        const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& inv_freq,
+                        const c10::optional<at::Tensor>& axes, bool adjacent, double rot_scale,
+                        const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight, double eps,
+                        const c10::optional<at::Tensor>& out_given) {
+    TORCH_CHECK(q_any.is_cuda() && q_any.dim() == 3, "q: [T, heads, dim]");
+    const auto t = q_any.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, "q: bf16 or fp16");
+    const esp_kv_cache c = kv_cache(k_cache, v_cache, k_scale, v_scale);
+    on_device(k_cache, q_any, "cache");
+    const int64_t T = q_any.size(0);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q_any.device());
+    const at::Tensor out = head_out(out_given, q_any);
+    const at::Tensor q = head_rows(q_any, t, q_any, T, c.dim, "q"), k = head_rows(k_any, t, q_any, T, c.dim, "k"),
+                     v = head_rows(v_any, t, q_any, T, c.dim, "v");
+    TORCH_CHECK(k.size(1) == c.heads && v.size(1) == c.heads, "k / v: the cache's heads");
+    check(slots, at::kLong, "slots");
+    on_device(slots, q, "slots");
+    TORCH_CHECK(slots.numel() == T, "slots: [T]");
+    int64_t n_axes = 1, half = 0;
+    if (inv_freq.has_value()) {
+        TORCH_CHECK(positions.has_value(), "a rotation needs positions");
+        check(*positions, at::kLong, "positions");
+        check(*inv_freq, at::kDouble, "inv_freq");
+        all_on_device("cache_append", q, *positions, *inv_freq);
+        half = inv_freq->numel();
+        TORCH_CHECK((positions->dim() == 1 || positions->dim() == 2) && positions->size(-1) == T, "positions: [T] or [axes, T]");
+        if (positions->dim() == 2) n_axes = positions->size(0);
+        if (axes.has_value()) {
+            check(*axes, at::kInt, "axes");
+            on_device(*axes, q, "axes");
+            TORCH_CHECK(axes->numel() == half, "axes: one a frequency");
+        }
+    }
+    for (const auto* w : {&q_weight, &k_weight})
+        if (w->has_value()) {
+            check(**w, t, "norm weights");
+            on_device(**w, q, "norm weights");
+            TORCH_CHECK((*w)->numel() == c.dim, "norm weights: [dim]");
+        }
+    call(esp_cache_append(q.data_ptr(), row_stride(q), head_stride(q), k.data_ptr(), row_stride(k), head_stride(k), v.data_ptr(),
+                          row_stride(v), head_stride(v), T, q.size(1), dtype_code(q), &c, cptr<int64_t>(slots),
+                          half ? cptr<int64_t>(*positions) : nullptr, T, n_axes, half ? cptr<double>(*inv_freq) : nullptr,
+                          half && axes.has_value() ? cptr<int32_t>(*axes) : nullptr, half, adjacent, rot_scale,
+                          q_weight.has_value() ? q_weight->data_ptr() : nullptr,
+                          k_weight.has_value() ? k_weight->data_ptr() : nullptr, eps, out.data_ptr(), row_stride(out),
+                          head_stride(out), cur_stream()));
+    return out;
+}
+
+// esp_paged_attention (csrc/attention.hip): q [T, Hq, dim], tables [B, pages a request], lengths / first / n_new [B]
+at::Tensor paged_attention(const at::Tensor& q_any, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale,
+                           const at::Tensor& tables, const at::Tensor& lengths, const c10::optional<at::Tensor>& first,
+                           const c10::optional<at::Tensor>& n_new, int64_t max_new, double scale, int64_t window, int64_t split,
+                           const c10::optional<at::Tensor>& out_given) {
+    TORCH_CHECK(q_any.is_cuda() && q_any.dim() == 3, "q: [T, heads, dim]");
+    const auto t = q_any.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, "q: bf16 or fp16");
+    const esp_kv_cache c = kv_cache(k_cache, v_cache, k_scale, v_scale);
+    on_device(k_cache, q_any, "cache");
+    const int64_t T = q_any.size(0);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q_any.device());
+    const at::Tensor out = head_out(out_given, q_any);
+    const at::Tensor q = head_rows(q_any, t, q_any, T, c.dim, "q");
+    TORCH_CHECK(tables.is_cuda() && tables.scalar_type() == at::kInt && tables.dim() == 2 &&
+                    (tables.size(1) <= 1 || tables.stride(1) == 1), "tables: int32 [B, pages], unit column stride");
+    const int64_t B = tables.size(0), max_pages = tables.size(1);
+    check(lengths, at::kInt, "lengths");
+    all_on_device("paged_attention", q, tables, lengths);
+    TORCH_CHECK(lengths.numel() == B, "lengths: [B]");
+    for (const auto* v : {&first, &n_new})
+        if (v->has_value()) {
+            check(**v, at::kInt, "first / n_new");
+            on_device(**v, q, "first / n_new");
+            TORCH_CHECK((*v)->numel() == B, "first / n_new: [B]");
+        }
+    const int64_t bytes = esp_paged_attention_scratch(B, max_new, q.size(1), &c, max_pages, split);
+    const at::Tensor scratch = at::empty({bytes}, q.options().dtype(at::kByte));
+    call(esp_paged_attention(q.data_ptr(), row_stride(q), head_stride(q), T, q.size(1), dtype_code(q), &c, cptr<int32_t>(tables),
+                             B > 1 ? tables.stride(0) : max_pages, max_pages, cptr<int32_t>(lengths),
+                             first.has_value() ? cptr<int32_t>(*first) : nullptr,
+                             n_new.has_value() ? cptr<int32_t>(*n_new) : nullptr, B, max_new, scale, window, split,
+                             out.data_ptr(), row_stride(out), head_stride(out), scratch.data_ptr(), bytes, cur_stream()));
+    return out;
+}
+
+// esp_token_logprobs (csrc/logprobs.hip): logits [R, V], tokens [R]; (logprobs, ranks, entropies, top_ids, top_logprobs), `out`'s
+// own if given
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
+    const at::Tensor& logits, const at::Tensor& tokens, int64_t top, const c10::optional<at::Tensor>& temperature,
+    const c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>>& out) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+                "logits: [R, V], unit column stride");
+    const auto t = logits.scalar_type();
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, "logits: bf16, fp16 or fp32");
+    const int64_t R = logits.size(0), V = logits.size(1);
+    check(tokens, at::kInt, "tokens");
+    on_device(tokens, logits, "tokens");
+    TORCH_CHECK(tokens.numel() == R, "tokens: [R]");
+    TORCH_CHECK(top >= 0, "top: at least 0");
+    if (temperature.has_value()) {
+        check(*temperature, at::kFloat, "temperature");
+        on_device(*temperature, logits, "temperature");
+        TORCH_CHECK(temperature->numel() == R, "temperature: [R]");
+    }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+    at::Tensor lp, ranks, entropies, ids, top_lp;
+    if (out.has_value()) {
+        std::tie(lp, ranks, entropies, ids, top_lp) = *out;
+        check(lp, at::kFloat, "logprobs");
+        check(ranks, at::kInt, "ranks");
+        check(entropies, at::kFloat, "entropies");
+        check(ids, at::kInt, "top_ids");
+        check(top_lp, at::kFloat, "top_logprobs");
+        all_on_device("token_logprobs", logits, lp, ranks, entropies, ids, top_lp);
+        TORCH_CHECK(lp.numel() == R && ranks.numel() == R && entropies.numel() == R && ids.numel() == R * top &&
+                        top_lp.numel() == R * top, "out: [R] three times, then [R, top] twice");
+    } else {
+        lp = at::empty({R}, logits.options().dtype(at::kFloat));
+        ranks = at::empty({R}, tokens.options());
+        entropies = at::empty_like(lp);
+        ids = at::empty({R, top}, tokens.options());
+        top_lp = at::empty({R, top}, lp.options());
+    }
+    const int64_t bytes = esp_token_logprobs_scratch(R, V, top);
+    const at::Tensor scratch = at::empty({bytes}, logits.options().dtype(at::kByte));
+    call(esp_token_logprobs(logits.data_ptr(), dtype_code(logits), logits.stride(0), R, V, cptr<int32_t>(tokens),
+                            temperature.has_value() ? cptr<float>(*temperature) : nullptr, top, mptr<float>(lp),
+                            mptr<int32_t>(ranks), mptr<float>(entropies), top ? mptr<int32_t>(ids) : nullptr,
+                            top ? mptr<float>(top_lp) : nullptr, scratch.data_ptr(), bytes, cur_stream()));
+    return {lp, ranks, entropies, ids, top_lp};
+}
+
 // several dense launches as one (esp_dense_multi; no reference counterpart): per group its input rows, matrices,
 // output columns and plan; after[g] != 0 when group g's x is a view of group g - 1's y. The optional norm (h, d1, d2,
 // w, h_out, eps) makes group 0's input RMSNorm(h + d1 + d2) * w, as dense_rmsnorm does.
@@ -1015,6 +1205,9 @@ PYBIND11_MODULE(espalier_ext, m) {
     m.def("lora", &lora, py::arg("x"), py::arg("y"), py::arg("out"), py::arg("rows"), py::arg("a"), py::arg("b"),
           py::arg("ranks"), py::arg("scales"), py::arg("n_cols"), py::arg("in_features") = 0);
     m.def("verify", &verify);
+    m.def("cache_append", &cache_append);
+    m.def("paged_attention", &paged_attention);
+    m.def("token_logprobs", &token_logprobs);
     m.def("argmax", &argmax, py::arg("logits"), py::arg("ids"), py::arg("part") = py::none(),
           py::arg("counters") = py::none());
 }

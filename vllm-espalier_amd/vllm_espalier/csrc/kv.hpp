@@ -1,0 +1,51 @@
+// What the kernels over a paged cache of keys and values share: its 16- and 8-bit elements, and the host's checks of it.
+#pragma once
+
+#include "../../../include/espalier.h"
+#include "common.hpp"
+
+namespace esp {
+
+constexpr int E4M3 = ESP_E4M3;
+constexpr float E4M3_MAX = 448.0f;
+
+// Bytes of an element
+__host__ __device__ constexpr int kv_bytes(int dtype) { return dtype == E4M3 ? 1 : 2; }
+
+// Two floats as e4m3 in the low (or, HI, the high) half of w, to nearest even, those past the largest (infinities too) as the
+// largest, a NaN as a NaN
+template <bool HI>
+__device__ __forceinline__ int pack_e4m3(float a, float b, int w) {
+    a = a > E4M3_MAX ? E4M3_MAX : a < -E4M3_MAX ? -E4M3_MAX : a;      // (a NaN compares false and stays)
+    b = b > E4M3_MAX ? E4M3_MAX : b < -E4M3_MAX ? -E4M3_MAX : b;
+    return __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, HI);
+}
+
+}  // namespace esp
+
+namespace esp_host {
+
+// nullptr, or what is wrong with a cache. `align`: the bytes that its rows of D elements are aligned to
+inline const char* kv_cache_error(const esp_kv_cache* c, int dtype) {
+    if (!c) return "null cache";
+    if (c->dtype != dtype && c->dtype != ESP_E4M3) return "a cache has the rows' dtype or e4m3";
+    if (c->dim != 64 && c->dim != 128 && c->dim != 256) return "heads of 64, 128 or 256 elements";
+    if (c->heads < 1 || c->heads > 1024) return "1 to 1024 heads in the cache";
+    if (c->pages < 1 || c->pages >= (int64_t(1) << 31)) return "1 to 2^31 - 1 pages";
+    if (c->page < 16 || c->page > 65536 || c->page % 16) return "pages of a multiple of 16 tokens, at most 65536";
+    if (!c->k || !c->v) return "null pointer";
+    if ((c->dtype == ESP_E4M3) != (c->k_scale != nullptr) || (c->dtype == ESP_E4M3) != (c->v_scale != nullptr))
+        return "an e4m3 cache has a scale a head for k and for v, one of 16 bits has none";
+    const int64_t size = esp::kv_bytes(c->dtype);
+    const int64_t strides[6] = {c->k_page, c->k_token, c->k_head, c->v_page, c->v_token, c->v_head};
+    for (const int64_t s : strides) {
+        if (s < 0 || s >= (int64_t(1) << 40)) return "cache strides of 0 to 2^40 elements";
+        if (s * size % 16) return "cache rows must be aligned to 16 bytes";
+    }
+    if (((uintptr_t)c->k | (uintptr_t)c->v) % 16) return "cache rows must be aligned to 16 bytes";
+    if (c->k_token < c->dim || c->v_token < c->dim) return "the cache's tokens overlap";
+    if (c->k_token >= (1 << 24) || c->v_token >= (1 << 24)) return "a token's stride of at most 2^24 elements";
+    return nullptr;
+}
+
+}  // namespace esp_host
