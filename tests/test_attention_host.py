@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import paged
+from vllm_espalier import step as S
 from vllm_espalier.attention import PagedCache, Rotary
 
 LIB = Path(__file__).resolve().parent.parent / "vllm-espalier_amd" / "vllm_espalier" / "libespalier_hip.so"
@@ -185,3 +186,15 @@ def test_plain_attention_by_torch():
     mask = torch.arange(40)[None, :] <= torch.arange(37, 40)[:, None]
     want = torch.nn.functional.scaled_dot_product_attention(q[1:].double().permute(1, 0, 2), k, v, attn_mask=mask)
     assert torch.allclose(out[1:], want.permute(1, 0, 2))
+
+def test_place():
+    """Where the rows of a decoder's pass stand, and what does not fit."""
+    s = S.Sequences(6, 3, 3, 4, 16, "cpu")
+    s.place([[5, 2], [9]], [18, 2], [3, 2])
+    assert s.slots.tolist() == [5 * 16 + 15, 32, 33, 144, 145, -1] and s.positions.tolist() == [15, 16, 17, 0, 1, 0]
+    assert s.tables.tolist() == [[5, 2, -1, -1], [9, -1, -1, -1], [-1] * 4]
+    assert s.lengths.tolist() == [18, 2, 0] and s.first.tolist() == [0, 3, 0] and s.n_new.tolist() == [3, 2, -1]
+    for bad in (([[1]] * 4, [1] * 4, None), ([[1]], [17], [1]), ([[1]], [3], [4]), ([[1]], [2], [3]), ([[1, 2, 3, 4, 5]], [2], [1]),
+                ([[1], [2], [3]], [3, 3, 3], [3, 3, 3]), ([[1]], [2, 3], None)):
+        with pytest.raises(ValueError):
+            s.place(*bad)

@@ -4,7 +4,7 @@ step: 40 layers of the dense block and the grouped MoE block, an mcg LM head, gr
 Per layer, on rows h (bf16 [T, 2048], the residual stream):
   a   = RMSNorm(h + the previous layer's MoE outputs)     add_rmsnorm (csrc/step.hip)
   qkv = [q | k | v](a)                                    one dense launch (2048 -> 4096 + 512 + 512, int6)
-        attention is not part of this layer set: o reads q itself (qkv[:, :4096]) as a placeholder
+        attention over a paged cache (use_cache); without one, o reads q itself (qkv[:, :4096]) as a placeholder
   o   = o(q)                                              one dense launch (4096 -> 2048, int6)
   a   = RMSNorm(h + o)                                    add_rmsnorm
   route_group, then the grouped launches                  256 routed experts (top-8) + the gated shared expert
@@ -24,13 +24,17 @@ MoE after the routing is one chained launch too (experts.routed2: esp_moe_chain)
 Rows never interact (the dense and grouped kernels keep rows apart, norms are per row), so a window of T rows
 gives each row the bits it gets alone.
 
-Three things of a served model can stand in the step, off by default:
+Four things of a served model can stand in the step, off by default:
+  * use_cache(pages, ...): a paged cache of keys and values for every layer; the rows of a pass are the new tokens of requests
+    (Buffers.sequences), whose q and k are normed and turned, k and v appended, and o reads their attention over the cache;
   * use_adapters(slots, max_rank): low-rank adapters beside qkv and o, each row's own (Buffers.rows names their slots);
   * post_norms=True: every block's output has a norm of its own before it joins the residual (sandwich_rmsnorm instead of
     add_rmsnorm);
   * verify(b, ...): the rows of a pass are requests' last tokens and their drafts, verified against the logits
-    (speculative.verify).
-A layer that has one of the first two runs its launches apart (qkv's adapters stand between qkv and o); rows stay independent.
+    (speculative.verify); score(b, ...): the log-probabilities of given tokens under them (logprobs.token_logprobs).
+A layer that has one of the first three runs its launches apart (the attention and qkv's adapters stand between qkv and o). Rows
+stay independent but for what a request's rows see of one another; with a cache and no split of its own (use_cache), the lengths of
+all requests decide how their keys are cut up, and with that a row's last bits.
 """
 from __future__ import annotations
 
@@ -43,10 +47,13 @@ from . import experts as G
 from . import speculative
 from . import workloads as WL
 from .adapters import Adapters
+from .attention import PagedCache, Rotary
 from .experts import ext
+from .logprobs import token_logprobs
 
 D_MODEL = 2048
 Q_OUT, KV_OUT = 4096, 512
+HEAD_DIM = 128               # 32 query heads over 4 of the cache
 EXPERT_I = 512
 VOCAB = 151936
 TOPK = 8
@@ -71,6 +78,9 @@ class DecoderLayer:
     post_o: torch.Tensor | None = None
     qkv_adapters: Adapters | None = None
     o_adapters: Adapters | None = None
+    cache: PagedCache | None = None
+    q_norm: torch.Tensor | None = None       # the norms of q and k a head, with a cache
+    k_norm: torch.Tensor | None = None
 
     @property
     def adapted(self) -> bool:
@@ -79,7 +89,7 @@ class DecoderLayer:
     @property
     def plain(self) -> bool:
         """Whether the layer runs in the launches that hold several of its steps: none of what may stand between them."""
-        return self.post_in is None and self.post_o is None and not self.adapted
+        return self.post_in is None and self.post_o is None and not self.adapted and self.cache is None
 
 
 def _norm_weight(gen, dev, D):
@@ -107,6 +117,45 @@ def build_layer(gen: torch.Generator, dev, E: int = 256, D: int = D_MODEL, I: in
                         shared)
 
 
+class Sequences:
+    """Where the rows of a pass stand: the new tokens of up to B requests, at most max_new of each, and the requests' pages. The
+    tensors keep their addresses, so a captured graph follows what place() writes into them."""
+
+    def __init__(self, T: int, B: int, max_new: int, pages: int, page: int, dev):
+        self.page, self.max_new = page, max_new
+        self.slots = torch.full((T,), -1, dtype=torch.int64, device=dev)
+        self.positions = torch.zeros((T,), dtype=torch.int64, device=dev)
+        self.tables = torch.full((B, pages), -1, dtype=torch.int32, device=dev)
+        self.lengths = torch.zeros((B,), dtype=torch.int32, device=dev)
+        self.first = torch.zeros((B,), dtype=torch.int32, device=dev)
+        self.n_new = torch.full((B,), -1, dtype=torch.int32, device=dev)
+
+    def place(self, tables, lengths, n_new=None) -> None:
+        """Requests of lengths[b] tokens in the pages tables[b], the last n_new[b] (default: one) of them the rows of the next
+        pass, one request after the other. Rows and requests that are left over belong to nobody."""
+        n_new = [1] * len(lengths) if n_new is None else list(n_new)
+        T, (B, width) = self.slots.numel(), self.tables.shape
+        if not len(tables) == len(lengths) == len(n_new) <= B or sum(n_new) > T:
+            raise ValueError(f"at most {B} requests of {T} new tokens together, each with its pages and length")
+        slots, positions, first = [-1] * T, [0] * T, []
+        at = 0
+        for pages, length, n in zip(tables, lengths, n_new):
+            if not 0 <= n <= min(length, self.max_new) or len(pages) > width or len(pages) * self.page < length:
+                raise ValueError(f"a request has up to {self.max_new} new tokens among its own, in up to {width} pages that hold them")
+            first.append(at)
+            for p in range(length - n, length):
+                slots[at], positions[at] = pages[p // self.page] * self.page + p % self.page, p
+                at += 1
+        put = lambda t, v: t.copy_(torch.tensor(v, dtype=t.dtype))  # noqa: E731
+        spare = B - len(lengths)
+        put(self.slots, slots)
+        put(self.positions, positions)
+        put(self.tables, [list(pages) + [-1] * (width - len(pages)) for pages in tables] + [[-1] * width] * spare)
+        put(self.lengths, list(lengths) + [0] * spare)
+        put(self.first, first + [0] * spare)
+        put(self.n_new, n_new + [-1] * spare)
+
+
 class Buffers:
     """Every activation of a T-row pass, allocated once (graph capture needs fixed addresses)."""
 
@@ -124,6 +173,8 @@ class Buffers:
         self.moe = torch.zeros((T, D), dtype=bf, device=dev)
         self.moe_shared = torch.zeros((T, D), dtype=bf, device=dev)
         self.logits = torch.zeros((T, vocab), dtype=bf, device=dev)
+        self.sequences: Sequences | None = None                                # where the rows stand (use_cache)
+        self.attn: torch.Tensor | None = None
         self.argmax_part = torch.zeros((T * -(-vocab // 4096),), dtype=torch.int64, device=dev)   # a key a slice
         self.argmax_cnt = torch.zeros((T * 32,), dtype=torch.int32, device=dev)                   # zero between uses
 
@@ -153,6 +204,42 @@ class SyntheticDecoder:
         for L in self.layers:
             L.qkv_adapters = Adapters(D_MODEL, [Q_OUT, KV_OUT, KV_OUT], slots, max_rank, device=self.dev)
             L.o_adapters = Adapters(Q_OUT, [D_MODEL], slots, max_rank, device=self.dev)
+
+    def use_cache(self, pages: int, page: int = 64, dtype=torch.bfloat16, scale: float | None = None, base: float = 1e6,
+                  split: int = 0, seed: int = 0) -> None:
+        """A cache of `pages` pages for every layer, q and k norms a head, and the rotation of positions; dtype bf16, or e4m3 with
+        one scale. split: PagedCache.attend's. The rows of the passes that follow are those of Buffers.sequences (sequences())."""
+        gen = torch.Generator(device=self.dev).manual_seed(seed)
+        self.rotary, self.split = Rotary.of_base(HEAD_DIM, base, device=self.dev), split
+        for L in self.layers:
+            L.cache = PagedCache.empty(pages, page, KV_OUT // HEAD_DIM, HEAD_DIM, dtype, self.dev, scale, scale)
+            L.q_norm, L.k_norm = _norm_weight(gen, self.dev, HEAD_DIM), _norm_weight(gen, self.dev, HEAD_DIM)
+
+    def sequences(self, b: Buffers, requests: int | None = None, max_new: int = 1, pages: int | None = None) -> Sequences:
+        """The places of the rows of b, for up to `requests` (default: one a row) with max_new new tokens and `pages` pages each
+        (default: the whole cache's)."""
+        cache = self.layers[0].cache
+        b.sequences = Sequences(b.T, b.T if requests is None else requests, max_new, cache.k.shape[0] if pages is None else pages,
+                                cache.k.shape[1], self.dev)
+        b.attn = torch.zeros((b.T, Q_OUT), dtype=torch.bfloat16, device=self.dev)
+        return b.sequences
+
+    def _mixed(self, L: DecoderLayer, b: Buffers) -> torch.Tensor:
+        """What o reads of b.qkv: the rows' attention over the layer's cache, theirs appended, or, without one, q itself."""
+        q = b.qkv[:, :Q_OUT]
+        if L.cache is None:
+            return q
+        s = b.sequences
+        if s is None:
+            raise RuntimeError("a pass over a cache needs sequences(buffers) to say where its rows stand")
+        q, k, v = (t.view(b.T, -1, HEAD_DIM) for t in b.qkv.split([Q_OUT, KV_OUT, KV_OUT], dim=1))
+        L.cache.append(q, k, v, s.slots, s.positions, self.rotary, L.q_norm, L.k_norm, EPS, out=q)
+        L.cache.attend(q, s.tables, s.lengths, s.first, s.n_new, s.max_new, split=self.split, out=b.attn.view(b.T, -1, HEAD_DIM))
+        return b.attn
+
+    def score(self, b: Buffers, tokens, top: int = 0, temperature=None, out=None):
+        """The log-probabilities of `tokens` [rows], one a row, under the logits of a pass over b (logprobs.token_logprobs)."""
+        return token_logprobs(b.logits, tokens, top, temperature, out)
 
     def verify(self, b: Buffers, first, n_drafts, drafts, uniform, race, temperature, draft_probs=None, out=None):
         """The drafts of the requests whose rows a pass over b ran, against its logits (speculative.verify)."""
@@ -198,15 +285,16 @@ class SyntheticDecoder:
             G.route_rmsnorm(b.h2, b.o, L.norm2, EPS, b.h, b.a, L.router, TOPK, L.moe, self.scratch)
         else:
             self._join(b, d1, d2, L.post_in, L.norm1)
-            if MULTI_ATTN and not L.adapted:
+            if MULTI_ATTN and not L.adapted and L.cache is None:
                 L.attn.forward([b.a, q], [b.qkv, b.o])
             else:
                 L.qkv.forward(b.a, out=b.qkv)
                 if L.qkv_adapters is not None:
                     L.qkv_adapters.apply(b.a, b.qkv, b.rows)
-                L.o.forward(q, out=b.o)
+                mixed = self._mixed(L, b)
+                L.o.forward(mixed, out=b.o)
                 if L.o_adapters is not None:
-                    L.o_adapters.apply(q, b.o, b.rows)
+                    L.o_adapters.apply(mixed, b.o, b.rows)
             self._join(b, b.o, None, L.post_o, L.norm2)
             G.route(b.a, L.router, TOPK, L.moe, self.scratch)
         if picks is not None:                     # eager runs only: the distinct experts this layer reads
@@ -247,14 +335,14 @@ class SyntheticDecoder:
         """One layer of prefill over the rows of b: the dense layers as prompt launches, the MoE over the whole prompt
         (its picks left in ps.pick, slots a row)."""
         d1, d2 = (None, None) if first else (b.moe, b.moe_shared)
-        q = b.qkv[:, :Q_OUT]
         self._join(b, d1, d2, L.post_in, L.norm1)
         L.qkv.forward_tile(b.a, out=b.qkv)
         if L.qkv_adapters is not None:
             L.qkv_adapters.apply(b.a, b.qkv, b.rows)
-        L.o.forward_tile(q, out=b.o)
+        mixed = self._mixed(L, b)
+        L.o.forward_tile(mixed, out=b.o)
         if L.o_adapters is not None:
-            L.o_adapters.apply(q, b.o, b.rows)
+            L.o_adapters.apply(mixed, b.o, b.rows)
         self._join(b, b.o, None, L.post_o, L.norm2)
         G.prefill(b.a, None, None, L.moe, ps, TOPK, gate=L.router, out=b.moe, out_shared=b.moe_shared)
 
