@@ -518,9 +518,11 @@ int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k
  * entry outside [0, pages) hides its tokens): out = sum_j softmax_j(scale * q k_j) v_j, query head h over the cache's head
  * h / (Hq / heads), zeros where it sees nothing. What a row does not see does not change it, whatever it holds. Rows of no request,
  * and those of a request with n outside [0, max_new] or rows outside [0, T), are left as they are. Scores and sums in fp32, the
- * weights rounded to dtype for the product with the values.
+ * weights rounded to dtype for the product with the values; where a row sees a value that is NaN or infinite, its output is NaN or
+ * infinite.
  * split: tokens a piece of a request's keys (a multiple of 128); pieces run apart and are joined in order. 0: chosen from all the
- * batch's lengths, so that a row's bits depend on them; with a split of its own a row's bits depend on that row alone.
+ * batch's lengths, so that a row's bits depend on them; with a split of its own a row's bits depend on its request alone (requests
+ * of more than 32 rows a head of the cache, n * Hq / heads, are then not cut at all).
  * q, out [T][Hq][dim] of dtype ESP_BF16 or ESP_F16 with row and head strides, 16-byte aligned (strides multiples of 8); out must
  * not overlap q (refused), nor anything else. Hq a multiple of heads; scale > 0; max_pages * page <= 2^28. scratch: at least
  * esp_paged_attention_scratch bytes, 16-byte aligned, any values. */
@@ -531,8 +533,8 @@ int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head, int64_t T,
                         void* stream);
 
 /* Bytes of scratch that esp_paged_attention needs (the cache's heads, dim and page are read). */
-int64_t esp_paged_attention_scratch(int64_t B, int64_t max_new, int64_t Hq, const esp_kv_cache* cache, int64_t max_pages,
-                                    int64_t split);
+int64_t esp_paged_attention_scratch(int64_t B, int64_t T, int64_t max_new, int64_t Hq, const esp_kv_cache* cache,
+                                    int64_t max_pages, int64_t split);
 
 /* ---- Log-probabilities of given tokens (csrc/logprobs.hip). No counterpart in the reference. ---- */
 

@@ -27,7 +27,7 @@ def lib(ext):
     L.esp_last_error.restype = ctypes.c_char_p
     L.esp_cache_append.argtypes = [P, I64, I64] * 3 + [I64, I64, INT, C, P, P, I64, I64, P, P, I64, INT, F64, P, P, F64, P, I64, I64, P]
     L.esp_paged_attention.argtypes = [P, I64, I64, I64, I64, INT, C, P, I64, I64, P, P, P, I64, I64, F64, I64, I64, P, I64, I64, P, I64, P]
-    L.esp_paged_attention_scratch.argtypes, L.esp_paged_attention_scratch.restype = [I64, I64, I64, C, I64, I64], I64
+    L.esp_paged_attention_scratch.argtypes, L.esp_paged_attention_scratch.restype = [I64, I64, I64, I64, C, I64, I64], I64
     L.esp_token_logprobs.argtypes = [P, INT, I64, I64, I64, P, P, I64, P, P, P, P, P, P, I64, P]
     L.esp_token_logprobs_scratch.argtypes, L.esp_token_logprobs_scratch.restype = [I64] * 3, I64
     return L
@@ -108,11 +108,13 @@ def test_no_rows_is_no_call(lib):
 def test_attend_scratch(lib):
     """Scratch for every piece of a tile that can have several: at most as many as the lengths' choice makes, none without any."""
     c = Cache(dim=128, heads=4, page=16)
-    size = lambda B, new, Hq, width, split: lib.esp_paged_attention_scratch(B, new, Hq, ctypes.byref(c), width, split)  # noqa: E731
+    size = lambda B, new, Hq, width, split: lib.esp_paged_attention_scratch(B, B * new, new, Hq, ctypes.byref(c), width, split)  # noqa: E731
     assert size(1, 1, 32, 8, 0) == 16                          # 128 keys: one piece
     assert size(4, 1, 32, 64, 128) >= 4 * 4 * 8 * 16 * 130 * 4
     assert size(1, 1, 32, 1 << 13, 0) >= 512 * 16 * 130 * 4
     assert size(64, 1, 32, 1 << 13, 0) >= 1024 * 16 * 130 * 4
+    assert size(2, 100, 32, 1 << 10, 0) >= 1024 * (32 + 128) * 130 * 4
+    assert size(2, 100, 32, 1 << 10, 256) == 16 + 2 * 4 * 64 * 32 * 130 * 4           # prompts are not cut then
     for bad in ((0, 1, 32, 8, 0), (1, 0, 32, 8, 0), (1, 1, 30, 8, 0), (1, 1, 32, -1, 0), (1, 1, 32, 8, 100), (1, 1, 32, 1 << 25, 0)):
         assert size(*bad) == 0
 

@@ -5,7 +5,7 @@
 //
 // A request's rows that share a head of the cache (its new tokens times the query heads of the group) are tiles of ROWS rows; the
 // keys that a tile sees are cut into pieces, and a workgroup takes a piece of a tile: its four waves take 32 keys in turn, each with
-// a running maximum and sum of its own, joined at the end. Tiles of one piece are written at once, the others' pieces go to scratch
+// a running maximum and sum of its own, joined at the end (requests of more than 32 rows are attention_prompt.hip's). Tiles of one piece are written at once, the others' pieces go to scratch
 // (fp32) and a second launch joins them, in their order.
 //
 // All in registers: with S^T = K Q^T (keys are the rows of the product, queries its columns) a lane loads 8 consecutive elements of
@@ -17,192 +17,20 @@
 //
 // Scores, statistics and sums are fp32; the weights are rounded to the rows' dtype for the second product (off by at most half a
 // step of themselves; their sum is that of the unrounded ones), e4m3 keys and values are exact in either dtype.
-#include "kv.hpp"
-#include "norm.hpp"
+#include "attention.hpp"
 
 namespace esp {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr int64_t JOIN_GRID = 2048;            // workgroups of a join: what fits at once
 
-constexpr int STEP = 32;                       // keys a wave takes at once
-constexpr int WAVES = 4;
-constexpr int PIECE = WAVES * STEP;            // pieces are multiples of this many keys
-constexpr int TARGET = 512;                    // pieces that a batch is cut into, about: two workgroups a CU
-
-struct AttendArgs {
-    const uint16_t* q;
-    int64_t q_row, q_head;                      // elements
-    uint16_t* out;
-    int64_t o_row, o_head;
-    const char *k, *v;
-    int64_t k_page, k_token, k_head, v_page, v_token, v_head, pages;       // bytes
-    const float *ks, *vs;
-    const int32_t* tables;
-    int64_t table_row;
-    const int32_t *lengths, *first, *n_new;
-    float* part;                                // [pieces][ROWS][D], then [pieces][ROWS][2]: a row's maximum and sum
-    float* stats;
-    int2* plan;                                 // [B]: a request's first piece in scratch and its pieces a tile
-    int B, T, Hkv, group, max_new, window, split, capacity;                // capacity: tokens that a table can name
-    int page16, page_shift;                     // tokens of a page / 16, and its reciprocal: 2 n page_mul >> (32 + page_shift)
-    uint32_t page_mul;
-    float scale;                                // scale * log2(e)
-};
-
-template <typename T>
-__device__ __forceinline__ T load_uniform(const T* p) {       // through the scalar cache: nothing writes it while the kernel runs
-    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
-}
-
-// ---- which piece a workgroup has
-
-// A request: its rows, and the keys [lo, hi) that any of them sees, lo down to a whole step
-struct Request {
-    int n, first, length, lo, hi;
-};
-__device__ __forceinline__ Request request(const AttendArgs& a, int n, int first, int length) {
-    Request r = {n, first, max(length, 0), 0, 0};
-    if (n < 0 || n > a.max_new || first < 0 || first > a.T - n) r.n = 0;        // no such request
-    r.hi = min(r.length, a.capacity);
-    if (a.window) r.lo = max(0, min(r.hi, r.length - r.n + 1 - a.window)) & ~(STEP - 1);
-    return r;
-}
-__device__ __forceinline__ Request request_of(const AttendArgs& a, int b) {              // any lane's
-    return b < a.B ? request(a, a.n_new ? a.n_new[b] : 1, a.first ? a.first[b] : b, a.lengths[b]) : Request{0, 0, 0, 0, 0};
-}
-__device__ __forceinline__ Request uniform_request(const AttendArgs& a, int b) {
-    return request(a, a.n_new ? load_uniform(a.n_new + b) : 1, a.first ? load_uniform(a.first + b) : b, load_uniform(a.lengths + b));
-}
-
-struct Piece {
-    int b, tile, head, at, pieces;              // at: which of the tile's pieces
-    int64_t slot;                               // its place in scratch
-    int size;                                   // keys a piece
-};
-
-__device__ __forceinline__ int wave_scan(int v) {             // inclusive sum over the lanes
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
-// Piece `item` of the batch, found by every wave for itself: the requests' lengths give the size of the pieces (a.split, or so
-// that there are about TARGET of them) and the requests' first ones. false: there are fewer
-template <int ROWS>
-__device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p) {
-    const int lane = threadIdx.x & 63;
-    int size = a.split;
-    if (!size) {
-        double keys = 0.0;                                     // exact: below 2^53
-        for (int b0 = 0; b0 < a.B; b0 += 64) {
-            const Request r = request_of(a, b0 + lane);
-            keys += (double)((r.n * a.group + ROWS - 1) / ROWS) * (double)(r.hi - r.lo);
-        }
-        keys = wave_sum_f64_dpp(keys) * a.Hkv;
-        size = ((int)fmin(keys / TARGET, (double)(1 << 28)) / PIECE + 1) * PIECE;
-    }
-    int before = 0, slots = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const Request r = request_of(a, b0 + lane);
-        const int tiles = (r.n * a.group + ROWS - 1) / ROWS, pieces = max(1, (r.hi - r.lo + size - 1) / size);
-        const int mine = tiles * a.Hkv * pieces, in_scratch = pieces > 1 ? mine : 0;
-        const int upto = wave_scan(mine), slots_upto = wave_scan(in_scratch);
-        const uint64_t hit = __ballot(item >= before + upto - mine && item < before + upto);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
-            const int in = item - before - of(upto - mine), per_tile = of(pieces);
-            p.b = b0 + l;
-            p.size = size;
-            p.pieces = per_tile;
-            // the tiles of a head and piece read the same keys: next to one another
-            const int n_tiles = of(tiles);
-            p.tile = in % n_tiles;
-            p.at = in / n_tiles % per_tile;
-            p.head = in / n_tiles / per_tile;
-            const int base = slots + of(slots_upto - in_scratch);
-            p.slot = base + (int64_t)(p.head * n_tiles + p.tile) * per_tile + p.at;
-            if (in == 0 && threadIdx.x == 0) a.plan[p.b] = make_int2(base, per_tile);
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-        slots += __builtin_amdgcn_readlane(slots_upto, 63);
-    }
-    return false;
-}
-
-// ---- the products
-
-template <bool BF>
-__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
-    if constexpr (BF)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {              // to nearest even
-    const f32x2 v = {a, b};
-    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-}
-// two e4m3 values of w's low (HI: high) half as two of dtype, exact
-template <bool BF, bool HI>
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
-    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
-    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
-}
-
-// the largest over the four 16-lane rows of a wave, each lane with those at its place; their sum
-__device__ __forceinline__ float rows_max(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    v = fmaxf(__builtin_bit_cast(float, (uint32_t)s[0]), __builtin_bit_cast(float, (uint32_t)s[1]));
-    const uint32_t w = __builtin_bit_cast(uint32_t, v);
-    s = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)s[0]), __builtin_bit_cast(float, (uint32_t)s[1]));
-}
-__device__ __forceinline__ float rows_sum(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    v = __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
-    const uint32_t w = __builtin_bit_cast(uint32_t, v);
-    s = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-    return __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
-}
-
-// whether any of the values in w is a NaN or an infinity (e4m3 has no infinities)
-template <bool BF, bool E8>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    if constexpr (E8) return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-    constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
-    return (w & E) == E || (w >> 16 & E) == E;
-}
-
-// The pages of 16 keys each, of which a step has two: a page that the table does not have, or that does not exist, is none
+// The pages of a step's two times 16 keys
 struct Pages {
-    int64_t page[2];                            // -1: none
-    int off[2];                                 // keys into the page
+    int64_t page[2];
+    int off[2];
 };
 __device__ __forceinline__ Pages pages_of(const AttendArgs& a, const int32_t* table, int key) {
-    Pages p;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const uint32_t n = (uint32_t)(key + 16 * u) >> 4;
-        const uint32_t at = __umulhi(2 * n, a.page_mul) >> a.page_shift;
-        const bool in = key + 16 * u < a.capacity;
-        const int id = load_uniform(table + (in ? at : 0));
-        p.page[u] = in && id >= 0 && id < a.pages ? id : -1;
-        p.off[u] = (int)(n - at * (uint32_t)a.page16) * 16;
-    }
-    return p;
+    const Page p = page_of(a, table, key), q = page_of(a, table, key + 16);
+    return {{p.page, q.page}, {p.off, q.off}};
 }
 
 // A wave's 32 keys or values. Keys: operand c of tile u holds elements 32 c + 8 g .. + 8 of key l (16 bits), or, two operands a
@@ -266,9 +94,9 @@ __device__ __forceinline__ u32x4 turned(const uint32_t (&w)[8], int e) {
     return r;
 }
 
-// One step of 32 keys from `key`. edge: some of them are not every row's. hi, lo: the keys [lo, hi) that the lane's query sees
+// One step of 32 keys from `key`; whether values went in as zeros (mark_not_finite). edge: some of them are not every row's. hi, lo: the keys [lo, hi) that the lane's query sees
 template <int D, bool BF, bool E8, int NT>
-__device__ __forceinline__ void step(const u32x4 (&q)[NT][D / 32], const Keys<D, E8>& k, Values<D, E8>& v, bool edge, int key,
+__device__ __forceinline__ bool step(const u32x4 (&q)[NT][D / 32], const Keys<D, E8>& k, Values<D, E8>& v, bool edge, int key,
                                      const Pages& p, const int (&lo)[NT], const int (&hi)[NT], int any_lo, int any_hi, float scale,
                                      State<D, NT>& st) {
     using V = Values<D, E8>;
@@ -293,7 +121,7 @@ __device__ __forceinline__ void step(const u32x4 (&q)[NT][D / 32], const Keys<D,
 #pragma unroll
             for (int t = 0; t < NT; ++t) s[t][u] = mfma<BF>(kw, q[t][c], s[t][u]);
         }
-    bool odd = false;                                         // a NaN or an infinity: some rows may see it and others not
+    bool odd = false;
     if (edge) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -309,11 +137,11 @@ __device__ __forceinline__ void step(const u32x4 (&q)[NT][D / 32], const Keys<D,
                 for (int h = 0; h < V::HALVES; ++h)
 #pragma unroll
                     for (int w = 0; w < V::WORDS; ++w) {
-                        v.w[4 * u + i][h][w] &= keep;
-                        odd |= not_finite<BF, E8>(v.w[4 * u + i][h][w]);
+                        const uint32_t x = v.w[4 * u + i][h][w] & keep, f = finite<BF, E8>(x);
+                        odd |= f != x;
+                        v.w[4 * u + i][h][w] = f;
                     }
             }
-        odd = __any(odd);
     }
     u32x4 pw[NT];
 #pragma unroll
@@ -352,33 +180,14 @@ __device__ __forceinline__ void step(const u32x4 (&q)[NT][D / 32], const Keys<D,
                 if constexpr (E8) w[j] = i % 2 ? widen2<BF, true>(v.w[j][h][i / 2]) : widen2<BF, false>(v.w[j][h][i / 2]);
                 else w[j] = v.w[j][h][i];
             }
-            if (!odd) {
 #pragma unroll
-                for (int e = 2 * i; e < 2 * i + 2; ++e) {
-                    const u32x4 vw = turned(w, e);
+            for (int e = 2 * i; e < 2 * i + 2; ++e) {
+                const u32x4 vw = turned(w, e);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) st.o[t][h * 8 + e] = mfma<BF>(vw, pw[t], st.o[t][h * 8 + e]);
-                }
-            } else {                                          // rarely: a product a query, without the values that it does not see
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    for (int c = 0; c < 16; ++c) {
-                        const int from = __builtin_amdgcn_readlane(lo[t], c), to = __builtin_amdgcn_readlane(hi[t], c);
-                        uint32_t x[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int at = key + 16 * (j / 4) + 4 * g + j % 4;
-                            x[j] = at < from || at >= to ? 0 : w[j];
-                        }
-#pragma unroll
-                        for (int e = 2 * i; e < 2 * i + 2; ++e) {
-                            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                            const f32x4 r = mfma<BF>(turned(x, e), pw[t], zero);
-                            if ((lane & 15) == c) st.o[t][h * 8 + e] += r;
-                        }
-                    }
+                for (int t = 0; t < NT; ++t) st.o[t][h * 8 + e] = mfma<BF>(vw, pw[t], st.o[t][h * 8 + e]);
             }
         }
+    return odd;
 }
 
 template <int D, bool BF, bool E8, int NT>
@@ -422,6 +231,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     }
     const float scale = E8 ? a.scale * load_uniform(a.ks + pc.head) : a.scale;
     const int end = min(k1, any_hi);
+    bool odd = false;
     int key = k0 + STEP * wave;
     if (any_lo > key) key += (any_lo - key) / PIECE * PIECE;
     for (; key < end; key += PIECE) {
@@ -431,7 +241,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
         load_keys<D, E8>(a, kb, p, lane, k);
         load_values<D, E8>(a, vb, p, lane, v);
         const bool edge = key < all_lo || key + STEP > all_hi || p.page[0] < 0 || p.page[1] < 0;
-        step<D, BF, E8, NT>(q, k, v, edge, key, p, lo, hi, any_lo, any_hi, scale, st);
+        odd |= step<D, BF, E8, NT>(q, k, v, edge, key, p, lo, hi, any_lo, any_hi, scale, st);
     }
 
     // the four waves' shares: scaled to one maximum, summed in two rounds through the LDS
@@ -474,12 +284,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
                 for (int e = 0; e < OPS; ++e) st.o[t][e] += sh_o[wave][t * OPS + e][lane];
         __syncthreads();
     }
-    if (wave != 0) return;
     const float vscale = E8 ? load_uniform(a.vs + pc.head) : 1.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int row = pc.tile * ROWS + 16 * t + (lane & 15), i = row / a.group, gh = row % a.group;
-        if (i >= r.n) continue;
+        if (wave != 0 || i >= r.n) continue;
         // operand e of half h, output i of row group g: element 128 h + E (4 g + i) + e
         constexpr int E = Values<D, E8>::E, HALVES = Values<D, E8>::HALVES;
         if (pc.pieces == 1) {
@@ -497,7 +306,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
                     else *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
                 }
         } else {
-            float* to = a.part + (pc.slot * ROWS + 16 * t + (lane & 15)) * D;
+            float* to = a.part + (pc.row + 16 * t + (lane & 15)) * D;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
@@ -507,108 +316,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
                         *reinterpret_cast<float4*>(to + 128 * h + E * (4 * g + u) + e) =
                             make_float4(st.o[t][h * 8 + e][u], st.o[t][h * 8 + e + 1][u], st.o[t][h * 8 + e + 2][u],
                                         st.o[t][h * 8 + e + 3][u]);
-            if (g == 0) *reinterpret_cast<float2*>(a.stats + (pc.slot * ROWS + 16 * t + lane) * 2) = make_float2(m[t], l[t]);
+            if (g == 0) a.stats[pc.row + 16 * t + lane] = make_float2(m[t], l[t]);
         }
     }
+    if (__syncthreads_or(odd)) mark_not_finite<D, BF, E8, ROWS>(a, pc, r, table, k0, end);
 }
 
-// The pieces of one row joined: a workgroup a row of a request with more than one; D / 4 lanes a piece, the pieces in order within
-// every 256 / (D / 4)-th, then those sums in order
-template <int D, bool BF, bool E8, int NT>
-__global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
-    constexpr int ROWS = 16 * NT, LANES = D / 4, SIDE = 256 / LANES;
-    __shared__ float4 sh[SIDE][LANES];
-    __shared__ float sh_m[4], sh_l[4];
-    const int heads = a.Hkv * a.group, head = blockIdx.x % heads, i = blockIdx.x / heads % a.max_new,
-              b = blockIdx.x / heads / a.max_new;
-    const Request r = uniform_request(a, b);
-    if (i >= r.n) return;
-    const int2 plan = a.plan[b];
-    const int pieces = plan.y;
-    if (pieces == 1) return;
-    const int row = i * a.group + head % a.group, tiles = (r.n * a.group + ROWS - 1) / ROWS;
-    const int64_t slot = plan.x + (int64_t)(head / a.group * tiles + row / ROWS) * pieces;
-    const float* part = a.part + (slot * ROWS + row % ROWS) * D;
-    const float2* stats = reinterpret_cast<const float2*>(a.stats) + slot * ROWS + row % ROWS;
-    float m = -INFINITY;
-    for (int p = threadIdx.x; p < pieces; p += 256) m = fmaxf(m, stats[(int64_t)p * ROWS].x);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0) sh_m[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-    const float base = m == -INFINITY ? 0.f : m;
-    const int lane = threadIdx.x % LANES, side = threadIdx.x / LANES;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int p = side; p < pieces; p += SIDE) {
-        const float2 s = stats[(int64_t)p * ROWS];
-        const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)p * ROWS * D + 4 * lane);
-        const float w = __builtin_amdgcn_exp2f(s.x - base);
-        l += s.y * w;
-        o.x += v.x * w;
-        o.y += v.y * w;
-        o.z += v.z * w;
-        o.w += v.w * w;
-    }
-    sh[side][lane] = o;
-    __shared__ float sides[SIDE];
-    if (lane == 0) sides[side] = l;
-    __syncthreads();
-    if (side != 0) return;
-    l = sides[0];
-#pragma unroll
-    for (int k = 1; k < SIDE; ++k) {
-        const float4 v = sh[k][lane];
-        l += sides[k];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
-    }
-    const float vscale = E8 ? a.vs[head / a.group] : 1.f;
-    const float f = l > 0.f ? vscale / l : l == 0.f ? 0.f : __builtin_nanf("");
-    *reinterpret_cast<uint2*>(a.out + (int64_t)(r.first + i) * a.o_row + (int64_t)head * a.o_head + 4 * lane) =
-        make_uint2(pack2<BF>(o.x * f, o.y * f), pack2<BF>(o.z * f, o.w * f));
-}
-
-// ---- the host's side
-
-// Rows a tile: 32 where a request has more than 16
-inline int attend_rows(int64_t max_new, int64_t group) { return max_new * group > 16 ? 32 : 16; }
-
-struct AttendSizes {
-    int64_t tiles, items, slots, part, stats, bytes;          // offsets in bytes behind the plan
-    AttendSizes(int64_t B, int64_t max_new, int64_t group, int64_t Hkv, int64_t D, int64_t capacity, int64_t split) {
-        const int64_t rows = attend_rows(max_new, group);
-        tiles = (max_new * group + rows - 1) / rows * Hkv;
-        const int64_t size = split ? split : PIECE, most = (capacity + size - 1) / size;      // pieces a tile, at most
-        items = B * tiles * std::max<int64_t>(1, most);
-        slots = most > 1 ? items : 0;
-        if (!split) {                                          // sum of ceil(k / size) over all tiles: at most TARGET + tiles
-            items = std::min(items, B * tiles + TARGET);
-            slots = std::min<int64_t>(slots, 2 * TARGET);      // of those with k > size: at most twice sum of k / size
-        }
-        part = (B * 8 + 15) / 16 * 16;
-        stats = part + slots * rows * D * 4;
-        bytes = stats + slots * rows * 8;
-    }
-};
-
-template <int D, bool BF, bool E8, int NT>
-void attend_launch(const AttendArgs& a, const AttendSizes& z, hipStream_t st) {
-    attend_kernel<D, BF, E8, NT><<<(unsigned)z.items, 256, 0, st>>>(a);
-    if (z.slots) join_kernel<D, BF, E8, NT><<<(unsigned)((int64_t)a.B * a.max_new * a.Hkv * a.group), 256, 0, st>>>(a);
-}
 template <int D, bool BF, bool E8>
-void attend_tiles(const AttendArgs& a, const AttendSizes& z, hipStream_t st) {
-    attend_rows(a.max_new, a.group) == 16 ? attend_launch<D, BF, E8, 1>(a, z, st) : attend_launch<D, BF, E8, 2>(a, z, st);
+void attend_launch(const AttendArgs& a, const AttendSizes& z, hipStream_t st) {
+    if (z.tile_rows == 16) attend_kernel<D, BF, E8, 1><<<(unsigned)z.few, 256, 0, st>>>(a);
+    else attend_kernel<D, BF, E8, 2><<<(unsigned)z.few, 256, 0, st>>>(a);
+    if (z.many) attend_prompt(a, z, D, BF, E8, st);
+    const int64_t rows = (int64_t)a.B * a.max_new * a.Hkv * a.group;
+    if (z.rows) join_kernel<D, BF, E8><<<(unsigned)std::min<int64_t>(rows, JOIN_GRID), 256, 0, st>>>(a);
 }
 template <int D>
 void attend_types(const AttendArgs& a, const AttendSizes& z, bool bf, bool e8, hipStream_t st) {
-    if (bf) e8 ? attend_tiles<D, true, true>(a, z, st) : attend_tiles<D, true, false>(a, z, st);
-    else e8 ? attend_tiles<D, false, true>(a, z, st) : attend_tiles<D, false, false>(a, z, st);
+    if (bf) e8 ? attend_launch<D, true, true>(a, z, st) : attend_launch<D, true, false>(a, z, st);
+    else e8 ? attend_launch<D, false, true>(a, z, st) : attend_launch<D, false, false>(a, z, st);
 }
 
 }  // namespace esp
@@ -620,13 +345,13 @@ using namespace esp;
 
 constexpr int64_t ATTEND_CAPACITY = int64_t(1) << 28;
 
-extern "C" int64_t esp_paged_attention_scratch(int64_t B, int64_t max_new, int64_t Hq, const esp_kv_cache* cache,
+extern "C" int64_t esp_paged_attention_scratch(int64_t B, int64_t T, int64_t max_new, int64_t Hq, const esp_kv_cache* cache,
                                                int64_t max_pages, int64_t split) {
-    if (!cache || B <= 0 || B > (1 << 20) || max_new <= 0 || max_new >= (1 << 24) || cache->heads < 1 || Hq < cache->heads ||
+    if (!cache || T <= 0 || T >= (1 << 24) || B <= 0 || B > (1 << 20) || max_new <= 0 || max_new >= (1 << 24) || cache->heads < 1 || Hq < cache->heads ||
         Hq % cache->heads || Hq > 65536 || cache->page < 1 || max_pages < 0 || max_pages * cache->page > ATTEND_CAPACITY ||
         split < 0 || split % PIECE)
         return 0;
-    return AttendSizes(B, max_new, Hq / cache->heads, cache->heads, cache->dim, max_pages * cache->page, split).bytes;
+    return AttendSizes(B, T, max_new, Hq / cache->heads, cache->heads, cache->dim, max_pages * cache->page, split).bytes;
 }
 
 extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head, int64_t T, int64_t Hq, int dtype,
@@ -661,8 +386,9 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     // other workgroups still read the queries when one writes its rows
     ESP_REQUIRE(!esp_host::rows_meet(out, out_row * 2, ((Hq - 1) * out_head + c.dim) * 2, q, q_row * 2,
                                      ((Hq - 1) * q_head + c.dim) * 2, T), "paged_attention: the output overlaps q");
-    const AttendSizes z(B, max_new, group, c.heads, c.dim, max_pages * c.page, split);
-    ESP_REQUIRE(z.items < (1 << 24) && B * max_new * Hq < (int64_t(1) << 31), "paged_attention: at most 2^24 - 1 pieces of tiles");
+    const AttendSizes z(B, T, max_new, group, c.heads, c.dim, max_pages * c.page, split);
+    ESP_REQUIRE(z.few < (1 << 24) && z.many < (1 << 24) && z.rows < (1 << 30) && B * max_new * Hq < (int64_t(1) << 31),
+                "paged_attention: at most 2^24 - 1 pieces of tiles");
     ESP_REQUIRE(scratch_bytes >= z.bytes, "paged_attention: the scratch needs esp_paged_attention_scratch bytes");
     AttendArgs a;
     a.q = static_cast<const uint16_t*>(q);
@@ -691,7 +417,9 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     char* base = static_cast<char*>(scratch);
     a.plan = reinterpret_cast<int2*>(base);
     a.part = reinterpret_cast<float*>(base + z.part);
-    a.stats = reinterpret_cast<float*>(base + z.stats);
+    a.stats = reinterpret_cast<float2*>(base + z.stats);
+    a.tile_rows = z.tile_rows;
+    a.first_row = z.first_row;
     a.B = (int)B;
     a.T = (int)T;
     a.Hkv = (int)c.heads;

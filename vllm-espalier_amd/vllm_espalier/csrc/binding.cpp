@@ -1020,7 +1020,7 @@ at::Tensor paged_attention(const at::Tensor& q_any, const at::Tensor& k_cache, c
             on_device(**v, q, "first / n_new");
             TORCH_CHECK((*v)->numel() == B, "first / n_new: [B]");
         }
-    const int64_t bytes = esp_paged_attention_scratch(B, max_new, q.size(1), &c, max_pages, split);
+    const int64_t bytes = esp_paged_attention_scratch(B, T, max_new, q.size(1), &c, max_pages, split);
     const at::Tensor scratch = at::empty({bytes}, q.options().dtype(at::kByte));
     call(esp_paged_attention(q.data_ptr(), row_stride(q), head_stride(q), T, q.size(1), dtype_code(q), &c, cptr<int32_t>(tables),
                              B > 1 ? tables.stride(0) : max_pages, max_pages, cptr<int32_t>(lengths),

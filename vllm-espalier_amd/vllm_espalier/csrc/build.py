@@ -2,7 +2,7 @@
 
   libespalier_hip.so   the HIP kernels and the C ABI of include/espalier.h (dense.hip, dense_multi.hip, dense_tile.hip,
                        dense_stream.hip, prompt.hip, moe.hip, moe_prompt.hip, step.hip, sandwich.hip, lora.hip, verify.hip,
-                       cache.hip, attention.hip, logprobs.hip, abi.cpp)
+                       cache.hip, attention.hip, attention_prompt.hip, logprobs.hip, abi.cpp)
   espalier_ext*.so     the torch extension module (binding.cpp, host code only), linked to libespalier_hip.so
   libespalier_probe.so bench.py --probes' measurement kernels (probe.hip), apart from the kernel layer
 
@@ -66,6 +66,7 @@ def build_lib(jobs: int, incremental: bool = False, pkg: Path = PKG, build_dir: 
     srcs = [CSRC / "dense.hip", CSRC / "dense_multi.hip", CSRC / "dense_tile.hip",
             CSRC / "dense_stream.hip", CSRC / "prompt.hip", CSRC / "moe.hip", CSRC / "moe_prompt.hip", CSRC / "step.hip",
             CSRC / "sandwich.hip", CSRC / "lora.hip", CSRC / "verify.hip", CSRC / "cache.hip", CSRC / "attention.hip",
+            CSRC / "attention_prompt.hip",
             CSRC / "logprobs.hip", CSRC / "abi.cpp"]
     objs = [build_dir / (s.stem + ".o") for s in srcs]
     headers = [*CSRC.glob("*.hpp"), REPO / "include" / "espalier.h"]
