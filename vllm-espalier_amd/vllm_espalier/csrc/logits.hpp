@@ -11,26 +11,32 @@ namespace esp {
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// elements i .. i + 8 of a row
+template <int DT>
+__device__ __forceinline__ void load_whole_group(const void* row, int i, float (&v)[8]) {
+    if constexpr (DT == F32) {
+        const f32x4_a4* p = reinterpret_cast<const f32x4_a4*>(static_cast<const float*>(row) + i);
+        const f32x4_a4 a = p[0], b = p[1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = a[k];
+            v[4 + k] = b[k];
+        }
+    } else {
+        const u32x4_a2 u = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(row) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[2 * k] = from16((uint16_t)(u[k] & 0xFFFFu), DT == BF16);
+            v[2 * k + 1] = from16((uint16_t)(u[k] >> 16), DT == BF16);
+        }
+    }
+}
+
 // elements i .. i + 8 of a row of V, `past` past its end
 template <int DT>
 __device__ __forceinline__ void load_group(const void* row, int i, int V, float past, float (&v)[8]) {
     if (i + 8 <= V) {
-        if constexpr (DT == F32) {
-            const f32x4_a4* p = reinterpret_cast<const f32x4_a4*>(static_cast<const float*>(row) + i);
-            const f32x4_a4 a = p[0], b = p[1];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[k] = a[k];
-                v[4 + k] = b[k];
-            }
-        } else {
-            const u32x4_a2 u = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(row) + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[2 * k] = from16((uint16_t)(u[k] & 0xFFFFu), DT == BF16);
-                v[2 * k + 1] = from16((uint16_t)(u[k] >> 16), DT == BF16);
-            }
-        }
+        load_whole_group<DT>(row, i, v);
     } else {                                                 // eight loads at once here too, and none wholly past the end
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = past;

@@ -1,14 +1,19 @@
 // Log-probabilities of given tokens, with their ranks, the rows' entropies and the likeliest alternatives, on gfx950. With
-// p = softmax(row / T), m the row's largest logit, d = l - m, z = sum exp(d / T):
-//   log p_t = d_t / T - log z,   -sum p log p = log z - (sum exp(d / T) d / T) / z.
+// p = softmax(row / T), c = log2(e) / T and x = c l of a logit l:
+//   log2 p_t = x_t - log2 z,   -sum p log2 p = log2 z - (sum 2^x x) / z,   z = sum 2^x.
 // Tokens are ordered by their logits, equal ones by their indices; a token's rank is its place in that order.
 //
 // Two launches. The first reads every row once: a wave takes 1024 logits into registers and leaves their maximum, their sums and
-// how many of them come before the row's token, so no workgroup waits for another. The second puts a row together, a workgroup a
-// row, and finds the alternatives without another pass over it: the k first tokens lie in the k pieces whose largest logits are
-// the first (each other piece has k elements before all of its own), and in there in the k lanes of 16 logits for which the same
-// holds. So it reads k pieces again, and keeps one key a lane. Keys hold the index: they are all different, and a key's place is
-// the number of larger ones.
+// how many of them come before the row's token, so no workgroup waits for another. Sums are over 2^(x - K) with K the whole number
+// nearest to the piece's largest x, so that an exponent costs one exact multiply-add; c's rounding to fp32, which shifts x by x times a
+// constant, is taken out of the sums afterwards (its first order is that constant times the sum of 2^(x - K) x, which is there).
+//
+// The second launch puts a row together, a workgroup a row, and finds the alternatives without another pass over it: the k first
+// tokens lie in the k pieces whose largest logits are the first (each other piece has k elements before all of its own), so it reads
+// these again and keeps the logits that are no smaller than the least of the k maxima, mostly little more than k. A row of fewer pieces
+// gets that bar from the largest logits of its lanes, 16 logits each. Where equal logits make them too many, the first key of each
+// lane is kept instead, of which the same holds once more, and sorted. Keys hold the index: they are all different, and a key's place
+// is the number of larger ones.
 #include "../../../include/espalier.h"
 #include "common.hpp"
 #include "logits.hpp"
@@ -23,9 +28,15 @@ constexpr int PIECE = 1024;                    // logits a wave takes: 16 a lane
 constexpr int PIECES_MAX = 1024;
 
 struct LogitsPiece {
-    float m, s, w;                             // largest logit (a NaN if there is one), sum of e = exp((l - m) / T), sum of e (l - m)
+    float m, s, w;                             // the largest logit (a NaN if there is one), sums of e = 2^(x - K) and of e (x - K)
     int above;                                 // logits before the row's token
 };
+
+// K of a piece, where c m is a number of moderate size; elsewhere (rows of a type's lowest values) the sums are over x - c m
+__device__ __forceinline__ bool whole_base(float m, float c, float& base) {
+    base = rintf(m * c);
+    return fabsf(m * c) < 16777216.0f;
+}
 
 struct LogprobsArgs {
     const void* logits;
@@ -49,211 +60,413 @@ __device__ __forceinline__ double inv_temperature_of(const LogprobsArgs& a, int 
     return a.temperature ? inv_temperature(load_uniform(a.temperature + r)) : 1.0;
 }
 
-// The statistics of the rows: a wave a piece, four to a workgroup
-template <int DT>
+// The statistics of the rows: a wave PER pieces, all on their way at once, four to a workgroup
+template <int DT, int PER>
 __global__ __launch_bounds__(256) void logprobs_stats_kernel(const LogprobsArgs a) {
-    const int quads = (a.pieces + 3) / 4, r = blockIdx.x / quads, lane = threadIdx.x & 63;
-    const int piece = (int)(blockIdx.x % quads) * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    if (piece >= a.pieces) return;
+    const int groups = (a.pieces + 4 * PER - 1) / (4 * PER), r = blockIdx.x / groups, lane = threadIdx.x & 63;
+    const int piece0 = ((int)(blockIdx.x % groups) * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))) * PER;
+    if (piece0 >= a.pieces) return;
     const void* row = row_of<DT>(a, r);
-    const int i0 = piece * PIECE + lane * 8;
-    float v[2][8];
+    float all[PER][2][8];
+    if ((piece0 + PER) * PIECE <= a.V) {                    // (whole pieces without a branch between their loads)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_group<DT>(row, i0 + u * 512, a.V, -INFINITY, v[u]);
+        for (int j = 0; j < PER; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) load_whole_group<DT>(row, (piece0 + j) * PIECE + lane * 8 + u * 512, all[j][u]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) load_group<DT>(row, (piece0 + j) * PIECE + lane * 8 + u * 512, a.V, -INFINITY, all[j][u]);
+    }
     const int token = load_uniform(a.tokens + r);
     const bool given = token >= 0 && token < a.V;
     const float mine = load_elem(row, DT, (size_t)(given ? token : 0));
     float hi, lo;
     exponent_factor(inv_temperature_of(a, r), hi, lo);
-    float m = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, v[u][k]);
-    m = wave_max_f32(m);                                    // NaN is passed over here and found in the sum
-    const float base = m == -INFINITY ? 0.f : m;
-    float s = 0.f, w = 0.f;
-    int above = 0;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float d = v[u][k] - base, e = exp_scaled(d, hi, lo);
-            s += e;
-            w += e * fmaxf(d, -3.0e38f);                    // a masked logit: 0 times a number
-            above += v[u][k] > mine || (v[u][k] == mine && i0 + u * 512 + k < token);
-        }
-    s = wave_sum_f32(s);
-    w = wave_sum_f32(w);
-    bool nan = false;
-    if (s != s || mine != mine) {                           // a NaN, or +inf: counted by their order
-        above = 0;
-        const unsigned long long key = key32(mine, token);
+    const auto one = [&](int piece, const float (&v)[2][8]) __attribute__((always_inline)) {
+        const int i0 = piece * PIECE + lane * 8;
+        float m = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int i = i0 + u * 512 + k;
-                nan |= v[u][k] != v[u][k];
-                above += i < a.V && key32(v[u][k], i) > key;
-            }
-        nan = __any(nan);
-    }
+            for (int k = 0; k < 8; ++k) m = fmaxf(m, v[u][k]);
+        m = wave_max_f32(m);                                    // NaN is passed over here and found in the sum
+        float s = 0.f, w = 0.f, base;
+        if (whole_base(m, hi, base)) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) above += __shfl_xor(above, d);
-    if (lane == 0) a.part[(size_t)r * a.pieces + piece] = {nan ? __builtin_nanf("") : m, s, w, given ? above : 0};
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    float x = __builtin_fmaf(v[u][k], hi, -base);
+                    const float e = __builtin_amdgcn_exp2f(x);
+                    s += e;
+                    w = __builtin_fmaf(e, fmaxf(x, -1024.0f), w);      // a masked logit: 0 times a number
+                }
+        } else {
+            base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float d = v[u][k] - base, e = exp_scaled(d, hi, lo);
+                    s += e;
+                    w = __builtin_fmaf(e, fmaxf(d * hi, -1024.0f), w);
+                }
+        }
+        s = wave_sum_f32(s);
+        w = wave_sum_f32(w);
+        int above = 0;
+        const int begin = piece * PIECE;
+        if (token < begin) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) above += __popcll(__ballot(v[u][k] > mine));
+        } else if (token >= begin + PIECE) {                    // (never of a piece that ends past the row)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) above += __popcll(__ballot(v[u][k] >= mine));
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    above += __popcll(__ballot(v[u][k] > mine || (v[u][k] == mine && i0 + u * 512 + k < token)));
+        }
+        bool nan = false;
+        if (s != s || mine != mine) {                           // a NaN, or +inf: counted by their order
+            above = 0;
+            const unsigned long long key = key32(mine, token);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int i = i0 + u * 512 + k;
+                    nan |= v[u][k] != v[u][k];
+                    above += __popcll(__ballot(i < a.V && key32(v[u][k], i) > key));
+                }
+            nan = __any(nan);
+        }
+        if (lane == 0) a.part[(size_t)r * a.pieces + piece] = {nan ? __builtin_nanf("") : m, s, w, given ? above : 0};
+    };
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (piece0 + j < a.pieces) one(piece0 + j, all[j]);
 }
 
-// How many of the n keys are larger
+// Keys in the LDS: of all pieces, of the lanes of `top` pieces or of the logits of `top` lanes, whole powers of two, and a zero; at
+// least some hundred logits
+__host__ __device__ inline int keys_room(int pieces, int top) {
+    int n = 512;
+    while (n < pieces || n < top * 64) n *= 2;
+    return n;
+}
+// the logit of a key (zeros of both signs alike)
+__device__ __forceinline__ float logit_of(unsigned long long key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __builtin_bit_cast(float, o & 0x80000000u ? (o == 0xFFFFFFFFu ? 0x7FC00000u : o & 0x7FFFFFFFu) : ~o);
+}
+
+// How many of the n keys are larger; a zero follows the last
 __device__ __forceinline__ int place_of(unsigned long long key, const unsigned long long* keys, int n) {
+    const ulonglong2* two = reinterpret_cast<const ulonglong2*>(keys);
     int larger = 0;
-    for (int i = 0; i < n; ++i) larger += keys[i] > key;
+#pragma unroll 8
+    for (int i = 0; i < (n + 1) / 2; ++i) larger += (two[i].x > key) + (two[i].y > key);
     return larger;
 }
 
+// The k-th largest of values[0 .. n) (a multiple of 256), by 256 threads a byte at a time from the top: how many have each value of
+// it, of those that agree above it. bins: 256 counts and two more
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int n, int k, int* bins) {
+    const int t = threadIdx.x, lane = t & 63;
+    uint32_t found = 0;
+#pragma unroll
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        bins[t] = 0;
+        __syncthreads();
+        for (int i = t; i < n; i += 256)
+            if (shift == 24 || (values[i] ^ found) >> (shift + 8) == 0) atomicAdd(&bins[values[i] >> shift & 255], 1);
+        __syncthreads();
+        if (t < 64) {                                       // lane l: bins 255 - 4 l down
+            int c[4], upto = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) upto += c[j] = bins[255 - 4 * lane - j];
+            const int mine = upto;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(upto, d);
+                if (lane >= d) upto += o;
+            }
+            int before = upto - mine;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (before < k && before + c[j] >= k) {
+                    bins[256] = 255 - 4 * lane - j;
+                    bins[257] = k - before;
+                }
+                before += c[j];
+            }
+        }
+        __syncthreads();
+        found |= (uint32_t)bins[256] << shift;
+        k = bins[257];
+        __syncthreads();
+    }
+    return found;
+}
+
+// keys[0 .. n), n a power of two, from the largest down, by 256 threads
+__device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
+    for (int size = 2; size <= n; size *= 2)
+        for (int log = 30 - __clz(size); log >= 0; --log) {
+            const int step = 1 << log;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n / 2; i += 256) {
+                const int lo = (i >> log) * 2 * step + (i & (step - 1)), hi = lo + step;
+                const unsigned long long x = keys[lo], y = keys[hi];
+                if ((x < y) == ((lo & size) == 0)) {
+                    keys[lo] = y;
+                    keys[hi] = x;
+                }
+            }
+        }
+    __syncthreads();
+}
+__device__ __forceinline__ int power_of_two(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
+
 struct LogprobsRow {
-    double z, w;                               // over the row's maximum
+    double z, w;
     float m;
     int above;
 };
 
-// A row from its pieces, and its alternatives
-template <int DT>
+// A row from its pieces, and its alternatives: the logits that these are chosen from are on their way, of AHEAD pieces a wave at once,
+// while the row's sums are made
+template <int DT, int AHEAD>
 __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a) {
-    __shared__ unsigned long long keys[TOP_MAX * 64];       // of pieces, then of lanes, then of logits
+    extern __shared__ __attribute__((aligned(16))) unsigned long long keys[];        // keys_room and two more
     __shared__ int chosen[TOP_MAX];
-    __shared__ unsigned long long least[4];
+    __shared__ uint32_t bar;
     __shared__ LogprobsRow part[4];
-    __shared__ int count;
+    __shared__ int count, nan, bins[258];
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const LogitsPiece* p = a.part + (size_t)r * a.pieces;
     const void* row = row_of<DT>(a, r);
+    // a thread's pieces t, t + 256, ..
+    LogitsPiece held[PIECES_MAX / 256];
+#pragma unroll
+    for (int k = 0; k < PIECES_MAX / 256; ++k)
+        held[k] = t + 256 * k < a.pieces ? p[t + 256 * k] : LogitsPiece{-INFINITY, 0.f, 0.f, 0};
     const int token = load_uniform(a.tokens + r);
     const bool given = token >= 0 && token < a.V;
     const float mine = load_elem(row, DT, (size_t)(given ? token : 0));
-    const double inv_t = inv_temperature_of(a, r);
-    // a thread's pieces t, t + 256, ..: the maximum, then the sums over it
-    LogitsPiece held[PIECES_MAX / 256];
-    float m = -INFINITY;
+    const int n_pieces = min(a.pieces, a.top);
+    if (a.top) {                                            // the pieces that the alternatives lie in
+#pragma unroll
+        for (int k = 0; k < PIECES_MAX / 256; ++k)
+            if (t + 256 * k <= a.pieces) keys[t + 256 * k] = t + 256 * k < a.pieces ? key32(held[k].m, t + 256 * k) : 0;
+        if (t == 0) {
+            keys[a.pieces] = 0;
+            count = 0;
+        }
+        __syncthreads();
+        for (int i = t; i < a.pieces; i += 256) {
+            const unsigned long long key = keys[i];
+            const int at = place_of(key, keys, a.pieces);
+            if (at < n_pieces) chosen[at] = i;
+            if (at == a.top - 1) bar = (uint32_t)(key >> 32);
+            if (at == 0) nan = key >> 32 == 0xFFFFFFFFull;
+        }
+        __syncthreads();
+    }
+    float v[AHEAD][2][8];
+    int first[AHEAD];
+    const auto load_ahead = [&](int from) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (from + 4 * j < n_pieces) {
+                const int piece = __builtin_amdgcn_readfirstlane(chosen[from + 4 * j]);
+                first[j] = piece * PIECE + lane * 8;
+                if ((piece + 1) * PIECE <= a.V) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) load_whole_group<DT>(row, first[j] + u * 512, v[j][u]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) load_group<DT>(row, first[j] + u * 512, a.V, 0.f, v[j][u]);
+                }
+            }
+    };
+    load_ahead(wave);
+    if (n_pieces < a.top) {                                 // the bar from the lanes (those without a logit: 0)
+        uint32_t* order = reinterpret_cast<uint32_t*>(keys);
+        const int n = (n_pieces * 64 + 255) / 256 * 256;
+        for (int i = n_pieces * 64 + t; i < n; i += 256) order[i] = 0;
+        for (int from = wave; from < n_pieces; from += 4 * AHEAD) {
+            if (from != wave) load_ahead(from);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+                if (from + 4 * j < n_pieces) {
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (first[j] + u * 512 + k < a.V) most = max(most, (uint32_t)(key32(v[j][u][k], 0) >> 32));
+                    order[(from + 4 * j) * 64 + lane] = most;
+                }
+        }
+        __syncthreads();
+        const uint32_t b = kth_largest(order, n, min(a.top, n), bins);
+        if (t == 0) bar = b;
+        if (n_pieces > 4 * AHEAD) load_ahead(wave);
+        __syncthreads();
+    }
+    // the pieces' sums over 2^base, and those over the largest base
+    const double inv_t = inv_temperature_of(a, r), c = inv_t * 1.4426950408889634;
+    float hi, lo;
+    exponent_factor(inv_t, hi, lo);
+    const double off = (float)(c - (double)hi) / hi;
+    double base[PIECES_MAX / 256], s[PIECES_MAX / 256], w[PIECES_MAX / 256];
+    float most = -INFINITY;
+    int above = 0;
 #pragma unroll
     for (int k = 0; k < PIECES_MAX / 256; ++k) {
-        held[k] = t + 256 * k < a.pieces ? p[t + 256 * k] : LogitsPiece{-INFINITY, 0.f, 0.f, 0};
-        m = fmaxf(m, held[k].m);
+        float b;
+        s[k] = held[k].s;
+        w[k] = held[k].w;
+        base[k] = held[k].m == -INFINITY ? -INFINITY : (double)held[k].m * c;
+        if (s[k] != 0.0 && whole_base(held[k].m, hi, b)) {
+            const double shift = off * (w[k] + (double)b * s[k]);       // sum of e (c - hi) l
+            base[k] = b;
+            s[k] += 0.6931471805599453 * shift;
+            w[k] += shift;
+        }
+        most = fmaxf(most, held[k].m);
+        above += held[k].above;
     }
-    m = wave_max_f32(m);
-    if (lane == 0) part[wave].m = m;
-    if (t == 0) count = 0;
+    most = wave_max_f32(most);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) above += __shfl_xor(above, d);
+    if (lane == 0) {
+        part[wave].m = most;
+        part[wave].above = above;
+    }
     __syncthreads();
-    m = fmaxf(fmaxf(part[0].m, part[1].m), fmaxf(part[2].m, part[3].m));
-    const double base = m == -INFINITY ? 0.0 : (double)m;
-    double z = 0.0, w = 0.0, above = 0.0;
+    most = fmaxf(fmaxf(part[0].m, part[1].m), fmaxf(part[2].m, part[3].m));
+    float whole;
+    const double top = whole_base(most, hi, whole) ? (double)whole : most == -INFINITY ? 0.0 : (double)most * c;
+    double z = 0.0, sum_w = 0.0;
 #pragma unroll
     for (int k = 0; k < PIECES_MAX / 256; ++k)
-        if (held[k].s != 0.f) {
-            const double d = (double)held[k].m - base, e = exp(d * inv_t);
-            z += (double)held[k].s * e;
-            w += ((double)held[k].w + (double)held[k].s * d) * e;
+        if (s[k] != 0.0) {
+            const double d = base[k] - top, e = __builtin_amdgcn_exp2f((float)d);     // (of whole numbers, a power of two)
+            z += s[k] * e;
+            sum_w += e != 0.0 ? (w[k] + s[k] * d) * e : 0.0;
         }
-#pragma unroll
-    for (int k = 0; k < PIECES_MAX / 256; ++k) above += held[k].above;
     z = wave_sum_f64_dpp(z);
-    w = wave_sum_f64_dpp(w);
-    above = wave_sum_f64_dpp(above);
+    sum_w = wave_sum_f64_dpp(sum_w);
     if (lane == 0) {
         part[wave].z = z;
-        part[wave].w = w;
-        part[wave].above = (int)above;
+        part[wave].w = sum_w;
     }
-    if (a.top)
-        for (int i = t; i < a.pieces; i += 256) keys[i] = key32(p[i].m, i);
+    // their logits from the bar on
+    const uint32_t reach = bar;
+    const float least = nan ? __builtin_nanf("") : logit_of((unsigned long long)reach << 32);      // (a NaN: all are looked at)
+    const int room = keys_room(a.pieces, a.top);
+    for (int from = wave; from < n_pieces; from += 4 * AHEAD) {
+        if (from != wave) load_ahead(from);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (from + 4 * j < n_pieces)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (v[j][u][k] < least) continue;
+                        const int i = first[j] + u * 512 + k;
+                        const unsigned long long key = key32(v[j][u][k], i);
+                        if (i < a.V && (uint32_t)(key >> 32) >= reach) {
+                            const int at = atomicAdd(&count, 1);
+                            if (at < room) keys[at] = key;
+                        }
+                    }
+    }
     __syncthreads();
     z = ((part[0].z + part[1].z) + part[2].z) + part[3].z;
-    w = ((part[0].w + part[1].w) + part[2].w) + part[3].w;
+    sum_w = ((part[0].w + part[1].w) + part[2].w) + part[3].w;
     const bool some = z > 0.0 && z < INFINITY;
-    const double log_z = some ? log(z) : (double)__builtin_nanf("");
+    // log2 z in two parts: a whole number, and that of a number in [1/2, 1)
+    const double small = __builtin_amdgcn_frexp_mant(z);
+    const double log_s = (double)__builtin_amdgcn_frexp_exp(z) + (double)__builtin_amdgcn_logf((float)small);
+    const double log_z = some ? log_s + top : (double)__builtin_nanf("");
+    const auto log_p = [&](float l) __attribute__((always_inline)) { return (float)(0.6931471805599453 * ((double)l * c - log_z)); };
     if (t == 0) {
-        a.logprobs[r] = given ? (float)(((double)mine - base) * inv_t - log_z) : 0.f;
+        a.logprobs[r] = given ? log_p(mine) : 0.f;
         if (a.ranks) a.ranks[r] = given ? 1 + part[0].above + part[1].above + part[2].above + part[3].above : 0;
-        if (a.entropies) a.entropies[r] = (float)(log_z - w * inv_t / z);
+        if (a.entropies) a.entropies[r] = some ? (float)(0.6931471805599453 * (log_s - (double)((float)sum_w / (float)z))) : __builtin_nanf("");
     }
     if (!a.top) return;
-    // the pieces that the alternatives lie in
-    const int n_pieces = min(a.pieces, a.top);
-    for (int i = t; i < a.pieces; i += 256) {
-        const int at = place_of(keys[i], keys, a.pieces);
-        if (at < n_pieces) chosen[at] = i;
-    }
-    __syncthreads();
-    // the first key of each of their lanes
-    unsigned long long first = ~0ull;
-    for (int c = wave; c < n_pieces; c += 4) {
-        const int i0 = chosen[c] * PIECE + lane * 8;
-        unsigned long long key = 0;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float v[8];
-            load_group<DT>(row, i0 + u * 512, a.V, 0.f, v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (i0 + u * 512 + k < a.V) key = max(key, key32(v[k], i0 + u * 512 + k));
+    int n = count;
+    if (n <= min(room, 1024)) {
+        if (t == 0) keys[n] = 0;
+        __syncthreads();
+        for (int i = t; i < n; i += 256) {
+            const unsigned long long key = keys[i];
+            const int at = place_of(key, keys, n);
+            if (at < a.top) {
+                a.top_ids[(size_t)r * a.top + at] = (int)~(uint32_t)key;
+                a.top_logprobs[(size_t)r * a.top + at] = log_p(logit_of(key));
+            }
         }
-        keys[c * 64 + lane] = key;
-        first = min(first, wave_max_key(key));
+        return;
     }
-    if (lane == 0) least[wave] = first;
+    // Too many: the first key of each lane of the pieces, sorted; then the logits of the first lanes, sorted
     __syncthreads();
-    // (with fewer pieces than alternatives there is nothing that a key has to reach)
-    unsigned long long bar = n_pieces < a.top ? 1 : min(min(least[0], least[1]), min(least[2], least[3]));
-    unsigned long long mine_keys[TOP_MAX / 4];
+    n = power_of_two(n_pieces * 64);
+    for (int i = n_pieces * 64 + t; i < n; i += 256) keys[i] = 0;
+    for (int from = wave; from < n_pieces; from += 4 * AHEAD) {
+        load_ahead(from);
 #pragma unroll
-    for (int k = 0; k < TOP_MAX / 4; ++k) mine_keys[k] = t + 256 * k < n_pieces * 64 ? keys[t + 256 * k] : 0;
-    __syncthreads();
+        for (int j = 0; j < AHEAD; ++j)
+            if (from + 4 * j < n_pieces) {
+                unsigned long long key = 0;
 #pragma unroll
-    for (int k = 0; k < TOP_MAX / 4; ++k)
-        if (mine_keys[k] >= bar) keys[atomicAdd(&count, 1)] = mine_keys[k];
-    __syncthreads();
-    const int n_lanes = count;
-    __syncthreads();
-    if (t == 0) {
-        count = 0;
-        least[0] = 1;
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (first[j] + u * 512 + k < a.V) key = max(key, key32(v[j][u][k], first[j] + u * 512 + k));
+                keys[(from + 4 * j) * 64 + lane] = key;
+            }
+    }
+    sort_keys(keys, n);
+    if (t < a.top) {
+        const int id = t < n && keys[t] ? (int)~(uint32_t)keys[t] : -1;
+        chosen[t] = id < 0 ? -1 : id - id % 8 - (id % PIECE >= 512 ? 512 : 0);      // the first of the lane's logits
     }
     __syncthreads();
-    for (int i = t; i < n_lanes; i += 256) {
-        const unsigned long long key = keys[i];
-        const int at = place_of(key, keys, n_lanes);
-        if (at < a.top) {
-            const int id = (int)~(uint32_t)key;
-            chosen[at] = id - id % 512 % 8 - (id % PIECE >= 512 ? 512 : 0);     // the first of the lane's logits
-            if (at == a.top - 1) least[0] = key;
-        }
-    }
-    __syncthreads();
-    // their logits
-    bar = least[0];
-    const int n_chosen = min(n_lanes, a.top);
-    for (int i = t; i < n_chosen * 16; i += 256) {
-        const int id = chosen[i / 16] + (i % 16 >= 8 ? 512 : 0) + i % 8;
-        const unsigned long long key = id < a.V ? key32(load_elem(row, DT, (size_t)id), id) : 0;
-        if (key >= bar) keys[atomicAdd(&count, 1)] = key;
-    }
-    __syncthreads();
-    const int n = count;
+    n = power_of_two(a.top * 16);
     for (int i = t; i < n; i += 256) {
-        const unsigned long long key = keys[i];
-        const int at = place_of(key, keys, n);
-        if (at < a.top) {
-            const int id = (int)~(uint32_t)key;
-            a.top_ids[(size_t)r * a.top + at] = id;
-            a.top_logprobs[(size_t)r * a.top + at] = (float)(((double)load_elem(row, DT, (size_t)id) - base) * inv_t - log_z);
-        }
+        const int begin = i < a.top * 16 ? chosen[i / 16] : -1, id = begin + (i % 16 >= 8 ? 512 : 0) + i % 8;
+        keys[i] = begin >= 0 && id < a.V ? key32(load_elem(row, DT, (size_t)id), id) : 0;
+    }
+    sort_keys(keys, n);
+    if (t < a.top) {
+        a.top_ids[(size_t)r * a.top + t] = (int)~(uint32_t)keys[t];
+        a.top_logprobs[(size_t)r * a.top + t] = log_p(logit_of(keys[t]));
     }
 }
 
 template <int DT>
 int logprobs_launch(const LogprobsArgs& a, hipStream_t st) {
-    logprobs_stats_kernel<DT><<<(unsigned)((int64_t)a.R * ((a.pieces + 3) / 4)), 256, 0, st>>>(a);
-    logprobs_row_kernel<DT><<<(unsigned)a.R, 256, 0, st>>>(a);
+    // Two pieces a wave where there are waves enough (64 a CU): 2043 rows of 151935 bf16 logits (621 MB) 145 -> 124 us, 5.0 TB/s
+    if ((int64_t)a.R * a.pieces < 32768) logprobs_stats_kernel<DT, 1><<<(unsigned)((int64_t)a.R * ((a.pieces + 3) / 4)), 256, 0, st>>>(a);
+    else logprobs_stats_kernel<DT, 2><<<(unsigned)((int64_t)a.R * ((a.pieces + 7) / 8)), 256, 0, st>>>(a);
+    const size_t lds = a.top ? (keys_room(a.pieces, a.top) + 2) * 8 : 0;
+    if (a.top <= 4) logprobs_row_kernel<DT, 1><<<(unsigned)a.R, 256, lds, st>>>(a);
+    else logprobs_row_kernel<DT, 4><<<(unsigned)a.R, 256, lds, st>>>(a);
     return esp_host::launch_check("token_logprobs");
 }
 
