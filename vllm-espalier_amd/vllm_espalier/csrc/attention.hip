@@ -23,15 +23,10 @@ namespace esp {
 
 constexpr int64_t JOIN_GRID = 2048;            // workgroups of a join: what fits at once
 
-// The pages of a step's two times 16 keys
+// The pages of a step's two times 16 keys (-1: none), and the keys' places in them
 struct Pages {
-    int64_t page[2];
-    int off[2];
+    int page[2], off[2];
 };
-__device__ __forceinline__ Pages pages_of(const AttendArgs& a, const int32_t* table, int key) {
-    const Page p = page_of(a, table, key), q = page_of(a, table, key + 16);
-    return {{p.page, q.page}, {p.off, q.off}};
-}
 
 // A wave's 32 keys or values. Keys: operand c of tile u holds elements 32 c + 8 g .. + 8 of key l (16 bits), or, two operands a
 // load, 64 (c / 2) + 16 g + 8 (c % 2) .. + 8 (8 bits). Values: words of elements E l .. + E (in halves of 128) of keys 4 g + j
@@ -50,7 +45,7 @@ __device__ __forceinline__ void load_keys(const AttendArgs& a, const char* base,
     const int to = (lane & 15) * (int)a.k_token + (lane >> 4) * 16;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const char* row = base + (p.page[u] < 0 ? 0 : p.page[u]) * a.k_page + p.off[u] * a.k_token;
+        const char* row = base + (int64_t)max(p.page[u], 0) * a.k_page + p.off[u] * a.k_token;
 #pragma unroll
         for (int c = 0; c < (E8 ? D / 64 : D / 32); ++c) k.w[u][c] = *reinterpret_cast<const u32x4*>(row + to + c * 64);
     }
@@ -61,7 +56,7 @@ __device__ __forceinline__ void load_values(const AttendArgs& a, const char* bas
     const int to = (lane >> 4) * 4 * (int)a.v_token + (lane & 15) * V::WORDS * 4;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const char* row = base + (p.page[j / 4] < 0 ? 0 : p.page[j / 4]) * a.v_page + (p.off[j / 4] + j % 4) * a.v_token;
+        const char* row = base + (int64_t)max(p.page[j / 4], 0) * a.v_page + (p.off[j / 4] + j % 4) * a.v_token;
 #pragma unroll
         for (int h = 0; h < V::HALVES; ++h) {
             const char* at = row + to + h * (E8 ? 128 : 256);
@@ -94,14 +89,9 @@ __device__ __forceinline__ u32x4 turned(const uint32_t (&w)[8], int e) {
     return r;
 }
 
-// One step of 32 keys from `key`; whether values went in as zeros (mark_not_finite). edge: some of them are not every row's. hi, lo: the keys [lo, hi) that the lane's query sees
+// The scores of 32 keys
 template <int D, bool BF, bool E8, int NT>
-__device__ __forceinline__ bool step(const u32x4 (&q)[NT][D / 32], const Keys<D, E8>& k, Values<D, E8>& v, bool edge, int key,
-                                     const Pages& p, const int (&lo)[NT], const int (&hi)[NT], int any_lo, int any_hi, float scale,
-                                     State<D, NT>& st) {
-    using V = Values<D, E8>;
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    f32x4 s[NT][2];
+__device__ __forceinline__ void scores(const u32x4 (&q)[NT][D / 32], const Keys<D, E8>& k, f32x4 (&s)[NT][2]) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -121,6 +111,14 @@ __device__ __forceinline__ bool step(const u32x4 (&q)[NT][D / 32], const Keys<D,
 #pragma unroll
             for (int t = 0; t < NT; ++t) s[t][u] = mfma<BF>(kw, q[t][c], s[t][u]);
         }
+}
+
+// 32 keys from `key` by their scores and values; whether values went in as zeros (mark_not_finite). edge: some of them are not every row's. hi, lo: the keys [lo, hi) that the lane's query sees
+template <int D, bool BF, bool E8, int NT>
+__device__ __forceinline__ bool weigh(f32x4 (&s)[NT][2], Values<D, E8>& v, bool edge, int key, const Pages& p, const int (&lo)[NT],
+                                      const int (&hi)[NT], int any_lo, int any_hi, float scale, State<D, NT>& st) {
+    using V = Values<D, E8>;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
     bool odd = false;
     if (edge) {
 #pragma unroll
@@ -196,7 +194,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     Piece pc;
     if (!piece_of<ROWS>(a, (int)blockIdx.x, pc)) return;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, g = lane >> 4;
-    const Request r = uniform_request(a, pc.b);
+    const Request& r = pc.r;
     const int k0 = r.lo + pc.at * pc.size, k1 = min(k0 + pc.size, r.hi);
     const int32_t* table = a.tables + pc.b * a.table_row;
     const char *kb = a.k + pc.head * a.k_head, *vb = a.v + pc.head * a.v_head;
@@ -206,7 +204,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     int lo[NT], hi[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int row = pc.tile * ROWS + 16 * t + (lane & 15), i = row / a.group, gh = row % a.group;
+        const int row = 16 * t + (lane & 15), i = quotient(row, a.group), gh = row - i * a.group;
         const bool here = i < r.n;
         hi[t] = here ? max(0, min(r.length - r.n + i + 1, r.hi)) : 0;
         lo[t] = a.window && here ? max(0, r.length - r.n + i + 1 - a.window) : 0;
@@ -216,7 +214,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
             q[t][c] = *reinterpret_cast<const u32x4*>(p + (E8 ? c / 2 * 64 + g * 16 + c % 2 * 8 : c * 32 + g * 8));
     }
     // the keys that all of the tile's rows see, and those that any of them does
-    const int i0 = pc.tile * ROWS / a.group, i1 = min((pc.tile * ROWS + ROWS - 1) / a.group, r.n - 1);
+    const int i0 = 0, i1 = r.n - 1;                           // (a request is one tile)
     const int all_hi = min(r.length - r.n + i0 + 1, r.hi), any_hi = max(0, min(r.length - r.n + i1 + 1, r.hi));
     const int all_lo = a.window ? max(0, r.length - r.n + i1 + 1 - a.window) : 0;
     const int any_lo = a.window ? max(0, r.length - r.n + i0 + 1 - a.window) : 0;
@@ -234,14 +232,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     bool odd = false;
     int key = k0 + STEP * wave;
     if (any_lo > key) key += (any_lo - key) / PIECE * PIECE;
-    for (; key < end; key += PIECE) {
-        const Pages p = pages_of(a, table, key);
+    // Lane 2 i + u: the page of the wave's 16 keys u of step i from where it was last asked, 32 steps at once
+    Place ahead = {};
+    int steps = 0;
+    const auto pages_at = [&](int from) __attribute__((always_inline)) {
+        if (steps == 0) ahead = place_of(a, table, from + (lane >> 1) * PIECE + 16 * (lane & 1));
+        Pages p;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            p.page[u] = __builtin_amdgcn_readlane(ahead.page, 2 * steps + u);
+            p.off[u] = __builtin_amdgcn_readlane(ahead.off, 2 * steps + u);
+        }
+        steps = (steps + 1) & 31;
+        return p;
+    };
+    if (key < end) {
+        Pages p = pages_at(key);
         Keys<D, E8> k;
         Values<D, E8> v;
         load_keys<D, E8>(a, kb, p, lane, k);
         load_values<D, E8>(a, vb, p, lane, v);
-        const bool edge = key < all_lo || key + STEP > all_hi || p.page[0] < 0 || p.page[1] < 0;
-        odd |= step<D, BF, E8, NT>(q, k, v, edge, key, p, lo, hi, any_lo, any_hi, scale, st);
+        while (true) {                                        // the next keys are on their way while these are weighed, the next
+            const int next = key + PIECE;                     // values as soon as these are added up
+            const bool more = next < end;
+            f32x4 s[NT][2];
+            scores<D, BF, E8, NT>(q, k, s);
+            const Pages now = p;
+            if (more) {
+                p = pages_at(next);
+                load_keys<D, E8>(a, kb, p, lane, k);
+            }
+            const bool edge = key < all_lo || key + STEP > all_hi || now.page[0] < 0 || now.page[1] < 0;
+            odd |= weigh<D, BF, E8, NT>(s, v, edge, key, now, lo, hi, any_lo, any_hi, scale, st);
+            if (!more) break;
+            load_values<D, E8>(a, vb, p, lane, v);
+            key = next;
+        }
     }
 
     // the four waves' shares: scaled to one maximum, summed in two rounds through the LDS
@@ -287,7 +313,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     const float vscale = E8 ? load_uniform(a.vs + pc.head) : 1.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int row = pc.tile * ROWS + 16 * t + (lane & 15), i = row / a.group, gh = row % a.group;
+        const int row = 16 * t + (lane & 15), i = quotient(row, a.group), gh = row - i * a.group;
         if (wave != 0 || i >= r.n) continue;
         // operand e of half h, output i of row group g: element 128 h + E (4 g + i) + e
         constexpr int E = Values<D, E8>::E, HALVES = Values<D, E8>::HALVES;
@@ -306,7 +332,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
                     else *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
                 }
         } else {
-            float* to = a.part + (pc.row + 16 * t + (lane & 15)) * D;
+            const int64_t at = pc.row + (16 * t + (lane & 15)) * pc.pieces;
+            float* to = a.part + at * D;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
@@ -316,7 +343,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
                         *reinterpret_cast<float4*>(to + 128 * h + E * (4 * g + u) + e) =
                             make_float4(st.o[t][h * 8 + e][u], st.o[t][h * 8 + e + 1][u], st.o[t][h * 8 + e + 2][u],
                                         st.o[t][h * 8 + e + 3][u]);
-            if (g == 0) a.stats[pc.row + 16 * t + lane] = make_float2(m[t], l[t]);
+            if (g == 0) a.stats[at] = make_float2(m[t], l[t]);
         }
     }
     if (__syncthreads_or(odd)) mark_not_finite<D, BF, E8, ROWS>(a, pc, r, table, k0, end);
@@ -328,7 +355,12 @@ void attend_launch(const AttendArgs& a, const AttendSizes& z, hipStream_t st) {
     else attend_kernel<D, BF, E8, 2><<<(unsigned)z.few, 256, 0, st>>>(a);
     if (z.many) attend_prompt(a, z, D, BF, E8, st);
     const int64_t rows = (int64_t)a.B * a.max_new * a.Hkv * a.group;
-    if (z.rows) join_kernel<D, BF, E8><<<(unsigned)std::min<int64_t>(rows, JOIN_GRID), 256, 0, st>>>(a);
+    if (!z.rows) return;
+    // Few tiles have many pieces a row (64 of one request of 131072 keys: 4.8 us, 5.8 with 256 threads); others, and rows whose bits
+    // are to be their own, go by one order (1024 rows of up to 11 pieces: 4.3 us, 6.8 with 512 threads)
+    const unsigned grid = (unsigned)std::min<int64_t>(rows, JOIN_GRID);
+    if (!a.split && a.B * a.Hkv <= LONG_TILES) join_kernel<D, BF, E8, 512, 8><<<grid, 512, 0, st>>>(a);
+    else join_kernel<D, BF, E8, 256, 2><<<grid, 256, 0, st>>>(a);
 }
 template <int D>
 void attend_types(const AttendArgs& a, const AttendSizes& z, bool bf, bool e8, hipStream_t st) {
@@ -418,6 +450,7 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     a.plan = reinterpret_cast<int2*>(base);
     a.part = reinterpret_cast<float*>(base + z.part);
     a.stats = reinterpret_cast<float2*>(base + z.stats);
+    a.slots = z.slots;
     a.tile_rows = z.tile_rows;
     a.first_row = z.first_row;
     a.B = (int)B;
@@ -426,7 +459,7 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     a.group = (int)group;
     a.max_new = (int)max_new;
     a.window = (int)window;
-    a.split = (int)split;
+    a.split = split ? (int)split : z.rows ? 0 : PIECE;            // (tables of one piece: there is nothing to choose)
     a.capacity = (int)(max_pages * c.page);
     a.page16 = (int)(c.page / 16);
     a.page_shift = 31 - __builtin_clz((unsigned)a.page16);

@@ -19,7 +19,8 @@ constexpr int WAVES = 4;
 constexpr int FEW_ROWS = 32;                   // requests of up to this many rows a head of the cache are attention.hip's, a tile each,
 constexpr int PROMPT_ROWS = 128;               // those of more attention_prompt.hip's, in tiles of this many
 constexpr int PIECE = WAVES * STEP;            // pieces are multiples of this many keys
-constexpr int TARGET = 512;                    // pieces that a batch is cut into, about: two workgroups a CU
+constexpr int PROMPT_SLOTS = 512;              // workgroups that fit at once: attention_prompt.hip's (two a CU)
+constexpr int LONG_SLOTS = 256, LONG_TILES = 16;    // and attention.hip's where a batch has few tiles, whose rows would have many pieces
 
 struct AttendArgs {
     const uint16_t* q;
@@ -32,10 +33,11 @@ struct AttendArgs {
     const int32_t* tables;
     int64_t table_row;
     const int32_t *lengths, *first, *n_new;
-    float* part;                                // [rows][D]: a piece's rows one after the other
-    float2* stats;                              // [rows]: a row's maximum and sum
-    int2* plan;                                 // [B]: a request's first row in scratch and its pieces a tile
-    int tile_rows, first_row;                   // of attention.hip's tiles; attention_prompt.hip's first row in scratch
+    float* part;                                // [a tile's rows][its pieces][D]
+    float2* stats;                              // a row's maximum and sum in a piece
+    int2* plan;                                 // [B]: a request's first place in scratch and its pieces a tile
+    int slots;                                  // workgroups of attention.hip that fit at once
+    int tile_rows, first_row;                   // of attention.hip's tiles; attention_prompt.hip's first place in scratch
     int B, T, Hkv, group, max_new, window, split, capacity;                // capacity: tokens that a table can name
     int page16, page_shift;                     // tokens of a page / 16, and its reciprocal: 2 n page_mul >> (32 + page_shift)
     uint32_t page_mul;
@@ -68,23 +70,33 @@ __device__ __forceinline__ Request uniform_request(const AttendArgs& a, int b) {
 }
 
 struct Piece {
+    Request r;
     int b, tile, head, at, pieces;              // at: which of the tile's pieces
-    int64_t row;                                // its first row in scratch
+    int64_t row;                                // its first row's place in scratch, a row's pieces are next to one another
     int size;                                   // keys a piece
 };
 
-__device__ __forceinline__ int wave_scan(int v) {             // inclusive sum over the lanes
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+__device__ __forceinline__ int wave_scan(int v) {             // inclusive sum over the lanes: rows of 16, then over the rows
+    v += (int)dpp_u32<0x111>((uint32_t)v, 0u);                // row_shr 1, 2, 4, 8
+    v += (int)dpp_u32<0x112>((uint32_t)v, 0u);
+    v += (int)dpp_u32<0x114>((uint32_t)v, 0u);
+    v += (int)dpp_u32<0x118>((uint32_t)v, 0u);
+    v += (int)dpp_u32<0x142, 0xA>((uint32_t)v, 0u);           // row_bcast:15 into rows 1, 3
+    v += (int)dpp_u32<0x143, 0xC>((uint32_t)v, 0u);           // row_bcast:31 into rows 2, 3
     return v;
 }
 
-// Piece `item` of the requests that are tiles of ROWS rows, found by every wave for itself: the requests' lengths give the size of
-// the pieces (a.split, or so that there are about TARGET of them) and the requests' first ones. false: there are fewer
+// n / d of non-negative numbers below 2^30 (the reciprocal's quotient is off by one at most)
+__device__ __forceinline__ int quotient(int n, int d) {
+    int q = (int)((float)n * __builtin_amdgcn_rcpf((float)d));
+    const int r = n - q * d;
+    q += r >= d ? 1 : r < 0 ? -1 : 0;
+    return q;
+}
+
+// Piece `item` of the requests that are tiles of ROWS rows, found by every wave for itself from the requests' lengths: the size of the
+// pieces (a.split, or the smallest, about, with which all pieces fit on the CUs at once) and the requests' first ones. false: there are
+// fewer. 32 requests of up to 8171 keys, 273 MB: 53 us with pieces that fit, 57 with smaller and 66 with larger ones
 template <int ROWS>
 __device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p) {
     constexpr bool MANY = ROWS == PROMPT_ROWS;
@@ -94,21 +106,40 @@ __device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p
         if ((r.n * a.group > FEW_ROWS) != MANY) r.n = 0;
         return r;
     };
+    const auto tiles_of = [&](const Request& r) __attribute__((always_inline)) { return (r.n * a.group + ROWS - 1) / ROWS * a.Hkv; };
+    const Request r0 = mine_of(lane);                         // the first 64, loaded once
+    const auto request_at = [&](int b0) __attribute__((always_inline)) { return b0 ? mine_of(b0 + lane) : r0; };
     // (a prompt has tiles enough to run apart, and is not cut where rows are to be their own)
     int size = MANY && a.split ? 1 << 28 : a.split;
     if (!size) {
         double keys = 0.0;                                     // exact: below 2^53
+        int tiles = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
-            const Request r = mine_of(b0 + lane);
-            keys += (double)((r.n * a.group + ROWS - 1) / ROWS) * (double)(r.hi - r.lo);
+            const Request r = request_at(b0);
+            const int mine = tiles_of(r);
+            keys += (double)mine * (double)(r.hi - r.lo);
+            tiles += mine;
         }
-        keys = wave_sum_f64_dpp(keys) * a.Hkv;
-        size = ((int)fmin(keys / TARGET, (double)(1 << 28)) / PIECE + 1) * PIECE;
+        keys = wave_sum_f64_dpp(keys);
+        tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+        const int slots = MANY ? PROMPT_SLOTS : tiles <= LONG_TILES ? min(LONG_SLOTS, a.slots) : a.slots;
+        // a tile's last piece is half a piece, on average; then a little more at a time
+        const float most = (float)max(slots - tiles / 2, slots / 4);
+        size = ((int)fminf((float)keys * __builtin_amdgcn_rcpf(most), (float)(1 << 28)) / PIECE + 1) * PIECE;
+        for (int k = 0; k < 4 && !MANY && tiles < slots; ++k) {
+            int pieces = 0;
+            for (int b0 = 0; b0 < a.B; b0 += 64) {
+                const Request r = request_at(b0);
+                pieces += tiles_of(r) * max(1, quotient(r.hi - r.lo + size - 1, size));
+            }
+            if (__builtin_amdgcn_readlane(wave_scan(pieces), 63) <= slots) break;
+            size += (size / (16 * PIECE) + 1) * PIECE;
+        }
     }
     int before = 0, rows = MANY ? a.first_row : 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const Request r = mine_of(b0 + lane);
-        const int tiles = (r.n * a.group + ROWS - 1) / ROWS, pieces = max(1, (r.hi - r.lo + size - 1) / size);
+        const Request r = request_at(b0);
+        const int tiles = (r.n * a.group + ROWS - 1) / ROWS, pieces = max(1, quotient(r.hi - r.lo + size - 1, size));
         const int mine = tiles * a.Hkv * pieces, in_scratch = pieces > 1 ? mine * ROWS : 0;
         const int upto = wave_scan(mine), rows_upto = wave_scan(in_scratch);
         const uint64_t hit = __ballot(item >= before + upto - mine && item < before + upto);
@@ -116,16 +147,18 @@ __device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p
             const int l = __builtin_ctzll(hit);
             const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
             const int in = item - before - of(upto - mine), per_tile = of(pieces);
+            p.r = {of(r.n), of(r.first), of(r.length), of(r.lo), of(r.hi)};
             p.b = b0 + l;
             p.size = size;
             p.pieces = per_tile;
             // the tiles of a head and piece read the same keys: next to one another
             const int n_tiles = of(tiles);
-            p.tile = n_tiles - 1 - in % n_tiles;               // the last rows see the most
-            p.at = in / n_tiles % per_tile;
-            p.head = in / n_tiles / per_tile;
+            const int stack = MANY ? __builtin_amdgcn_readfirstlane(quotient(in, n_tiles)) : in;
+            p.tile = MANY ? n_tiles - 1 - (in - stack * n_tiles) : 0;       // the last rows see the most
+            p.head = __builtin_amdgcn_readfirstlane(quotient(stack, per_tile));
+            p.at = stack - p.head * per_tile;
             const int base = rows + of(rows_upto - in_scratch);
-            p.row = base + (int64_t)((p.head * n_tiles + p.tile) * per_tile + p.at) * ROWS;
+            p.row = base + (int64_t)(p.head * n_tiles + p.tile) * per_tile * ROWS + p.at;
             if (in == 0 && threadIdx.x == 0) a.plan[p.b] = make_int2(base, per_tile);
             return true;
         }
@@ -203,6 +236,17 @@ __device__ __forceinline__ Page page_of(const AttendArgs& a, const int32_t* tabl
     return {in && id >= 0 && id < a.pages ? id : -1, (int)(n - at * (uint32_t)a.page16) * 16};
 }
 
+// The same by every lane for a key of its own: a wave looks its next pages up together, ahead of their turn
+struct Place {
+    int page, off;
+};
+__device__ __forceinline__ Place place_of(const AttendArgs& a, const int32_t* table, int key) {
+    const uint32_t n = (uint32_t)key >> 4, at = __umulhi(2 * n, a.page_mul) >> a.page_shift;
+    const bool in = key < a.capacity;
+    const int id = table[in ? at : 0];
+    return {in && id >= 0 && id < a.pages ? id : -1, (int)(n - at * (uint32_t)a.page16) * 16};
+}
+
 // What a product cannot say: where only some of a tile's rows see a key, its values that are NaN or infinite went in as zeros (a
 // weight of zero would have made NaNs of them for every row). If there were any, the tile's outputs are gone over once more, after
 // they are stored, and those of the rows that see one become NaN. All threads of the workgroup
@@ -226,60 +270,78 @@ __device__ __forceinline__ void mark_not_finite(const AttendArgs& a, const Piece
             if (pc.pieces == 1)
                 a.out[(int64_t)(r.first + i) * a.o_row + (int64_t)(pc.head * a.group + n % a.group) * a.o_head + d] = BF ? 0x7FC0 : 0x7E00;
             else
-                a.part[(pc.row + t) * D + d] = __builtin_nanf("");
+                a.part[(pc.row + t * pc.pieces) * D + d] = __builtin_nanf("");
         }
     }
 }
 
-// Output row `row` (token i, head) of request b from its pieces: D / 4 lanes a piece, the pieces in order within every
-// 256 / (D / 4)-th, then those sums in order
-template <int D, bool BF, bool E8>
-__device__ __forceinline__ void join_row(const AttendArgs& a, const Request& r, int2 plan, int i, int head) {
-    constexpr int LANES = D / 4, SIDE = 256 / LANES;
+// Output row (token i, head) of a request from its pieces: D / 4 lanes a piece, the pieces in order within every SIDE-th with a running
+// maximum, then those sums in order; AHEAD pieces of a thread are on their way at once
+template <int D, bool BF, bool E8, int THREADS, int AHEAD>
+__device__ __forceinline__ void join_row(const AttendArgs& a, const Request& r, int first_row, int pieces, int i, int head) {
+    constexpr int LANES = D / 4, SIDE = THREADS / LANES;
     __shared__ float4 sh[SIDE][LANES];
-    __shared__ float sh_m[4], sides[SIDE];
-    const int pieces = plan.y, rows = r.n * a.group > FEW_ROWS ? PROMPT_ROWS : a.tile_rows;
-    const int row = i * a.group + head % a.group, tiles = (r.n * a.group + rows - 1) / rows;
-    const int64_t at = plan.x + (int64_t)((head / a.group * tiles + row / rows) * pieces) * rows + row % rows;
-    const float* part = a.part + at * D;
-    const float2* stats = a.stats + at;
-    float m = -INFINITY;
-    for (int p = threadIdx.x; p < pieces; p += 256) m = fmaxf(m, stats[(int64_t)p * rows].x);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0) sh_m[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-    const float base = m == -INFINITY ? 0.f : m;
+    __shared__ float2 sides[SIDE];
+    const int rows = r.n * a.group > FEW_ROWS ? PROMPT_ROWS : a.tile_rows;
+    const int kv = __builtin_amdgcn_readfirstlane(quotient(head, a.group)), row = i * a.group + head - kv * a.group;
+    const int tiles = (r.n * a.group + rows - 1) / rows;
+    const int64_t at = first_row + ((int64_t)(kv * tiles + row / rows) * rows + row % rows) * pieces;
     const int lane = threadIdx.x % LANES, side = threadIdx.x / LANES;
+    const float* part = a.part + at * D + 4 * lane;
+    const float2* stats = a.stats + at;
+    float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int p = side; p < pieces; p += SIDE) {
-        const float2 s = stats[(int64_t)p * rows];
-        const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)p * rows * D + 4 * lane);
-        const float w = __builtin_amdgcn_exp2f(s.x - base);
-        l += s.y * w;
-        o.x += v.x * w;
-        o.y += v.y * w;
-        o.z += v.z * w;
-        o.w += v.w * w;
+    for (int p0 = side; p0 < pieces; p0 += SIDE * AHEAD) {
+        float2 s[AHEAD];
+        float4 v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {                     // (the last ones again where there are no more)
+            const int p = min(p0 + SIDE * k, pieces - 1);
+            s[k] = stats[p];
+            v[k] = *reinterpret_cast<const float4*>(part + p * D);
+        }
+        float next = m;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (p0 + SIDE * k < pieces) next = fmaxf(next, s[k].x);
+        const float base = next == -INFINITY ? 0.f : next, alpha = __builtin_amdgcn_exp2f(m - base);
+        m = next;
+        l *= alpha;
+        o.x *= alpha;
+        o.y *= alpha;
+        o.z *= alpha;
+        o.w *= alpha;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (p0 + SIDE * k >= pieces) break;
+            const float w = __builtin_amdgcn_exp2f(s[k].x - base);
+            l += s[k].y * w;
+            o.x += v[k].x * w;
+            o.y += v[k].y * w;
+            o.z += v[k].z * w;
+            o.w += v[k].w * w;
+        }
     }
     sh[side][lane] = o;
-    if (lane == 0) sides[side] = l;
+    if (lane == 0) sides[side] = make_float2(m, l);
     __syncthreads();
     if (side == 0) {
-        l = sides[0];
 #pragma unroll
-        for (int k = 1; k < SIDE; ++k) {
+        for (int k = 1; k < SIDE; ++k) m = fmaxf(m, sides[k].x);
+        const float base = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < SIDE; ++k) {
             const float4 v = sh[k][lane];
-            l += sides[k];
-            o.x += v.x;
-            o.y += v.y;
-            o.z += v.z;
-            o.w += v.w;
+            const float w = __builtin_amdgcn_exp2f(sides[k].x - base);
+            l += sides[k].y * w;
+            o.x += v.x * w;
+            o.y += v.y * w;
+            o.z += v.z * w;
+            o.w += v.w * w;
         }
-        const float vscale = E8 ? a.vs[head / a.group] : 1.f;
+        const float vscale = E8 ? a.vs[kv] : 1.f;
         const float f = l > 0.f ? vscale / l : l == 0.f ? 0.f : __builtin_nanf("");
         *reinterpret_cast<uint2*>(a.out + (int64_t)(r.first + i) * a.o_row + (int64_t)head * a.o_head + 4 * lane) =
             make_uint2(pack2<BF>(o.x * f, o.y * f), pack2<BF>(o.z * f, o.w * f));
@@ -288,20 +350,21 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, const Request& r, 
 }
 
 // The rows of requests with more than one piece, a workgroup every gridDim.x-th of them
-template <int D, bool BF, bool E8>
-__global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
+template <int D, bool BF, bool E8, int THREADS, int AHEAD>
+__global__ __launch_bounds__(THREADS) void join_kernel(const AttendArgs a) {
     const int lane = threadIdx.x & 63, heads = a.Hkv * a.group;
     int before = 0, row = blockIdx.x;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int b = b0 + lane;
+        const int2 plan = b < a.B ? a.plan[b] : make_int2(0, 0);              // (of no request: anything)
         const Request r = request_of(a, b);
-        int mine = 0;
-        if (r.n > 0 && a.plan[b].y > 1) mine = r.n * heads;
-        const int upto = wave_scan(mine), all = before + __builtin_amdgcn_readlane(upto, 63);
+        const int mine = r.n > 0 && plan.y > 1 ? r.n * heads : 0, upto = wave_scan(mine);
+        const int all = before + __builtin_amdgcn_readlane(upto, 63);
         for (; row < all; row += gridDim.x) {
             const int l = __builtin_ctzll(__ballot(row < before + upto));
-            const int in = row - before - __builtin_amdgcn_readlane(upto - mine, l);
-            join_row<D, BF, E8>(a, uniform_request(a, b0 + l), a.plan[b0 + l], in / heads, in % heads);
+            const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
+            const int in = row - before - of(upto - mine), i = __builtin_amdgcn_readfirstlane(quotient(in, heads));
+            join_row<D, BF, E8, THREADS, AHEAD>(a, {of(r.n), of(r.first), 0, 0, 0}, of(plan.x), of(plan.y), i, in - i * heads);
         }
         before = all;
     }
@@ -311,28 +374,29 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
 
 struct AttendSizes {
     int64_t few, many, rows, part, stats, bytes;              // workgroups of either kernel; rows in scratch; byte offsets
-    int tile_rows, first_row;
+    int tile_rows, first_row, slots;
     AttendSizes(int64_t B, int64_t T, int64_t max_new, int64_t group, int64_t Hkv, int64_t D, int64_t capacity, int64_t split) {
         tile_rows = max_new * group <= 16 ? 16 : FEW_ROWS;
+        slots = 256 * (D == 256 ? 1 : D == 128 && tile_rows == FEW_ROWS ? 2 : 3);
         const int64_t size = split ? split : PIECE, most = std::max<int64_t>(1, (capacity + size - 1) / size);   // pieces a tile
-        // chosen pieces: the sum of ceil(k / size) over all tiles is at most TARGET more than there are tiles, and that of the
-        // tiles with k > size, whose pieces go to scratch, at most twice the sum of k / size
+        // the size chosen is at least keys / slots: the sum of ceil(k / size) over all tiles is at most `slots` more than there are
+        // tiles, and that of the tiles with k > size, whose pieces go to scratch, at most twice the sum of k / size
         few = B * Hkv * most;
-        int64_t slots = most > 1 ? few : 0;
+        int64_t in_scratch = most > 1 ? few : 0;
         if (!split) {
-            few = std::min(few, B * Hkv + TARGET);
-            slots = std::min<int64_t>(slots, 2 * TARGET);
+            few = std::min(few, B * Hkv + slots);
+            in_scratch = std::min<int64_t>(in_scratch, 2 * slots);
         }
         first_row = 0;
-        rows = slots * tile_rows;
+        rows = in_scratch * tile_rows;
         many = 0;
         if (max_new * group > FEW_ROWS) {
             // requests' rows are apart, so there are no more tiles than all rows make, and a part of one more each
             many = std::min(B * ((max_new * group + PROMPT_ROWS - 1) / PROMPT_ROWS), T * group / PROMPT_ROWS + B) * Hkv;
             first_row = (int)std::min<int64_t>(rows, 1 << 30);
             if (!split && most > 1) {
-                many += TARGET;
-                rows += 2 * TARGET * PROMPT_ROWS;
+                many += PROMPT_SLOTS;
+                rows += 2 * PROMPT_SLOTS * PROMPT_ROWS;
             }
         }
         part = (B * 8 + 15) / 16 * 16;

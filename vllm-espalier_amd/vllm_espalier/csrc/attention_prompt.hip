@@ -50,24 +50,32 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
 }
 
-// A wave's 16 keys of a tile, of which nobody sees those outside [lo, hi): pieces straight into the LDS, or 8-bit ones into
-// registers and from there
+// A wave's 16 keys of a tile: pieces straight into the LDS, or 8-bit ones into registers and from there
 template <int D, bool E8>
 struct Loader {
-    static constexpr int ROW = D * 2, PIECES = D / 8, N = E8 ? D / 64 : D / 32;       // LDS bytes and pieces a row; loads
+    static constexpr int ROW = D * 2, N = E8 ? D / 64 : D / 32, UNITS = E8 ? D / 16 : D / 8;      // LDS bytes a row; loads; their pieces a row
     u32x4 held[E8 ? 2 * N : 1];
+    int k_at[N], v_at[N];                                     // where the lane reads, from the first key
 
-    __device__ __forceinline__ void load(const AttendArgs& a, const char* kb, const char* vb, Page p, int key, int lo, int hi, char* lds) {
-        const int lane = threadIdx.x & 63;
-        const bool dead = p.page < 0;
-        const char *k = kb + (dead ? 0 : p.page) * a.k_page + p.off * a.k_token, *v = vb + (dead ? 0 : p.page) * a.v_page + p.off * a.v_token;
+    __device__ __forceinline__ explicit Loader(const AttendArgs& a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int unit = i * 64 + lane, units = E8 ? D / 16 : PIECES, r = unit / units, c = unit % units;
-            const int from = (E8 ? c : c ^ spread<D>(r)) * 16;
-            const bool none = dead || key + r < lo || key + r >= hi;
-            const char *ks = none ? reinterpret_cast<const char*>(no_keys) : k + r * a.k_token + from;
-            const char *vs = none ? reinterpret_cast<const char*>(no_keys) : v + r * a.v_token + from;
+            const int unit = i * 64 + (int)(threadIdx.x & 63), r = unit / UNITS, c = unit % UNITS;
+            k_at[i] = r * (int)a.k_token + (E8 ? c : c ^ spread<D>(r)) * 16;
+            v_at[i] = r * (int)a.v_token + (E8 ? c : c ^ spread<D>(r)) * 16;
+        }
+    }
+    // part: only the keys in [lo, hi) of them, and none without a page, are anybody's
+    __device__ __forceinline__ void load(const AttendArgs& a, const char* kb, const char* vb, int page, int off, bool part, int key, int lo,
+                                         int hi, char* lds) {
+        const char *k = kb + (int64_t)max(page, 0) * a.k_page + off * a.k_token, *v = vb + (int64_t)max(page, 0) * a.v_page + off * a.v_token;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const char *ks = k + k_at[i], *vs = v + v_at[i];
+            if (part) {
+                const int at = key + (i * 64 + (int)(threadIdx.x & 63)) / UNITS;
+                if (page < 0 || at < lo || at >= hi) ks = vs = reinterpret_cast<const char*>(no_keys);
+            }
             if constexpr (E8) {
                 held[i] = *reinterpret_cast<const u32x4*>(ks);
                 held[N + i] = *reinterpret_cast<const u32x4*>(vs);
@@ -105,12 +113,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
     Piece pc;
     if (!piece_of<ROWS>(a, (int)blockIdx.x, pc)) return;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, h = lane >> 5;
-    const Request r = uniform_request(a, pc.b);
+    const Request& r = pc.r;
     const int32_t* table = a.tables + pc.b * a.table_row;
     const char *kb = a.k + pc.head * a.k_head, *vb = a.v + pc.head * a.v_head;
 
     // the lane's query, the keys that it sees, those that all and any of the wave's do, and those that any of the workgroup's do
-    const int before = r.length - r.n + 1, row0 = pc.tile * ROWS + 32 * wave, row = row0 + (lane & 31), i = row / a.group, gh = row % a.group;
+    const int before = r.length - r.n + 1, row0 = pc.tile * ROWS + 32 * wave, row = row0 + (lane & 31), i = quotient(row, a.group), gh = row - i * a.group;
     const bool here = i < r.n, some = row0 / a.group < r.n;
     const auto upto = [&](int t) __attribute__((always_inline)) { return max(0, min(before + t, r.hi)); };
     const auto from = [&](int t) __attribute__((always_inline)) { return a.window ? max(0, before + t - a.window) : 0; };
@@ -151,17 +159,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
         return u32x4{u.x, u.y, w.x, w.y};
     };
 
-    Loader<D, E8> loader;
+    Loader<D, E8> loader(a);
     const int mine = 16 * wave;                               // the wave's keys of a tile
+    // Lane i: the page of the wave's keys of tile i from where it was last asked, and which of the tile's 16 keys have none
+    Place ahead = {};
+    int none_ahead = 0, tiles = 0;
+    const auto load = [&](int key, char* lds) __attribute__((always_inline)) {
+        if (tiles == 0) {
+            none_ahead = 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const Place p = place_of(a, table, key + lane * TILE + 16 * u);
+                if (p.page < 0) none_ahead |= 1 << u;
+                if (u == wave) ahead = p;
+            }
+        }
+        const int none = __builtin_amdgcn_readlane(none_ahead, tiles);
+        const bool part = none || key < wg_lo || key + TILE > wg_hi;
+        loader.load(a, kb, vb, __builtin_amdgcn_readlane(ahead.page, tiles), __builtin_amdgcn_readlane(ahead.off, tiles), part, key + mine,
+                    wg_lo, wg_hi, lds + mine * ROW);
+        tiles = (tiles + 1) & 63;
+        return none;
+    };
+    int none_next = 0;
     if (start < end) {
-        loader.load(a, kb, vb, page_of(a, table, start + mine), start + mine, wg_lo, wg_hi, lds0 + mine * ROW);
+        none_next = load(start, lds0);
         loader.template store<BF>(lds0 + mine * ROW);
     }
     const int wg_all_hi = upto(pc.tile * ROWS / a.group), wg_all_lo = from(min((pc.tile * ROWS + ROWS - 1) / a.group, r.n - 1));
     bool odd = false;                                         // a NaN or an infinity among values that some rows see and others do not
     const auto tile = [&](int key, char* buf, char* other) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);                        // this wave's part of the tile has come
-        if (key < wg_all_lo || key + TILE > wg_all_hi) {
+        if (key < wg_all_lo || key + TILE > wg_all_hi || none_next) {
             u32x4* v = reinterpret_cast<u32x4*>(buf + (TILE + mine) * ROW) + lane;
 #pragma unroll
             for (int c = 0; c < ROW / 64; ++c) {
@@ -173,7 +202,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
         }
         __syncthreads();                                      // and everybody's; the other buffer is read by nobody any more
         const int next = key + TILE;
-        if (next < end) loader.load(a, kb, vb, page_of(a, table, next + mine), next + mine, wg_lo, wg_hi, other + mine * ROW);
+        const int none = none_next;                           // which 16 keys have no page
+        if (next < end) none_next = load(next, other);
         if (some && key < any_hi && key + TILE > any_lo) {
             f32x16 s[2];
 #pragma unroll
@@ -192,9 +222,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
 #pragma unroll
                 for (int u = 0; u < 2; ++u) s[u] = mfma32<BF>(k[kk & 1][u], q[kk], s[u]);
             }
-            uint32_t none = 0;                                // which 16 keys have no page
-#pragma unroll
-            for (int u = 0; u < 4; ++u) none |= (page_of(a, table, key + 16 * u).page < 0 ? 1u : 0u) << u;
             const bool edge = key < all_lo || key + TILE > all_hi || none;
             if (edge) {
 #pragma unroll
@@ -259,7 +286,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
                 *reinterpret_cast<uint2*>(to + 32 * db + 2 * j) =
                     make_uint2(pack2<BF>(o[db][j] * f, o[db][j + 1] * f), pack2<BF>(o[db][j + 2] * f, o[db][j + 3] * f));
     } else if (here) {
-        const int64_t at = pc.row + 32 * wave + (lane & 31);
+        const int64_t at = pc.row + (32 * wave + (lane & 31)) * pc.pieces;
         float* to = a.part + at * D + 4 * h;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
