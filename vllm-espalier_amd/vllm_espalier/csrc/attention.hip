@@ -195,7 +195,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     if (!piece_of<ROWS>(a, (int)blockIdx.x, pc)) return;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, g = lane >> 4;
     const Request& r = pc.r;
-    const int k0 = r.lo + pc.at * pc.size, k1 = min(k0 + pc.size, r.hi);
+    // (readfirstlane: what all lanes share is kept in scalar registers)
+    const auto shared = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
+    const int k0 = shared(r.lo + pc.at * pc.size), k1 = shared(min(k0 + pc.size, r.hi));
     const int32_t* table = a.tables + pc.b * a.table_row;
     const char *kb = a.k + pc.head * a.k_head, *vb = a.v + pc.head * a.v_head;
 
@@ -215,9 +217,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const Att
     }
     // the keys that all of the tile's rows see, and those that any of them does
     const int i0 = 0, i1 = r.n - 1;                           // (a request is one tile)
-    const int all_hi = min(r.length - r.n + i0 + 1, r.hi), any_hi = max(0, min(r.length - r.n + i1 + 1, r.hi));
-    const int all_lo = a.window ? max(0, r.length - r.n + i1 + 1 - a.window) : 0;
-    const int any_lo = a.window ? max(0, r.length - r.n + i0 + 1 - a.window) : 0;
+    const int all_hi = shared(min(r.length - r.n + i0 + 1, r.hi)), any_hi = shared(max(0, min(r.length - r.n + i1 + 1, r.hi)));
+    const int all_lo = shared(a.window ? max(0, r.length - r.n + i1 + 1 - a.window) : 0);
+    const int any_lo = shared(a.window ? max(0, r.length - r.n + i0 + 1 - a.window) : 0);
 
     State<D, NT> st;
 #pragma unroll

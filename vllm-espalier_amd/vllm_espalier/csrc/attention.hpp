@@ -94,6 +94,45 @@ __device__ __forceinline__ int quotient(int n, int d) {
     return q;
 }
 
+// The same of up to 64 requests, a lane each (r, pieces of `size` keys), those of the tiles that see the most keys first, so that the
+// last workgroups are short ones: item counts down the tiles that see more than 64 x keys, for the x at which they are more than
+// item (-1: all tiles). Heads next to one another: with the workgroups dealt to the XCDs in turn, an XCD's L2 has a few heads' keys.
+template <int ROWS>
+__device__ __forceinline__ bool piece_by_length(const AttendArgs& a, int item, int size, const Request& r, Piece& p) {
+    const int lane = threadIdx.x & 63;
+    const int tiles = (r.n * a.group + ROWS - 1) / ROWS, pieces = max(1, quotient(r.hi - r.lo + size - 1, size));
+    const float per_key = (float)a.group / ROWS;              // tiles a key further down
+    const auto above = [&](int x) __attribute__((always_inline)) {           // the request's tiles that see more
+        return x < 0 ? tiles : max(0, min(tiles, (int)ceilf((float)min(r.hi - 64 * x, 1 << 24) * per_key)));
+    };
+    const auto all = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
+    if (item >= all(tiles * a.Hkv * pieces)) return false;
+    int x = -1, end = (int)(wave_max_u32((uint32_t)r.hi) >> 6) + 1;
+    while (end - x > 1) {
+        const int mid = (x + end) >> 1;
+        if (all(above(mid) * a.Hkv * pieces) > item) x = mid;
+        else end = mid;
+    }
+    const int higher = above(x + 1), rest = item - all(higher * a.Hkv * pieces);
+    const int mine = (above(x) - higher) * a.Hkv * pieces, upto = wave_scan(mine);
+    const int in_scratch = pieces > 1 ? tiles * a.Hkv * pieces * ROWS : 0, rows_upto = wave_scan(in_scratch);
+    const int l = __builtin_ctzll(__ballot(rest < upto));
+    const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
+    const int in = rest - of(upto - mine), stack = __builtin_amdgcn_readfirstlane(quotient(in, a.Hkv));
+    p.r = {of(r.n), of(r.first), of(r.length), of(r.lo), of(r.hi)};
+    p.b = l;
+    p.size = size;
+    p.pieces = of(pieces);
+    p.head = in - stack * a.Hkv;
+    const int level = __builtin_amdgcn_readfirstlane(quotient(stack, p.pieces));
+    p.at = stack - level * p.pieces;
+    p.tile = of(tiles) - 1 - of(higher) - level;
+    const int base = a.first_row + of(rows_upto - in_scratch);
+    p.row = base + (int64_t)(p.head * of(tiles) + p.tile) * p.pieces * ROWS + p.at;
+    if (p.tile == 0 && p.head == 0 && p.at == 0 && threadIdx.x == 0) a.plan[l] = make_int2(base, p.pieces);
+    return true;
+}
+
 // Piece `item` of the requests that are tiles of ROWS rows, found by every wave for itself from the requests' lengths: the size of the
 // pieces (a.split, or the smallest, about, with which all pieces fit on the CUs at once) and the requests' first ones. false: there are
 // fewer. 32 requests of up to 8171 keys, 273 MB: 53 us with pieces that fit, 57 with smaller and 66 with larger ones
@@ -136,6 +175,7 @@ __device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p
             size += (size / (16 * PIECE) + 1) * PIECE;
         }
     }
+    if (MANY && a.B <= 64) return piece_by_length<ROWS>(a, item, size, r0, p);
     int before = 0, rows = MANY ? a.first_row : 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const Request r = request_at(b0);
@@ -154,7 +194,7 @@ __device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p
             // the tiles of a head and piece read the same keys: next to one another
             const int n_tiles = of(tiles);
             const int stack = MANY ? __builtin_amdgcn_readfirstlane(quotient(in, n_tiles)) : in;
-            p.tile = MANY ? n_tiles - 1 - (in - stack * n_tiles) : 0;       // the last rows see the most
+            p.tile = MANY ? n_tiles - 1 - (in - stack * n_tiles) : 0;
             p.head = __builtin_amdgcn_readfirstlane(quotient(stack, per_tile));
             p.at = stack - p.head * per_tile;
             const int base = rows + of(rows_upto - in_scratch);

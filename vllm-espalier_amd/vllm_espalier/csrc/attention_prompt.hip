@@ -55,7 +55,7 @@ template <int D, bool E8>
 struct Loader {
     static constexpr int ROW = D * 2, N = E8 ? D / 64 : D / 32, UNITS = E8 ? D / 16 : D / 8;      // LDS bytes a row; loads; their pieces a row
     u32x4 held[E8 ? 2 * N : 1];
-    int k_at[N], v_at[N];                                     // where the lane reads, from the first key
+    uint32_t k_at[N], v_at[N];                                // where the lane reads, from the first key
 
     __device__ __forceinline__ explicit Loader(const AttendArgs& a) {
 #pragma unroll
@@ -69,19 +69,25 @@ struct Loader {
     __device__ __forceinline__ void load(const AttendArgs& a, const char* kb, const char* vb, int page, int off, bool part, int key, int lo,
                                          int hi, char* lds) {
         const char *k = kb + (int64_t)max(page, 0) * a.k_page + off * a.k_token, *v = vb + (int64_t)max(page, 0) * a.v_page + off * a.v_token;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const char *ks = k + k_at[i], *vs = v + v_at[i];
-            if (part) {
-                const int at = key + (i * 64 + (int)(threadIdx.x & 63)) / UNITS;
-                if (page < 0 || at < lo || at >= hi) ks = vs = reinterpret_cast<const char*>(no_keys);
-            }
+        const auto one = [&](int i, const char* ks, const char* vs) __attribute__((always_inline)) {
             if constexpr (E8) {
                 held[i] = *reinterpret_cast<const u32x4*>(ks);
                 held[N + i] = *reinterpret_cast<const u32x4*>(vs);
             } else {
                 __builtin_amdgcn_global_load_lds((global_void_ptr)ks, (lds_void_ptr)(lds + i * 1024), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((global_void_ptr)vs, (lds_void_ptr)(lds + TILE * ROW + i * 1024), 16, 0, 0);
+            }
+        };
+        if (!part) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) one(i, k + k_at[i], v + v_at[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int at = key + (i * 64 + (int)(threadIdx.x & 63)) / UNITS;
+                const bool none = page < 0 || at < lo || at >= hi;
+                const char* zeros = reinterpret_cast<const char*>(no_keys);
+                one(i, none ? zeros : k + k_at[i], none ? zeros : v + v_at[i]);
             }
         }
     }
@@ -107,6 +113,7 @@ struct Loader {
 template <int D, bool BF, bool E8>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(const AttendArgs a) {
     constexpr int ROWS = PROMPT_ROWS, ROW = D * 2, KK = D / 16, DB = D / 32, BUFFER = 2 * TILE * ROW;
+    constexpr int K_AHEAD = D == 256 ? 1 : 2, V_AHEAD = D == 256 ? 2 : 4;     // steps that operands are read ahead of their products
     // two buffers, each an object of its own and each step of the loop with its own: a read of one is then known not to wait for what
     // is on its way into the other
     __shared__ __attribute__((aligned(1024))) char lds0[BUFFER], lds1[BUFFER];
@@ -119,21 +126,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
 
     // the lane's query, the keys that it sees, those that all and any of the wave's do, and those that any of the workgroup's do
     const int before = r.length - r.n + 1, row0 = pc.tile * ROWS + 32 * wave, row = row0 + (lane & 31), i = quotient(row, a.group), gh = row - i * a.group;
-    const bool here = i < r.n, some = row0 / a.group < r.n;
+    const bool here = i < r.n, some = row0 < r.n * a.group;
+    // (readfirstlane: what all lanes share is kept in scalar registers)
+    const auto shared = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
     const auto upto = [&](int t) __attribute__((always_inline)) { return max(0, min(before + t, r.hi)); };
     const auto from = [&](int t) __attribute__((always_inline)) { return a.window ? max(0, before + t - a.window) : 0; };
     const int hi = here ? upto(i) : 0, lo = here ? from(i) : 0;
-    const int i0 = row0 / a.group, i1 = min((row0 + 31) / a.group, r.n - 1);
-    const int all_hi = upto(i0), any_hi = upto(i1), all_lo = from(i1), any_lo = from(i0);
-    const int wg_hi = upto(min((pc.tile * ROWS + ROWS - 1) / a.group, r.n - 1)), wg_lo = from(pc.tile * ROWS / a.group);
+    const int i0 = shared(quotient(row0, a.group)), i1 = min(shared(quotient(row0 + 31, a.group)), r.n - 1);
+    const int wg_i0 = shared(quotient(pc.tile * ROWS, a.group)), wg_i1 = min(shared(quotient(pc.tile * ROWS + ROWS - 1, a.group)), r.n - 1);
+    const int all_hi = shared(upto(i0)), any_hi = shared(upto(i1)), all_lo = shared(from(i1)), any_lo = shared(from(i0));
+    const int wg_hi = shared(upto(wg_i1)), wg_lo = shared(from(wg_i0));
     u32x4 q[KK];
     {
         const uint16_t* p = a.q + (int64_t)(r.first + (here ? i : 0)) * a.q_row + (int64_t)(pc.head * a.group + gh) * a.q_head;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) q[kk] = *reinterpret_cast<const u32x4*>(p + kk * 16 + h * 8);
     }
-    const int k0 = r.lo + pc.at * pc.size, end = min(min(k0 + pc.size, r.hi), wg_hi);
-    const int start = k0 + (wg_lo > k0 ? (wg_lo - k0) / TILE * TILE : 0);
+    const int k0 = shared(r.lo + pc.at * pc.size), end = shared(min(min(k0 + pc.size, r.hi), wg_hi));
+    const int start = shared(k0 + (wg_lo > k0 ? (wg_lo - k0) / TILE * TILE : 0));
 
     f32x16 o[DB];
 #pragma unroll
@@ -186,7 +196,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
         none_next = load(start, lds0);
         loader.template store<BF>(lds0 + mine * ROW);
     }
-    const int wg_all_hi = upto(pc.tile * ROWS / a.group), wg_all_lo = from(min((pc.tile * ROWS + ROWS - 1) / a.group, r.n - 1));
+    const int wg_all_hi = shared(upto(wg_i0)), wg_all_lo = shared(from(wg_i1));
     bool odd = false;                                         // a NaN or an infinity among values that some rows see and others do not
     const auto tile = [&](int key, char* buf, char* other) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);                        // this wave's part of the tile has come
@@ -210,18 +220,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) s[u][j] = 0.f;
-            u32x4 k[2][2];                                    // operands a step ahead
+            u32x4 k[K_AHEAD + 1][2];                          // operands some steps ahead
 #pragma unroll
-            for (int u = 0; u < 2; ++u) k[0][u] = read_k(buf, u, 0);
+            for (int kk = 0; kk < K_AHEAD; ++kk)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) k[kk][u] = read_k(buf, u, kk);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                if (kk + 1 < KK)
+                if (kk + K_AHEAD < KK)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) k[(kk + 1) & 1][u] = read_k(buf, u, kk + 1);
+                    for (int u = 0; u < 2; ++u) k[(kk + K_AHEAD) % (K_AHEAD + 1)][u] = read_k(buf, u, kk + K_AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) s[u] = mfma32<BF>(k[kk & 1][u], q[kk], s[u]);
+                for (int u = 0; u < 2; ++u) s[u] = mfma32<BF>(k[kk % (K_AHEAD + 1)][u], q[kk], s[u]);
             }
+            u32x4 v[V_AHEAD + 1];
+#pragma unroll
+            for (int n = 0; n < V_AHEAD; ++n) v[n] = read_v(buf, n / DB, n % DB);
             const bool edge = key < all_lo || key + TILE > all_hi || none;
             if (edge) {
 #pragma unroll
@@ -257,13 +272,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
                     l += x + y;
                     p[2 * u + j / 8][j % 8 / 2] = pack2<BF>(x, y);
                 }
-            u32x4 v[2];
-            v[0] = read_v(buf, 0, 0);
 #pragma unroll
             for (int n = 0; n < 4 * DB; ++n) {
-                if (n + 1 < 4 * DB) v[(n + 1) & 1] = read_v(buf, (n + 1) / DB, (n + 1) % DB);
+                if (n + V_AHEAD < 4 * DB) v[(n + V_AHEAD) % (V_AHEAD + 1)] = read_v(buf, (n + V_AHEAD) / DB, (n + V_AHEAD) % DB);
                 __builtin_amdgcn_sched_barrier(0);
-                o[n % DB] = mfma32<BF>(v[n & 1], p[n / DB], o[n % DB]);
+                o[n % DB] = mfma32<BF>(v[n % (V_AHEAD + 1)], p[n / DB], o[n % DB]);
             }
         }
         if (next < end) loader.template store<BF>(other + mine * ROW);
