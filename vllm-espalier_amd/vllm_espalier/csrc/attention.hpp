@@ -10,9 +10,7 @@
 namespace esp {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int STEP = 32;                       // keys a wave takes at once
 constexpr int WAVES = 4;
@@ -43,11 +41,6 @@ struct AttendArgs {
     uint32_t page_mul;
     float scale;                                // scale * log2(e)
 };
-
-template <typename T>
-__device__ __forceinline__ T load_uniform(const T* p) {       // through the scalar cache: nothing writes it while the kernel runs
-    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
-}
 
 // ---- which piece a workgroup has
 
@@ -216,12 +209,6 @@ __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {              // to nearest even
-    const f32x2 v = {a, b};
-    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
 // two e4m3 values of w's low (HI: high) half as two of dtype, exact
 template <bool BF, bool HI>

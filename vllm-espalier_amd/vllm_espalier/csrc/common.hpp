@@ -33,6 +33,12 @@ __device__ __forceinline__ float bf2f(uint16_t b) { return __builtin_bit_cast(fl
 // u + 0x7FFF + (u >> 16 & 1) with a NaN branch, compared over all 2^32 inputs, in one instruction instead of a dozen)
 __device__ __forceinline__ uint16_t f2bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 
+// a value that every lane of the wave reads, through the scalar cache (nothing writes it while the kernel runs)
+template <typename T>
+__device__ __forceinline__ T load_uniform(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 // one element of a 16-bit (f16 / bf16) or f32 array as f32
 __device__ __forceinline__ float load_elem(const void* p, int dtype, size_t i) {
     if (dtype == F32) return static_cast<const float*>(p)[i];

@@ -12,6 +12,17 @@ constexpr float E4M3_MAX = 448.0f;
 // Bytes of an element
 __host__ __device__ constexpr int kv_bytes(int dtype) { return dtype == E4M3 ? 1 : 2; }
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Two floats as bf16 or fp16, to nearest even
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 v = {a, b};
+    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
 // Two floats as e4m3 in the low (or, HI, the high) half of w, to nearest even, those past the largest (infinities too) as the
 // largest, a NaN as a NaN
 template <bool HI>

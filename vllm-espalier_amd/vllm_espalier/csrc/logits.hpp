@@ -105,10 +105,4 @@ __device__ __forceinline__ float exp_scaled(float d, float hi, float lo) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, hi, d * lo));
 }
 
-// a value that every lane of the wave reads, through the scalar cache (nothing writes it while the kernel runs)
-template <typename T>
-__device__ __forceinline__ T load_uniform(const T* p) {
-    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
-}
-
 }  // namespace esp
