@@ -191,6 +191,11 @@ __device__ __forceinline__ bool weigh(f32x4 (&s)[NT][2], Values<D, E8>& v, bool 
 template <int D, bool BF, bool E8, int NT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(const AttendArgs a) {
     constexpr int ROWS = 16 * NT, OPS = D / 16;
+    // All arguments at once: left to where they are used, they come one after the other, a trip to memory each (one token over 113: 6.3 -> 5.7 us)
+    asm volatile("" ::"s"(a.lengths), "s"(a.first), "s"(a.n_new), "s"(a.tables), "s"(a.table_row), "s"(a.q), "s"(a.q_row), "s"(a.q_head),
+                 "s"(a.k), "s"(a.v), "s"(a.k_page), "s"(a.k_token), "s"(a.k_head), "s"(a.v_page), "s"(a.v_token), "s"(a.v_head),
+                 "s"(a.pages), "s"(a.B), "s"(a.T), "s"(a.Hkv), "s"(a.group), "s"(a.max_new), "s"(a.window), "s"(a.split), "s"(a.capacity),
+                 "s"(a.page16), "s"(a.page_shift), "s"(a.page_mul), "s"(a.slots));
     Piece pc;
     if (!piece_of<ROWS>(a, (int)blockIdx.x, pc)) return;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, g = lane >> 4;

@@ -90,7 +90,7 @@ __device__ __forceinline__ Turn turn_of(const AppendArgs& p, const float2* turn,
         const float2 cs = !t.turns ? make_float2(1.f, 0.f) : p.adjacent ? turn[d / 2 + j / 2] : turn[d % half + j];
         const bool first = p.adjacent ? j % 2 == 0 : low;
         t.a[j] = w[j] * cs.x;
-        t.b[j] = (p.adjacent ? v[j ^ 1] : v[j]) * (first ? -cs.y : cs.y);
+        t.b[j] = t.turns ? (p.adjacent ? v[j ^ 1] : v[j]) * (first ? -cs.y : cs.y) : -0.0f;      // (a zero keeps its sign)
     }
     return t;
 }
@@ -124,10 +124,10 @@ __device__ __forceinline__ void turned(const AppendArgs& p, const Turn& t, bool 
 }
 
 // x / scale from 1 / scale, to nearest: many quotients of 16-bit values lie on the borders of 8-bit ones, and the product alone, off by
-// one last place, would put them on either side (beyond what eight bits hold it does, infinities among it)
+// one last place, would put them on either side (beyond what eight bits hold it does, infinities among it; a zero keeps its sign)
 __device__ __forceinline__ float quotient_of(float x, float scale, float over) {
     const float q = x * over;
-    return fabsf(q) <= 1024.0f ? __builtin_fmaf(__builtin_fmaf(-q, scale, x), over, q) : q;
+    return q != 0.0f && fabsf(q) <= 1024.0f ? __builtin_fmaf(__builtin_fmaf(-q, scale, x), over, q) : q;
 }
 
 // one of three values by a row's kind (by value: the arguments stay where they are)

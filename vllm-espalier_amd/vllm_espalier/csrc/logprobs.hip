@@ -178,16 +178,17 @@ __device__ __forceinline__ int place_of(unsigned long long key, const unsigned l
     return larger;
 }
 
-// The k-th largest of values[0 .. n) (a multiple of 256), by 256 threads a byte at a time from the top: how many have each value of
+// The k-th largest of values[0 .. n) (a multiple of 256), a byte at a time from the top: how many have each value of
 // it, of those that agree above it. bins: 256 counts and two more
+template <int THREADS>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int n, int k, int* bins) {
     const int t = threadIdx.x, lane = t & 63;
     uint32_t found = 0;
 #pragma unroll
     for (int shift = 24; shift >= 0; shift -= 8) {
-        bins[t] = 0;
+        if (t < 256) bins[t] = 0;
         __syncthreads();
-        for (int i = t; i < n; i += 256)
+        for (int i = t; i < n; i += THREADS)
             if (shift == 24 || (values[i] ^ found) >> (shift + 8) == 0) atomicAdd(&bins[values[i] >> shift & 255], 1);
         __syncthreads();
         if (t < 64) {                                       // lane l: bins 255 - 4 l down
@@ -218,13 +219,14 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int n, i
     return found;
 }
 
-// keys[0 .. n), n a power of two, from the largest down, by 256 threads
+// keys[0 .. n), n a power of two, from the largest down
+template <int THREADS>
 __device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
     for (int size = 2; size <= n; size *= 2)
         for (int log = 30 - __clz(size); log >= 0; --log) {
             const int step = 1 << log;
             __syncthreads();
-            for (int i = threadIdx.x; i < n / 2; i += 256) {
+            for (int i = threadIdx.x; i < n / 2; i += THREADS) {
                 const int lo = (i >> log) * 2 * step + (i & (step - 1)), hi = lo + step;
                 const unsigned long long x = keys[lo], y = keys[hi];
                 if ((x < y) == ((lo & size) == 0)) {
@@ -245,35 +247,38 @@ struct LogprobsRow {
 
 // A row from its pieces, and its alternatives: the logits that these are chosen from are on their way, of AHEAD pieces a wave at once,
 // while the row's sums are made
-template <int DT, int AHEAD>
-__global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a) {
+template <int DT, int AHEAD, int THREADS>
+__global__ __launch_bounds__(THREADS) void logprobs_row_kernel(const LogprobsArgs a) {
+    constexpr int WAVES = THREADS / 64, HELD = THREADS == 256 ? PIECES_MAX / 256 : 1;       // (512: at most 256 pieces)
+    asm volatile("" ::"s"(a.logits), "s"(a.stride), "s"(a.V), "s"(a.pieces), "s"(a.top), "s"(a.tokens), "s"(a.temperature),
+                 "s"(a.logprobs), "s"(a.ranks), "s"(a.entropies), "s"(a.top_ids), "s"(a.top_logprobs), "s"(a.part));      // all at once
     extern __shared__ __attribute__((aligned(16))) unsigned long long keys[];        // keys_room and two more
     __shared__ int chosen[TOP_MAX];
     __shared__ uint32_t bar;
-    __shared__ LogprobsRow part[4];
+    __shared__ LogprobsRow part[WAVES];
     __shared__ int count, nan, bins[258];
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const LogitsPiece* p = a.part + (size_t)r * a.pieces;
     const void* row = row_of<DT>(a, r);
     // a thread's pieces t, t + 256, ..
-    LogitsPiece held[PIECES_MAX / 256];
+    LogitsPiece held[HELD];
 #pragma unroll
-    for (int k = 0; k < PIECES_MAX / 256; ++k)
-        held[k] = t + 256 * k < a.pieces ? p[t + 256 * k] : LogitsPiece{-INFINITY, 0.f, 0.f, 0};
+    for (int k = 0; k < HELD; ++k)
+        held[k] = t + THREADS * k < a.pieces ? p[t + THREADS * k] : LogitsPiece{-INFINITY, 0.f, 0.f, 0};
     const int token = load_uniform(a.tokens + r);
     const bool given = token >= 0 && token < a.V;
     const float mine = load_elem(row, DT, (size_t)(given ? token : 0));
     const int n_pieces = min(a.pieces, a.top);
     if (a.top) {                                            // the pieces that the alternatives lie in
 #pragma unroll
-        for (int k = 0; k < PIECES_MAX / 256; ++k)
-            if (t + 256 * k <= a.pieces) keys[t + 256 * k] = t + 256 * k < a.pieces ? key32(held[k].m, t + 256 * k) : 0;
+        for (int k = 0; k < HELD; ++k)
+            if (t + THREADS * k <= a.pieces) keys[t + THREADS * k] = t + THREADS * k < a.pieces ? key32(held[k].m, t + THREADS * k) : 0;
         if (t == 0) {
             keys[a.pieces] = 0;
             count = 0;
         }
         __syncthreads();
-        for (int i = t; i < a.pieces; i += 256) {
+        for (int i = t; i < a.pieces; i += THREADS) {
             const unsigned long long key = keys[i];
             const int at = place_of(key, keys, a.pieces);
             if (at < n_pieces) chosen[at] = i;
@@ -287,8 +292,8 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     const auto load_ahead = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
-            if (from + 4 * j < n_pieces) {
-                const int piece = __builtin_amdgcn_readfirstlane(chosen[from + 4 * j]);
+            if (from + WAVES * j < n_pieces) {
+                const int piece = __builtin_amdgcn_readfirstlane(chosen[from + WAVES * j]);
                 first[j] = piece * PIECE + lane * 8;
                 if ((piece + 1) * PIECE <= a.V) {
 #pragma unroll
@@ -303,25 +308,25 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     if (n_pieces < a.top) {                                 // the bar from the lanes (those without a logit: 0)
         uint32_t* order = reinterpret_cast<uint32_t*>(keys);
         const int n = (n_pieces * 64 + 255) / 256 * 256;
-        for (int i = n_pieces * 64 + t; i < n; i += 256) order[i] = 0;
-        for (int from = wave; from < n_pieces; from += 4 * AHEAD) {
+        for (int i = n_pieces * 64 + t; i < n; i += THREADS) order[i] = 0;
+        for (int from = wave; from < n_pieces; from += WAVES * AHEAD) {
             if (from != wave) load_ahead(from);
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
-                if (from + 4 * j < n_pieces) {
+                if (from + WAVES * j < n_pieces) {
                     uint32_t most = 0;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                             if (first[j] + u * 512 + k < a.V) most = max(most, (uint32_t)(key32(v[j][u][k], 0) >> 32));
-                    order[(from + 4 * j) * 64 + lane] = most;
+                    order[(from + WAVES * j) * 64 + lane] = most;
                 }
         }
         __syncthreads();
-        const uint32_t b = kth_largest(order, n, min(a.top, n), bins);
+        const uint32_t b = kth_largest<THREADS>(order, n, min(a.top, n), bins);
         if (t == 0) bar = b;
-        if (n_pieces > 4 * AHEAD) load_ahead(wave);
+        if (n_pieces > WAVES * AHEAD) load_ahead(wave);
         __syncthreads();
     }
     // the pieces' sums over 2^base, and those over the largest base
@@ -329,11 +334,11 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     float hi, lo;
     exponent_factor(inv_t, hi, lo);
     const double off = (float)(c - (double)hi) / hi;
-    double base[PIECES_MAX / 256], s[PIECES_MAX / 256], w[PIECES_MAX / 256];
+    double base[HELD], s[HELD], w[HELD];
     float most = -INFINITY;
     int above = 0;
 #pragma unroll
-    for (int k = 0; k < PIECES_MAX / 256; ++k) {
+    for (int k = 0; k < HELD; ++k) {
         float b;
         s[k] = held[k].s;
         w[k] = held[k].w;
@@ -355,12 +360,13 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
         part[wave].above = above;
     }
     __syncthreads();
-    most = fmaxf(fmaxf(part[0].m, part[1].m), fmaxf(part[2].m, part[3].m));
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) most = fmaxf(most, part[k].m);
     float whole;
     const double top = whole_base(most, hi, whole) ? (double)whole : most == -INFINITY ? 0.0 : (double)most * c;
     double z = 0.0, sum_w = 0.0;
 #pragma unroll
-    for (int k = 0; k < PIECES_MAX / 256; ++k)
+    for (int k = 0; k < HELD; ++k)
         if (s[k] != 0.0) {
             const double d = base[k] - top, e = __builtin_amdgcn_exp2f((float)d);     // (of whole numbers, a power of two)
             z += s[k] * e;
@@ -376,11 +382,11 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     const uint32_t reach = bar;
     const float least = nan ? __builtin_nanf("") : logit_of((unsigned long long)reach << 32);      // (a NaN: all are looked at)
     const int room = keys_room(a.pieces, a.top);
-    for (int from = wave; from < n_pieces; from += 4 * AHEAD) {
+    for (int from = wave; from < n_pieces; from += WAVES * AHEAD) {
         if (from != wave) load_ahead(from);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
-            if (from + 4 * j < n_pieces)
+            if (from + WAVES * j < n_pieces)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -395,8 +401,15 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
                     }
     }
     __syncthreads();
-    z = ((part[0].z + part[1].z) + part[2].z) + part[3].z;
-    sum_w = ((part[0].w + part[1].w) + part[2].w) + part[3].w;
+    z = part[0].z;
+    sum_w = part[0].w;
+    above = part[0].above;
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) {
+        z += part[k].z;
+        sum_w += part[k].w;
+        above += part[k].above;
+    }
     const bool some = z > 0.0 && z < INFINITY;
     // log2 z in two parts: a whole number, and that of a number in [1/2, 1)
     const double small = __builtin_amdgcn_frexp_mant(z);
@@ -405,7 +418,7 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     const auto log_p = [&](float l) __attribute__((always_inline)) { return (float)(0.6931471805599453 * ((double)l * c - log_z)); };
     if (t == 0) {
         a.logprobs[r] = given ? log_p(mine) : 0.f;
-        if (a.ranks) a.ranks[r] = given ? 1 + part[0].above + part[1].above + part[2].above + part[3].above : 0;
+        if (a.ranks) a.ranks[r] = given ? 1 + above : 0;
         if (a.entropies) a.entropies[r] = some ? (float)(0.6931471805599453 * (log_s - (double)((float)sum_w / (float)z))) : __builtin_nanf("");
     }
     if (!a.top) return;
@@ -413,7 +426,7 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     if (n <= min(room, 1024)) {
         if (t == 0) keys[n] = 0;
         __syncthreads();
-        for (int i = t; i < n; i += 256) {
+        for (int i = t; i < n; i += THREADS) {
             const unsigned long long key = keys[i];
             const int at = place_of(key, keys, n);
             if (at < a.top) {
@@ -426,33 +439,33 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(const LogprobsArgs a)
     // Too many: the first key of each lane of the pieces, sorted; then the logits of the first lanes, sorted
     __syncthreads();
     n = power_of_two(n_pieces * 64);
-    for (int i = n_pieces * 64 + t; i < n; i += 256) keys[i] = 0;
-    for (int from = wave; from < n_pieces; from += 4 * AHEAD) {
+    for (int i = n_pieces * 64 + t; i < n; i += THREADS) keys[i] = 0;
+    for (int from = wave; from < n_pieces; from += WAVES * AHEAD) {
         load_ahead(from);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
-            if (from + 4 * j < n_pieces) {
+            if (from + WAVES * j < n_pieces) {
                 unsigned long long key = 0;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         if (first[j] + u * 512 + k < a.V) key = max(key, key32(v[j][u][k], first[j] + u * 512 + k));
-                keys[(from + 4 * j) * 64 + lane] = key;
+                keys[(from + WAVES * j) * 64 + lane] = key;
             }
     }
-    sort_keys(keys, n);
+    sort_keys<THREADS>(keys, n);
     if (t < a.top) {
         const int id = t < n && keys[t] ? (int)~(uint32_t)keys[t] : -1;
         chosen[t] = id < 0 ? -1 : id - id % 8 - (id % PIECE >= 512 ? 512 : 0);      // the first of the lane's logits
     }
     __syncthreads();
     n = power_of_two(a.top * 16);
-    for (int i = t; i < n; i += 256) {
+    for (int i = t; i < n; i += THREADS) {
         const int begin = i < a.top * 16 ? chosen[i / 16] : -1, id = begin + (i % 16 >= 8 ? 512 : 0) + i % 8;
         keys[i] = begin >= 0 && id < a.V ? key32(load_elem(row, DT, (size_t)id), id) : 0;
     }
-    sort_keys(keys, n);
+    sort_keys<THREADS>(keys, n);
     if (t < a.top) {
         a.top_ids[(size_t)r * a.top + t] = (int)~(uint32_t)keys[t];
         a.top_logprobs[(size_t)r * a.top + t] = log_p(logit_of(keys[t]));
@@ -465,8 +478,10 @@ int logprobs_launch(const LogprobsArgs& a, hipStream_t st) {
     if ((int64_t)a.R * a.pieces < 32768) logprobs_stats_kernel<DT, 1><<<(unsigned)((int64_t)a.R * ((a.pieces + 3) / 4)), 256, 0, st>>>(a);
     else logprobs_stats_kernel<DT, 2><<<(unsigned)((int64_t)a.R * ((a.pieces + 7) / 8)), 256, 0, st>>>(a);
     const size_t lds = a.top ? (keys_room(a.pieces, a.top) + 2) * 8 : 0;
-    if (a.top <= 4) logprobs_row_kernel<DT, 1><<<(unsigned)a.R, 256, lds, st>>>(a);
-    else logprobs_row_kernel<DT, 4><<<(unsigned)a.R, 256, lds, st>>>(a);
+    // Twice the waves where rows are few and alternatives many (48 rows of 151936 with 20: 9.6 -> 8.0 us); a row's pieces are summed alike
+    if (a.top <= 4) logprobs_row_kernel<DT, 1, 256><<<(unsigned)a.R, 256, lds, st>>>(a);
+    else if (a.R <= 256 && a.pieces <= 256) logprobs_row_kernel<DT, 4, 512><<<(unsigned)a.R, 512, lds, st>>>(a);
+    else logprobs_row_kernel<DT, 4, 256><<<(unsigned)a.R, 256, lds, st>>>(a);
     return esp_host::launch_check("token_logprobs");
 }
 
