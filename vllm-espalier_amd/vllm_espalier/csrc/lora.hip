@@ -79,12 +79,6 @@ __device__ __forceinline__ void store8_nt(uint16_t* p, uint4 v) {
     __builtin_nontemporal_store(u32x4_a8{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_a8*>(p));
 }
 
-// a value that every lane of the wave reads, through the scalar cache (nothing writes it while the kernel runs)
-template <typename T>
-__device__ __forceinline__ T load_uniform(const T* p) {
-    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
-}
-
 // The distinct adapters of a tile of 16 * MG rows (a lane each), one after the other: next() gives an adapter and the mask of
 // its rows, those of `rest` that are left; an id outside [0, slots) is none
 template <int MG>
