@@ -503,7 +503,7 @@ typedef struct esp_kv_cache {
  * cache (-1: the padding of a batch) stores no key and value, its queries are turned all the same. Slots of a call are distinct;
  * of tokens that share one, each 16 bytes are either's. e4m3: to nearest even of the value over the head's scale, beyond +-448
  * (infinities too) +-448. half a multiple of 8 (0: no rotation). out may be q (in place) and must else overlap none of q, k and v
- * (refused), nor the cache any of them. Alignment: rows and weights 16 bytes, strides a multiple of 8 elements. T < 2^24. A row's
+ * (refused), nor the cache any of them; the cache's elements must lie apart (refused). Alignment: rows and weights 16 bytes, strides a multiple of 8 elements. T < 2^24. A row's
  * bits depend on that row alone. */
 int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
                      int64_t v_row, int64_t v_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
@@ -512,7 +512,7 @@ int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k
                      const void* k_weight, double eps, void* out, int64_t out_row, int64_t out_head, void* stream);
 
 /* Attention of new tokens over the cache. Request b has n = n_new[b] new tokens (at most max_new; NULL: 1), whose queries are rows
- * first[b] .. first[b] + n of q (NULL: row b), and lengths[b] tokens in the cache, the new ones the last of them; token j is in
+ * first[b] .. first[b] + n of q (NULL, with max_new 1: row b), which are its own, and lengths[b] tokens in the cache, the new ones the last of them; token j is in
  * page tables[b * table_row + j / page] at j % page. New token i, at position p = lengths[b] - n + i, sees the tokens j <= p, of
  * a window (0: none) those with j > p - window, that lie in the table (j < max_pages * page) and in a page that exists (a table
  * entry outside [0, pages) hides its tokens): out = sum_j softmax_j(scale * q k_j) v_j, query head h over the cache's head

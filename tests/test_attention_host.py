@@ -49,6 +49,17 @@ CACHE_ERRORS = [
     (dict(v_token=32), "overlap"), (dict(k_token=1 << 24), "at most 2^24"), (dict(dtype=3, k_scale=16, v_scale=16, k_token=72), "aligned")]
 
 
+def test_overlapping_caches(lib):
+    """A cache that is written must lie apart: pages, tokens and heads in any order, but none over another."""
+    for over in (dict(k_head=0), dict(v_head=48), dict(k_page=1024), dict(v_page=0), dict(k_token=128, k_head=64, k_page=1024),
+                 dict(v_token=64, v_head=1024, v_page=2040)):
+        assert _append(lib, **over) == 1 and "overlap" in lib.esp_last_error().decode(), over
+    for over in (dict(k_token=128, k_head=64), dict(k_page=64, k_token=512, k_head=8192), dict(heads=1, k_head=0, v_head=0, kr=64, vr=64),
+                 dict(pages=1, k_page=0, v_page=0)):
+        assert _append(lib, T=0, **over) == 0, (over, lib.esp_last_error())
+    assert _attend(lib, T=0, k_head=0, v_head=0) == 0          # what is only read may be one head for all
+
+
 def _append(lib, **over):
     cache = _cache(over)
     a = dict(q=FAR, qr=256, qh=64, k_rows=2 * FAR, kr=128, kh=64, v_rows=3 * FAR, vr=128, vh=64, T=4, Hq=4, rows=1, slots=16, pos=16, axis=4,
@@ -89,7 +100,7 @@ def _attend(lib, **over):
     (dict(window=-1), "window"), (dict(window=1 << 30), "window"), (dict(split=64), "split"), (dict(split=-128), "split"), (dict(split=1 << 30), "split"),
     (dict(width=-1), "tables"), (dict(width=(1 << 24) + 1, tr=1 << 25), "tables"), (dict(width=0), "at least one page"),
     (dict(q=None), "null"), (dict(out=None), "null"), (dict(tables=None), "null"), (dict(lengths=None), "null"), (dict(scratch=None), "null"),
-    (dict(tr=7), "overlap"), (dict(qr=260), "multiples of 8"), (dict(outh=-64), "multiples of 8"), (dict(out=4 * FAR + 8), "aligned"),
+    (dict(first=None), "first rows"), (dict(Hq=1 << 16, T=(1 << 24) - 1, heads=1 << 10, qr=0, outr=1 << 31), "rows of heads"), (dict(tr=7), "overlap"), (dict(qr=260), "multiples of 8"), (dict(outh=-64), "multiples of 8"), (dict(out=4 * FAR + 8), "aligned"),
     (dict(scratch=24), "aligned"), (dict(outh=32), "overlap"), (dict(outr=192), "overlap"), (dict(out=FAR), "overlaps q"),
     (dict(out=FAR + 1024), "overlaps q"), (dict(new=(1 << 23) + 1), "rows a request"), (dict(bytes=15), "scratch"),
     (dict(width=1 << 24, tr=1 << 24, split=128, B=1 << 10), "pieces")])

@@ -221,6 +221,28 @@ def test_many_requests(dev):
     batch(gen, dev, lengths[:70], [1 + i % 3 for i in range(70)], 4, 2, 64, 16, split=128)
 
 
+@pytest.mark.parametrize("split", [0, 128])
+def test_many_prompts(dev, split):
+    """More prompts than a wave has lanes, some of few rows among them, padding, and prompts long enough to be cut."""
+    gen = torch.Generator().manual_seed(14)
+    n_new = [-1 if i % 13 == 4 else 1 + i * 5 % 19 for i in range(70)]
+    batch(gen, dev, [max(n, 0) + i * 11 % 50 for i, n in enumerate(n_new)], n_new, 8, 2, 64, 16, split=split)
+    batch(gen, dev, [1500, 40, 900], [20, 20, 1], 8, 2, 128, 32, split=split)
+
+
+def test_one_head_of_the_cache_for_all(dev):
+    """A cache that is only read may show one head as many (a stride of zero)."""
+    gen = torch.Generator().manual_seed(15)
+    one = make_cache(gen, dev, 6, 32, 1, 64, BF)
+    wide = PagedCache(*(t.expand(6, 32, 4, 64) for t in (one.k, one.v)))
+    q = torch.randn((2, 8, 64), generator=gen).to(BF).to(dev)
+    args = (q, i32([[3, 1], [2, 5]], dev), i32([60, 33], dev))
+    assert torch.equal(one.attend(*args, split=128), wide.attend(*args, split=128))
+    with pytest.raises(RuntimeError, match="overlap"):
+        wide.append(q, torch.zeros((2, 4, 64), dtype=BF, device=dev), torch.zeros((2, 4, 64), dtype=BF, device=dev),
+                    torch.arange(2, device=dev))
+
+
 def test_one_long_request(dev):
     gen = torch.Generator().manual_seed(6)
     for lengths, n_new in (([20011], [1]), ([9000, 12], [3, 1])):
@@ -455,7 +477,7 @@ def test_refusals(dev):
         cache.append(q, buf[:, 4:6], buf[:, 6:], slots, out=buf[:, 3:7])
     for bad in (dict(q=q.half()), dict(q=torch.zeros((3, 3, 64), dtype=BF, device=dev)), dict(tables=tables.long()),
                 dict(tables=tables[:, :0]), dict(tables=tables.cpu()), dict(lengths=lengths[:2]), dict(lengths=lengths.long()),
-                dict(first=lengths[:2]), dict(n_new=lengths.long()), dict(max_new=0), dict(scale=0.0), dict(scale=-1.0), dict(window=-1),
+                dict(first=lengths[:2]), dict(n_new=lengths.long()), dict(max_new=2), dict(max_new=0), dict(scale=0.0), dict(scale=-1.0), dict(window=-1),
                 dict(split=100), dict(split=-128), dict(out=q), dict(out=q.half())):
         args = {**dict(q=q, tables=tables, lengths=lengths), **bad}
         with pytest.raises(RuntimeError):

@@ -109,8 +109,8 @@ class PagedCache:
         tables    int32 [B, pages a request]: token j of request b is in page tables[b, j // page]; an entry outside the cache
                   hides its tokens
         lengths   int32 [B]: a request's tokens in the cache, its new ones the last of them
-        first, n_new  int32 [B]: its new tokens are rows first .. first + n_new of q (default: row b alone); n_new outside
-                  [0, max_new]: no such request, the padding of a fixed batch
+        first, n_new  int32 [B]: its new tokens are rows first .. first + n_new of q, its own (default, with max_new 1: row b);
+                  n_new outside [0, max_new]: no such request, the padding of a fixed batch
         max_new   the most that n_new may hold: what the launches are sized for
         scale     of the scores; default 1 / sqrt(dim)
         window    how many tokens a row sees, its own the last; 0: all

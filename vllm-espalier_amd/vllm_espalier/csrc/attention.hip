@@ -413,6 +413,7 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     if (T == 0 || B == 0) return esp_host::ok();
     ESP_REQUIRE(q && out && lengths && (tables || max_pages == 0) && scratch, "paged_attention: null pointer");
     ESP_REQUIRE(max_pages >= 1, "paged_attention: tables of at least one page");
+    ESP_REQUIRE(first || max_new == 1, "paged_attention: requests of more than one new token need their first rows");
     ESP_REQUIRE(B == 1 || table_row >= max_pages, "paged_attention: the tables' rows overlap");
     const int64_t strides[4] = {q_row, q_head, out_row, out_head};
     for (const int64_t s : strides)
@@ -426,8 +427,8 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     ESP_REQUIRE(!esp_host::rows_meet(out, out_row * 2, ((Hq - 1) * out_head + c.dim) * 2, q, q_row * 2,
                                      ((Hq - 1) * q_head + c.dim) * 2, T), "paged_attention: the output overlaps q");
     const AttendSizes z(B, T, max_new, group, c.heads, c.dim, max_pages * c.page, split);
-    ESP_REQUIRE(z.few < (1 << 24) && z.many < (1 << 24) && z.rows < (1 << 30) && B * max_new * Hq < (int64_t(1) << 31),
-                "paged_attention: at most 2^24 - 1 pieces of tiles");
+    ESP_REQUIRE(z.few < (1 << 24) && z.many < (1 << 24) && z.rows < (1 << 30) && T * Hq < (int64_t(1) << 31),
+                "paged_attention: at most 2^24 - 1 pieces of tiles, 2^31 - 1 rows of heads");
     ESP_REQUIRE(scratch_bytes >= z.bytes, "paged_attention: the scratch needs esp_paged_attention_scratch bytes");
     AttendArgs a;
     a.q = static_cast<const uint16_t*>(q);
@@ -460,6 +461,7 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     a.slots = z.slots;
     a.tile_rows = z.tile_rows;
     a.first_row = z.first_row;
+    a.rows = z.rows;
     a.B = (int)B;
     a.T = (int)T;
     a.Hkv = (int)c.heads;

@@ -36,6 +36,7 @@ struct AttendArgs {
     int2* plan;                                 // [B]: a request's first place in scratch and its pieces a tile
     int slots;                                  // workgroups of attention.hip that fit at once
     int tile_rows, first_row;                   // of attention.hip's tiles; attention_prompt.hip's first place in scratch
+    int64_t rows;                               // places in scratch
     int B, T, Hkv, group, max_new, window, split, capacity;                // capacity: tokens that a table can name
     int page16, page_shift;                     // tokens of a page / 16, and its reciprocal: 2 n page_mul >> (32 + page_shift)
     uint32_t page_mul;
@@ -87,6 +88,13 @@ __device__ __forceinline__ int quotient(int n, int d) {
     return q;
 }
 
+// Whether what was found lies in the request and in scratch. It does, but where requests that claim the same rows make more tiles than
+// all rows have
+__device__ __forceinline__ bool sound(const AttendArgs& a, const Piece& p, int tiles, int rows, int base, int first) {
+    return p.tile >= 0 && p.tile < tiles && p.head >= 0 && p.head < a.Hkv && p.at >= 0 && p.at < p.pieces &&
+           (p.pieces == 1 || (base >= first && base + (int64_t)tiles * a.Hkv * p.pieces * rows <= a.rows));
+}
+
 // The same of up to 64 requests, a lane each (r, pieces of `size` keys), those of the tiles that see the most keys first, so that the
 // last workgroups are short ones: item counts down the tiles that see more than 64 x keys, for the x at which they are more than
 // item (-1: all tiles). Heads next to one another: with the workgroups dealt to the XCDs in turn, an XCD's L2 has a few heads' keys.
@@ -109,7 +117,9 @@ __device__ __forceinline__ bool piece_by_length(const AttendArgs& a, int item, i
     const int higher = above(x + 1), rest = item - all(higher * a.Hkv * pieces);
     const int mine = (above(x) - higher) * a.Hkv * pieces, upto = wave_scan(mine);
     const int in_scratch = pieces > 1 ? tiles * a.Hkv * pieces * ROWS : 0, rows_upto = wave_scan(in_scratch);
-    const int l = __builtin_ctzll(__ballot(rest < upto));
+    const uint64_t hit = __ballot(rest < upto);
+    if (!hit) return false;
+    const int l = __builtin_ctzll(hit);
     const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
     const int in = rest - of(upto - mine), stack = __builtin_amdgcn_readfirstlane(quotient(in, a.Hkv));
     p.r = {of(r.n), of(r.first), of(r.length), of(r.lo), of(r.hi)};
@@ -122,6 +132,7 @@ __device__ __forceinline__ bool piece_by_length(const AttendArgs& a, int item, i
     p.tile = of(tiles) - 1 - of(higher) - level;
     const int base = a.first_row + of(rows_upto - in_scratch);
     p.row = base + (int64_t)(p.head * of(tiles) + p.tile) * p.pieces * ROWS + p.at;
+    if (!sound(a, p, of(tiles), ROWS, base, a.first_row)) return false;
     if (p.tile == 0 && p.head == 0 && p.at == 0 && threadIdx.x == 0) a.plan[l] = make_int2(base, p.pieces);
     return true;
 }
@@ -192,6 +203,7 @@ __device__ __forceinline__ bool piece_of(const AttendArgs& a, int item, Piece& p
             p.at = stack - p.head * per_tile;
             const int base = rows + of(rows_upto - in_scratch);
             p.row = base + (int64_t)(p.head * n_tiles + p.tile) * per_tile * ROWS + p.at;
+            if (!sound(a, p, n_tiles, ROWS, base, MANY ? a.first_row : 0)) return false;
             if (in == 0 && threadIdx.x == 0) a.plan[p.b] = make_int2(base, per_tile);
             return true;
         }
@@ -385,12 +397,17 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const AttendArgs a) {
         const int b = b0 + lane;
         const int2 plan = b < a.B ? a.plan[b] : make_int2(0, 0);              // (of no request: anything)
         const Request r = request_of(a, b);
-        const int mine = r.n > 0 && plan.y > 1 ? r.n * heads : 0, upto = wave_scan(mine);
+        const int rows = r.n * a.group > FEW_ROWS ? PROMPT_ROWS : a.tile_rows, tiles = (r.n * a.group + rows - 1) / rows;
+        const bool joined = r.n > 0 && plan.x >= 0 && plan.y > 1 && plan.x + (int64_t)tiles * a.Hkv * plan.y * rows <= a.rows;
+        const int mine = joined ? r.n * heads : 0, upto = wave_scan(mine);
         const int all = before + __builtin_amdgcn_readlane(upto, 63);
         for (; row < all; row += gridDim.x) {
-            const int l = __builtin_ctzll(__ballot(row < before + upto));
+            const uint64_t hit = __ballot(row < before + upto);
+            if (!hit) return;
+            const int l = __builtin_ctzll(hit);
             const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
             const int in = row - before - of(upto - mine), i = __builtin_amdgcn_readfirstlane(quotient(in, heads));
+            if (in < 0 || i >= of(r.n)) return;
             join_row<D, BF, E8, THREADS, AHEAD>(a, {of(r.n), of(r.first), 0, 0, 0}, of(plan.x), of(plan.y), i, in - i * heads);
         }
         before = all;

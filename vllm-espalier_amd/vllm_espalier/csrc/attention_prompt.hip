@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
 #pragma unroll
             for (int n = 0; n < 4 * DB; ++n) {
                 if (n + V_AHEAD < 4 * DB) v[(n + V_AHEAD) % (V_AHEAD + 1)] = read_v(buf, (n + V_AHEAD) / DB, (n + V_AHEAD) % DB);
-                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (D != 64) __builtin_amdgcn_sched_barrier(0);      // (there the registers hold more: 87 -> 82 us)
                 o[n % DB] = mfma32<BF>(v[n % (V_AHEAD + 1)], p[n / DB], o[n % DB]);
             }
         }

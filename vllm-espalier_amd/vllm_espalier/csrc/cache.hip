@@ -263,6 +263,9 @@ extern "C" int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, co
     const char* wrong = esp_host::kv_cache_error(cache, dtype);
     ESP_REQUIRE(!wrong, "cache_append: %s", wrong);
     const esp_kv_cache& c = *cache;
+    ESP_REQUIRE(!esp_host::kv_overlaps(c.dim, c.pages, c.k_page, c.page, c.k_token, c.heads, c.k_head) &&
+                    !esp_host::kv_overlaps(c.dim, c.pages, c.v_page, c.page, c.v_token, c.heads, c.v_head),
+                "cache_append: elements of the cache overlap");
     ESP_REQUIRE(T >= 0 && T < (1 << 24), "cache_append: at most 2^24 - 1 rows");
     ESP_REQUIRE(Hq >= 0 && Hq <= 1024, "cache_append: at most 1024 query heads");
     ESP_REQUIRE(half >= 0 && half % 8 == 0 && 2 * half <= c.dim,

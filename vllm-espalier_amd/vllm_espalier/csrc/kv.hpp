@@ -4,6 +4,8 @@
 #include "../../../include/espalier.h"
 #include "common.hpp"
 
+#include <utility>
+
 namespace esp {
 
 constexpr int E4M3 = ESP_E4M3;
@@ -57,6 +59,24 @@ inline const char* kv_cache_error(const esp_kv_cache* c, int dtype) {
     if (c->k_token < c->dim || c->v_token < c->dim) return "the cache's tokens overlap";
     if (c->k_token >= (1 << 24) || c->v_token >= (1 << 24)) return "a token's stride of at most 2^24 elements";
     return nullptr;
+}
+
+// Whether two of the cache's elements share a place (no call may write into such a one): a dimension's stride must be past all that the
+// ones of smaller strides span
+inline bool kv_overlaps(int64_t dim, int64_t pages, int64_t page_stride, int64_t page, int64_t token_stride, int64_t heads, int64_t head_stride) {
+    int64_t sizes[3] = {pages, page, heads}, strides[3] = {page_stride, token_stride, head_stride}, span = dim;
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (strides[j] < strides[i]) {
+                std::swap(strides[i], strides[j]);
+                std::swap(sizes[i], sizes[j]);
+            }
+    for (int i = 0; i < 3; ++i) {
+        if (sizes[i] == 1) continue;
+        if (strides[i] < span) return true;
+        span += strides[i] * (sizes[i] - 1);
+    }
+    return false;
 }
 
 }  // namespace esp_host
