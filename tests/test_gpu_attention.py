@@ -230,6 +230,25 @@ def test_many_prompts(dev, split):
     batch(gen, dev, [1500, 40, 900], [20, 20, 1], 8, 2, 128, 32, split=split)
 
 
+@pytest.mark.parametrize("dim,hq,hkv", [(64, 8, 2), (128, 8, 2), (128, 12, 1), (256, 4, 1)])
+@pytest.mark.parametrize("cache_dtype", [BF, E8])
+@pytest.mark.parametrize("window", [0, 700])
+def test_tokens_beside_prompts(dev, dim, hq, hkv, cache_dtype, window):
+    """A batch of prompts, tokens far into their answers (cut into pieces) and drafts; with a split the tokens' bits are those of a
+    batch without prompts."""
+    gen = torch.Generator().manual_seed(dim + hq + window)
+    lengths, n_new = [6000, 430, 3001, 12, 129, 1700], [1, 300, 2, 1, 129, 1]
+    batch(gen, dev, lengths, n_new, hq, hkv, dim, 32, BF, cache_dtype, window=window)
+    cache, q, tables, first, out = batch(gen, dev, lengths, n_new, hq, hkv, dim, 32, BF, cache_dtype, window=window, split=256)
+    few = [0, 2, 3, 5]
+    pick = lambda v: i32([v[b] for b in few], dev)  # noqa: E731
+    alone = torch.zeros_like(out)
+    cache.attend(q, tables[few].contiguous(), pick(lengths), pick(first), pick(n_new), 2, window=window, split=256, out=alone)
+    for b in few:
+        rows = slice(first[b], first[b] + n_new[b])
+        assert torch.equal(alone[rows].view(torch.int16), out[rows].view(torch.int16)), b
+
+
 def test_one_head_of_the_cache_for_all(dev):
     """A cache that is only read may show one head as many (a stride of zero)."""
     gen = torch.Generator().manual_seed(15)

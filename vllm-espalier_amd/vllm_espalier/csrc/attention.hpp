@@ -35,6 +35,7 @@ struct AttendArgs {
     float2* stats;                              // a row's maximum and sum in a piece
     int2* plan;                                 // [B]: a request's first place in scratch and its pieces a tile
     int slots;                                  // workgroups of attention.hip that fit at once
+    int many;                                   // of attention_prompt.hip's launch, those for requests of many rows
     int tile_rows, first_row;                   // of attention.hip's tiles; attention_prompt.hip's first place in scratch
     int64_t rows;                               // places in scratch
     int B, T, Hkv, group, max_new, window, split, capacity;                // capacity: tokens that a table can name
@@ -449,7 +450,12 @@ struct AttendSizes {
     }
 };
 
-// attention_prompt.hip: tiles of PROMPT_ROWS rows
+// attention_prompt.hip: tiles of PROMPT_ROWS rows, and, FEW_TOO, the requests of few rows as well: a prompt of 2048 new tokens beside
+// 31 requests of one over 4000, heads 32/8 of 128, takes 149 us in one launch and 171 in two (the same prompt alone 62 and 64), 512
+// beside 31 over 2000 77 and 85. With workgroups of both kinds in turn, by eights, the second is 93 (the requests of one token, bound
+// by memory, want all slots at once). Heads of 256 would lose: 174 us for 168 at 4 prompts of 1024 over 2048 (registers spill).
+template <int D>
+constexpr bool FEW_TOO = D != 256;
 void attend_prompt(const AttendArgs& a, const AttendSizes& z, int D, bool bf, bool e8, hipStream_t st);
 
 }  // namespace esp

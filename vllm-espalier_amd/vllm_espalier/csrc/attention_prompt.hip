@@ -11,7 +11,13 @@
 //
 // LDS rows are the head's elements in pieces of 16 bytes, piece c of key r at c ^ spread(r): the 16 keys that a read of K goes through
 // at one piece lie in different banks, and so do the 4 keys of 64 bytes that a transposed read goes through.
-#include "attention.hpp"
+//
+// What bounds it is neither products nor memory alone but a wave's order: its products (34 % of the cycles), then its softmax (41 %
+// on the vector units), with two waves a SIMD to fill in for each other, which is what the registers of 32 x 128 outputs leave.
+// Three requests of up to 2048 new tokens over up to 4096, heads 32/4 of 128, bf16 (105 GFLOP of visible pairs): 144 to 158 us
+// (0.7 PFLOP/s), where the tiles that see most decide the end; one of 4096 over 8192, heads 32/8 (412 GFLOP), 445 us (0.93 PFLOP/s).
+// A large matrix product reaches 1.5.
+#include "attention_few.hpp"
 
 namespace esp {
 
@@ -117,6 +123,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
     // two buffers, each an object of its own and each step of the loop with its own: a read of one is then known not to wait for what
     // is on its way into the other
     __shared__ __attribute__((aligned(1024))) char lds0[BUFFER], lds1[BUFFER];
+    if constexpr (FEW_TOO<D>) {
+        static_assert(FEW_LDS<D, 2> <= BUFFER, "the few rows' shares");
+        if ((int)blockIdx.x >= a.many) {                      // behind the others: they fill in where these end
+            attend_few<D, BF, E8, 2>(a, (int)blockIdx.x - a.many, lds0);
+            return;
+        }
+    }
     Piece pc;
     if (!piece_of<ROWS>(a, (int)blockIdx.x, pc)) return;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, h = lane >> 5;
@@ -313,7 +326,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
 
 template <int D, bool BF, bool E8>
 void prompt_launch(const AttendArgs& a, const AttendSizes& z, hipStream_t st) {
-    attend_prompt_kernel<D, BF, E8><<<(unsigned)z.many, 256, 0, st>>>(a);
+    attend_prompt_kernel<D, BF, E8><<<(unsigned)(z.many + (FEW_TOO<D> ? z.few : 0)), 256, 0, st>>>(a);
 }
 template <int D>
 void prompt_types(const AttendArgs& a, const AttendSizes& z, bool bf, bool e8, hipStream_t st) {
