@@ -503,8 +503,8 @@ typedef struct esp_kv_cache {
  * cache (-1: the padding of a batch) stores no key and value, its queries are turned all the same. Slots of a call are distinct;
  * of tokens that share one, each 16 bytes are either's. e4m3: to nearest even of the value over the head's scale, beyond +-448
  * (infinities too) +-448. half a multiple of 8 (0: no rotation). out may be q (in place) and must else overlap none of q, k and v
- * (refused), nor the cache any of them; the cache's elements must lie apart (refused). Alignment: rows and weights 16 bytes, strides a multiple of 8 elements. T < 2^24. A row's
- * bits depend on that row alone. */
+ * (refused), nor the cache any of them; the cache's elements must lie apart (refused). Alignment: rows and weights 16 bytes, strides
+ * a multiple of 8 elements. T < 2^24. A row's bits depend on that row alone. */
 int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
                      int64_t v_row, int64_t v_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
                      const int64_t* slots, const int64_t* positions, int64_t pos_axis, int64_t n_axes, const double* inv_freq,
@@ -512,8 +512,8 @@ int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k
                      const void* k_weight, double eps, void* out, int64_t out_row, int64_t out_head, void* stream);
 
 /* Attention of new tokens over the cache. Request b has n = n_new[b] new tokens (at most max_new; NULL: 1), whose queries are rows
- * first[b] .. first[b] + n of q (NULL, with max_new 1: row b), which are its own, and lengths[b] tokens in the cache, the new ones the last of them; token j is in
- * page tables[b * table_row + j / page] at j % page. New token i, at position p = lengths[b] - n + i, sees the tokens j <= p, of
+ * first[b] .. first[b] + n of q (NULL, with max_new 1: row b), which are its own, and lengths[b] tokens in the cache, the new ones the
+ * last of them; token j is in page tables[b * table_row + j / page] at j % page. New token i, at position p = lengths[b] - n + i, sees the tokens j <= p, of
  * a window (0: none) those with j > p - window, that lie in the table (j < max_pages * page) and in a page that exists (a table
  * entry outside [0, pages) hides its tokens): out = sum_j softmax_j(scale * q k_j) v_j, query head h over the cache's head
  * h / (Hq / heads), zeros where it sees nothing. What a row does not see does not change it, whatever it holds. Rows of no request,
@@ -524,8 +524,8 @@ int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k
  * batch's lengths, so that a row's bits depend on them; with a split of its own a row's bits depend on its request alone (requests
  * of more than 32 rows a head of the cache, n * Hq / heads, are then not cut at all).
  * q, out [T][Hq][dim] of dtype ESP_BF16 or ESP_F16 with row and head strides, 16-byte aligned (strides multiples of 8); out must
- * not overlap q (refused), nor anything else. Hq a multiple of heads; scale > 0; max_pages * page <= 2^28. scratch: at least
- * esp_paged_attention_scratch bytes, 16-byte aligned, any values. */
+ * not overlap q (refused), nor anything else. Hq a multiple of heads; scale > 0; max_pages * page <= 2^28; T < 2^24, T * Hq < 2^31,
+ * max_new * Hq / heads < 2^23. scratch: at least esp_paged_attention_scratch bytes, 16-byte aligned, any values. */
 int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
                         const int32_t* tables, int64_t table_row, int64_t max_pages, const int32_t* lengths,
                         const int32_t* first, const int32_t* n_new, int64_t B, int64_t max_new, double scale, int64_t window,

@@ -109,6 +109,13 @@ def test_attend_argument_errors(lib, over, needle):
     assert needle in lib.esp_last_error().decode()
 
 
+def test_rows_of_a_request_stay_countable(lib):
+    """Rows a request and head of the cache are told apart by reciprocals in fp32: 2^23 are refused, one fewer not for that."""
+    heads = dict(Hq=4, heads=1, outr=256, bytes=15)
+    assert _attend(lib, new=1 << 21, **heads) == 1 and "rows a request" in lib.esp_last_error().decode()
+    assert _attend(lib, new=(1 << 21) - 1, **heads) == 1 and "scratch" in lib.esp_last_error().decode()
+
+
 def test_no_rows_is_no_call(lib):
     assert _append(lib, T=0, q=None, k_rows=None, v_rows=None, out=None) == 0
     assert _attend(lib, T=0, q=None, out=None) == 0

@@ -103,7 +103,7 @@ extern "C" int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head,
     ESP_REQUIRE((Hq == 1 || out_head >= c.dim) && (T == 1 || out_row >= (Hq - 1) * out_head + c.dim),
                 "paged_attention: the output's rows overlap");
     const int64_t group = Hq / c.heads;
-    ESP_REQUIRE(max_new * group < (1 << 24), "paged_attention: at most 2^24 - 1 rows a request and head of the cache");
+    ESP_REQUIRE(max_new * group < (1 << 23), "paged_attention: at most 2^23 - 1 rows a request and head of the cache");
     // other workgroups still read the queries when one writes its rows
     ESP_REQUIRE(!esp_host::rows_meet(out, out_row * 2, ((Hq - 1) * out_head + c.dim) * 2, q, q_row * 2,
                                      ((Hq - 1) * q_head + c.dim) * 2, T), "paged_attention: the output overlaps q");

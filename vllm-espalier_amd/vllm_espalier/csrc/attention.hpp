@@ -81,7 +81,8 @@ __device__ __forceinline__ int wave_scan(int v) {             // inclusive sum o
     return v;
 }
 
-// n / d of non-negative numbers below 2^30 (the reciprocal's quotient is off by one at most)
+// n / d of non-negative numbers with a quotient below 2^22 (its relative error is 2^-22 at most: the reciprocal's quotient is off by
+// one at most), or n below 2^24 and d a power of two
 __device__ __forceinline__ int quotient(int n, int d) {
     int q = (int)((float)n * __builtin_amdgcn_rcpf((float)d));
     const int r = n - q * d;
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const AttendArgs a) {
             if (!hit) return;
             const int l = __builtin_ctzll(hit);
             const auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, l); };
-            const int in = row - before - of(upto - mine), i = __builtin_amdgcn_readfirstlane(quotient(in, heads));
+            const int in = row - before - of(upto - mine), i = __builtin_amdgcn_readfirstlane((int)((uint32_t)in / (uint32_t)heads));
             if (in < 0 || i >= of(r.n)) return;
             join_row<D, BF, E8, THREADS, AHEAD>(a, {of(r.n), of(r.first), 0, 0, 0}, of(plan.x), of(plan.y), i, in - i * heads);
         }
