@@ -5,8 +5,10 @@
 //
 // Two launches. The first reads every row once: a wave takes 1024 logits into registers and leaves their maximum, their sums and
 // how many of them come before the row's token, so no workgroup waits for another. Sums are over 2^(x - K) with K the whole number
-// nearest to the piece's largest x, so that an exponent costs one exact multiply-add; c's rounding to fp32, which shifts x by x times a
-// constant, is taken out of the sums afterwards (its first order is that constant times the sum of 2^(x - K) x, which is there).
+// nearest to the piece's largest x, so that an exponent costs one multiply-add. That is with c rounded down to fp32, hi: what it leaves
+// out, x - K times off = (c - hi) / hi below 2^-23 and K times the same, comes back in the second launch. A piece's base is K (1 + off)
+// there, in fp64 (K off passes 1 where logits times c pass 2^23: no first order of it would do), and off times x - K, a small number for
+// every logit that counts, is taken into the sums by its first order, which is off times the sum of 2^(x - K) (x - K), which is there.
 //
 // The second launch puts a row together, a workgroup a row, and finds the alternatives without another pass over it: the k first
 // tokens lie in the k pieces whose largest logits are the first (each other piece has k elements before all of its own), so it reads
@@ -333,8 +335,9 @@ __global__ __launch_bounds__(THREADS) void logprobs_row_kernel(const LogprobsArg
     const double inv_t = inv_temperature_of(a, r), c = inv_t * 1.4426950408889634;
     float hi, lo;
     exponent_factor(inv_t, hi, lo);
-    const double off = (float)(c - (double)hi) / hi;
+    const double off = (c - (double)hi) / (double)hi;
     double base[HELD], s[HELD], w[HELD];
+    bool whole[HELD];
     float most = -INFINITY;
     int above = 0;
 #pragma unroll
@@ -342,12 +345,12 @@ __global__ __launch_bounds__(THREADS) void logprobs_row_kernel(const LogprobsArg
         float b;
         s[k] = held[k].s;
         w[k] = held[k].w;
+        whole[k] = s[k] != 0.0 && whole_base(held[k].m, hi, b);
         base[k] = held[k].m == -INFINITY ? -INFINITY : (double)held[k].m * c;
-        if (s[k] != 0.0 && whole_base(held[k].m, hi, b)) {
-            const double shift = off * (w[k] + (double)b * s[k]);       // sum of e (c - hi) l
-            base[k] = b;
-            s[k] += 0.6931471805599453 * shift;
-            w[k] += shift;
+        if (whole[k]) {
+            base[k] = b;                                      // K; below, K (1 + off)
+            s[k] += 0.6931471805599453 * off * w[k];
+            w[k] += off * w[k];
         }
         most = fmaxf(most, held[k].m);
         above += held[k].above;
@@ -362,13 +365,23 @@ __global__ __launch_bounds__(THREADS) void logprobs_row_kernel(const LogprobsArg
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) most = fmaxf(most, part[k].m);
-    float whole;
-    const double top = whole_base(most, hi, whole) ? (double)whole : most == -INFINITY ? 0.0 : (double)most * c;
+    float top_k;
+    const bool top_whole = whole_base(most, hi, top_k);
+    const double top = top_whole ? (double)top_k * (1.0 + off) : most == -INFINITY ? 0.0 : (double)most * c;
     double z = 0.0, sum_w = 0.0;
 #pragma unroll
     for (int k = 0; k < HELD; ++k)
         if (s[k] != 0.0) {
-            const double d = base[k] - top, e = __builtin_amdgcn_exp2f((float)d);     // (of whole numbers, a power of two)
+            double d, e;
+            if (whole[k] && top_whole) {                      // 2^(a whole number) times 2^(off times it), off times 150 at most where it counts
+                const double between = base[k] - (double)top_k;
+                d = between * (1.0 + off);
+                e = __builtin_amdgcn_exp2f((float)between);
+                e = e != 0.0 ? e * (1.0 + 0.6931471805599453 * off * between) : 0.0;
+            } else {
+                d = (whole[k] ? base[k] * (1.0 + off) : base[k]) - top;
+                e = __builtin_amdgcn_exp2f((float)d);
+            }
             z += s[k] * e;
             sum_w += e != 0.0 ? (w[k] + s[k] * d) * e : 0.0;
         }
@@ -414,8 +427,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_row_kernel(const LogprobsArg
     // log2 z in two parts: a whole number, and that of a number in [1/2, 1)
     const double small = __builtin_amdgcn_frexp_mant(z);
     const double log_s = (double)__builtin_amdgcn_frexp_exp(z) + (double)__builtin_amdgcn_logf((float)small);
-    const double log_z = some ? log_s + top : (double)__builtin_nanf("");
-    const auto log_p = [&](float l) __attribute__((always_inline)) { return (float)(0.6931471805599453 * ((double)l * c - log_z)); };
+    const double less = some ? log_s : (double)__builtin_nanf("");       // (the largest logit's difference is exact, however large it is)
+    const auto log_p = [&](float l) __attribute__((always_inline)) { return (float)(0.6931471805599453 * ((double)l * c - top - less)); };
     if (t == 0) {
         a.logprobs[r] = given ? log_p(mine) : 0.f;
         if (a.ranks) a.ranks[r] = given ? 1 + above : 0;
