@@ -231,6 +231,17 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
     else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
 }
 
+// What the exponents of a row's weights are taken from, by its running maximum m (-inf where it has seen nothing). bf16 weights: m. fp16 has
+// ten binary places down to 2^-14 only: over m - 13 a weight is off by at most half a step of itself down to 2^-27 of the largest, and by
+// 2^-38 of that below (over m, thousands of keys some 2^-25 below one whose value is small would come out as nothing, though their weights
+// are in the sum). Weights stay below 2^15.5 so, prompts' LAG among them, while scores are below 2^22; past that, where fp32's own steps
+// move an exponent by whole numbers, over m. Sums, outputs and statistics are over the same, and it cancels.
+template <bool BF>
+__device__ __forceinline__ float reference(float m) {
+    if constexpr (BF) return m;
+    return m - (fabsf(m) < 4194304.0f ? 13.0f : 0.0f);
+}
+
 // the largest over the four 16-lane rows of a wave, each lane with those at its place; their sum
 __device__ __forceinline__ float rows_max(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);

@@ -133,9 +133,9 @@ __device__ __forceinline__ bool weigh(f32x4 (&s)[NT][2], Values<D, E8>& v, bool 
 #pragma unroll
             for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][u][i] * scale);
         m = rows_max(m);
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = m == -INFINITY ? 0.f : reference<BF>(m);
         if (__any(m != st.m[t])) {
-            const float alpha = __builtin_amdgcn_exp2f(st.m[t] - base);
+            const float alpha = __builtin_amdgcn_exp2f(reference<BF>(st.m[t]) - base);
             st.l[t] *= alpha;
 #pragma unroll
             for (int e = 0; e < State<D, NT>::OPS; ++e) st.o[t][e] *= alpha;
@@ -268,6 +268,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int item, char* 
     f32x4(*sh_o)[NT * OPS][64] = reinterpret_cast<f32x4(*)[NT * OPS][64]>(lds);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+        st.m[t] = reference<BF>(st.m[t]);                     // (from here on what the sums are over)
         st.l[t] = rows_sum(st.l[t]);
         if (g == 0) {
             sh_m[wave][16 * t + lane] = st.m[t];

@@ -6,8 +6,8 @@
 // they are what O^T = V^T P^T wants; V^T comes from the LDS by its transposed reads, 4 keys of an element at a time. A query's
 // statistics are two lanes' business.
 //
-// The maximum that the weights are taken from may lie up to 2^LAG below the largest score: sums and outputs, fp32, keep their
-// relative errors, and the outputs are rarely scaled.
+// The maximum that the weights are taken from may lie up to LAG below the largest score (as exponents of 2): sums and outputs, fp32, keep
+// their relative errors, and the outputs are rarely scaled.
 //
 // LDS rows are the head's elements in pieces of 16 bytes, piece c of key r at c ^ spread(r): the 16 keys that a read of K goes through
 // at one piece lie in different banks, and so do the 4 keys of 64 bytes that a transposed read goes through.
@@ -27,7 +27,10 @@ using global_void_ptr = const __attribute__((address_space(1))) void*;
 using lds_void_ptr = __attribute__((address_space(3))) void*;
 
 constexpr int TILE = 64;                       // keys in the LDS
-constexpr float LAG = 8.0f;
+// (fp16: what reference() leaves of its range. The outputs are scaled more often: 4 prompts of 1024 over 2047, 32/4 heads of 64 125 us for
+// 123 with 8, 16/2 of 256 252 for 235)
+template <bool BF>
+constexpr float LAG = BF ? 8.0f : 2.0f;
 
 __device__ const uint4 no_keys[1] = {};        // what keys that nobody sees are read from
 
@@ -116,8 +119,9 @@ struct Loader {
     }
 };
 
+// (three waves a SIMD hold the plain heads of 64 by themselves in bf16; fp16, one register over, has to be told)
 template <int D, bool BF, bool E8>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 && !E8 && !BF ? 3 : 2) void attend_prompt_kernel(const AttendArgs a) {
     constexpr int ROWS = PROMPT_ROWS, ROW = D * 2, KK = D / 16, DB = D / 32, BUFFER = 2 * TILE * ROW;
     constexpr int K_AHEAD = D == 256 ? 1 : 2, V_AHEAD = D == 256 ? 2 : 4;     // steps that operands are read ahead of their products
     // two buffers, each an object of its own and each step of the loop with its own: a read of one is then known not to wait for what
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[db][j] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, over = -INFINITY;          // over: reference(m), of fp16 (made from m for every tile it costs 27 registers)
     const float scale = E8 ? a.scale * load_uniform(a.ks + pc.head) : a.scale;
 
     // where the lane reads: K operand kk of key lane % 32; V^T, elements 32 db + lane % 32, keys 4 h .. of 16 (and 8 further on)
@@ -266,15 +270,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, s[1][j]);
             top = halves_max(top) * scale;
-            if (__any(top > m + LAG)) {
+            if (__any(top > m + LAG<BF>)) {
                 const float next_m = fmaxf(m, top);
-                const float alpha = __builtin_amdgcn_exp2f(m - (next_m == -INFINITY ? 0.f : next_m));
+                const float next = reference<BF>(next_m), alpha = __builtin_amdgcn_exp2f((BF ? m : over) - (next == -INFINITY ? 0.f : next));
                 m = next_m;
+                over = next;
                 l *= alpha;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) o[db] *= alpha;
             }
-            const float base = m == -INFINITY ? 0.f : m;
+            const float base = (BF ? m : over) == -INFINITY ? 0.f : BF ? m : over;
             u32x4 p[4];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -319,7 +324,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_prompt_kernel(co
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
                 *reinterpret_cast<float4*>(to + 32 * db + 2 * j) = make_float4(o[db][j], o[db][j + 1], o[db][j + 2], o[db][j + 3]);
-        if (h == 0) a.stats[at] = make_float2(m, l);
+        if (h == 0) a.stats[at] = make_float2(BF ? m : over, l);
     }
     if (__syncthreads_or(odd)) mark_not_finite<D, BF, E8, ROWS>(a, pc, r, table, start, end);
 }
