@@ -503,7 +503,8 @@ typedef struct esp_kv_cache {
  * cache (-1: the padding of a batch) stores no key and value, its queries are turned all the same. Slots of a call are distinct;
  * of tokens that share one, each 16 bytes are either's. e4m3: to nearest even of the value over the head's scale, beyond +-448
  * (infinities too) +-448. half a multiple of 8 (0: no rotation). out may be q (in place) and must else overlap none of q, k and v
- * (refused), nor the cache any of them; the cache's elements must lie apart (refused). Alignment: rows and weights 16 bytes, strides
+ * (refused), nor the cache any of them; the cache's elements must lie apart, k's from v's too (refused; of k and v with different strides
+ * the caller sees to it). Alignment: rows and weights 16 bytes, strides
  * a multiple of 8 elements. T < 2^24. A row's bits depend on that row alone. */
 int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
                      int64_t v_row, int64_t v_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,

@@ -62,7 +62,8 @@ class Rotary:
 class PagedCache:
     """The keys and values of a layer in pages: k and v [pages, page, heads, dim] of any strides with a head's elements side by
     side (16-byte aligned), bf16, fp16 or e4m3. e4m3 has a scale a head (fp32 [heads], positive) for k and for v: a value stands
-    for itself times its head's scale. dim is 64, 128 or 256, page a multiple of 16."""
+    for itself times its head's scale. dim is 64, 128 or 256, page a multiple of 16. append needs k and v apart; attend may have one
+    tensor for both."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):

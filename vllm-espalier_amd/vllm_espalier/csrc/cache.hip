@@ -266,6 +266,9 @@ extern "C" int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, co
     ESP_REQUIRE(!esp_host::kv_overlaps(c.dim, c.pages, c.k_page, c.page, c.k_token, c.heads, c.k_head) &&
                     !esp_host::kv_overlaps(c.dim, c.pages, c.v_page, c.page, c.v_token, c.heads, c.v_head),
                 "cache_append: elements of the cache overlap");
+    ESP_REQUIRE(c.k_page != c.v_page || c.k_token != c.v_token || c.k_head != c.v_head ||
+                    !esp_host::kv_share(((intptr_t)c.v - (intptr_t)c.k) / kv_bytes(c.dtype), c.dim, c.pages, c.k_page, c.page, c.k_token, c.heads, c.k_head),
+                "cache_append: k and v of the cache overlap");
     ESP_REQUIRE(T >= 0 && T < (1 << 24), "cache_append: at most 2^24 - 1 rows");
     ESP_REQUIRE(Hq >= 0 && Hq <= 1024, "cache_append: at most 1024 query heads");
     ESP_REQUIRE(half >= 0 && half % 8 == 0 && 2 * half <= c.dim,

@@ -4,6 +4,7 @@
 #include "../../../include/espalier.h"
 #include "common.hpp"
 
+#include <algorithm>
 #include <utility>
 
 namespace esp {
@@ -77,6 +78,25 @@ inline bool kv_overlaps(int64_t dim, int64_t pages, int64_t page_stride, int64_t
         span += strides[i] * (sizes[i] - 1);
     }
     return false;
+}
+
+// Whether k and v of one layout (kv_overlaps is false of it) share an element: whether what lies between their first ones, v - k elements,
+// is a difference of two places. The largest stride first: all that the smaller ones span is less than it, so one of two multiples of it
+// is in the difference, if any
+inline bool kv_share(int64_t between, int64_t dim, int64_t pages, int64_t page_stride, int64_t page, int64_t token_stride, int64_t heads,
+                     int64_t head_stride) {
+    std::pair<int64_t, int64_t> by[3] = {{page_stride, pages}, {token_stride, page}, {head_stride, heads}};
+    std::sort(by, by + 3);
+    const auto reached = [&](const auto& self, int level, int64_t d) -> bool {
+        if (level < 0) return d > -dim && d < dim;
+        const auto [stride, n] = by[level];
+        if (n == 1) return self(self, level - 1, d);
+        const int64_t q = d >= 0 ? d / stride : -((-d + stride - 1) / stride);
+        for (int64_t k = q; k <= q + 1; ++k)
+            if (k > -n && k < n && self(self, level - 1, d - k * stride)) return true;
+        return false;
+    };
+    return reached(reached, 2, between);
 }
 
 }  // namespace esp_host
