@@ -7,6 +7,7 @@ import random
 import pytest
 
 from test_attention_host import Cache, FAR, lib  # noqa: F401
+from vllm_espalier.attention import Rotary
 
 
 def append(lib, k, v, strides, pages, page, heads, dim, dtype=1):  # noqa: F811
@@ -60,3 +61,16 @@ def test_keys_and_values_apart_by_enumeration(lib):  # noqa: F811
             assert got == int(want), (order, strides, between)
             seen[got] += 1
     assert min(seen) > 100, seen
+
+
+def test_interleaved_shares():
+    """Every axis has as many pairs as it was given, or the rotation is refused."""
+    for sections in ([16, 8, 8], [12, 10, 10], [32], [16, 16], [11, 11, 10], [32, 0, 0], [20, 2, 10], [8, 8, 8, 8], [17, 5, 5, 5]):
+        axes = Rotary.of_base(64, sections=sections, interleaved=True, device="cpu").axes
+        assert [int((axes == a).sum()) for a in range(len(sections))] == sections
+        assert all(a in (0, f % len(sections)) for f, a in enumerate(axes.tolist()))
+    for sections in ([4, 14, 14], [0, 16, 16], [10, 11, 11], [15, 17], [7, 9, 8, 8], [0, 32]):
+        with pytest.raises(ValueError, match="turns"):
+            Rotary.of_base(64, sections=sections, interleaved=True, device="cpu")
+        axes = Rotary.of_base(64, sections=sections, device="cpu").axes                  # (one axis after the other any shares fit)
+        assert [int((axes == a).sum()) for a in range(len(sections))] == sections

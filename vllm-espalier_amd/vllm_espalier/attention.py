@@ -38,7 +38,7 @@ class Rotary:
     def of_base(cls, elements: int, base: float = 10000.0, sections=None, interleaved: bool = False, device="cuda", **more):
         """base^(-2 f / elements) for the pairs of `elements` elements. sections: how many pairs each axis has, one axis after
         the other, or (interleaved) in turn, pair f on axis f mod the number of axes as long as that one has pairs left, else on
-        axis 0."""
+        axis 0. An axis behind the first that has more pairs than turns is refused."""
         half = elements // 2
         if elements <= 0 or elements % 16:
             raise ValueError("a rotation takes a positive multiple of 16 elements")
@@ -53,6 +53,8 @@ class Rotary:
                 for f in range(half):
                     a = f % len(sections)
                     order.append(a if f // len(sections) < left[a] else 0)
+                if [order.count(a) for a in range(len(sections))] != sections:
+                    raise ValueError(f"sections: an axis has more pairs than turns among {half} interleaved ones")
             else:
                 order = [a for a, n in enumerate(sections) for _ in range(n)]
             axes = torch.tensor(order, dtype=torch.int32, device=device)
