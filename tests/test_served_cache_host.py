@@ -7,6 +7,7 @@ import random
 import pytest
 
 from test_attention_host import Cache, FAR, lib  # noqa: F401
+from vllm_espalier import step as S
 from vllm_espalier.attention import Rotary
 
 
@@ -74,3 +75,13 @@ def test_interleaved_shares():
             Rotary.of_base(64, sections=sections, interleaved=True, device="cpu")
         axes = Rotary.of_base(64, sections=sections, device="cpu").axes                  # (one axis after the other any shares fit)
         assert [int((axes == a).sum()) for a in range(len(sections))] == sections
+
+
+@pytest.fixture(scope="module")
+def decoder():
+    return S.SyntheticDecoder(n_layers=2, seed=9, device="cpu", E=4, vocab=1024)
+
+
+def test_no_places_without_caches(decoder):
+    with pytest.raises(RuntimeError, match="use_cache"):
+        decoder.sequences(decoder.buffers(3))

@@ -219,6 +219,8 @@ class SyntheticDecoder:
         """The places of the rows of b, for up to `requests` (default: one a row) with max_new new tokens and `pages` pages each
         (default: the whole cache's)."""
         cache = self.layers[0].cache
+        if cache is None:
+            raise RuntimeError("sequences(): the layers have no cache (use_cache)")
         b.sequences = Sequences(b.T, b.T if requests is None else requests, max_new, cache.k.shape[0] if pages is None else pages,
                                 cache.k.shape[1], self.dev)
         b.attn = torch.zeros((b.T, Q_OUT), dtype=torch.bfloat16, device=self.dev)
