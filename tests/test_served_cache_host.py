@@ -85,3 +85,17 @@ def decoder():
 def test_no_places_without_caches(decoder):
     with pytest.raises(RuntimeError, match="use_cache"):
         decoder.sequences(decoder.buffers(3))
+
+
+def test_places_belong_to_the_caches(decoder):
+    """None of the former caches' pages after others have come."""
+    b = decoder.buffers(3)
+    decoder.use_cache(4, 32)
+    s = decoder.sequences(b, max_new=3)
+    s.place([[1, 2]], [34], [3])
+    assert s.page == 32 and s.slots.tolist() == [63, 64, 65]
+    assert b.sequences is s
+    decoder.use_cache(8, 16)
+    with pytest.raises(RuntimeError, match="sequences"):
+        decoder._mixed(decoder.layers[0], b)
+    assert decoder.sequences(b).page == 16 and b.sequences.tables.shape == (3, 8)

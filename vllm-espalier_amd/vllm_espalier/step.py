@@ -208,7 +208,10 @@ class SyntheticDecoder:
     def use_cache(self, pages: int, page: int = 64, dtype=torch.bfloat16, scale: float | None = None, base: float = 1e6,
                   split: int = 0, seed: int = 0) -> None:
         """A cache of `pages` pages for every layer, q and k norms a head, and the rotation of positions; dtype bf16, or e4m3 with
-        one scale. split: PagedCache.attend's. The rows of the passes that follow are those of Buffers.sequences (sequences())."""
+        one scale. split: PagedCache.attend's. The rows of the passes that follow are those of Buffers.sequences (sequences()),
+        which is asked for anew where there were caches before: its places are those of their pages."""
+        for b in self._bufs.values():
+            b.sequences = None
         gen = torch.Generator(device=self.dev).manual_seed(seed)
         self.rotary, self.split = Rotary.of_base(HEAD_DIM, base, device=self.dev), split
         for L in self.layers:
