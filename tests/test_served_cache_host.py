@@ -5,6 +5,7 @@ import itertools
 import random
 
 import pytest
+import torch
 
 from test_attention_host import Cache, FAR, lib  # noqa: F401
 from vllm_espalier import step as S
@@ -99,3 +100,13 @@ def test_places_belong_to_the_caches(decoder):
     with pytest.raises(RuntimeError, match="sequences"):
         decoder._mixed(decoder.layers[0], b)
     assert decoder.sequences(b).page == 16 and b.sequences.tables.shape == (3, 8)
+
+
+def test_algorithmic_bytes_count_the_norms_of_q_and_k():
+    dec = S.SyntheticDecoder(n_layers=2, seed=9, device="cpu", E=4, vocab=1024)
+    picks = [torch.empty((0,), dtype=torch.int32)] * 2
+    plain = dec.algorithmic_bytes(picks, 3)
+    dec.use_cache(4, 32)
+    assert dec.algorithmic_bytes(picks, 3) - plain == 2 * 2 * S.HEAD_DIM * 2
+    dec.layers[1].cache = None                                # a layer without a cache reads none of them
+    assert dec.algorithmic_bytes(picks, 3) - plain == 2 * S.HEAD_DIM * 2

@@ -373,11 +373,14 @@ class SyntheticDecoder:
     def algorithmic_bytes(self, picks: list[torch.Tensor], tokens: int, head: bool = True) -> int:
         """Weight bytes a pass over `tokens` rows reads: trellis + suh + svh of q/k/v/o, of the shared expert and of
         every distinct routed expert picked (picks from an eager forward), the bf16 router, the RMSNorm weights (behind
-        the blocks too), one embedding row a token, and the head. Adapters, of which rows name the slots, are not in it."""
+        the blocks and, with a cache, of q and k too), one embedding row a token, and the head. Adapters, of which rows name the
+        slots, and what a cache holds are not in it."""
         total = tokens * D_MODEL * 2
         for L, ids in zip(self.layers, picks):
             total += WL.nbytes(L.qkv.mats) + WL.nbytes(L.o.mats) + WL.nbytes(L.shared)
             total += L.router.numel() * 2 + WL.norm_bytes(L.norm1, L.norm2, L.post_in, L.post_o)
+            if L.cache is not None:
+                total += WL.norm_bytes(L.q_norm, L.k_norm)
             for u in ids.tolist():
                 if u < len(L.experts):
                     total += WL.nbytes(L.experts[u])
