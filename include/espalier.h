@@ -547,7 +547,7 @@ int64_t esp_paged_attention_scratch(int64_t B, int64_t T, int64_t max_new, int64
  * A token outside [0, V) has rank 0 and log-probability 0. A row without a distribution (a NaN or +inf in it, or nothing above
  * -inf) has NaN for its entropy and all its log-probabilities; ids and ranks as ever. Exponentials are summed in fp32 within 1024
  * logits, in fp64 above. ranks, entropies may be NULL; top <= V. Outputs contiguous, apart from one another and from the inputs.
- * Rows may start at any element. R < 2^31, V <= 2^24, R * ceil(V / 4096) < 2^24. scratch: esp_token_logprobs_scratch bytes,
+ * Rows may start at any element. R < 2^31, V <= 2^20, R * ceil(V / 4096) < 2^24. scratch: esp_token_logprobs_scratch bytes,
  * 16-byte aligned, any values. A row's bits depend on that row alone. */
 int esp_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t R, int64_t V, const int32_t* tokens,
                        const float* temperature, int64_t top, float* logprobs, int32_t* ranks, float* entropies,

@@ -3,6 +3,8 @@ and the synthetic decoder's bookkeeping around its caches."""
 import ctypes
 import itertools
 import random
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -110,3 +112,13 @@ def test_algorithmic_bytes_count_the_norms_of_q_and_k():
     assert dec.algorithmic_bytes(picks, 3) - plain == 2 * 2 * S.HEAD_DIM * 2
     dec.layers[1].cache = None                                # a layer without a cache reads none of them
     assert dec.algorithmic_bytes(picks, 3) - plain == 2 * S.HEAD_DIM * 2
+
+
+def test_the_largest_vocabulary_is_the_headers(lib):  # noqa: F811
+    """What include/espalier.h says of V, the scratch's size and the call's own check are one number."""
+    text = (Path(__file__).resolve().parent.parent / "include" / "espalier.h").read_text()
+    most = 1 << int(re.search(r"R < 2\^31, V <= 2\^(\d+), R \* ceil", text).group(1))
+    call = lambda V: lib.esp_token_logprobs(FAR, 1, V, 1, V, 16, None, 0, 16, None, None, None, None, 16, 0, None)  # noqa: E731
+    assert lib.esp_token_logprobs_scratch(1, most, 0) > 0 and lib.esp_token_logprobs_scratch(1, most + 1, 0) == 0
+    assert call(most) == 1 and "scratch" in lib.esp_last_error().decode()
+    assert call(most + 1) == 1 and "V" in lib.esp_last_error().decode()

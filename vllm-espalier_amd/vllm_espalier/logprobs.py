@@ -9,7 +9,7 @@ from .experts import ext
 def token_logprobs(logits, tokens, top: int = 0, temperature=None, out=None):
     """(logprobs fp32 [R], ranks int32 [R], entropies fp32 [R], top_ids int32 [R, top], top_logprobs fp32 [R, top]).
 
-    logits       [R, V], bf16, fp16 or fp32, rows that start at any element. Masked tokens are -inf.
+    logits       [R, V], bf16, fp16 or fp32, rows that start at any element, V at most 2^20. Masked tokens are -inf.
     tokens       int32 [R]; one outside [0, V): rank and log-probability 0
     top          how many of the likeliest tokens, at most 64; among equal ones the lowest first
     temperature  fp32 [R]: p = softmax(row / temperature); below 1e-5 (a greedy request), or None: 1
