@@ -60,9 +60,6 @@ __device__ __forceinline__ Request request(const AttendArgs& a, int n, int first
 __device__ __forceinline__ Request request_of(const AttendArgs& a, int b) {              // any lane's
     return b < a.B ? request(a, a.n_new ? a.n_new[b] : 1, a.first ? a.first[b] : b, a.lengths[b]) : Request{0, 0, 0, 0, 0};
 }
-__device__ __forceinline__ Request uniform_request(const AttendArgs& a, int b) {
-    return request(a, a.n_new ? load_uniform(a.n_new + b) : 1, a.first ? load_uniform(a.first + b) : b, load_uniform(a.lengths + b));
-}
 
 struct Piece {
     Request r;
