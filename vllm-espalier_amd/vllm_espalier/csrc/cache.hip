@@ -142,10 +142,6 @@ template <int D, bool BF, bool E8, int TOKENS>
 __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
     constexpr int LANES = D / 8, ROWS = 64 / LANES;           // lanes a row, rows a wave
     __shared__ float2 turn[TOKENS][D / 2];                    // (cos, sin) of a token's angles
-    // All arguments at once: left to where they are used, they come one after the other, a trip to memory each
-    asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.q_row), "s"(a.k_row), "s"(a.v_row), "s"(a.q_head), "s"(a.k_head), "s"(a.v_head),
-                 "s"(a.wq), "s"(a.wk), "s"(a.slots), "s"(a.positions), "s"(a.pos_axis), "s"(a.inv_freq), "s"(a.axes), "s"(a.T), "s"(a.Hq),
-                 "s"(a.Hkv), "s"(a.half), "s"(a.page), "s"(a.pages), "s"(a.rot_scale), "s"(a.eps), "s"(a.adjacent), "s"(a.n_axes));
     const int t0 = blockIdx.x * TOKENS, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int token = TOKENS == 1 ? 0 : wave, t = min(t0 + token, a.T - 1), d = lane % LANES * 8, sub = lane / LANES;
     const int q_passes = (a.Hq + ROWS - 1) / ROWS, kv_passes = (a.Hkv + ROWS - 1) / ROWS, passes = q_passes + 2 * kv_passes;
@@ -232,8 +228,8 @@ void append_launch(const AppendArgs& a, hipStream_t st) {
     constexpr int ROWS = 512 / D;
     const int passes = (a.Hq + ROWS - 1) / ROWS + 2 * ((a.Hkv + ROWS - 1) / ROWS);
     // From 256 tokens on four share a workgroup, whose angles a wave's worth of threads makes at once; as many shares of their rows
-    // as fill the CUs, two passes at least. 8192 tokens of 32 + 2 x 4 heads of 128 (168 MB): 41 us, 4.1 TB/s (73 us a token a workgroup);
-    // 1531: 15 us (21 us); 300: 6.5 us (5.5 us); one: 3.4 us, bound by its chain of loads
+    // as fill the CUs, two passes at least. 8192 tokens of 32 + 2 x 4 heads of 128 (168 MB): 42 us, 4.0 TB/s (73 us a token a workgroup);
+    // 1531: 15 us (21 us); 300: 6.5 us (5.5 us); one: 3.6 us by the kernel trace (3.4 at least), bound by its chain of loads
     if (a.T >= 256) {
         const int shares = std::max(1, std::min((passes + 1) / 2, 8192 / a.T));
         append_kernel<D, BF, E8, 4><<<dim3((unsigned)((a.T + 3) / 4), (unsigned)shares), 256, 0, st>>>(a);
