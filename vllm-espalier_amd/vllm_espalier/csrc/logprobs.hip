@@ -252,8 +252,6 @@ struct LogprobsRow {
 template <int DT, int AHEAD, int THREADS>
 __global__ __launch_bounds__(THREADS) void logprobs_row_kernel(const LogprobsArgs a) {
     constexpr int WAVES = THREADS / 64, HELD = THREADS == 256 ? PIECES_MAX / 256 : 1;       // (512: at most 256 pieces)
-    asm volatile("" ::"s"(a.logits), "s"(a.stride), "s"(a.V), "s"(a.pieces), "s"(a.top), "s"(a.tokens), "s"(a.temperature),
-                 "s"(a.logprobs), "s"(a.ranks), "s"(a.entropies), "s"(a.top_ids), "s"(a.top_logprobs), "s"(a.part));      // all at once
     extern __shared__ __attribute__((aligned(16))) unsigned long long keys[];        // keys_room and two more
     __shared__ int chosen[TOP_MAX];
     __shared__ uint32_t bar;
