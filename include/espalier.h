@@ -482,7 +482,8 @@ int64_t esp_verify_scratch(int64_t B, int64_t G, int64_t V);
 /* `pages` pages of `page` tokens (a multiple of 16, at most 65536), `heads` heads of dim (64, 128 or 256) elements each: element d
  * of head h of token t of page p at k[p * k_page + t * k_token + h * k_head + d] and v likewise, strides in elements. dtype
  * ESP_F16, ESP_BF16, or ESP_E4M3 with k_scale and v_scale (fp32 [heads] on the device, positive): a value stands for itself times
- * its head's scale; without scales NULL. k, v and every stride 16-byte aligned; k_token, v_token at least dim. */
+ * its head's scale; without scales NULL. k, v and every stride 16-byte aligned; k_token, v_token at least dim,
+ * below 2^24. At most 1024 heads. */
 typedef struct esp_kv_cache {
     void* k;
     void* v;
@@ -505,7 +506,7 @@ typedef struct esp_kv_cache {
  * (infinities too) +-448. half a multiple of 8 (0: no rotation). out may be q (in place) and must else overlap none of q, k and v
  * (refused), nor the cache any of them; the cache's elements must lie apart, k's from v's too (refused; of k and v with different strides
  * the caller sees to it). Alignment: rows and weights 16 bytes, strides
- * a multiple of 8 elements. T < 2^24. A row's bits depend on that row alone. */
+ * a multiple of 8 elements. T < 2^24, Hq <= 1024, n_axes <= 16. A row's bits depend on that row alone. */
 int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
                      int64_t v_row, int64_t v_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
                      const int64_t* slots, const int64_t* positions, int64_t pos_axis, int64_t n_axes, const double* inv_freq,
@@ -520,13 +521,14 @@ int esp_cache_append(const void* q, int64_t q_row, int64_t q_head, const void* k
  * h / (Hq / heads), zeros where it sees nothing. What a row does not see does not change it, whatever it holds. Rows of no request,
  * and those of a request with n outside [0, max_new] or rows outside [0, T), are left as they are. Scores and sums in fp32, the
  * weights rounded to dtype for the product with the values; where a row sees a value that is NaN or infinite, its output is NaN or
- * infinite.
+ * infinite (values from 2^90 on may do the same: they are summed in fp32 and divided at the end).
  * split: tokens a piece of a request's keys (a multiple of 128); pieces run apart and are joined in order. 0: chosen from all the
  * batch's lengths, so that a row's bits depend on them; with a split of its own a row's bits depend on its request alone (requests
- * of more than 32 rows a head of the cache, n * Hq / heads, are then not cut at all).
+ * of more than 32 rows a head of the cache, n * Hq / heads, are then not cut at all, and take long where their rows are few and their
+ * keys many), and scratch and launch go by max_pages * page / split.
  * q, out [T][Hq][dim] of dtype ESP_BF16 or ESP_F16 with row and head strides, 16-byte aligned (strides multiples of 8); out must
- * not overlap q (refused), nor anything else. Hq a multiple of heads; scale > 0; max_pages * page <= 2^28; T < 2^24, T * Hq < 2^31,
- * max_new * Hq / heads < 2^23. scratch: at least esp_paged_attention_scratch bytes, 16-byte aligned, any values. */
+ * not overlap q (refused), nor anything else. Hq a multiple of heads, at most 65536; scale > 0; window, split < 2^30;
+ * max_pages * page <= 2^28; T < 2^24, T * Hq < 2^31, max_new * Hq / heads < 2^23. scratch: at least esp_paged_attention_scratch bytes, 16-byte aligned, any values. */
 int esp_paged_attention(const void* q, int64_t q_row, int64_t q_head, int64_t T, int64_t Hq, int dtype, const esp_kv_cache* cache,
                         const int32_t* tables, int64_t table_row, int64_t max_pages, const int32_t* lengths,
                         const int32_t* first, const int32_t* n_new, int64_t B, int64_t max_new, double scale, int64_t window,

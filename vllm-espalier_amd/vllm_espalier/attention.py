@@ -119,7 +119,8 @@ class PagedCache:
         window    how many tokens a row sees, its own the last; 0: all
         split     tokens a piece of a request's keys (a multiple of 128) where pieces run apart; 0: chosen on the device from
                   the batch's lengths. With a split of its own a row's bits depend on its request alone (one of more than 32 rows
-                  a head of the cache, n_new times the heads of a group, is then not cut).
+                  a head of the cache, n_new times the heads of a group, is then not cut: few such rows over many tokens take long).
+                  Scratch and launch are then sized by what the tables could hold.
 
         Rows that see nothing are zeros; rows of no request are left as they are (in a new tensor: undefined). Nothing is kept
         between calls, so calls on several streams do not meet."""

@@ -23,7 +23,8 @@
 // token over up to 8171, heads 32/4 of 128 (273 MB), take 54 us (5.0 TB/s) and the join 4.9; one over 131072 (268 MB) 49 us
 // (5.4 TB/s) and 5.4; 64 over 4000, 8 heads of 64 (524 MB), 88 us (5.9 TB/s). An e4m3 cache is bound by its widening, heads of 256
 // with two tiles' outputs by one workgroup a CU: 40 requests of up to 4 new tokens over up to 6001, heads 16/2, e4m3 (128 MB), 37 us
-// (3.5 TB/s). One token over 113 is bound by its chain of loads: length, table, keys, values, 6.3 us.
+// (3.5 TB/s). One token over 113 is bound by its chain of loads: length, table, keys, values, 6.2 us
+// in a table of up to 128 tokens; a wider one could hold a second piece, and the join's launch, of nothing here, makes it 8.8.
 #include "attention_few.hpp"
 
 namespace esp {

@@ -14,8 +14,9 @@
 //
 // What bounds it is neither products nor memory alone but a wave's order: its products (34 % of the cycles), then its softmax (41 %
 // on the vector units), with two waves a SIMD to fill in for each other, which is what the registers of 32 x 128 outputs leave.
-// Three requests of up to 2048 new tokens over up to 4096, heads 32/4 of 128, bf16 (105 GFLOP of visible pairs): 144 to 158 us
-// (0.7 PFLOP/s), where the tiles that see most decide the end; one of 4096 over 8192, heads 32/8 (412 GFLOP), 445 us (0.93 PFLOP/s).
+// Three requests of up to 2048 new tokens over up to 4096, heads 32/4 of 128, bf16 (105 GFLOP of visible pairs): 134 to 139 us
+// a pass with its join (0.78 PFLOP/s; a kernel trace, which slows it, has 143 at least), where the tiles that see most decide the end;
+// one of 4096 over 8192, heads 32/8 (412 GFLOP), 445 us (0.93 PFLOP/s).
 // A large matrix product reaches 1.5.
 #include "attention_few.hpp"
 
@@ -27,7 +28,7 @@ using global_void_ptr = const __attribute__((address_space(1))) void*;
 using lds_void_ptr = __attribute__((address_space(3))) void*;
 
 constexpr int TILE = 64;                       // keys in the LDS
-// (fp16: what reference() leaves of its range. The outputs are scaled more often: 4 prompts of 1024 over 2047, 32/4 heads of 64 125 us for
+// (fp16: what reference() leaves of its range. The outputs are scaled more often: 4 prompts of 1024 over 3071, 32/4 heads of 64 125 us for
 // 123 with 8, 16/2 of 256 252 for 235)
 template <bool BF>
 constexpr float LAG = BF ? 8.0f : 2.0f;
